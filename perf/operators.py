@@ -1,0 +1,493 @@
+"""The operators of the serving path as timed and checked cases: attention over whole prompts, the paged
+8-bit cache (filling it and reading it back, decoding over it) and what is done with its pages (forking,
+freeing, moving them).
+
+``listed()`` names the fixed cases, ``draw(rng)`` gives more of the same ranges, ``prepare`` makes what a
+program holds before the call, ``run`` is one pass, ``work`` the bytes and operations that it cannot do
+without, and ``exact`` the same outputs in 64 bits, written apart from ``run``.  With ``own`` false ``run``
+computes in plain torch operations of 32 bits, with ``own`` true it calls the package.
+
+The cache: a sequence's tokens lie in blocks of ``page`` tokens.  A full block of a KV head is held in 8 bits
+with one float32 scale for its keys and one for its values: with a = max(|x|, 2^-100) over the block and
+top = 127 (int8) or 448 (e4m3), scale = a / top and code = x * (top / a), each operation rounded to float32,
+the code to the nearest of its type (ties to even).  The open block stays as it came.
+"""
+from __future__ import annotations
+
+import math
+import sys
+from pathlib import Path
+from types import SimpleNamespace
+
+import torch
+
+own = False
+
+_PACKAGE = str(Path(__file__).resolve().parent.parent / "kv-project_amd")
+if _PACKAGE not in sys.path:
+    sys.path.insert(0, _PACKAGE)
+
+DEV = "cuda"
+DTYPES = {"bf16": torch.bfloat16, "fp16": torch.float16}
+TOP = {"int8": 127.0, "e4m3": 448.0}
+ROUNDS = 4                                     # a served sequence's pages lie between those of others
+
+
+# ---- the cases ------------------------------------------------------------------------------
+
+def listed():
+    return [
+        # one short question: latency
+        dict(name="prompt_bf16_1x20", op="prompt", dtype="bf16", Hq=32, Hkv=8, d=128, n_seq=1, lo=20, hi=20, past=0,
+             causal=True),
+        # a batch of requests of very different lengths, packed
+        dict(name="prompt_fp16_24_ragged", op="prompt", dtype="fp16", Hq=32, Hkv=8, d=128, n_seq=24, lo=1, hi=2901, past=0,
+             causal=True),
+        # a long prompt of an 8B-shaped layer; the matrix cores
+        dict(name="prompt_bf16_16k", op="prompt", dtype="bf16", Hq=32, Hkv=8, d=128, n_seq=1, lo=16384, hi=16384, past=0,
+             causal=True),
+        # chunks of prompts behind what is there of them, head_dim 64
+        dict(name="prompt_bf16_d64_chunks", op="prompt", dtype="bf16", Hq=32, Hkv=8, d=64, n_seq=4, lo=512, hi=1531,
+             past=9000, causal=True),
+        # a few requests enter the cache, one layer, and are read back; small
+        dict(name="fill_fp16_e4m3_ragged", op="fill", dtype="fp16", code="e4m3", page=32, Hkv=8, d=64, n_seq=5, lo=1, hi=700,
+             held=45),
+        # a batch of prompts enters the cache and is read back; bandwidth
+        dict(name="fill_bf16_int8_16x8k", op="fill", dtype="bf16", code="int8", page=64, Hkv=8, d=128, n_seq=16, lo=6001,
+             hi=8200, held=0),
+        # one sequence, one token: latency
+        dict(name="decode_fp16_e4m3_4k", op="decode", dtype="fp16", code="e4m3", page=64, Hq=32, Hkv=8, d=128, n_seq=1,
+             lo=4096, hi=4096, Tq=1, uneven=False),
+        # many sequences of different lengths, one to four drafted tokens each
+        dict(name="decode_bf16_int8_48_ragged", op="decode", dtype="bf16", code="int8", page=32, Hq=32, Hkv=8, d=64,
+             n_seq=48, lo=90, hi=12000, Tq=4, uneven=True),
+        # 16 sequences at 32k of an 8B-shaped layer; bandwidth
+        dict(name="decode_bf16_int8_16x32k", op="decode", dtype="bf16", code="int8", page=64, Hq=32, Hkv=8, d=128, n_seq=16,
+             lo=32700, hi=32768, Tq=1, uneven=False),
+        # eight continuations of one prompt: forked, a step of two tokens through the layers, freed
+        dict(name="branch_bf16_int8_8_of_6k", op="branch", dtype="bf16", code="int8", page=64, Hq=32, Hkv=8, d=128, n_seq=8,
+             lo=6019, hi=6019, Tq=2, layers=4),
+        # a small pool, half of it freed, brought to its size
+        dict(name="resize_small", op="resize", dtype="fp16", code="int8", page=32, Hkv=4, d=64, n_seq=7, lo=40, hi=500,
+             layers=2),
+        # a model's whole pool after a third of its sequences have left
+        dict(name="resize_32_layers", op="resize", dtype="bf16", code="int8", page=64, Hkv=8, d=128, n_seq=12, lo=2500, hi=5100,
+             layers=32),
+    ]
+
+
+def _log_int(rng, lo, hi):
+    return int(round(math.exp(rng.uniform(math.log(lo), math.log(hi)))))
+
+
+def draw(rng):
+    op = rng.choice(["prompt", "prompt", "prompt", "fill", "fill", "decode", "decode", "decode", "branch", "resize"])
+    c = dict(op=op, dtype=rng.choice(["bf16", "fp16"]), Hkv=rng.choice([1, 2, 4, 8]), d=rng.choice([64, 128, 128]))
+    if op in ("prompt", "decode", "branch"):
+        c["Hq"] = c["Hkv"] * rng.choice([1, 2, 3, 4, 4, 7, 8] if c["Hkv"] < 8 else [1, 2, 3, 4])
+    if op != "prompt":
+        c.update(code=rng.choice(["int8", "e4m3"]), page=rng.choice([32, 64, 128]))
+    if op == "prompt":
+        c.update(n_seq=_log_int(rng, 1, 32), past=rng.choice([0, 0, _log_int(rng, 1, 16000)]),
+                 causal=rng.choice([True, True, True, False]))
+        pairs = 16384 * 16384 / 2 / c["n_seq"]                               # of a sequence: hi (hi + past) at most
+        c["hi"] = _log_int(rng, 1, int((math.sqrt(c["past"] ** 2 + 4 * pairs) - c["past"]) / 2))
+    elif op == "fill":
+        c.update(n_seq=_log_int(rng, 1, 24), held=rng.choice([0, rng.randint(1, 300)]))
+        c["hi"] = _log_int(rng, 1, 96000 // c["n_seq"])
+    elif op == "decode":
+        c.update(n_seq=_log_int(rng, 1, 64), Tq=rng.choice([1, 1, 2, 5]), uneven=rng.choice([True, False]))
+        c["hi"] = _log_int(rng, 8, min(131072, 16 * 30000 * 8 // (c["n_seq"] * c["Hkv"])))
+    elif op == "branch":
+        c.update(n_seq=rng.randint(2, 12), Tq=rng.randint(1, 4), layers=rng.randint(1, 4), hi=_log_int(rng, 10, 12000))
+    else:
+        c.update(code="int8", n_seq=rng.randint(3, 12), layers=rng.choice([1, 3, 8, 16]), hi=_log_int(rng, 300, 5000))
+    c["lo"] = c["hi"] if op == "branch" else rng.randint(max(1, c["hi"] // (2 if op == "resize" else 8)), c["hi"])
+    if op == "decode":
+        c["lo"] = max(c["lo"], min(c["hi"], c["Tq"]))
+        c["Tq"] = min(c["Tq"], c["lo"])
+    return c
+
+
+def _lens(c):
+    """The sequences' lengths: spread evenly in their logarithm from ``lo`` to ``hi``, not in order."""
+    n, lo, hi = c["n_seq"], c["lo"], c["hi"]
+    if n == 1:
+        return [hi]
+    at = [round(math.exp(math.log(lo) + (math.log(hi) - math.log(lo)) * i / (n - 1))) for i in range(n)]
+    step = next(s for s in (7, 5, 11, 13, 17) if math.gcd(s, n) == 1)
+    return [at[(i * step + n // 2) % n] for i in range(n)]
+
+
+def _past(c):
+    """Keys in front of the new ones, a different number for each sequence."""
+    return [c["past"] * (i + 1) // c["n_seq"] for i in range(c["n_seq"])]
+
+
+def _held(c):
+    return [c["held"] * (i + 1) // c["n_seq"] for i in range(c["n_seq"])]
+
+
+def _counts(c):
+    return [1 + i % c["Tq"] if c["uneven"] else c["Tq"] for i in range(c["n_seq"])]
+
+
+def work(case):
+    c = case
+    Hkv, d, lens = c["Hkv"], c["d"], _lens(c)
+    if c["op"] == "prompt":
+        past = _past(c)
+        keys = sum(n + p for n, p in zip(lens, past))
+        pairs = sum(n * p + (n * (n + 1) // 2 if c["causal"] else n * n) for n, p in zip(lens, past))
+        return {"bytes": 2 * d * (2 * c["Hq"] * sum(lens) + 2 * Hkv * keys), "flops": 4 * d * c["Hq"] * pairs}
+    P = c["page"]
+    if c["op"] == "fill":
+        held = _held(c)
+        rows = Hkv * d * 2
+        full = sum((n + h) // P * P - h // P * P for n, h in zip(lens, held))
+        return {"bytes": rows * (2 * sum(lens) + full + 2 * (sum(lens) + sum(held))), "flops": 5 * rows * sum(lens)}
+    token = 2 * Hkv * d
+    if c["op"] == "decode":
+        codes = sum(n // P * P for n in lens)
+        nq = sum(_counts(c))
+        return {"bytes": token * codes + 8 * Hkv * codes // P + 2 * token * (sum(lens) - codes) + 4 * nq * c["Hq"] * d,
+                "flops": 4 * d * c["Hq"] * sum(n * t for n, t in zip(lens, _counts(c)))}
+    if c["op"] == "branch":
+        H, n, t = c["hi"], c["n_seq"], c["Tq"]
+        kept = H // P * P
+        return {"bytes": c["layers"] * (token * kept + 8 * Hkv * kept // P + 2 * token * (H - kept) * 2 * n
+                                        + 2 * token * t * n * 2 + 4 * n * t * c["Hq"] * d),
+                "flops": c["layers"] * 4 * d * c["Hq"] * n * t * (H + t)}
+    live = sum(n // P for i, n in enumerate(lens) if i % 3 != 1)
+    return {"bytes": 2 * c["layers"] * live * (token * P + 8 * Hkv), "flops": 0}
+
+
+# ---- inputs ---------------------------------------------------------------------------------
+
+def _randn(g, *shape):
+    return torch.randn(shape, generator=g, device=DEV)
+
+
+def _kv(g, c, n):
+    """Keys and values of n tokens (n, Hkv, d): heavy-tailed channel magnitudes in the keys."""
+    H, d, dt = c["Hkv"], c["d"], DTYPES[c["dtype"]]
+    t3 = (_randn(g, H, d) / (_randn(g, H, d, 3).square().sum(-1) / 3.0).sqrt()).abs().clamp(0.2, 8.0)
+    return (_randn(g, n, H, d) * t3).to(dt), _randn(g, n, H, d).to(dt)
+
+
+def _q(g, c, n):
+    return _randn(g, n, c["Hq"], c["d"]).to(DTYPES[c["dtype"]])
+
+
+def _quantise(x, page, code):
+    """Full blocks x (n page, H, d) -> codes (n, H, page, d) and scales (n, H)."""
+    b = x.reshape(-1, page, x.shape[1], x.shape[2]).transpose(1, 2).float()
+    a = b.abs().amax((2, 3)).clamp_min(2.0 ** -100)
+    y = b * (TOP[code] / a)[..., None, None]
+    codes = y.round().to(torch.int8) if code == "int8" else y.to(torch.float8_e4m3fn)
+    return codes, a / TOP[code]
+
+
+def _values(codes, scales):
+    """(n, H, page, d) codes -> (n page, H, d) float32."""
+    v = codes.float() * scales[..., None, None]
+    return v.transpose(1, 2).reshape(-1, v.shape[1], v.shape[3])
+
+
+def _chunks(lens, rounds=ROUNDS):
+    """[(sequence, first, end)] of each round in which the sequences are filled."""
+    return [[(i, n * r // rounds, n * (r + 1) // rounds) for i, n in enumerate(lens)] for r in range(rounds)]
+
+
+def _cache(c, lens, slots, layers=1):
+    import kvq
+    pages = sum(-(-n // c["page"]) for n in lens)
+    return kvq.PagedCache(layers, slots, pages, max(lens), c["Hkv"], c["d"], page=c["page"], code=c["code"],
+                          dtype=DTYPES[c["dtype"]], device=DEV)
+
+
+def _fill(cache, layers, lens):
+    """Tokens of sequences 0, 1, .. into the cache's slots of these numbers, in rounds. ``layers``: lists of each
+    sequence's (k, v)."""
+    for chunk in _chunks(lens):
+        step = cache.extend([i for i, _, _ in chunk], [b - a for _, a, b in chunk])
+        for l, kv in enumerate(layers):
+            k, v = (torch.cat([kv[i][s][a:b] for i, a, b in chunk]) for s in (0, 1))
+            cache.append(l, k, v, step)
+
+
+class _Pages:
+    """A sequence's tokens in plain form: full blocks as codes and scales, the open block as it came."""
+
+    def __init__(self, k, v, page, code):
+        n = k.shape[0] // page * page
+        self.k, self.v = _quantise(k[:n], page, code), _quantise(v[:n], page, code)
+        self.k_open, self.v_open = k[n:], v[n:]
+
+    def rows(self):
+        """float32 keys and values (n, H, d)."""
+        return (torch.cat([_values(*self.k), self.k_open.float()]), torch.cat([_values(*self.v), self.v_open.float()]))
+
+
+def prepare(case, seed):
+    c, g = case, torch.Generator(device=DEV).manual_seed(int(seed))
+    st = SimpleNamespace(c=c, own=own, lens=_lens(c), scaling=c["d"] ** -0.5)
+    n, lens = c["n_seq"], st.lens
+    if c["op"] == "prompt":
+        st.lens_k = [a + b for a, b in zip(lens, _past(c))]
+        st.q = _q(g, c, sum(lens))
+        st.k, st.v = _kv(g, c, sum(st.lens_k))
+        if own:
+            import kvq
+            st.plan = kvq.PromptPlan(lens, c["Hq"], c["Hkv"], lens_k=st.lens_k, causal=c["causal"], device=DEV)
+        return st
+    if c["op"] == "fill":
+        st.held = _held(c)
+        st.before = [_kv(g, c, h) for h in st.held]
+        st.k, st.v = _kv(g, c, sum(lens))
+        if own:
+            whole = [a + b for a, b in zip(lens, st.held)]
+            st.cache = _cache(c, whole + st.held, 2 * n)
+            _fill(st.cache, [st.before], st.held)
+        else:
+            st.before = [_Pages(k, v, c["page"], c["code"]) for k, v in st.before]
+    elif c["op"] == "decode":
+        kv = [_kv(g, c, m) for m in lens]
+        st.counts = _counts(c)
+        st.q = _q(g, c, sum(st.counts))
+        if own:
+            st.cache = _cache(c, lens, n)
+            _fill(st.cache, [[(k[:k.shape[0] - t], v[:v.shape[0] - t]) for (k, v), t in zip(kv, st.counts)]],
+                  [m - t for m, t in zip(lens, st.counts)])
+            st.step = st.cache.extend(list(range(n)), st.counts)
+            st.cache.append(0, torch.cat([k[k.shape[0] - t:] for (k, _), t in zip(kv, st.counts)]),
+                            torch.cat([v[v.shape[0] - t:] for (_, v), t in zip(kv, st.counts)]), st.step)
+        else:
+            st.pages = [_Pages(k, v, c["page"], c["code"]) for k, v in kv]
+    elif c["op"] == "branch":
+        prefix = [_kv(g, c, c["hi"]) for _ in range(c["layers"])]
+        st.new = [_kv(g, c, n * c["Tq"]) for _ in range(c["layers"])]
+        st.q = [_q(g, c, n * c["Tq"]) for _ in range(c["layers"])]
+        if own:
+            st.cache = _cache(c, [c["hi"]] + [c["Tq"] + c["page"]] * n + [c["hi"] + c["Tq"]], n + 1, c["layers"])
+            _fill(st.cache, [[kv] for kv in prefix], [c["hi"]])
+        else:
+            st.pages = [_Pages(k, v, c["page"], c["code"]) for k, v in prefix]
+            st.table = torch.arange(c["hi"] // c["page"], dtype=torch.int32, device=DEV)
+    else:
+        st.left = [i for i in range(n) if i % 3 != 1]
+        kv = ([_kv(g, c, m) for m in lens] for _ in range(c["layers"]))
+        st.pages = sum(lens[i] // c["page"] for i in st.left)
+        if own:
+            st.cache = _cache(c, lens, n, c["layers"])
+            steps = [(chunk, st.cache.extend([i for i, _, _ in chunk], [b - a for _, a, b in chunk]))
+                     for chunk in _chunks(lens)]
+            for l, layer in enumerate(kv):
+                for chunk, step in steps:
+                    k, v = (torch.cat([layer[i][s][a:b] for i, a, b in chunk]) for s in (0, 1))
+                    st.cache.append(l, k, v, step)
+            st.cache.free([i for i in range(n) if i % 3 == 1])
+        else:
+            st.ids, total = _page_ids(lens, c["page"])
+            shape = (c["layers"], total, c["Hkv"])
+            st.codes = [torch.empty((*shape, c["page"], c["d"]), dtype=torch.int8, device=DEV) for _ in (0, 1)]
+            st.scales = [torch.empty(shape, device=DEV) for _ in (0, 1)]
+            for l, layer in enumerate(kv):
+                for i, x in enumerate(layer):
+                    at = torch.tensor(st.ids[i], dtype=torch.long, device=DEV)
+                    for s in (0, 1):
+                        m = lens[i] // c["page"] * c["page"]
+                        st.codes[s][l, at], st.scales[s][l, at] = _quantise(x[s][:m], c["page"], c["code"])
+            st.ids = [torch.tensor(x, dtype=torch.long, device=DEV) for x in st.ids]
+    return st
+
+
+def _page_ids(lens, page):
+    """Pages of each sequence when the sequences are filled in rounds: the lowest free page for each block that
+    gets full, in the order of the sequences."""
+    ids, total = [[] for _ in lens], 0
+    for chunk in _chunks(lens):
+        for i, a, b in chunk:
+            for _ in range(b // page - a // page):
+                ids[i].append(total)
+                total += 1
+    return ids, total
+
+
+# ---- one pass -------------------------------------------------------------------------------
+
+def _attend(q, k, v, scaling, causal=True):
+    """q (t, Hq, d) over k, v (n, Hkv, d) float32, the last query at the last key -> (t, Hq, d) float32."""
+    (t, Hq, d), (n, Hkv, _) = q.shape, k.shape
+    rep = Hq // Hkv
+    out = torch.zeros((t, Hq, d), device=q.device)
+    if n == 0 or t == 0:
+        return out
+    hidden = (torch.arange(n, device=q.device)[None] > torch.arange(t, device=q.device)[:, None] + (n - t)) if causal else None
+    per = max(1, min(Hkv, (1 << 30) // (rep * t * n)))                      # KV heads of a product: scores of 4 GB at most
+    for h in range(0, Hkv, per):
+        m = min(per, Hkv - h)
+        qs = q[:, h * rep:(h + m) * rep].float().reshape(t, m, rep, d).permute(1, 2, 0, 3).reshape(m, rep * t, d)
+        s = (qs @ k[:, h:h + m].permute(1, 2, 0).contiguous()) * scaling
+        if hidden is not None:
+            s.view(m, rep, t, n).masked_fill_(hidden, -math.inf)
+        top = s.amax(-1, keepdim=True)
+        s.sub_(torch.where(top == -math.inf, torch.zeros_like(top), top)).exp_()
+        o = (s @ v[:, h:h + m].transpose(0, 1).contiguous()) / s.sum(-1, keepdim=True).clamp_min(1e-30)
+        out[:, h * rep:(h + m) * rep] = o.view(m, rep, t, d).permute(2, 0, 1, 3).reshape(t, m * rep, d)
+    return out
+
+
+def _spans(counts):
+    at = 0
+    for n in counts:
+        yield at, at + n
+        at += n
+
+
+def run(state):
+    st, c = state, state.c
+    n, dt = c["n_seq"], DTYPES[c["dtype"]]
+    if st.own:
+        import kvq
+    if c["op"] == "prompt":
+        if st.own:
+            return kvq.prompt_attention(st.q, st.k, st.v, st.scaling, st.plan)
+        out = torch.empty_like(st.q)
+        for (a, b), (x, y) in zip(_spans(st.lens), _spans(st.lens_k)):
+            out[a:b] = _attend(st.q[a:b], st.k[x:y].float(), st.v[x:y].float(), st.scaling, c["causal"])
+        return out
+    if c["op"] == "fill":
+        if st.own:
+            slots = list(range(n, 2 * n))
+            if c["held"]:
+                st.cache.fork(list(range(n)), slots)
+            st.cache.append(0, st.k, st.v, st.cache.extend(slots, st.lens))
+            out = st.cache.rows(0, slots)
+            st.cache.free(slots)
+            return out
+        ks, vs = [], []
+        for p, (a, b) in zip(st.before, _spans(st.lens)):
+            x = _Pages(torch.cat([p.k_open, st.k[a:b]]), torch.cat([p.v_open, st.v[a:b]]), c["page"], c["code"])
+            k, v = x.rows()
+            ks += [_values(*p.k).to(dt), k.to(dt)]
+            vs += [_values(*p.v).to(dt), v.to(dt)]
+        return torch.cat(ks), torch.cat(vs)
+    if c["op"] == "decode":
+        if st.own:
+            return kvq.paged_decode(st.q, st.scaling, st.cache, 0, st.step)
+        return torch.cat([_attend(st.q[a:b], *p.rows(), st.scaling) for p, (a, b) in zip(st.pages, _spans(st.counts))]).to(dt)
+    if c["op"] == "branch":
+        t, P = c["Tq"], c["page"]
+        if st.own:
+            slots = list(range(1, n + 1))
+            st.cache.fork([0] * n, slots)
+            step = st.cache.extend(slots, [t] * n)
+            out = []
+            for l in range(c["layers"]):
+                st.cache.append(l, *st.new[l], step)
+                out.append(kvq.paged_decode(st.q[l], st.scaling, st.cache, l, step))
+            out.append(st.cache.table[1:n + 1, :(c["hi"] + t) // P])
+            st.cache.free(slots)
+            return out
+        out = []
+        for l in range(c["layers"]):
+            p = st.pages[l]
+            k0, v0 = _values(*p.k), _values(*p.v)
+            o = []
+            for a in range(0, n * t, t):
+                x = _Pages(torch.cat([p.k_open, st.new[l][0][a:a + t]]), torch.cat([p.v_open, st.new[l][1][a:a + t]]),
+                           P, c["code"])
+                k, v = x.rows()
+                o.append(_attend(st.q[l][a:a + t], torch.cat([k0, k]), torch.cat([v0, v]), st.scaling))
+            out.append(torch.cat(o).to(dt))
+        m = (c["hi"] + t) // P - c["hi"] // P
+        new = c["hi"] // P + torch.arange(n * m, dtype=torch.int32, device=DEV).view(n, m)
+        out.append(torch.cat([st.table.expand(n, -1), new], 1))
+        return out
+    if st.own:
+        st.cache.resize(st.pages)
+        codes, scales = st.cache.codes(), st.cache.scales()
+        return [*codes, *scales, *[st.cache.table[i, :st.lens[i] // c["page"]] for i in st.left]]
+    live = torch.cat([st.ids[i] for i in st.left]).sort().values
+    stay = live < st.pages                     # pages beyond the new end go to the free places below it, both in order
+    free = torch.ones(st.pages, dtype=torch.bool, device=DEV)
+    free[live[stay]] = False
+    to = live.clone()
+    to[~stay] = free.nonzero()[:, 0]
+    origin = torch.empty_like(live)
+    origin[to] = live
+    place = torch.empty(st.codes[0].shape[1], dtype=torch.int32, device=DEV)
+    place[live] = to.int()
+    return [*[x[:, origin] for x in st.codes], *[x[:, origin] for x in st.scales], *[place[st.ids[i]] for i in st.left]]
+
+
+# ---- 64 bits --------------------------------------------------------------------------------
+
+def _exact_cache(x, page, code):
+    """Tokens (n, H, d) as the cache stands for them, float64."""
+    y = x.double().clone()
+    top = torch.tensor(TOP[code], dtype=torch.float64, device=x.device)
+    n = x.shape[0] // page
+    if n == 0:
+        return y
+    b = y[:n * page].view(n, page, *x.shape[1:])
+    a = b.abs().amax((1, 3), keepdim=True).clamp_min(2.0 ** -100)
+    z = (b * (top / a).float().double()).float()                             # two roundings to float32: part of the definition
+    z = torch.round(z).double() if code == "int8" else z.to(torch.float8_e4m3fn).double()
+    b.copy_(z * (a / top).float().double())
+    return y
+
+
+def _exact_rows(q, k, v, scaling, causal):
+    """One sequence, head by head and in pieces of queries, float64."""
+    (t, Hq, d), (n, Hkv, _) = q.shape, k.shape
+    out = torch.zeros((t, Hq, d), dtype=torch.float64, device=q.device)
+    if n == 0:
+        return out
+    j = torch.arange(n, device=q.device)
+    for h in range(Hq):
+        kh, vh = k[:, h * Hkv // Hq].double(), v[:, h * Hkv // Hq].double()
+        kt, vh = kh.t().contiguous(), vh.contiguous()
+        for a in range(0, t, 8192):
+            b = min(t, a + 8192)
+            m = min(n, max(0, b + n - t)) if causal else n                   # later keys: hidden from all of these
+            s = torch.matmul(q[a:b, h].double(), kt[:, :m]) * scaling
+            if causal:
+                s = torch.where(j[None, :m] <= torch.arange(a, b, device=q.device)[:, None] + (n - t), s, -math.inf)
+            if m:
+                p = torch.softmax(s, -1)
+                out[a:b, h] = torch.matmul(torch.nan_to_num(p, nan=0.0), vh[:m])
+    return out
+
+
+def exact(case, seed):
+    """What ``run`` returns, from the formulas in 64 bits."""
+    c = case
+    lens, n, scaling = _lens(c), c["n_seq"], c["d"] ** -0.5
+    g = torch.Generator(device=DEV).manual_seed(int(seed))
+    if c["op"] == "prompt":
+        q = _q(g, c, sum(lens))
+        lens_k = [a + b for a, b in zip(lens, _past(c))]
+        k, v = _kv(g, c, sum(lens_k))
+        return torch.cat([_exact_rows(q[a:b], k[x:y], v[x:y], scaling, c["causal"])
+                          for (a, b), (x, y) in zip(_spans(lens), _spans(lens_k))])
+    if c["op"] == "fill":
+        before = [_kv(g, c, h) for h in _held(c)]
+        new = _kv(g, c, sum(lens))
+        return tuple(torch.cat([_exact_cache(torch.cat([p[s], new[s][a:b]]), c["page"], c["code"])
+                                for p, (a, b) in zip(before, _spans(lens))]) for s in (0, 1))
+    if c["op"] == "decode":
+        kv = [_kv(g, c, m) for m in lens]
+        q = _q(g, c, sum(_counts(c)))
+        return torch.cat([_exact_rows(q[a:b], *(_exact_cache(x, c["page"], c["code"]) for x in pair), scaling, True)
+                          for pair, (a, b) in zip(kv, _spans(_counts(c)))])
+    if c["op"] == "branch":
+        t = c["Tq"]
+        prefix = [_kv(g, c, c["hi"]) for _ in range(c["layers"])]
+        new = [_kv(g, c, n * t) for _ in range(c["layers"])]
+        qs = [_q(g, c, n * t) for _ in range(c["layers"])]
+        return [torch.cat([_exact_rows(qs[l][a:a + t], *(_exact_cache(torch.cat([prefix[l][s], new[l][s][a:a + t]]), c["page"],
+                                                                      c["code"]) for s in (0, 1)), scaling, True)
+                           for a in range(0, n * t, t)]) for l in range(c["layers"])] + [None]
+    return None                                # moved bytes: nothing is computed
