@@ -659,6 +659,80 @@ int kvq_quasar_values(const float* pv, int64_t Hkv, int64_t rows, int64_t n_c, c
  * ---------------------------------------------------------------------------------------- */
 int kvq_selftest_mfma_layout(const uint16_t* a, const uint16_t* b, float* out, void* stream);
 
+/* ------------------------------------------------------------------------------------------
+ * Attention over whole prompts (the reference leaves it to SDPA: STRATA_KV.py:499-504).
+ * Packed rows of n sequences: q (sum lens_q, Hq, D), k, v (sum lens_k, Hq / rep, D) of one 16-bit dtype,
+ * element strides per row and head, channels contiguous, pointers and strides multiples of 16 bytes; D 64
+ * or 128, rep <= 128.  Query t of a sequence sees keys 0 .. t + len_k - len_q (causal), or all of them; one
+ * that sees none gets zeros.  out (sum lens_q, Hq, D), contiguous.
+ * kvq_prompt_plan (host memory): fills `items` (8 int32 each) for a call over such sequences and returns
+ * their number (-1: bad sizes; more than items_cap: nothing to be used, call again with room).  The items
+ * go to the device as they are; they bound what kvq_prompt_attention reads.
+ * ---------------------------------------------------------------------------------------- */
+int64_t kvq_prompt_plan(const int64_t* lens_q, const int64_t* lens_k, int64_t n, int64_t rep, int causal,
+                        int32_t* items, int64_t items_cap);
+int kvq_prompt_attention(const void* q, int64_t q_st, int64_t q_sh, const void* k, int64_t k_st, int64_t k_sh,
+                         const void* v, int64_t v_st, int64_t v_sh, int dtype, int64_t Hq, int64_t H, int64_t D,
+                         float scaling, const int32_t* items, int64_t n_items, void* out, void* stream);
+
+/* ------------------------------------------------------------------------------------------
+ * The paged 8-bit cache (no counterpart in the reference, whose caches are dense in the batch).
+ * A sequence (slot) holds full blocks of `page` tokens (32, 64, 128) as pages, shared by count, and one
+ * open block in 16 bits.  Per layer:
+ *   kc (pages, H, page, D) codes, vc (pages, H, D, page) codes, sc (pages, H, 2) float (key, value scale),
+ *   ko (slots, 2, H, page, D) and vo (slots, 2, H, D, page) 16-bit rows of the open blocks (two buffers).
+ * All layers share table (slots, max_blocks) int32 on the device and the accounts in host memory:
+ *   lens (slots) int64, table (slots, max_blocks) int32, refs (pages) int32 users of each page,
+ *   open (slots) uint8 the current open buffer, account[2] = {free pages, no free page below this one}.
+ * code: 0 int8, 1 e4m3.  a = max(|x|, 2^-100) over a block of one head, scale = a / top, code =
+ * rne(x * (top / a)), top 127 or 448, in float32; a block with an infinity or a NaN has the scale NaN.
+ *
+ * kvq_pages_extend claims counts[i] tokens for slot seq[i]: the lowest free page for each block that gets
+ * full, in order; refused whole ("decode buffer exhausted") when a slot's max_tokens or the free pages do
+ * not suffice.  It writes the step's description to `desc` (host, kvq_pages_step_words words) and, by
+ * value with launches on `stream`, to desc_device (NULL: host only).  split_cap >= n bounds the decode's split items.
+ * kvq_pages_whole describes whole sequences (for kvq_pages_rows; no page list).
+ * kvq_pages_append writes one layer's rows k, v (rows, H, D) of the step; running it again writes the same.
+ * kvq_pages_rows reads sequences back as dense rows (sum lens, H, D).  items: the description's second word.
+ * kvq_pages_fork makes empty slots dst share src's pages and copies the open blocks of all layers (ko,
+ * vo of layer 0, layers contiguous; table_device NULL: accounts only).  kvq_pages_free (host only) gives slots back.
+ * kvq_pages_move copies pages moves[i] = {from, to} (device) of all layers between pools (the same pool: no
+ * page both read and written) and maps the table's page numbers through place (device, `pages` entries).
+ * ---------------------------------------------------------------------------------------- */
+int64_t kvq_pages_step_words(int64_t page, const int64_t* counts, int64_t n);
+int kvq_pages_extend(int64_t* lens, int32_t* table, int32_t* refs, uint8_t* open, int64_t* account, int64_t slots,
+                     int64_t pages, int64_t max_blocks, int64_t page, int64_t max_tokens, const int64_t* seq,
+                     const int64_t* counts, int64_t n, int64_t split_cap, int32_t* desc, int64_t desc_words,
+                     int32_t* desc_device, void* stream);
+int kvq_pages_whole(const int64_t* lens, const uint8_t* open, int64_t slots, int64_t page, const int64_t* seq, int64_t n,
+                    int32_t* desc, int64_t desc_words, int32_t* desc_device, void* stream);
+int kvq_pages_append(const void* k, int64_t k_st, int64_t k_sh, const void* v, int64_t v_st, int64_t v_sh, int dtype,
+                     const int32_t* step, int64_t items, int32_t* table, int64_t max_blocks, int64_t H, int64_t D,
+                     int64_t page, int code, uint8_t* kc, uint8_t* vc, float* sc, void* ko, void* vo, void* stream);
+int kvq_pages_rows(const int32_t* step, int64_t items, const int32_t* table, int64_t max_blocks, int64_t H, int64_t D,
+                   int64_t page, int code, int dtype, const uint8_t* kc, const uint8_t* vc, const float* sc,
+                   const void* ko, const void* vo, void* k_out, void* v_out, void* stream);
+int kvq_pages_fork(int64_t* lens, int32_t* table, int32_t* refs, uint8_t* open, int64_t slots, int64_t max_blocks,
+                   int64_t page, const int64_t* src, const int64_t* dst, int64_t n, int64_t layers, int64_t H, int64_t D,
+                   int32_t* table_device, void* ko, void* vo, void* stream);
+int kvq_pages_free(int64_t* lens, const int32_t* table, int32_t* refs, uint8_t* open, int64_t* account, int64_t slots,
+                   int64_t max_blocks, int64_t page, const int64_t* seq, int64_t n);
+int kvq_pages_move(const uint8_t* kc, const uint8_t* vc, const float* sc, int64_t pages, uint8_t* kc_to, uint8_t* vc_to,
+                   float* sc_to, int64_t pages_to, int64_t layers, int64_t H, int64_t D, int64_t page,
+                   const int32_t* moves, int64_t n, const int32_t* place, int32_t* table, int64_t entries, void* stream);
+
+/* ------------------------------------------------------------------------------------------
+ * Attention of a step's query rows over the paged cache: q (rows, Hq, D), the step's rows in order; query
+ * i of a sequence with `count` new tokens sees all tokens up to its own.  split_items >= the description's
+ * third word and max_count >= every count give the grid.  out (rows, Hq, D) contiguous.  workspace:
+ * kvq_paged_decode_workspace floats, no clearing; calls that share one must not overlap in time.
+ * ---------------------------------------------------------------------------------------- */
+int64_t kvq_paged_decode_workspace(int64_t split_items, int64_t H, int64_t rep, int64_t max_count, int64_t D);
+int kvq_paged_decode(const void* q, int64_t q_st, int64_t q_sh, int dtype, int64_t rows, int64_t Hq, int64_t H, int64_t D,
+                     float scaling, const int32_t* step, int64_t split_items, int64_t max_count, const int32_t* table,
+                     int64_t max_blocks, int64_t page, int code, const uint8_t* kc, const uint8_t* vc, const float* sc,
+                     const void* ko, const void* vo, void* out, float* workspace, int64_t workspace_floats, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

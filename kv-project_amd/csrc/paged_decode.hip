@@ -1,0 +1,437 @@
+// Attention of a few query tokens per sequence over the paged 8-bit cache (layouts: pages.hpp).
+//
+// Rows of a KV head: (query token, query head) pairs, 16 to a workgroup, the columns of the matrix
+// products.  A unit is 64 tokens; a wavefront computes its scores S = K q (rows tokens, columns query
+// rows), the running maximum and sum of the softmax in base 2, and O += V^T P, all in registers:
+//   S tile s of a unit takes token 16 (m >> 2) + 4 s + (m & 3) as its row m, so lane group g = lane / 16 ends
+//   up with the scores of tokens 16 g .. 16 g + 15, which is the K-index order that V^T (channel major in the
+//   page) is read in with 16 bytes a lane.  No value crosses lanes but the maximum.
+// The key scale multiplies the scores, the value scale the probabilities; the codes themselves turn to
+// 16-bit numbers exactly.  Probabilities times scale keep 16 bits as a pair of bfloat16 (the range of a
+// scale is float32's), so they round at 2^-17.
+//
+// Workgroups take the units of one split item, their wavefronts in turn, and join in LDS; a sequence
+// of several items is joined by merge_kernel in the items' order.
+#include <type_traits>
+
+#include "mfma_common.hpp"
+#include "pages.hpp"
+
+namespace kvq {
+namespace {
+
+constexpr int kThreads = 256, kWaves = 4, kRows = 16;
+
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+typedef float f32x2 __attribute__((ext_vector_type(2)));
+
+template <bool BF16>
+__device__ __forceinline__ f32x4 mfma16(u32x4 a, u32x4 b, f32x4 c) {
+  if constexpr (BF16) return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+  else return __builtin_amdgcn_mfma_f32_16x16x32_f16(as_half8(a), as_half8(b), c, 0, 0, 0);
+}
+
+__device__ __forceinline__ uint32_t pack_bf16(float a, float b) {
+  const f32x2 v = {a, b};
+  return __builtin_bit_cast(uint32_t, __builtin_convertvector(v, bf16x2));
+}
+
+// Two codes as two numbers of the 16-bit type: exact.  `hi` selects the upper pair of the word.
+template <int CODE, bool BF16>
+__device__ __forceinline__ void widen4(uint32_t w, uint32_t& a, uint32_t& b) {
+  if constexpr (CODE == kCodeE4M3) {
+    if constexpr (BF16) {
+      a = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, 1.0f, false));
+      b = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, 1.0f, true));
+    } else {
+      a = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, 1.0f, false));
+      b = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, 1.0f, true));
+    }
+  } else if constexpr (BF16) {
+    const int s = static_cast<int>(w);
+    a = pack_bf16(static_cast<float>(static_cast<int8_t>(s)), static_cast<float>(static_cast<int8_t>(s >> 8)));
+    b = pack_bf16(static_cast<float>(static_cast<int8_t>(s >> 16)), static_cast<float>(static_cast<int8_t>(s >> 24)));
+  } else {
+    // 0x6400 | u is the half 1024 + u; u = code + 128
+    const uint32_t u = w ^ 0x80808080u;
+    const half2v z = {static_cast<_Float16>(1152.0f), static_cast<_Float16>(1152.0f)};
+    a = w2(h2(__builtin_amdgcn_perm(0x64646464u, u, 0x07010700u)) - z);
+    b = w2(h2(__builtin_amdgcn_perm(0x64646464u, u, 0x07030702u)) - z);
+  }
+}
+
+template <int CODE, bool BF16>
+__device__ __forceinline__ u32x4 widen8(uint32_t x, uint32_t y) {
+  uint32_t r[4];
+  widen4<CODE, BF16>(x, r[0], r[1]);
+  widen4<CODE, BF16>(y, r[2], r[3]);
+  return u32x4{r[0], r[1], r[2], r[3]};
+}
+
+struct DecodeArgs {
+  const uint16_t* q;
+  int64_t q_st, q_sh;
+  const int* step;
+  const int* table;
+  int64_t max_blocks;
+  int H, rep, shift;                          // KV heads, query heads per KV head, log2 of the page
+  int pieces;                                 // of 16 rows
+  float scale;                                // scaling * log2(e)
+  const uint8_t *kc, *vc;
+  const float* sc;
+  const uint16_t *ko, *vo;
+  uint16_t* out;                              // (rows, Hq, D)
+  float* part;                                // (items, H, pieces): 16 x D sums, then 16 x {max, sum}
+};
+
+template <int D, bool BF16>
+struct Wave {                                 // one wavefront's running softmax: column lane % 16
+  f32x4 o[D / 16];                            // channels 16 c + 4 g + i
+  float m, l;                                 // base-2 maximum (of all groups), this lane's part of the sum
+};
+
+// Scores t (16 tokens of this lane, masked ones -inf) -> probabilities in t, o and l brought to the new maximum
+template <int D, bool BF16>
+__device__ __forceinline__ void soft(Wave<D, BF16>& w, float (&t)[16]) {
+  float m = t[0];
+#pragma unroll
+  for (int i = 1; i < 16; ++i) m = fmaxf(m, t[i]);
+  m = fmaxf(w.m, xmax32(xmax16(m)));
+  const float safe = m == -INFINITY ? 0.0f : m;
+  const float a = __builtin_amdgcn_exp2f(w.m - safe);
+  float sum = 0.0f;
+#pragma unroll
+  for (int i = 0; i < 16; ++i) {
+    t[i] = __builtin_amdgcn_exp2f(t[i] - safe);
+    sum += t[i];
+  }
+  w.l = w.l * a + sum;
+  if (__builtin_amdgcn_ballot_w64(a != 1.0f)) {
+#pragma unroll
+    for (int c = 0; c < D / 16; ++c) w.o[c] *= a;
+  }
+  w.m = m;
+}
+
+__device__ __forceinline__ void split_bf16(const float (&p)[16], int at, u32x4& hi, u32x4& lo) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float a = p[at + 2 * i], b = p[at + 2 * i + 1];
+    const uint32_t h = pack_bf16(a, b);
+    hi[i] = h;
+    lo[i] = pack_bf16(a - __uint_as_float(h << 16), b - __uint_as_float(h & 0xffff0000u));
+  }
+}
+__device__ __forceinline__ void split_f16(const float (&p)[16], int at, u32x4& hi, u32x4& lo) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const _Float16 a = static_cast<_Float16>(p[at + 2 * i]), b = static_cast<_Float16>(p[at + 2 * i + 1]);
+    hi[i] = pack_h2(a, b);
+    lo[i] = pack_h2(static_cast<_Float16>(p[at + 2 * i] - static_cast<float>(a)), static_cast<_Float16>(p[at + 2 * i + 1] - static_cast<float>(b)));
+  }
+}
+
+template <int D, int CODE, bool BF16>
+__global__ __launch_bounds__(kThreads, 2) void paged_split_kernel(DecodeArgs a) {
+  constexpr int kJ = D / 64, kC = D / 16;
+  __shared__ float join[kWaves][kRows][D + 4];
+  __shared__ float stat[kWaves][kRows][2];
+  const int* step = a.step;
+  const int n = step[0], per = step[3];
+  // pieces of one item and head on one of the 8 dies, next to each other: they read the same pages
+  const int group = blockIdx.x / (8 * a.pieces), within = blockIdx.x % (8 * a.pieces);
+  const int64_t ih = static_cast<int64_t>(group) * 8 + within % 8;
+  const int piece = within / 8, item = static_cast<int>(ih / a.H), h = static_cast<int>(ih % a.H);
+  if (item >= step[2]) return;
+  const int b = step_find(step, n, 5, item);
+  const StepSeq s = step_seq(step, b);
+  const int rows = a.rep * s.count;
+  if (piece * kRows >= rows) return;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, col = lane & 15, g = lane >> 4;
+  const int P = 1 << a.shift, len = s.pos0 + s.count, full = len >> a.shift << a.shift;
+  const int u_full = (full + kUnit - 1) / kUnit, u_all = u_full + (len - full + kUnit - 1) / kUnit;
+  const int u0 = (item - s.split0) * per, u1 = u0 + per < u_all ? u0 + per : u_all;
+
+  // the query rows: column col of B, channels 64 j + 16 g + 8 e ..
+  const int row = piece * kRows + col, tok = row / a.rep, hq = row % a.rep;
+  const bool live = row < rows;
+  const int visible = live ? s.pos0 + tok + 1 : 0;
+  u32x4 q[2 * kJ];
+  {
+    const uint16_t* qp = a.q + (s.row0 + (live ? tok : 0)) * a.q_st + (static_cast<int64_t>(h) * a.rep + (live ? hq : 0)) * a.q_sh;
+#pragma unroll
+    for (int j = 0; j < kJ; ++j)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const uint4 x = *reinterpret_cast<const uint4*>(qp + 64 * j + 16 * g + 8 * e);
+        q[2 * j + e] = live ? u32x4{x.x, x.y, x.z, x.w} : u32x4{0, 0, 0, 0};
+      }
+  }
+
+  Wave<D, BF16> w;
+#pragma unroll
+  for (int c = 0; c < kC; ++c) w.o[c] = f32x4{0, 0, 0, 0};
+  w.m = -INFINITY;
+  w.l = 0.0f;
+
+  const int m_tok = 16 * (col >> 2) + (col & 3);                    // + 4 s: the token of S row `col` in tile s
+  const int* pages = a.table + s.slot * a.max_blocks;
+  const int last = full / P - 1;                                    // last full block
+  int u = u0 + wave;
+  for (; u < u1 && u < u_full; u += kWaves) {
+    const int t0 = u * kUnit;
+    int bk = (t0 + m_tok) >> a.shift, bv = (t0 + 16 * g) >> a.shift; // blocks of this lane's key rows and value tokens
+    bk = bk < last ? bk : last;                                     // half a unit may lie behind the last page: masked
+    bv = bv < last ? bv : last;
+    const int64_t pk = static_cast<int64_t>(pages[bk]) * a.H + h, pv = static_cast<int64_t>(pages[bv]) * a.H + h;
+    const uint8_t* kp = a.kc + pk * P * D + ((t0 + m_tok) & (P - 1)) * D + 16 * g;
+    const uint8_t* vp = a.vc + pv * P * D + static_cast<int64_t>(col) * P + ((t0 + 16 * g) & (P - 1));
+    const float2 z = reinterpret_cast<const float2*>(a.sc)[pv];
+    uint4 kw[4][kJ], vw[kC];
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int j = 0; j < kJ; ++j) kw[i][j] = *reinterpret_cast<const uint4*>(kp + 4 * i * D + 64 * j);
+#pragma unroll
+    for (int c = 0; c < kC; ++c) vw[c] = *reinterpret_cast<const uint4*>(vp + 16 * c * P);
+    float t[16];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      f32x4 acc = {0, 0, 0, 0};
+#pragma unroll
+      for (int j = 0; j < kJ; ++j) {
+        acc = mfma16<BF16>(widen8<CODE, BF16>(kw[i][j].x, kw[i][j].y), q[2 * j], acc);
+        acc = mfma16<BF16>(widen8<CODE, BF16>(kw[i][j].z, kw[i][j].w), q[2 * j + 1], acc);
+      }
+#pragma unroll
+      for (int e = 0; e < 4; ++e) t[4 * i + e] = acc[e] * (z.x * a.scale);
+    }
+    const int end = visible < full ? visible : full;
+    const bool masked = t0 + kUnit > full || t0 + kUnit > s.pos0 + 1;
+    if (masked) {
+#pragma unroll
+      for (int i = 0; i < 16; ++i) t[i] = t0 + 16 * g + i < end ? t[i] : -INFINITY;
+    }
+    soft(w, t);
+#pragma unroll
+    for (int i = 0; i < 16; ++i) t[i] *= z.y;
+    if (masked) {                                                   // a NaN scale of a block that no row sees
+#pragma unroll
+      for (int i = 0; i < 16; ++i) t[i] = t0 + 16 * g + i < end ? t[i] : 0.0f;
+    }
+    u32x4 hi[2], lo[2];
+    split_bf16(t, 0, hi[0], lo[0]);
+    split_bf16(t, 8, hi[1], lo[1]);
+#pragma unroll
+    for (int c = 0; c < kC; ++c) {
+      const u32x4 x = widen8<CODE, true>(vw[c].x, vw[c].y), y = widen8<CODE, true>(vw[c].z, vw[c].w);
+      w.o[c] = mfma16<true>(x, hi[0], w.o[c]);
+      w.o[c] = mfma16<true>(y, hi[1], w.o[c]);
+      w.o[c] = mfma16<true>(x, lo[0], w.o[c]);
+      w.o[c] = mfma16<true>(y, lo[1], w.o[c]);
+    }
+  }
+
+  // units of the open block
+  const int64_t open = ((static_cast<int64_t>(s.slot) * 2 + (s.bufs >> 1 & 1)) * a.H + h) * P * D;
+  for (; u < u1; u += kWaves) {
+    const int off = (u - u_full) * kUnit, t0 = full + off;
+    const uint16_t* kp = a.ko + open;
+    const uint16_t* vp = a.vo + open + static_cast<int64_t>(col) * P + (off + 16 * g < P ? off + 16 * g : 0);
+    float t[16];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int r = off + m_tok + 4 * i < P ? off + m_tok + 4 * i : P - 1;
+      f32x4 acc = {0, 0, 0, 0};
+#pragma unroll
+      for (int j = 0; j < kJ; ++j)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const uint4 x = *reinterpret_cast<const uint4*>(kp + r * D + 64 * j + 16 * g + 8 * e);
+          acc = mfma16<BF16>(u32x4{x.x, x.y, x.z, x.w}, q[2 * j + e], acc);
+        }
+#pragma unroll
+      for (int e = 0; e < 4; ++e) t[4 * i + e] = t0 + 16 * g + 4 * i + e < visible ? acc[e] * a.scale : -INFINITY;
+    }
+    soft(w, t);
+    u32x4 hi[2], lo[2];
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      if constexpr (BF16) split_bf16(t, 8 * e, hi[e], lo[e]);
+      else split_f16(t, 8 * e, hi[e], lo[e]);
+    }
+    // what lies behind the sequence or is hidden from a row may be an infinity or a NaN: it goes in as zero, and
+    // the rows that do see such a value get it afterwards
+    constexpr uint32_t kInf = BF16 ? 0x7f80u : 0x7c00u;
+    bool bad = false;
+#pragma unroll
+    for (int c = 0; c < kC; ++c)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const uint4 x = *reinterpret_cast<const uint4*>(vp + 16 * c * P + 8 * e);
+        u32x4 v = {x.x, x.y, x.z, x.w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const bool b0 = (v[i] & kInf) == kInf, b1 = (v[i] >> 16 & kInf) == kInf;
+          bad |= b0 || b1;
+          v[i] = (b0 ? 0u : v[i] & 0xffffu) | (b1 ? 0u : v[i] & 0xffff0000u);
+        }
+        w.o[c] = mfma16<BF16>(v, hi[e], w.o[c]);
+        w.o[c] = mfma16<BF16>(v, lo[e], w.o[c]);
+      }
+    if (__builtin_amdgcn_ballot_w64(bad)) {
+      for (int i = 0; i < kUnit && t0 + i < len; ++i)
+#pragma unroll
+        for (int c = 0; c < kC; ++c)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const uint16_t x = a.vo[open + static_cast<int64_t>(16 * c + 4 * g + e) * P + off + i];
+            if ((x & kInf) == kInf && t0 + i < visible) w.o[c][e] += BF16 ? bf16_to_f32(x) : f16_to_f32(x);
+          }
+    }
+  }
+
+  w.l = xsum32(xsum16(w.l));
+#pragma unroll
+  for (int c = 0; c < kC; ++c) *reinterpret_cast<f32x4*>(&join[wave][col][16 * c + 4 * g]) = w.o[c];
+  if (g == 0) {
+    stat[wave][col][0] = w.m;
+    stat[wave][col][1] = w.l;
+  }
+  __syncthreads();
+  const int next = step[kStepHead + kStepSeq * (b + 1) + 5];
+  const bool single = next - s.split0 == 1;
+  constexpr int kPer = kRows * D / kThreads;                        // channels of a row per thread
+  const int r = threadIdx.x / (D / kPer), c0 = threadIdx.x % (D / kPer) * kPer;
+  float top = stat[0][r][0];
+#pragma unroll
+  for (int i = 1; i < kWaves; ++i) top = fmaxf(top, stat[i][r][0]);
+  const float safe = top == -INFINITY ? 0.0f : top;
+  float l = 0.0f, o[kPer] = {};
+#pragma unroll
+  for (int i = 0; i < kWaves; ++i) {
+    const float f = __builtin_amdgcn_exp2f(stat[i][r][0] - safe);
+    l += f * stat[i][r][1];
+#pragma unroll
+    for (int e = 0; e < kPer; ++e) o[e] += f * join[i][r][c0 + e];
+  }
+  const int R = piece * kRows + r;
+  if (R >= rows) return;
+  if (single) {
+    const float inv = 1.0f / l;
+    uint16_t* out = a.out + ((static_cast<int64_t>(s.row0) + R / a.rep) * a.H * a.rep + h * a.rep + R % a.rep) * D + c0;
+    uint32_t p[kPer / 2];
+#pragma unroll
+    for (int e = 0; e < kPer / 2; ++e)
+      p[e] = BF16 ? pack_bf16(o[2 * e] * inv, o[2 * e + 1] * inv)
+                  : pack_h2(static_cast<_Float16>(o[2 * e] * inv), static_cast<_Float16>(o[2 * e + 1] * inv));
+#pragma unroll
+    for (int e = 0; e < kPer / 4; ++e) *reinterpret_cast<uint2*>(out + 4 * e) = make_uint2(p[2 * e], p[2 * e + 1]);
+    return;
+  }
+  float* part = a.part + (ih * a.pieces + piece) * (kRows * (D + 2));
+#pragma unroll
+  for (int e = 0; e < kPer / 4; ++e)
+    *reinterpret_cast<float4*>(part + r * D + c0 + 4 * e) = make_float4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
+  if (c0 == 0) {
+    part[kRows * D + 2 * r] = top;
+    part[kRows * D + 2 * r + 1] = l;
+  }
+}
+
+// One wavefront per (packed row, query head): the items of its sequence, 64 maxima at a time.
+template <int D, bool BF16>
+__global__ __launch_bounds__(kThreads) void paged_merge_kernel(DecodeArgs a, int64_t total) {
+  const int64_t at = static_cast<int64_t>(blockIdx.x) * kWaves + (threadIdx.x >> 6);
+  if (at >= total) return;
+  const int Hq = a.H * a.rep, lane = threadIdx.x & 63;
+  const int n = static_cast<int>(at / Hq), head = static_cast<int>(at % Hq), h = head / a.rep;
+  const int b = step_find(a.step, a.step[0], 3, n);
+  const StepSeq s = step_seq(a.step, b);
+  const int items = a.step[kStepHead + kStepSeq * (b + 1) + 5] - s.split0;
+  if (n >= s.row0 + s.count || items < 2) return;
+  const int R = (n - s.row0) * a.rep + head % a.rep, piece = R / kRows, r = R % kRows;
+  constexpr int64_t kPart = kRows * (D + 2);
+  const int64_t stride = static_cast<int64_t>(a.H) * a.pieces * kPart;
+  const float* part = a.part + (static_cast<int64_t>(s.split0) * a.H + h) * a.pieces * kPart + piece * kPart;
+  float top = -INFINITY, l = 0.0f, o[D / 64] = {};
+  for (int i0 = 0; i0 < items; i0 += 64) {
+    const int i = i0 + lane;
+    const float2 st = i < items ? *reinterpret_cast<const float2*>(part + i * stride + kRows * D + 2 * r) : make_float2(-INFINITY, 0.0f);
+    const float m = fmaxf(top, wave_max(st.x)), safe = m == -INFINITY ? 0.0f : m;
+    const float old = __builtin_amdgcn_exp2f(top - safe), f = __builtin_amdgcn_exp2f(st.x - safe);
+    l = l * old + wave_sum(f * st.y);
+#pragma unroll
+    for (int e = 0; e < D / 64; ++e) o[e] *= old;
+    const int most = items - i0 < 64 ? items - i0 : 64;
+    for (int k = 0; k < most; ++k) {
+      const float fk = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(f), k));
+      const float* p = part + (i0 + k) * stride + r * D + lane * (D / 64);
+#pragma unroll
+      for (int e = 0; e < D / 64; ++e) o[e] += fk * p[e];
+    }
+    top = m;
+  }
+  const float inv = 1.0f / l;
+  uint16_t* out = a.out + at * D + lane * (D / 64);
+#pragma unroll
+  for (int e = 0; e < D / 64; ++e) out[e] = BF16 ? f32_to_bf16(o[e] * inv) : f32_to_f16(o[e] * inv);
+}
+
+int64_t pieces_of(int64_t rep, int64_t most) { return (rep * most + kRows - 1) / kRows; }
+
+}  // namespace
+}  // namespace kvq
+
+using namespace kvq;
+
+extern "C" int64_t kvq_paged_decode_workspace(int64_t split_items, int64_t H, int64_t rep, int64_t max_count, int64_t D) {
+  if (split_items < 1 || H < 1 || rep < 1 || max_count < 1 || (D != 64 && D != 128)) return -1;
+  return split_items * H * pieces_of(rep, max_count) * kRows * (D + 2);
+}
+
+extern "C" int kvq_paged_decode(const void* q, int64_t q_st, int64_t q_sh, int dtype, int64_t rows, int64_t Hq, int64_t H, int64_t D,
+                                float scaling, const int32_t* step, int64_t split_items, int64_t max_count, const int32_t* table,
+                                int64_t max_blocks, int64_t P, int code, const uint8_t* kc, const uint8_t* vc, const float* sc,
+                                const void* ko, const void* vo, void* out, float* workspace, int64_t workspace_floats, void* stream) {
+  KVQ_REQUIRE(D == 64 || D == 128, "kvq_paged_decode: head_dim must be 64 or 128 (got %lld)", static_cast<long long>(D));
+  KVQ_REQUIRE(P == 32 || P == 64 || P == 128, "kvq_paged_decode: pages hold 32, 64 or 128 tokens");
+  KVQ_REQUIRE(dtype == KVQ_F16 || dtype == KVQ_BF16, "kvq_paged_decode: queries must be fp16 or bf16");
+  KVQ_REQUIRE(code == kCodeInt8 || code == kCodeE4M3, "kvq_paged_decode: unknown code %d", code);
+  KVQ_REQUIRE(H > 0 && Hq > 0 && Hq % H == 0 && rows > 0 && max_count > 0 && split_items > 0, "kvq_paged_decode: bad sizes");
+  KVQ_REQUIRE(q && step && table && kc && vc && sc && ko && vo && out && workspace, "kvq_paged_decode: null pointer");
+  KVQ_REQUIRE(reinterpret_cast<uintptr_t>(q) % 16 == 0 && (q_st | q_sh) % 8 == 0 && reinterpret_cast<uintptr_t>(out) % 16 == 0 &&
+                  reinterpret_cast<uintptr_t>(workspace) % 16 == 0,
+              "kvq_paged_decode: rows and strides must be multiples of 16 bytes");
+  const int64_t rep = Hq / H, need = kvq_paged_decode_workspace(split_items, H, rep, max_count, D);
+  KVQ_REQUIRE(workspace_floats >= need, "kvq_paged_decode: workspace of %lld floats, %lld needed", static_cast<long long>(workspace_floats),
+              static_cast<long long>(need));
+  DecodeArgs a{static_cast<const uint16_t*>(q), q_st, q_sh, step, table, max_blocks, static_cast<int>(H), static_cast<int>(rep),
+               P == 32 ? 5 : P == 64 ? 6 : 7, static_cast<int>(pieces_of(rep, max_count)), scaling * 1.44269504088896341f, kc, vc, sc,
+               static_cast<const uint16_t*>(ko), static_cast<const uint16_t*>(vo), static_cast<uint16_t*>(out), workspace};
+  const int64_t blocks = (split_items * H + 7) / 8 * 8 * a.pieces, merges = (rows * Hq + kWaves - 1) / kWaves;
+  KVQ_REQUIRE(blocks < INT64_C(1) << 31 && merges < INT64_C(1) << 31, "kvq_paged_decode: too many rows");
+  auto run = [&](auto d, auto c, auto t) {
+    constexpr int D_ = decltype(d)::value, C_ = decltype(c)::value;
+    constexpr bool T_ = decltype(t)::value != 0;
+    hipLaunchKernelGGL((paged_split_kernel<D_, C_, T_>), dim3(static_cast<uint32_t>(blocks)), dim3(kThreads), 0,
+                       static_cast<hipStream_t>(stream), a);
+    hipLaunchKernelGGL((paged_merge_kernel<D_, T_>), dim3(static_cast<uint32_t>(merges)), dim3(kThreads), 0,
+                       static_cast<hipStream_t>(stream), a, rows * Hq);
+  };
+  using Zero = std::integral_constant<int, 0>;
+  using One = std::integral_constant<int, 1>;
+  auto by_type = [&](auto d, auto c) {
+    if (dtype == KVQ_BF16) run(d, c, One{});
+    else run(d, c, Zero{});
+  };
+  auto by_code = [&](auto d) {
+    if (code == kCodeInt8) by_type(d, Zero{});
+    else by_type(d, One{});
+  };
+  if (D == 64) by_code(std::integral_constant<int, 64>{});
+  else by_code(std::integral_constant<int, 128>{});
+  KVQ_LAUNCH_CHECK("kvq_paged_decode");
+  return KVQ_OK;
+}

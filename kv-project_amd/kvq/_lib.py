@@ -103,6 +103,19 @@ SIGNATURES = {
     "kvq_quasar_decode": (i32, [vp, i32, i64, i64, i64, i64, i64, i64, f32, vp, vp, i64, i64, vp, vp,
                                 vp, i64, vp, i64, vp, i32, i32, vp, i32, vp, vp, i64, vp, vp, i64, i64, vp, vp,
                                 vp, i32, vp, vp, i64, i32, vp]),
+    "kvq_prompt_plan": (i64, [vp, vp, i64, i64, i32, vp, i64]),
+    "kvq_prompt_attention": (i32, [vp, i64, i64, vp, i64, i64, vp, i64, i64, i32, i64, i64, i64, f32, vp, i64, vp, vp]),
+    "kvq_pages_step_words": (i64, [i64, vp, i64]),
+    "kvq_pages_extend": (i32, [vp, vp, vp, vp, vp, i64, i64, i64, i64, i64, vp, vp, i64, i64, vp, i64, vp, vp]),
+    "kvq_pages_whole": (i32, [vp, vp, i64, i64, vp, i64, vp, i64, vp, vp]),
+    "kvq_pages_append": (i32, [vp, i64, i64, vp, i64, i64, i32, vp, i64, vp, i64, i64, i64, i64, i32, vp, vp, vp, vp, vp, vp]),
+    "kvq_pages_rows": (i32, [vp, i64, vp, i64, i64, i64, i64, i32, i32, vp, vp, vp, vp, vp, vp, vp, vp]),
+    "kvq_pages_fork": (i32, [vp, vp, vp, vp, i64, i64, i64, vp, vp, i64, i64, i64, i64, vp, vp, vp, vp]),
+    "kvq_pages_free": (i32, [vp, vp, vp, vp, vp, i64, i64, i64, vp, i64]),
+    "kvq_pages_move": (i32, [vp, vp, vp, i64, vp, vp, vp, i64, i64, i64, i64, i64, vp, i64, vp, vp, i64, vp]),
+    "kvq_paged_decode_workspace": (i64, [i64, i64, i64, i64, i64]),
+    "kvq_paged_decode": (i32, [vp, i64, i64, i32, i64, i64, i64, i64, f32, vp, i64, i64, vp, i64, i64, i32, vp, vp, vp, vp, vp,
+                               vp, vp, i64, vp]),
 }
 
 
@@ -144,6 +157,14 @@ def call(name: str, *args) -> int:
         msg = load().kvq_last_error().decode(errors="replace")
         raise KVQError(f"{name} failed ({rc}): {msg}")
     return rc
+
+
+def call_on(device: torch.device, name: str, *args) -> int:
+    """``call`` with ``device`` as the current one: a launch on a default stream goes to the current device."""
+    if device.index == torch.cuda.current_device():
+        return call(name, *args)
+    with torch.cuda.device(device):
+        return call(name, *args)
 
 
 def ptr(t: torch.Tensor | None) -> int | None:

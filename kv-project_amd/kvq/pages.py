@@ -1,0 +1,294 @@
+"""A KV cache in pages of 8-bit codes, shared by sequences of any lengths, for all layers of a model.
+
+``PagedCache`` holds, per layer, a pool of pages: ``page`` tokens of every KV head as int8 or e4m3 codes with
+one float32 scale for the keys and one for the values of each head.  A sequence is a slot: a row of the
+page table and the block that is still open, in the model's type.  A block is coded when its last token
+comes, so what the cache holds does not depend on how the tokens arrived.  Full pages are never written
+again; forked sequences share them by count.
+
+A step: ``step = cache.extend(slots, counts)`` claims room for new tokens of some sequences, once for all
+layers; ``cache.append(layer, k, v, step)`` and ``paged_decode(q, scaling, cache, layer, step)`` run per layer.
+The page accounts live in host memory (libkvq's kvq_pages_* calls); the kernels read the table and the
+step's description on the device.  The reference's caches are dense in the batch (STRATA_KV.py:682-719):
+this one has no counterpart there.
+"""
+from __future__ import annotations
+
+from typing import List, Optional, Sequence, Tuple
+
+import numpy as np
+import torch
+
+from . import _lib
+from .prompt import device_of, rows16
+
+CODES = {"int8": 0, "e4m3": 1}
+PAGES = (32, 64, 128)
+SPLIT_BLOCKS = 768                             # workgroups a decode is split into at most: three on each of 256 CUs
+
+
+def _ints(x, what: str) -> np.ndarray:
+    a = np.array(x, dtype=np.int64).reshape(-1)
+    if a.size == 0:
+        raise ValueError(f"{what} must not be empty")
+    return a
+
+
+class Step:
+    """New tokens of some slots: ``rows`` packed rows, slot by slot.  Made by ``PagedCache.extend``."""
+
+    __slots__ = ("slots", "counts", "ends", "rows", "items", "splits", "max_count", "desc", "host", "generation")
+
+
+class PagedCache:
+    """``layers`` layers of ``pages`` pages for ``slots`` sequences of at most ``max_tokens`` tokens: ``Hkv`` KV heads of
+    head_dim ``d`` (64 or 128), blocks of ``page`` tokens (32, 64 or 128) held as ``code`` ("int8" or "e4m3"), rows of
+    ``dtype`` (bf16 or fp16)."""
+
+    def __init__(self, layers: int, slots: int, pages: int, max_tokens: int, Hkv: int, d: int, *, page: int = 64,
+                 code: str = "int8", dtype: torch.dtype = torch.bfloat16, device="cuda"):
+        if min(layers, slots, pages, max_tokens, Hkv) < 1:
+            raise ValueError("a cache needs at least one layer, slot, page, token and KV head")
+        if d not in (64, 128):
+            raise _lib.KVQError(f"PagedCache: head_dim must be 64 or 128 (got {d})")
+        if page not in PAGES:
+            raise ValueError(f"page must be one of {PAGES}")
+        if code not in CODES:
+            raise ValueError(f"code must be one of {tuple(CODES)}")
+        if dtype not in (torch.bfloat16, torch.float16):
+            raise TypeError("PagedCache holds bf16 or fp16 rows")
+        if max(pages, max_tokens, slots) >= 1 << 31 or layers * Hkv >= 65536:
+            raise ValueError("too many pages, tokens, slots or heads")
+        self.device = device_of(device)
+        self.layers, self.slots, self.pages, self.max_tokens = int(layers), int(slots), int(pages), int(max_tokens)
+        self.Hkv, self.d, self.page, self.code, self.dtype = int(Hkv), int(d), int(page), code, dtype
+        self.max_blocks = -(-self.max_tokens // self.page)
+        self._lens = np.zeros(self.slots, dtype=np.int64)
+        self._table = np.zeros((self.slots, self.max_blocks), dtype=np.int32)
+        self._open = np.zeros(self.slots, dtype=np.uint8)
+        self._set_refs(np.zeros(self.pages, dtype=np.int32))
+        self._generation = 0
+        self.table = torch.zeros((self.slots, self.max_blocks), dtype=torch.int32, device=self.device)
+        self.kc, self.vc, self.sc = self._pool(self.pages)
+        rows = (self.layers, self.slots, 2, self.Hkv, self.page * self.d)
+        self.k_open = torch.zeros(rows, dtype=dtype, device=self.device)     # token major, as a page's keys
+        self.v_open = torch.zeros(rows, dtype=dtype, device=self.device)     # channel major, as a page's values
+
+    def _pool(self, pages: int):
+        new = lambda *s, dt=torch.int8: torch.empty((self.layers, pages, self.Hkv, *s), dtype=dt, device=self.device)
+        return new(self.page, self.d), new(self.d, self.page), new(2, dt=torch.float32)
+
+    def _set_refs(self, refs: np.ndarray) -> None:
+        free = np.flatnonzero(refs == 0)
+        self._refs = refs
+        self._account = np.array([free.size, free[0] if free.size else refs.size], dtype=np.int64)
+        self._host = tuple(x.ctypes.data for x in (self._lens, self._table, self._refs, self._open, self._account))
+
+    # ---- what is held ------------------------------------------------------------------------
+
+    @property
+    def lengths(self) -> List[int]:
+        """Tokens of each slot."""
+        return self._lens.tolist()
+
+    @property
+    def free_pages(self) -> int:
+        return int(self._account[0])
+
+    def codes(self) -> Tuple[torch.Tensor, torch.Tensor]:
+        """The pools' key and value codes, (layers, pages, Hkv, page, d) views (the values' tokens vary fastest)."""
+        dt = torch.int8 if self.code == "int8" else torch.float8_e4m3fn
+        return self.kc.view(dt), self.vc.view(dt).transpose(-1, -2)
+
+    def scales(self) -> Tuple[torch.Tensor, torch.Tensor]:
+        """The pools' key and value scales, (layers, pages, Hkv) float32 views."""
+        return self.sc[..., 0], self.sc[..., 1]
+
+    def bytes_per_token(self) -> float:
+        """Bytes a full block holds per token, all layers."""
+        return self.layers * self.Hkv * (2.0 * self.d + 8.0 / self.page)
+
+    # ---- steps -------------------------------------------------------------------------------
+
+    def extend(self, slots: Sequence[int], counts: Sequence[int], *, into: Optional[Step] = None) -> Step:
+        """Claim room for counts[i] more tokens of slots[i] (each slot once): the lowest free page for each block that
+        gets full.  Raises KVQError ("decode buffer exhausted") and changes nothing when a slot or the pool is
+        full.  ``into``: a step of the same counts whose description is rewritten in place, so that a
+        captured graph of its append and decode runs the new step when it is replayed."""
+        s, c = _ints(slots, "slots"), _ints(counts, "counts")
+        if s.shape != c.shape:
+            raise ValueError("slots and counts must have the same length")
+        n = s.size
+        lib = _lib.load()
+        if into is None:
+            words = lib.kvq_pages_step_words(self.page, c.ctypes.data, n)
+            if words < 0:
+                raise ValueError("counts must be positive and below 2^31")
+            st = Step()
+            st.host = np.empty(words, dtype=np.int32)
+            st.desc = torch.empty(words, dtype=torch.int32, device=self.device)
+            st.splits = max(n, -(-SPLIT_BLOCKS // self.Hkv))
+        else:
+            st = into
+            if not np.array_equal(st.counts, c):
+                raise ValueError("a step is rewritten for the same counts only")
+        _lib.call_on(self.device, "kvq_pages_extend", *self._host, self.slots, self.pages, self.max_blocks, self.page,
+                     self.max_tokens, s.ctypes.data, c.ctypes.data, n, st.splits, st.host.ctypes.data, st.host.size,
+                     st.desc.data_ptr(), _lib.stream_of(st.desc))
+        if into is None:
+            st.splits = int(st.host[2])        # what later steps written into this one keep to
+            st.items = st.host.size - 8 * (n + 2)
+            st.rows, st.max_count = int(c.sum()), int(c.max())
+        st.slots, st.counts, st.ends, st.generation = s, c, self._lens[s], self._generation
+        return st
+
+    def check_step(self, step: Step, what: str) -> None:
+        """A step describes its slots only until they take more tokens or are freed."""
+        if not (self._lens[step.slots] == step.ends).all():
+            raise ValueError(f"{what}: the step's slots have changed since it was made")
+
+    @torch.no_grad()
+    def append(self, layer: int, k: torch.Tensor, v: torch.Tensor, step: Step) -> None:
+        """The step's new rows k, v (rows, Hkv, d) of one layer, slot by slot: full blocks to codes, the rest to the open
+        blocks.  Running it again writes the same."""
+        _lib.require_gpu(k, v)
+        self._layer(layer)
+        shape = (step.rows, self.Hkv, self.d)
+        if k.shape != shape or v.shape != shape:
+            raise ValueError(f"append: k {tuple(k.shape)} and v {tuple(v.shape)} must be {shape}")
+        if k.dtype != self.dtype or v.dtype != self.dtype:
+            raise TypeError("appended rows must have the cache's dtype")
+        if k.device != self.device or v.device != self.device:
+            raise ValueError(f"append: the cache is on {self.device}")
+        self.check_step(step, "append")
+        if step.generation != self._generation:
+            raise ValueError("append: the pages have moved since the step was made")
+        k, v = rows16(k), rows16(v)
+        _lib.call_on(self.device, "kvq_pages_append", k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(), v.stride(0), v.stride(1),
+                     _lib.DTYPE_CODE[self.dtype], step.desc.data_ptr(), step.items, self.table.data_ptr(), self.max_blocks,
+                     self.Hkv, self.d, self.page, CODES[self.code], *self._at(layer), _lib.stream_of(k))
+
+    def _layer(self, layer: int) -> None:
+        if not 0 <= layer < self.layers:
+            raise IndexError(f"no layer {layer} (of {self.layers})")
+
+    def _at(self, layer: int):
+        """Addresses of a layer's codes, scales and open blocks."""
+        return tuple(x.data_ptr() + layer * x.stride(0) * x.element_size()
+                     for x in (self.kc, self.vc, self.sc, self.k_open, self.v_open))
+
+    @torch.no_grad()
+    def rows(self, layer: int, slots: Sequence[int]) -> Tuple[torch.Tensor, torch.Tensor]:
+        """All tokens of the slots, one behind the other, as dense rows k, v (tokens, Hkv, d): code times scale, rounded
+        once, and the open blocks as they are.  With prompt_attention this is the attention of many new tokens."""
+        self._layer(layer)
+        s = _ints(slots, "slots")
+        n = s.size
+        host = np.empty(8 * (n + 2), dtype=np.int32)
+        desc = torch.empty(host.size, dtype=torch.int32, device=self.device)
+        stream = _lib.stream_of(desc)
+        _lib.call_on(self.device, "kvq_pages_whole", self._host[0], self._host[3], self.slots, self.page, s.ctypes.data, n,
+                     host.ctypes.data, host.size, desc.data_ptr(), stream)
+        total = int(self._lens[s].sum())
+        k, v = (torch.empty((total, self.Hkv, self.d), dtype=self.dtype, device=self.device) for _ in (0, 1))
+        if total:
+            _lib.call_on(self.device, "kvq_pages_rows", desc.data_ptr(), int(host[1]), self.table.data_ptr(), self.max_blocks, self.Hkv,
+                         self.d, self.page, CODES[self.code], _lib.DTYPE_CODE[self.dtype], *self._at(layer), k.data_ptr(),
+                         v.data_ptr(), stream)
+        return k, v
+
+    # ---- sequences and pages -----------------------------------------------------------------
+
+    def fork(self, src: Sequence[int], dst: Sequence[int]) -> None:
+        """Empty slots dst[i] become continuations of src[i]: they share its pages and get copies of its open block, in all
+        layers.  Call it when every layer has appended its steps."""
+        s, t = _ints(src, "src"), _ints(dst, "dst")
+        if s.shape != t.shape:
+            raise ValueError("src and dst must have the same length")
+        _lib.call_on(self.device, "kvq_pages_fork", *self._host[:4], self.slots, self.max_blocks, self.page, s.ctypes.data, t.ctypes.data,
+                     s.size, self.layers, self.Hkv, self.d, self.table.data_ptr(), self.k_open.data_ptr(), self.v_open.data_ptr(),
+                     _lib.stream_of(self.table))
+
+    def free(self, slots: Sequence[int]) -> None:
+        """Empty the slots; pages that no other sequence shares become free."""
+        s = _ints(slots, "slots")
+        _lib.call("kvq_pages_free", *self._host, self.slots, self.max_blocks, self.page, s.ctypes.data, s.size)
+
+    def compact(self) -> int:
+        """Move the pages at the end of the pool to the free places below, in order, so that the pages in use are the
+        first ones; returns their number.  In place: only the moved pages are read and written."""
+        used = self.pages - self.free_pages
+        self._move(used, None)
+        return used
+
+    def resize(self, pages: int) -> None:
+        """Give the pool ``pages`` pages: those beyond the new end move to the lowest free places, in order, the others
+        keep theirs.  New pools are allocated beside the old ones; graphs that were captured hold the old ones."""
+        pages = int(pages)
+        if pages < max(1, self.pages - self.free_pages):
+            raise ValueError(f"{self.pages - self.free_pages} pages are in use")
+        if pages >= 1 << 31:
+            raise ValueError("too many pages")
+        pool = self._pool(pages)
+        self._move(pages, pool)
+        (self.kc, self.vc, self.sc), self.pages = pool, pages
+
+    def _move(self, end: int, pool) -> None:
+        live = np.flatnonzero(self._refs)
+        high = live[live >= end]
+        place = np.zeros(self.pages, dtype=np.int32)
+        place[live] = live
+        place[high] = np.flatnonzero(self._refs[:end] == 0)[:high.size]
+        if pool is None and not high.size:
+            return
+        moved = live if pool is not None else high
+        moves = np.stack([moved, place[moved]], 1).astype(np.int32).reshape(-1)
+        # pinned, so that the copy is ordered on the stream without a wait here
+        words = torch.from_numpy(np.concatenate([moves, place])).pin_memory().to(self.device, non_blocking=True)
+        to = (self.kc, self.vc, self.sc) if pool is None else pool
+        _lib.call_on(self.device, "kvq_pages_move", self.kc.data_ptr(), self.vc.data_ptr(), self.sc.data_ptr(), self.pages,
+                     to[0].data_ptr(), to[1].data_ptr(), to[2].data_ptr(), self.pages if pool is None else end, self.layers, self.Hkv,
+                     self.d, self.page, words.data_ptr(), moved.size, words.data_ptr() + 4 * moves.size, self.table.data_ptr(),
+                     self.table.numel(), _lib.stream_of(self.table))
+        refs = np.zeros(self.pages if pool is None else end, dtype=np.int32)
+        refs[place[live]] = self._refs[live]
+        self._table[:] = place[self._table]
+        self._set_refs(refs)
+        self._generation += 1
+
+
+def paged_workspace_floats(step: Step, Hq: int, Hkv: int, d: int) -> int:
+    n = _lib.load().kvq_paged_decode_workspace(step.splits, Hkv, Hq // Hkv, step.max_count, d)
+    if n < 0:
+        raise _lib.KVQError("kvq_paged_decode_workspace rejected the shape")
+    return n
+
+
+@torch.no_grad()
+def paged_decode(q: torch.Tensor, scaling: float, cache: PagedCache, layer: int, step: Step, *,
+                 out: Optional[torch.Tensor] = None, workspace: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Attention of the step's query rows q (rows, Hq, d), slot by slot, over the cache; returns (rows, Hq, d).  Query i of
+    a slot's new tokens sees every token up to its own.  Meant for a few tokens per slot (16 rows = query
+    heads of a KV head times tokens go over the keys together); for many, ``cache.rows`` and prompt_attention."""
+    _lib.require_gpu(q)
+    cache._layer(layer)
+    if q.dim() != 3 or q.shape[0] != step.rows or q.shape[2] != cache.d or q.shape[1] < 1 or q.shape[1] % cache.Hkv:
+        raise ValueError(f"paged_decode: q {tuple(q.shape)} does not match the step ({step.rows} rows) and the cache "
+                         f"({cache.Hkv} KV heads, head_dim {cache.d})")
+    if q.dtype != cache.dtype:
+        raise TypeError("q must have the cache's dtype")
+    if q.device != cache.device:
+        raise ValueError(f"paged_decode: the cache is on {cache.device}")
+    cache.check_step(step, "paged_decode")
+    q = rows16(q)
+    Hq = q.shape[1]
+    out = _lib.out_or_new(out, (step.rows, Hq, cache.d), q.dtype, q.device, "paged_decode")
+    if workspace is None:
+        workspace = torch.empty((paged_workspace_floats(step, Hq, cache.Hkv, cache.d),), dtype=torch.float32, device=q.device)
+    elif workspace.dtype != torch.float32 or not workspace.is_contiguous() or workspace.device != q.device:
+        raise ValueError("workspace must be contiguous float32 on the cache's device")
+    _lib.call_on(q.device, "kvq_paged_decode", q.data_ptr(), q.stride(0), q.stride(1), _lib.DTYPE_CODE[q.dtype], step.rows, Hq, cache.Hkv,
+                 cache.d, float(scaling), step.desc.data_ptr(), step.splits, step.max_count, cache.table.data_ptr(),
+                 cache.max_blocks, cache.page, CODES[cache.code], *cache._at(layer), out.data_ptr(), workspace.data_ptr(),
+                 workspace.numel(), _lib.stream_of(q))
+    return out

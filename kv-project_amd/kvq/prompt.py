@@ -1,0 +1,91 @@
+"""Attention over whole prompts: packed sequences of any lengths, grouped heads.
+
+The reference leaves a prompt's attention to SDPA over a dense batch (STRATA_KV.py:499-504); here the
+sequences of a batch lie behind one another, (rows, heads, head_dim), with no padding, and a chunk of a
+prompt may attend over what is there of it already.  ``PromptPlan`` is built once from the lengths (on the
+host) and serves every layer of the step.
+"""
+from __future__ import annotations
+
+from typing import Optional, Sequence
+
+import numpy as np
+import torch
+
+from . import _lib
+
+MAX_REP = 128                                  # query heads per KV head of a kernel tile
+_WORDS = 8
+
+
+def device_of(device) -> torch.device:
+    """``device`` with an index (the current one when it names none)."""
+    device = torch.device(device)
+    if device.type != "cuda":
+        raise _lib.KVQError("kvq kernels run on the GPU only; there is no CPU path")
+    return device if device.index is not None else torch.device("cuda", torch.cuda.current_device())
+
+
+class PromptPlan:
+    """The work of an attention over packed sequences of ``lens`` new tokens each, in front of the last of
+    ``lens_k`` keys (as many as the new tokens when not given).  Causal: query t of a sequence sees keys
+    0 .. t + len_k - len; one that sees none gets zeros.  For ``Hq`` query heads over ``Hkv`` KV heads."""
+
+    def __init__(self, lens: Sequence[int], Hq: int, Hkv: int, *, lens_k: Optional[Sequence[int]] = None,
+                 causal: bool = True, device="cuda"):
+        lq = np.ascontiguousarray(lens, dtype=np.int64).reshape(-1)
+        lk = lq if lens_k is None else np.ascontiguousarray(lens_k, dtype=np.int64).reshape(-1)
+        if lq.shape != lk.shape:
+            raise ValueError("lens and lens_k must name the same sequences")
+        if (lq < 0).any() or (lk < 0).any():
+            raise ValueError("lengths must not be negative")
+        if Hkv < 1 or Hq < 1 or Hq % Hkv or Hq // Hkv > MAX_REP:
+            raise ValueError(f"{Hq} query heads over {Hkv} KV heads: the quotient must be whole and at most {MAX_REP}")
+        if int(lq.sum()) >= 1 << 31 or int(lk.sum()) >= 1 << 31:
+            raise ValueError("too many rows")
+        self.Hq, self.Hkv, self.causal = int(Hq), int(Hkv), bool(causal)
+        self.rows, self.keys = int(lq.sum()), int(lk.sum())
+        self.device = device_of(device)
+        rep = self.Hq // self.Hkv
+        lib = _lib.load()
+        args = (lq.ctypes.data, lk.ctypes.data, len(lq), rep, int(self.causal))
+        n = lib.kvq_prompt_plan(*args, None, 0)
+        items = np.empty((max(n, 1), _WORDS), dtype=np.int32)
+        if n < 0 or lib.kvq_prompt_plan(*args, items.ctypes.data, n) != n:
+            raise _lib.KVQError("kvq_prompt_plan rejected the lengths")
+        self.n_items = int(n)
+        self.items = torch.from_numpy(items).to(self.device)
+
+
+@torch.no_grad()
+def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, scaling: float, plan: PromptPlan, *,
+                     out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Attention of the packed rows q (rows, Hq, d) over k, v (keys, Hkv, d), bf16 or fp16 of one type, head_dim 64
+    or 128, any row and head strides of whole 16 bytes (others are copied); returns (rows, Hq, d)."""
+    _lib.require_gpu(q, k, v)
+    if q.dim() != 3 or k.dim() != 3 or v.shape != k.shape:
+        raise ValueError(f"prompt_attention takes q (rows, Hq, d) and k, v (keys, Hkv, d), got {tuple(q.shape)}, "
+                         f"{tuple(k.shape)}, {tuple(v.shape)}")
+    d = q.shape[2]
+    if q.shape[:2] != (plan.rows, plan.Hq) or k.shape != (plan.keys, plan.Hkv, d):
+        raise ValueError(f"prompt_attention: q {tuple(q.shape)} and k {tuple(k.shape)} do not match the plan "
+                         f"({plan.rows} rows of {plan.Hq} heads, {plan.keys} keys of {plan.Hkv})")
+    if q.dtype not in (torch.bfloat16, torch.float16) or k.dtype != q.dtype or v.dtype != q.dtype:
+        raise TypeError("prompt_attention takes bf16 or fp16 rows of one type")
+    if d not in (64, 128):
+        raise _lib.KVQError(f"prompt_attention: head_dim must be 64 or 128 (got {d})")
+    if q.device != plan.device or k.device != plan.device or v.device != plan.device:
+        raise ValueError(f"prompt_attention: the plan is for {plan.device}")
+    q, k, v = (rows16(x) for x in (q, k, v))
+    out = _lib.out_or_new(out, (plan.rows, plan.Hq, d), q.dtype, q.device, "prompt_attention")
+    _lib.call_on(q.device, "kvq_prompt_attention", q.data_ptr(), q.stride(0), q.stride(1), k.data_ptr(), k.stride(0), k.stride(1),
+                 v.data_ptr(), v.stride(0), v.stride(1), _lib.DTYPE_CODE[q.dtype], plan.Hq, plan.Hkv, d, float(scaling),
+                 plan.items.data_ptr(), plan.n_items, out.data_ptr(), _lib.stream_of(q))
+    return out
+
+
+def rows16(x: torch.Tensor) -> torch.Tensor:
+    """x (rows, heads, d) itself when the kernels can read it in 16-byte pieces, or a copy."""
+    if x.stride(2) != 1 or (x.stride(0) | x.stride(1)) % 8 or x.data_ptr() % 16:
+        return x.clone(memory_format=torch.contiguous_format)
+    return x

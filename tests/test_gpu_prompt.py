@@ -1,0 +1,165 @@
+"""Attention over packed prompts against the float64 oracle: lengths from none to many, chunks behind a past,
+rows without a key, grouped heads, strides, values that a row must not see, replays and other streams."""
+import pytest
+import torch
+
+from attention_bounds import HALF, check
+from oracle.paged import attend
+
+pytestmark = pytest.mark.gpu
+
+
+def _inputs(lens, lens_k, Hq, Hkv, d, dtype, seed):
+    g = torch.Generator().manual_seed(seed)
+    return tuple(torch.randn(n, h, d, generator=g).to(dtype) for n, h in ((sum(lens), Hq), (sum(lens_k), Hkv), (sum(lens_k), Hkv)))
+
+
+def _check(out, q, k, v, lens, lens_k, causal, dtype, what):
+    a = x = 0
+    d = q.shape[2]
+    for t, n in zip(lens, lens_k):
+        if t:
+            ref = attend(q[a:a + t], k[x:x + n], v[x:x + n], d ** -0.5, causal)
+            vmax = float(v[x:x + n].abs().max()) if n else 0.0
+            check(out[a:a + t], ref, vmax, n, d, dtype, HALF[dtype], f"{what} {t} of {n}")
+        a, x = a + t, x + n
+
+
+SHAPES = [
+    # lens, lens_k, Hq, Hkv, d, causal
+    ([1], [1], 1, 1, 64, True),
+    ([20], [20], 32, 8, 128, True),
+    ([63, 1, 64, 65, 0, 2], [63, 1, 64, 65, 0, 2], 4, 2, 64, True),
+    ([130, 7], [130, 7], 2, 2, 128, True),                   # one query head per KV head
+    ([37, 50], [37, 50], 7, 1, 128, True),                   # seven: tiles of 18 tokens
+    ([33, 5], [33, 5], 6, 2, 64, True),
+    ([4, 30, 1], [70, 200, 129], 8, 2, 64, True),            # behind a past
+    ([9, 3, 5], [4, 0, 5], 4, 1, 128, True),                 # more queries than keys: rows without a key
+    ([9, 3, 0], [77, 0, 5], 4, 4, 128, False),
+    ([2], [300], 128, 1, 64, True),                          # a tile per token
+    ([150], [150], 3, 1, 64, False),
+]
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("case", range(len(SHAPES)))
+def test_prompt_attention(case, dtype):
+    import kvq
+    lens, lens_k, Hq, Hkv, d, causal = SHAPES[case]
+    q, k, v = _inputs(lens, lens_k, Hq, Hkv, d, dtype, 100 + case)
+    plan = kvq.PromptPlan(lens, Hq, Hkv, lens_k=lens_k, causal=causal)
+    out = torch.full(q.shape, float("nan"), dtype=dtype, device="cuda")
+    got = kvq.prompt_attention(q.cuda(), k.cuda(), v.cuda(), d ** -0.5, plan, out=out)
+    assert got.data_ptr() == out.data_ptr()
+    _check(got, q, k, v, lens, lens_k, causal, dtype, f"case {case}")
+
+
+def test_large_scores_and_constant_rows():
+    """Scores of several hundred (one key takes all the weight, its maximum late) and equal scores."""
+    import kvq
+    lens, Hq, Hkv, d = [200], 4, 1, 128
+    q, k, v = _inputs(lens, lens, Hq, Hkv, d, torch.bfloat16, 5)
+    k[150] = 40 * q[180, 0] / q[180, 0].norm()
+    q[180] = q[180] * 8
+    q[10] = 0
+    out = kvq.prompt_attention(q.cuda(), k.cuda(), v.cuda(), d ** -0.5, kvq.PromptPlan(lens, Hq, Hkv))
+    _check(out, q, k, v, lens, lens, True, torch.bfloat16, "large")
+
+
+@pytest.mark.parametrize("layout", ["fused", "head_major", "odd"])
+def test_strides(layout):
+    """Rows of a fused projection, head-major rows, and rows the kernels cannot read in 16-byte pieces."""
+    import kvq
+    lens, Hq, Hkv, d = [70, 31], 8, 2, 64
+    q, k, v = _inputs(lens, lens, Hq, Hkv, d, torch.bfloat16, 9)
+    n = sum(lens)
+    if layout == "fused":
+        x = torch.cat([q, k, v], 1).cuda()
+        a, b, c = x[:, :Hq], x[:, Hq:Hq + Hkv], x[:, Hq + Hkv:]
+    elif layout == "head_major":
+        a, b, c = (x.transpose(0, 1).contiguous().cuda().transpose(0, 1) for x in (q, k, v))
+    else:
+        a, b, c = (torch.zeros((n, x.shape[1], d + 3), dtype=x.dtype, device="cuda")[:, :, 1:1 + d].copy_(x) for x in (q, k, v))
+    plan = kvq.PromptPlan(lens, Hq, Hkv)
+    got = kvq.prompt_attention(a, b, c, d ** -0.5, plan)
+    assert torch.equal(got, kvq.prompt_attention(q.cuda(), k.cuda(), v.cuda(), d ** -0.5, plan))
+    _check(got, q, k, v, lens, lens, True, torch.bfloat16, layout)
+
+
+@pytest.mark.parametrize("bad", [float("inf"), float("-inf"), float("nan")])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_values_that_a_row_does_not_see(bad, dtype):
+    """Keys and values behind a row, infinite or NaN, leave it as it is; a row that sees one does not hide it."""
+    import kvq
+    lens, Hq, Hkv, d, at = [90, 40], 4, 2, 64, 50
+    q, k, v = _inputs(lens, lens, Hq, Hkv, d, dtype, 21)
+    plan = kvq.PromptPlan(lens, Hq, Hkv)
+    clean = kvq.prompt_attention(q.cuda(), k.cuda(), v.cuda(), d ** -0.5, plan)
+    kb, vb = k.clone(), v.clone()
+    kb[at + 5], vb[at, :, 3] = bad, bad
+    got = kvq.prompt_attention(q.cuda(), kb.cuda(), vb.cuda(), d ** -0.5, plan)
+    assert torch.equal(got[:at], clean[:at]) and torch.equal(got[90:], clean[90:])
+    seen = got[at:at + 5].float()
+    assert not torch.isfinite(seen[:, :, 3]).any()
+    assert torch.equal(seen[:, :, :3], clean[at:at + 5, :, :3].float())
+    assert torch.equal(seen[:, :, 4:], clean[at:at + 5, :, 4:].float())
+
+
+def test_offsets_past_32_bits():
+    """Rows whose offsets pass 2^32 bytes and 2^31 elements."""
+    import kvq
+    lens, Hq, Hkv, d = [2100], 2, 1, 64
+    q, k, v = _inputs(lens, lens, Hq, Hkv, d, torch.bfloat16, 33)
+    step = 1 << 20
+    flat = torch.empty((2100 * step + d * 4,), dtype=torch.bfloat16, device="cuda")
+    rows = [flat.as_strided((2100, h, d), (step, d, 1), o * d) for o, h in ((0, 2), (2, 1), (3, 1))]
+    for r, x in zip(rows, (q, k, v)):
+        r.copy_(x)
+    plan = kvq.PromptPlan(lens, Hq, Hkv)
+    got = kvq.prompt_attention(*rows, d ** -0.5, plan)
+    assert torch.equal(got, kvq.prompt_attention(q.cuda(), k.cuda(), v.cuda(), d ** -0.5, plan))
+
+
+def test_replays_and_another_stream():
+    import kvq
+    lens, Hq, Hkv, d = [300, 41, 7], 8, 2, 128
+    q, k, v = (x.cuda() for x in _inputs(lens, lens, Hq, Hkv, d, torch.bfloat16, 41))
+    plan = kvq.PromptPlan(lens, Hq, Hkv)
+    out = torch.empty_like(q)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        first = kvq.prompt_attention(q, k, v, d ** -0.5, plan)
+    torch.cuda.current_stream().wait_stream(side)
+    assert torch.equal(first, kvq.prompt_attention(q, k, v, d ** -0.5, plan))
+    gr = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(gr):
+        kvq.prompt_attention(q, k, v, d ** -0.5, plan, out=out)
+    for i in range(3):
+        q.copy_(torch.randn_like(q))
+        _ = (q.float() * 2).sum()
+        torch.cuda.synchronize()
+        gr.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, kvq.prompt_attention(q, k, v, d ** -0.5, plan)), i
+
+
+def test_refusals():
+    import kvq
+    q = torch.zeros((5, 4, 64), dtype=torch.bfloat16, device="cuda")
+    k = torch.zeros((5, 2, 64), dtype=torch.bfloat16, device="cuda")
+    plan = kvq.PromptPlan([5], 4, 2)
+    with pytest.raises(ValueError, match="plan"):
+        kvq.prompt_attention(q[:4], k, k, 0.1, plan)
+    with pytest.raises(ValueError, match="plan"):
+        kvq.prompt_attention(q, k[:4], k[:4], 0.1, plan)
+    with pytest.raises(TypeError):
+        kvq.prompt_attention(q.float(), k.float(), k.float(), 0.1, plan)
+    with pytest.raises(TypeError):
+        kvq.prompt_attention(q, k.half(), k.half(), 0.1, plan)
+    with pytest.raises(kvq.KVQError, match="head_dim"):
+        kvq.prompt_attention(q[..., :32], k[..., :32], k[..., :32], 0.1, plan)
+    with pytest.raises(ValueError, match="out"):
+        kvq.prompt_attention(q, k, k, 0.1, plan, out=torch.empty((5, 64, 4), dtype=torch.bfloat16, device="cuda"))
+    with pytest.raises(kvq.KVQError):
+        kvq.prompt_attention(q.cpu(), k, k, 0.1, plan)

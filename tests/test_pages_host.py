@@ -1,0 +1,170 @@
+"""The page accounts and the plans of the paged cache and of prompt attention, on the host: against a plain
+model of the accounts, and everything that is refused."""
+import ctypes
+import random
+
+import numpy as np
+import pytest
+
+from oracle.paged import Accounts
+
+
+class Host:
+    """The accounts as PagedCache keeps them, without a device."""
+
+    def __init__(self, slots, pages, max_tokens, page):
+        from kvq import _lib
+        self.lib = _lib.load()
+        self.slots, self.pages, self.page, self.max_tokens, self.blocks = slots, pages, page, max_tokens, -(-max_tokens // page)
+        self.lens = np.zeros(slots, np.int64)
+        self.table = np.zeros((slots, self.blocks), np.int32)
+        self.refs = np.zeros(pages, np.int32)
+        self.open = np.zeros(slots, np.uint8)
+        self.account = np.array([pages, 0], np.int64)
+        self.p = [x.ctypes.data for x in (self.lens, self.table, self.refs, self.open, self.account)]
+
+    def extend(self, slots, counts, cap=64, words=None):
+        s, c = np.array(slots, np.int64), np.array(counts, np.int64)
+        n = self.lib.kvq_pages_step_words(self.page, c.ctypes.data, len(c)) if words is None else words
+        self.desc = np.zeros(max(n, 1), np.int32)
+        return self.lib.kvq_pages_extend(*self.p, self.slots, self.pages, self.blocks, self.page, self.max_tokens, s.ctypes.data,
+                                         c.ctypes.data, len(s), cap, self.desc.ctypes.data, n, None, None)
+
+    def fork(self, src, dst):
+        s, d = np.array(src, np.int64), np.array(dst, np.int64)
+        return self.lib.kvq_pages_fork(*self.p[:4], self.slots, self.blocks, self.page, s.ctypes.data, d.ctypes.data, len(s), 1, 1, 64,
+                                       None, None, None, None)
+
+    def free(self, slots):
+        s = np.array(slots, np.int64)
+        return self.lib.kvq_pages_free(*self.p, self.slots, self.blocks, self.page, s.ctypes.data, len(s))
+
+    def error(self):
+        return self.lib.kvq_last_error()
+
+    def same(self, model):
+        assert self.lens.tolist() == model.lens and self.refs.tolist() == model.refs
+        for s, pages in enumerate(model.table):
+            assert self.table[s, :len(pages)].tolist() == pages
+        free = [i for i, r in enumerate(model.refs) if r == 0]
+        assert self.account[0] == len(free) and (not free or self.account[1] <= free[0])
+
+
+@pytest.mark.parametrize("page", [32, 64, 128])
+def test_accounts_follow_the_model(page):
+    rng = random.Random(page)
+    host, model = Host(9, 40, 20 * page, page), Accounts(9, 40, page)
+    for _ in range(300):
+        op = rng.choice(["extend", "extend", "extend", "fork", "free"])
+        if op == "extend":
+            slots = rng.sample(range(9), rng.randint(1, 4))
+            counts = [rng.choice([1, 2, page - 1, page, rng.randint(1, 3 * page)]) for _ in slots]
+            need = sum((host.lens[s] + c) // page - host.lens[s] // page for s, c in zip(slots, counts))
+            fits = need <= host.account[0] and all(host.lens[s] + c <= host.max_tokens for s, c in zip(slots, counts))
+            rc = host.extend(slots, counts)
+            assert (rc == 0) == fits, host.error()
+            if fits:
+                model.extend(slots, counts)
+                _description(host, slots, counts)
+            else:
+                assert b"decode buffer exhausted" in host.error()
+        elif op == "fork":
+            empty = [s for s in range(9) if host.lens[s] == 0]
+            held = [s for s in range(9) if host.lens[s]]
+            if not empty or not held:
+                continue
+            dst = rng.sample(empty, rng.randint(1, len(empty)))
+            src = [rng.choice(held) for _ in dst]
+            assert host.fork(src, dst) == 0
+            model.fork(src, dst)
+        else:
+            slots = rng.sample(range(9), rng.randint(1, 3))
+            assert host.free(slots + slots[:1]) == 0              # a slot named twice is empty the second time
+            model.free(slots)
+        host.same(model)
+
+
+def _description(host, slots, counts):
+    """Rows, items, split items and the pages of what gets full."""
+    n, d, page = len(slots), host.desc, host.page
+    seq = d[8:8 + 8 * (n + 1)].reshape(n + 1, 8)
+    row = item = split = 0
+    for i, (s, c) in enumerate(zip(slots, counts)):
+        end = int(host.lens[s])
+        pos0 = end - c
+        assert seq[i, :6].tolist() == [s, pos0, c, row, item, split]
+        for j in range(pos0 // page, (end - 1) // page + 1):
+            want = host.table[s, j] if (j + 1) * page <= end else -1
+            assert d[8 + 8 * (n + 1) + item] == want
+            item += 1
+        row += c
+        full = end // page * page
+        units = -(-full // 64) + -(-(end - full) // 64)
+        split += -(-units // int(d[3]))
+    assert seq[n, 3:6].tolist() == [row, item, split] and d[:3].tolist() == [n, item, split] and split <= 64
+
+
+def test_refusals_change_nothing():
+    host = Host(4, 5, 400, 64)
+    assert host.extend([0, 1], [130, 70]) == 0
+    before = [x.copy() for x in (host.lens, host.table, host.refs, host.open, host.account)]
+    for slots, counts, message in (([0, 0], [1, 1], b"named twice"), ([4], [1], b"no slot"), ([-1], [1], b"no slot"),
+                                   ([2], [0], b"at least one"), ([2, 3], [64, -1], b"bad counts"), ([2], [401], b"exhausted"),
+                                   ([2, 3], [64, 128], b"exhausted")):
+        assert host.extend(slots, counts) == 1 and message in host.error(), (slots, counts, host.error())
+    assert host.extend([2], [1], cap=0) == 1 and host.extend([2], [1], words=10) == 1
+    for src, dst, message in (([0], [1], b"in use"), ([0, 0], [2, 2], b"twice"), ([0], [4], b"no slot"), ([-1], [2], b"no slot"),
+                              ([0], [0], b"in use"), ([2], [2], b"both"), ([0, 2], [2, 3], b"both")):
+        assert host.fork(src, dst) == 1 and message in host.error(), (src, dst, host.error())
+    assert host.free([0, 9]) == 1 and b"no slot" in host.error()
+    for a, b in zip(before, (host.lens, host.table, host.refs, host.open, host.account)):
+        assert np.array_equal(a, b)
+
+
+def test_prompt_plan_covers_every_row_once():
+    from kvq import _lib
+    lib = _lib.load()
+    rng = random.Random(3)
+    for _ in range(60):
+        n, rep, causal = rng.randint(1, 6), rng.choice([1, 2, 3, 4, 7, 8, 128]), rng.choice([0, 1])
+        lq = np.array([rng.choice([0, 1, 31, 32, rng.randint(0, 300)]) for _ in range(n)], np.int64)
+        lk = np.array([max(0, int(a) + rng.choice([0, 0, 50, -3])) for a in lq], np.int64)
+        count = lib.kvq_prompt_plan(lq.ctypes.data, lk.ctypes.data, n, rep, causal, None, 0)
+        items = np.zeros((max(count, 1), 8), np.int32)
+        assert lib.kvq_prompt_plan(lq.ctypes.data, lk.ctypes.data, n, rep, causal, items.ctypes.data, count) == count
+        seen = np.zeros(int(lq.sum()), np.int64)
+        rows, keys = np.concatenate([[0], np.cumsum(lq)]), np.concatenate([[0], np.cumsum(lk)])
+        for row, toks, key, nk, vis0, step, *_ in items[:count].tolist():
+            seen[row:row + toks] += 1
+            assert 0 < toks * rep <= 128
+            s = int(np.searchsorted(rows, row, "right") - 1)
+            assert row + toks <= rows[s + 1] and key == keys[s] and 0 <= nk <= lk[s]
+            t = row - rows[s]
+            assert (vis0, step) == ((lk[s] - lq[s] + t + 1, 1) if causal else (lk[s], 0))
+            assert nk == (max(0, vis0 + toks - 1) if causal else lk[s])
+        assert (seen == 1).all()
+    bad = np.array([-1], np.int64)
+    assert lib.kvq_prompt_plan(bad.ctypes.data, bad.ctypes.data, 1, 1, 1, None, 0) == -1
+    one = np.array([1], np.int64)
+    assert lib.kvq_prompt_plan(one.ctypes.data, one.ctypes.data, 1, 129, 1, None, 0) == -1
+
+
+def test_kernel_entries_refuse_before_any_launch():
+    from kvq import _lib
+    lib = _lib.load()
+    one = ctypes.c_void_p(16)
+    rc = lib.kvq_prompt_attention(one, 64, 64, one, 64, 64, one, 64, 64, 2, 4, 2, 96, 0.1, one, 1, one, None)
+    assert rc == 1 and b"head_dim" in lib.kvq_last_error()
+    rc = lib.kvq_prompt_attention(one, 64, 64, one, 64, 64, one, 64, 64, 0, 4, 2, 64, 0.1, one, 1, one, None)
+    assert rc == 1 and b"fp16 or bf16" in lib.kvq_last_error()
+    rc = lib.kvq_prompt_attention(one, 64, 60, one, 64, 64, one, 64, 64, 2, 4, 2, 64, 0.1, one, 1, one, None)
+    assert rc == 1 and b"16 bytes" in lib.kvq_last_error()
+    rc = lib.kvq_pages_append(one, 64, 64, one, 64, 64, 2, one, 1, one, 4, 2, 64, 48, 0, one, one, one, one, one, None)
+    assert rc == 1 and b"page" in lib.kvq_last_error()
+    rc = lib.kvq_pages_append(one, 64, 64, one, 64, 64, 2, one, 1, one, 4, 2, 64, 64, 3, one, one, one, one, one, None)
+    assert rc == 1 and b"code" in lib.kvq_last_error()
+    need = lib.kvq_paged_decode_workspace(4, 2, 2, 1, 64)
+    assert need == 4 * 2 * 16 * 66
+    rc = lib.kvq_paged_decode(one, 256, 64, 2, 1, 4, 2, 64, 0.1, one, 4, 1, one, 4, 64, 0, one, one, one, one, one, one, one, need - 1, None)
+    assert rc == 1 and b"workspace" in lib.kvq_last_error()
+    assert lib.kvq_paged_decode_workspace(4, 2, 2, 1, 96) == -1
