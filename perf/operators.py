@@ -280,12 +280,7 @@ def prepare(case, seed):
         st.pages = sum(lens[i] // c["page"] for i in st.left)
         if own:
             st.cache = _cache(c, lens, n, c["layers"])
-            steps = [(chunk, st.cache.extend([i for i, _, _ in chunk], [b - a for _, a, b in chunk]))
-                     for chunk in _chunks(lens)]
-            for l, layer in enumerate(kv):
-                for chunk, step in steps:
-                    k, v = (torch.cat([layer[i][s][a:b] for i, a, b in chunk]) for s in (0, 1))
-                    st.cache.append(l, k, v, step)
+            _fill(st.cache, list(kv), lens)
             st.cache.free([i for i in range(n) if i % 3 == 1])
         else:
             st.ids, total = _page_ids(lens, c["page"])
