@@ -687,7 +687,7 @@ int kvq_prompt_attention(const void* q, int64_t q_st, int64_t q_sh, const void* 
  * code: 0 int8, 1 e4m3.  a = max(|x|, 2^-100) over a block of one head, scale = a / top, code =
  * rne(x * (top / a)), top 127 or 448, in float32; a block with an infinity or a NaN has the scale NaN.
  *
- * kvq_pages_extend claims counts[i] tokens for slot seq[i]: the lowest free page for each block that gets
+ * kvq_pages_extend claims counts[i] >= 0 tokens for slot seq[i]: the lowest free page for each block that gets
  * full, in order; refused whole ("decode buffer exhausted") when a slot's max_tokens or the free pages do
  * not suffice.  It writes the step's description to `desc` (host, kvq_pages_step_words words) and, by
  * value with launches on `stream`, to desc_device (NULL: host only).  split_cap >= n bounds the decode's split items.

@@ -99,8 +99,7 @@ __global__ __launch_bounds__(kThreads) void append_kernel(Rows16 k, Rows16 v, co
   const int item = blockIdx.x / H, h = blockIdx.x % H, tid = threadIdx.x;
   const int n = step[0];
   if (item >= step[1]) return;
-  const int b = step[1] == n ? item : step_find(step, n, 4, item);
-  const StepSeq s = step_seq(step, b);
+  const StepSeq s = step_seq(step, step[4] ? item : step_find(step, n, 4, item));
   const int j = s.pos0 / P + item - s.item0;                        // block of the sequence
   const int first = j * P, end = s.pos0 + s.count;
   const int from = first > s.pos0 ? first : s.pos0;                 // tokens [from, to) of the block are new
@@ -348,10 +347,15 @@ int64_t units_of(int64_t len, int64_t page) {
   return (full + kUnit - 1) / kUnit + (len - full + kUnit - 1) / kUnit;
 }
 
+int64_t splits_of(const int32_t* e, int64_t page, int64_t per) {    // none for a sequence without new tokens
+  return e[2] ? (units_of(static_cast<int64_t>(e[1]) + e[2], page) + per - 1) / per : 0;
+}
+
 // Fills the description from lens (before), counts and open buffers.  Returns the number of items.
 int64_t describe(const int64_t* lens, const uint8_t* open, int64_t page, const int64_t* seq, const int64_t* counts, int64_t n,
                  int64_t split_cap, bool whole, int32_t* desc) {
   int64_t row = 0, item = 0, most = 0;
+  bool even = true;
   for (int64_t i = 0; i < n; ++i) {
     int32_t* e = desc + kStepHead + kStepSeq * i;
     const int64_t s = seq[i], len = lens[s], pos0 = whole ? 0 : len, count = whole ? len : counts[i], end = pos0 + count;
@@ -365,6 +369,7 @@ int64_t describe(const int64_t* lens, const uint8_t* open, int64_t page, const i
     e[7] = 0;
     row += count;
     item += count ? (end - 1) / page - pos0 / page + 1 : 0;
+    even = even && item == i + 1;
     const int64_t u = units_of(end, page);
     most = u > most ? u : most;
   }
@@ -374,7 +379,7 @@ int64_t describe(const int64_t* lens, const uint8_t* open, int64_t page, const i
     int64_t items = 0;
     for (int64_t i = 0; i < n; ++i) {
       const int32_t* e = desc + kStepHead + kStepSeq * i;
-      items += (units_of(static_cast<int64_t>(e[1]) + e[2], page) + mid - 1) / mid;
+      items += splits_of(e, page, mid);
     }
     if (items <= split_cap) hi = mid;
     else lo = mid + 1;
@@ -383,7 +388,7 @@ int64_t describe(const int64_t* lens, const uint8_t* open, int64_t page, const i
   for (int64_t i = 0; i < n; ++i) {
     int32_t* e = desc + kStepHead + kStepSeq * i;
     e[5] = static_cast<int32_t>(split);
-    split += (units_of(static_cast<int64_t>(e[1]) + e[2], page) + lo - 1) / lo;
+    split += splits_of(e, page, lo);
   }
   int32_t* e = desc + kStepHead + kStepSeq * n;
   memset(e, 0, sizeof(int32_t) * kStepSeq);
@@ -395,6 +400,7 @@ int64_t describe(const int64_t* lens, const uint8_t* open, int64_t page, const i
   desc[1] = static_cast<int32_t>(item);
   desc[2] = static_cast<int32_t>(split);
   desc[3] = static_cast<int32_t>(lo);
+  desc[4] = even;
   return item;
 }
 
@@ -461,7 +467,7 @@ extern "C" int kvq_pages_extend(int64_t* lens, int32_t* table, int32_t* refs, ui
   int64_t checked = 0;
   for (; checked < n; ++checked) {
     const int64_t s = seq[checked], c = counts[checked];
-    if (s < 0 || s >= slots || c < 1) { bad = checked; break; }
+    if (s < 0 || s >= slots) { bad = checked; break; }
     if (lens[s] < 0) { twice = s; break; }
     if (lens[s] + c > max_tokens) { bad = checked; break; }
     need += (lens[s] + c) / page - lens[s] / page;
@@ -473,7 +479,6 @@ extern "C" int kvq_pages_extend(int64_t* lens, int32_t* table, int32_t* refs, ui
   if (bad >= 0) {
     const int64_t s = seq[bad];
     KVQ_REQUIRE(s >= 0 && s < slots, "kvq_pages_extend: no slot %lld (of %lld)", static_cast<long long>(s), static_cast<long long>(slots));
-    KVQ_REQUIRE(counts[bad] >= 1, "kvq_pages_extend: a sequence takes at least one token");
     KVQ_REQUIRE(false, "decode buffer exhausted: slot %lld holds %lld tokens of %lld, %lld more asked for", static_cast<long long>(s),
                 static_cast<long long>(lens[s]), static_cast<long long>(max_tokens), static_cast<long long>(counts[bad]));
   }
@@ -486,7 +491,7 @@ extern "C" int kvq_pages_extend(int64_t* lens, int32_t* table, int32_t* refs, ui
   for (int64_t i = 0; i < n; ++i) {
     const int32_t* e = desc + kStepHead + kStepSeq * i;
     const int64_t s = seq[i], end = lens[s] + counts[i];
-    for (int64_t j = lens[s] / page; j <= (end - 1) / page; ++j) {
+    for (int64_t j = lens[s] / page; counts[i] && j <= (end - 1) / page; ++j) {
       int32_t id = -1;
       if ((j + 1) * page <= end) {
         while (low < pages && refs[low]) ++low;                     // the lowest free page

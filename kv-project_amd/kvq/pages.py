@@ -111,7 +111,7 @@ class PagedCache:
     # ---- steps -------------------------------------------------------------------------------
 
     def extend(self, slots: Sequence[int], counts: Sequence[int], *, into: Optional[Step] = None) -> Step:
-        """Claim room for counts[i] more tokens of slots[i] (each slot once): the lowest free page for each block that
+        """Claim room for counts[i] more tokens (or none) of slots[i] (each slot once): the lowest free page for each block that
         gets full.  Raises KVQError ("decode buffer exhausted") and changes nothing when a slot or the pool is
         full.  ``into``: a step of the same counts whose description is rewritten in place, so that a
         captured graph of its append and decode runs the new step when it is replayed."""
@@ -123,7 +123,7 @@ class PagedCache:
         if into is None:
             words = lib.kvq_pages_step_words(self.page, c.ctypes.data, n)
             if words < 0:
-                raise ValueError("counts must be positive and below 2^31")
+                raise ValueError("counts must not be negative, and below 2^31")
             st = Step()
             st.host = np.empty(words, dtype=np.int32)
             st.desc = torch.empty(words, dtype=torch.int32, device=self.device)
@@ -136,7 +136,7 @@ class PagedCache:
                      self.max_tokens, s.ctypes.data, c.ctypes.data, n, st.splits, st.host.ctypes.data, st.host.size,
                      st.desc.data_ptr(), _lib.stream_of(st.desc))
         if into is None:
-            st.splits = int(st.host[2])        # what later steps written into this one keep to
+            st.splits = max(1, int(st.host[2]))         # what later steps written into this one keep to
             st.items = st.host.size - 8 * (n + 2)
             st.rows, st.max_count = int(c.sum()), int(c.max())
         st.slots, st.counts, st.ends, st.generation = s, c, self._lens[s], self._generation
@@ -163,6 +163,8 @@ class PagedCache:
         self.check_step(step, "append")
         if step.generation != self._generation:
             raise ValueError("append: the pages have moved since the step was made")
+        if step.rows == 0:
+            return
         k, v = rows16(k), rows16(v)
         _lib.call_on(self.device, "kvq_pages_append", k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(), v.stride(0), v.stride(1),
                      _lib.DTYPE_CODE[self.dtype], step.desc.data_ptr(), step.items, self.table.data_ptr(), self.max_blocks,
@@ -283,6 +285,8 @@ def paged_decode(q: torch.Tensor, scaling: float, cache: PagedCache, layer: int,
     q = rows16(q)
     Hq = q.shape[1]
     out = _lib.out_or_new(out, (step.rows, Hq, cache.d), q.dtype, q.device, "paged_decode")
+    if step.rows == 0:
+        return out
     if workspace is None:
         workspace = torch.empty((paged_workspace_floats(step, Hq, cache.Hkv, cache.d),), dtype=torch.float32, device=q.device)
     elif workspace.dtype != torch.float32 or not workspace.is_contiguous() or workspace.device != q.device:

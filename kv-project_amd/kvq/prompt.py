@@ -78,6 +78,8 @@ def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, scaling:
         raise ValueError(f"prompt_attention: the plan is for {plan.device}")
     q, k, v = (rows16(x) for x in (q, k, v))
     out = _lib.out_or_new(out, (plan.rows, plan.Hq, d), q.dtype, q.device, "prompt_attention")
+    if plan.keys == 0:
+        return out.zero_()
     _lib.call_on(q.device, "kvq_prompt_attention", q.data_ptr(), q.stride(0), q.stride(1), k.data_ptr(), k.stride(0), k.stride(1),
                  v.data_ptr(), v.stride(0), v.stride(1), _lib.DTYPE_CODE[q.dtype], plan.Hq, plan.Hkv, d, float(scaling),
                  plan.items.data_ptr(), plan.n_items, out.data_ptr(), _lib.stream_of(q))

@@ -87,6 +87,8 @@ class Mirror:
         out = kvq.paged_decode(q.cuda(), c.d ** -0.5, c, layer, step)
         a = 0
         for s, n in zip(step.slots.tolist(), step.counts.tolist()):
+            if n == 0:
+                continue
             k, v = cached(self.k[layer][s], c.page, c.code), cached(self.v[layer][s], c.page, c.code)
             ref = attend(q[a:a + n], k, v, c.d ** -0.5)
             check(out[a:a + n], ref, float(v.abs().max()), k.shape[0], c.d, c.dtype, PAIR, f"{what} slot {s}, {n} of {k.shape[0]}")
@@ -103,7 +105,7 @@ def test_any_order_of_steps(page, d, Hkv, code, dtype):
     m.push([0, 2], [1, page])
     m.push([2, 0, 4], [1, page - 1, 3 * page + 5])
     m.check("prompts")
-    step = m.push([0, 2, 4], [1, 1, 1])
+    step = m.push([0, 1, 2, 4], [1, 0, 1, 1])                       # nothing for one of them
     m.check("tokens")
     m.decode(step, 4 * Hkv, what="one token")
     step = m.push([4, 0], [page - 3, 5])
@@ -212,7 +214,7 @@ def test_append_again_writes_the_same():
     """A step that fills a block and opens the next one, appended twice."""
     m = Mirror(seed=6, page=32)
     m.push([0, 1], [20, 31])
-    step, [(k, v)] = m.extend([0, 1], [25, 1])
+    step, [(k, v)] = m.extend([0, 2, 1], [25, 0, 1])
     for _ in range(3):
         m.cache.append(0, k.cuda(), v.cuda(), step)
         m.check("again")
@@ -348,6 +350,10 @@ def test_gpu_refusals():
         c.extend([0, 1], [192, 128])
     with pytest.raises(ValueError):
         c.extend([], [])
+    none = c.extend([0, 2], [0, 0])
+    empty = torch.empty((0, 2, 64), dtype=torch.bfloat16, device="cuda")
+    c.append(1, empty, empty, none)
+    assert kvq.paged_decode(torch.empty((0, 4, 64), dtype=torch.bfloat16, device="cuda"), 0.1, c, 0, none).shape == (0, 4, 64)
     with pytest.raises(kvq.KVQError, match="twice"):
         c.extend([1, 1], [1, 1])
     assert c.lengths == [0, 0, 0] and c.free_pages == 4

@@ -36,6 +36,8 @@ SHAPES = [
     ([4, 30, 1], [70, 200, 129], 8, 2, 64, True),            # behind a past
     ([9, 3, 5], [4, 0, 5], 4, 1, 128, True),                 # more queries than keys: rows without a key
     ([9, 3, 0], [77, 0, 5], 4, 4, 128, False),
+    ([5, 2], [0, 0], 4, 2, 64, True),
+    ([0, 0], [0, 7], 4, 2, 64, True),
     ([2], [300], 128, 1, 64, True),                          # a tile per token
     ([150], [150], 3, 1, 64, False),
 ]

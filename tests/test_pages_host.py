@@ -58,7 +58,7 @@ def test_accounts_follow_the_model(page):
         op = rng.choice(["extend", "extend", "extend", "fork", "free"])
         if op == "extend":
             slots = rng.sample(range(9), rng.randint(1, 4))
-            counts = [rng.choice([1, 2, page - 1, page, rng.randint(1, 3 * page)]) for _ in slots]
+            counts = [rng.choice([0, 1, 2, page - 1, page, rng.randint(1, 3 * page)]) for _ in slots]
             need = sum((host.lens[s] + c) // page - host.lens[s] // page for s, c in zip(slots, counts))
             fits = need <= host.account[0] and all(host.lens[s] + c <= host.max_tokens for s, c in zip(slots, counts))
             rc = host.extend(slots, counts)
@@ -93,14 +93,15 @@ def _description(host, slots, counts):
         end = int(host.lens[s])
         pos0 = end - c
         assert seq[i, :6].tolist() == [s, pos0, c, row, item, split]
-        for j in range(pos0 // page, (end - 1) // page + 1):
+        for j in range(pos0 // page, (end - 1) // page + 1 if c else 0):
             want = host.table[s, j] if (j + 1) * page <= end else -1
             assert d[8 + 8 * (n + 1) + item] == want
             item += 1
         row += c
         full = end // page * page
         units = -(-full // 64) + -(-(end - full) // 64)
-        split += -(-units // int(d[3]))
+        split += -(-units // int(d[3])) if c else 0
+    assert d[4] == all(b - a == 1 for a, b in zip(seq[:, 4], seq[1:, 4]))
     assert seq[n, 3:6].tolist() == [row, item, split] and d[:3].tolist() == [n, item, split] and split <= 64
 
 
@@ -109,7 +110,7 @@ def test_refusals_change_nothing():
     assert host.extend([0, 1], [130, 70]) == 0
     before = [x.copy() for x in (host.lens, host.table, host.refs, host.open, host.account)]
     for slots, counts, message in (([0, 0], [1, 1], b"named twice"), ([4], [1], b"no slot"), ([-1], [1], b"no slot"),
-                                   ([2], [0], b"at least one"), ([2, 3], [64, -1], b"bad counts"), ([2], [401], b"exhausted"),
+                                   ([2, 3], [64, -1], b"bad counts"), ([2], [401], b"exhausted"),
                                    ([2, 3], [64, 128], b"exhausted")):
         assert host.extend(slots, counts) == 1 and message in host.error(), (slots, counts, host.error())
     assert host.extend([2], [1], cap=0) == 1 and host.extend([2], [1], words=10) == 1
