@@ -684,8 +684,8 @@ int kvq_prompt_attention(const void* q, int64_t q_st, int64_t q_sh, const void* 
  * All layers share table (slots, max_blocks) int32 on the device and the accounts in host memory:
  *   lens (slots) int64, table (slots, max_blocks) int32, refs (pages) int32 users of each page,
  *   open (slots) uint8 the current open buffer, account[2] = {free pages, no free page below this one}.
- * code: 0 int8, 1 e4m3.  a = max(|x|, 2^-100) over a block of one head, scale = a / top, code =
- * rne(x * (top / a)), top 127 or 448, in float32; a block with an infinity or a NaN has the scale NaN.
+ * code: 0 int8, 1 e4m3.  a = max(|x|, 2^-100) over a block of one head, scale = a * (1 / top),
+ * code = rne(x * ((1 / a) * top)), top 127 or 448, each operation in float32; a block with an infinity or a NaN has the scale NaN.
  *
  * kvq_pages_extend claims counts[i] >= 0 tokens for slot seq[i]: the lowest free page for each block that gets
  * full, in order; refused whole ("decode buffer exhausted") when a slot's max_tokens or the free pages do

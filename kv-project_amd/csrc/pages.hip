@@ -1,8 +1,9 @@
 // The paged 8-bit cache: its page accounts (host), filling it, reading it back and moving its pages.
 //
 // A block is coded once, when its last token comes: a = max(|x|, 2^-100) over the P x D values of one KV
-// head, scale = a / top, code = rne(x * (top / a)), top = 127 (int8) or 448 (e4m3), each operation
-// rounded to float32.  The codes of a block therefore do not depend on how its tokens arrived.  A block
+// head, scale = a * (1 / top), code = rne(x * ((1 / a) * top)), top = 127 (int8) or 448 (e4m3), each
+// operation rounded to float32 (as torch divides by a number, and a number by a tensor, on this device;
+// bf16 values meet exact ties often enough for the last bit to count).  The codes of a block therefore do not depend on how its tokens arrived.  A block
 // that holds an infinity or a NaN gets the scale NaN: its tokens read as NaN.
 //
 // All of these kernels move bytes: filling reads 4 D and writes 2 D bytes per token and KV head.
@@ -80,7 +81,7 @@ __device__ __forceinline__ Scale block_scale(uint32_t bits) {
   constexpr float top = CODE == kCodeInt8 ? 127.0f : 448.0f;
   const float a = fmaxf(to_f32<BF16>(bits), 0x1p-100f);
   if (bits >= (BF16 ? 0x7f80u : 0x7c00u)) return {__uint_as_float(0x7fc00000u), 0.0f};
-  return {__fdiv_rn(a, top), __fdiv_rn(top, a)};
+  return {a * (1.0f / top), __fdiv_rn(1.0f, a) * top};
 }
 
 // One workgroup per (item, KV head).  Keys and values of the block are held in registers (16 bytes a

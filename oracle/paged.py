@@ -10,15 +10,16 @@ TOP = {"int8": 127.0, "e4m3": 448.0}
 
 
 def quantise(block: torch.Tensor, code: str):
-    """One head's block (page, d) -> (codes as float32, scale): a = max(|x|, 2^-100), scale = a / top,
-    code = rne(x * (top / a)); a block with an infinity or a NaN: zeros, scale NaN."""
+    """One head's block (page, d) -> (codes as float32, scale): a = max(|x|, 2^-100), scale =
+    a * (1 / top), code = rne(x * ((1 / a) * top)), each operation rounded; a block with an infinity or a NaN: zeros, scale NaN."""
     x = block.float()
     if not torch.isfinite(x).all():
         return torch.zeros_like(x), torch.tensor(float("nan"))
     a = x.abs().max().clamp_min(2.0 ** -100)
-    y = x * (torch.tensor(TOP[code]) / a)
+    top = torch.tensor(TOP[code])
+    y = x * ((torch.ones(()) / a) * top)
     c = torch.round(y) if code == "int8" else y.to(torch.float8_e4m3fn).float()
-    return c, a / TOP[code]
+    return c, a * (torch.ones(()) / top)
 
 
 def cached(x: torch.Tensor, page: int, code: str) -> torch.Tensor:
