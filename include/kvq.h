@@ -663,17 +663,20 @@ int kvq_selftest_mfma_layout(const uint16_t* a, const uint16_t* b, float* out, v
  * Attention over whole prompts (the reference leaves it to SDPA: STRATA_KV.py:499-504).
  * Packed rows of n sequences: q (sum lens_q, Hq, D), k, v (sum lens_k, Hq / rep, D) of one 16-bit dtype,
  * element strides per row and head, channels contiguous, pointers and strides multiples of 16 bytes; D 64
- * or 128, rep <= 128.  Query t of a sequence sees keys 0 .. t + len_k - len_q (causal), or all of them; one
+ * or 128, rep <= 128, row strides below 2^24.  Query t of a sequence sees keys 0 .. t + len_k - len_q (causal), or all of them; one
  * that sees none gets zeros.  out (sum lens_q, Hq, D), contiguous.
- * kvq_prompt_plan (host memory): fills `items` (8 int32 each) for a call over such sequences and returns
- * their number (-1: bad sizes; more than items_cap: nothing to be used, call again with room).  The items
- * go to the device as they are; they bound what kvq_prompt_attention reads.
+ * kvq_prompt_plan (host memory): fills `words` for a call over such sequences and H KV heads; info[3] = {items,
+ * merges, parts}.  8 items + 4 merges words are needed: with less room only info is set.  The words go to the
+ * device as they are; they bound what kvq_prompt_attention reads.  workspace: kvq_prompt_workspace floats
+ * (none without parts), no clearing; calls that share one must not overlap in time.
  * ---------------------------------------------------------------------------------------- */
-int64_t kvq_prompt_plan(const int64_t* lens_q, const int64_t* lens_k, int64_t n, int64_t rep, int causal,
-                        int32_t* items, int64_t items_cap);
+int kvq_prompt_plan(const int64_t* lens_q, const int64_t* lens_k, int64_t n, int64_t rep, int64_t H, int causal,
+                    int32_t* words, int64_t words_cap, int64_t* info);
+int64_t kvq_prompt_workspace(int64_t parts, int64_t H, int64_t D);
 int kvq_prompt_attention(const void* q, int64_t q_st, int64_t q_sh, const void* k, int64_t k_st, int64_t k_sh,
                          const void* v, int64_t v_st, int64_t v_sh, int dtype, int64_t Hq, int64_t H, int64_t D,
-                         float scaling, const int32_t* items, int64_t n_items, void* out, void* stream);
+                         float scaling, const int32_t* words, int64_t items, int64_t merges, int64_t parts, void* out,
+                         float* workspace, int64_t workspace_floats, void* stream);
 
 /* ------------------------------------------------------------------------------------------
  * The paged 8-bit cache (no counterpart in the reference, whose caches are dense in the batch).

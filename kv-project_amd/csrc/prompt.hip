@@ -4,12 +4,17 @@
 // A workgroup takes 128 rows of one KV head: (token, query head) pairs, token major, so that the query
 // heads of a group share the keys and values that are staged in LDS, 64 tokens at a time.  Each of its
 // four wavefronts holds 32 rows as the columns of the matrix products: S^T = K Q^T, the softmax in base
-// 2 with one running maximum and sum per column (two lanes hold a column; one swap joins them), and
+// 2 with one running reference and sum per column (two lanes hold a column; one swap joins them), and
 // O^T += V^T P^T.  The accumulator layout of S^T is the operand layout of P^T once V^T takes its tokens in
 // the same order, so probabilities never leave their lanes: V^T comes from LDS by transposing reads.
 // Probabilities are rounded to the inputs' type (half a step of the output's type); the sums, the
-// maximum and the accumulators are float32.
+// references and the accumulators are float32.
+//
+// Where the rows are too few to fill the chip, a tile of rows is cut along its keys into parts, each
+// with its own sums, and prompt_merge_kernel joins them in order.
+//
 #include <algorithm>
+#include <cmath>
 #include <type_traits>
 
 #include "mfma_common.hpp"
@@ -17,7 +22,7 @@
 namespace kvq {
 namespace {
 
-constexpr int kThreads = 256, kTileRows = 128, kTileKeys = 64, kItemWords = 8;
+constexpr int kThreads = 256, kTileRows = 128, kTileKeys = 64, kItemWords = 8, kSlots = 512;
 
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
@@ -26,6 +31,7 @@ typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
+typedef __attribute__((address_space(3))) void lds_void;
 
 template <bool BF16>
 __device__ __forceinline__ f32x16 mfma32(u32x4 a, u32x4 b, f32x16 c) {
@@ -45,22 +51,42 @@ __device__ __forceinline__ u32x2 read_tr(const uint16_t* p) {
   return __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(p)));
 }
 
+#define KVQ_INLINE __attribute__((always_inline))
+
+// f of the constants I .. N - 1: indexes of registers have to be known before any loop is unrolled
+template <int I, int N, class F>
+__device__ __forceinline__ void each(F&& f) {
+  if constexpr (I < N) {
+    f(std::integral_constant<int, I>{});
+    each<I + 1, N>(f);
+  }
+}
+
 struct PromptArgs {
   const uint16_t *q, *k, *v;
   int64_t q_st, q_sh, k_st, k_sh, v_st, v_sh;
-  const int* items;                           // {first row, tokens, first key, keys, visible to the first token, step}
+  const int* items;                           // {first row, tokens, first key, keys, visible to the first token, step, part or -1}
   int H, rep;
-  float scale;                                // scaling * log2(e)
+  float scale;                                // |scaling| * log2(e)
+  uint32_t sign;                              // of scaling, for both halves of a word of q
   uint16_t* out;                              // (rows, Hq, D)
+  float* part;                                // (parts, H): 128 x D sums, then 128 x {reference, sum}
 };
 
+// Iteration j takes a tile of 64 tokens through the softmax, beside matrix products that do not depend on it:
+// O += V(j-1) P(j-1); then S(j+1) = K(j+1) Q, alone, while the other wavefront of the SIMD is in its
+// softmax.  The order is written down step by step (a step is one operand from LDS, one product and a
+// share of the softmax) and fenced.  K(j+2) and V(j) go from memory to LDS during the iteration (two buffers each, one
+// barrier an iteration); the number of tiles is rounded up to an odd one, so that buffers and registers of even
+// and odd tiles have fixed places.
 template <int D, bool BF16>
 __global__ __launch_bounds__(kThreads, 2) void prompt_kernel(PromptArgs a) {
   constexpr int kRow = D / 8, kPer = kTileKeys * kRow / kThreads;   // 16-byte pieces of a row, of a thread
-  constexpr int kKMask = kRow - 1, kVMask = kRow / 2 - 1;
+  constexpr int kBuf = kTileKeys * D;                               // elements of a buffer
   constexpr uint32_t kInf = BF16 ? 0x7f80u : 0x7c00u;
-  __shared__ __align__(16) uint16_t ks[kTileKeys * D], vs[kTileKeys * D];
-  __shared__ int flag;
+  constexpr int kTiles = 5;                   // tiles that some row sees in part: 128 tokens, two ends, one of padding
+  __shared__ __align__(16) uint16_t k_even[kBuf], k_odd[kBuf], v_even[kBuf], v_odd[kBuf];
+  __shared__ int flag[kTiles];
   const int* it = a.items + kItemWords * (blockIdx.x / a.H);
   const int h = blockIdx.x % a.H;
   const int row0 = it[0], toks = it[1], key0 = it[2], keys = it[3], vis0 = it[4], vis_step = it[5];
@@ -68,155 +94,266 @@ __global__ __launch_bounds__(kThreads, 2) void prompt_kernel(PromptArgs a) {
 
   const int row = wave * 32 + col, tok = row / a.rep, hq = row % a.rep;
   const bool live = tok < toks;
-  int visible = vis0 + vis_step * tok;
-  visible = !live ? 0 : visible < keys ? visible : keys;
+  const int sees = vis0 + vis_step * tok, visible = !live ? 0 : sees < keys ? sees : keys;
   u32x4 q[D / 16];
   {
     const uint16_t* qp = a.q + (row0 + static_cast<int64_t>(live ? tok : 0)) * a.q_st + (static_cast<int64_t>(h) * a.rep + hq) * a.q_sh + 8 * g;
 #pragma unroll
     for (int i = 0; i < D / 16; ++i) {
       const uint4 x = *reinterpret_cast<const uint4*>(qp + 16 * i);
-      q[i] = live ? u32x4{x.x, x.y, x.z, x.w} : u32x4{0, 0, 0, 0};
+      q[i] = live ? u32x4{x.x, x.y, x.z, x.w} ^ a.sign : u32x4{0, 0, 0, 0};
     }
   }
-  f32x16 o[D / 32];
-#pragma unroll
-  for (int c = 0; c < D / 32; ++c)
-#pragma unroll
-    for (int e = 0; e < 16; ++e) o[c][e] = 0.0f;
-  float m = -INFINITY, l = 0.0f;
+  f32x16 o[D / 32], s[2][2];                  // s, p: of even and odd tiles
+  float m = -INFINITY, l = 0.0f, grow = 1.0f; // the exponents' reference, this lane's part of the sum, what o is to be scaled by
+  u32x4 p[2][4];
+  each<0, D / 32>([&](auto c) { each<0, 16>([&](auto e) { o[c.value][e.value] = 0.0f; }); });
 
+  // A thread's pieces of a tile: 16 bytes, the x-th of LDS, x = tid + i kThreads: row x / kRow, place x % kRow.
+  // A piece c of row r lies at place c ^ k_swz(r) or c ^ v_swz(r) of its row, so that 16 lanes of a read of K (16
+  // rows, one piece) and 32 of a read of V (4 rows, two pieces in two places) meet 256 different bytes of the banks.
+  auto k_swz = [](int r) { return D == 128 ? r & 15 : r >> 1 & 7; };
+  auto v_swz = [](int r) { return D == 128 ? (r & 3) << 2 : (r >> 1 & 1) << 2; };
+  const int xr = tid / kRow, xc = tid % kRow;
+  constexpr int kStep = kThreads / kRow;      // rows from one piece to the next: a multiple of kRow
   const uint16_t* kb = a.k + static_cast<int64_t>(key0) * a.k_st + h * a.k_sh;
   const uint16_t* vb = a.v + static_cast<int64_t>(key0) * a.v_st + h * a.v_sh;
-  uint4 kr[kPer], vr[kPer];
-  auto load = [&](int j) {                    // keys behind the last one: the last one again (masked)
+  const int k_at = (xr * static_cast<int>(a.k_st) + (xc ^ k_swz(xr)) * 8) * 2;
+  const int v_at = (xr * static_cast<int>(a.v_st) + (xc ^ v_swz(xr)) * 8) * 2;
+  const int wave0 = __builtin_amdgcn_readfirstlane(wave) * 512;     // elements
+  auto fetch = [&](uint16_t* to, const uint16_t* base, int64_t st, int at, int j) KVQ_INLINE {
+    // rows behind the last one read as zeros: the buffer ends with the last row
+    const int64_t left = keys - static_cast<int64_t>(j) * kTileKeys;
+    const int64_t bytes = left > 0 ? ((left - 1) * st + D) * 2 : 0;
+    const auto rsrc = make_rsrc(base + (left > 0 ? static_cast<int64_t>(j) * kTileKeys * st : 0),
+                                static_cast<uint32_t>(bytes < 0x7fffffff ? bytes : 0x7fffffff));
 #pragma unroll
-    for (int i = 0; i < kPer; ++i) {
-      const int p = tid + i * kThreads, c = p % kRow * 8;
-      int64_t r = j * kTileKeys + p / kRow;
-      r = r < keys ? r : keys - 1;
-      kr[i] = *reinterpret_cast<const uint4*>(kb + r * a.k_st + c);
-      vr[i] = *reinterpret_cast<const uint4*>(vb + r * a.v_st + c);
+    for (int i = 0; i < kPer; ++i)
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (lds_void*)(to + wave0 + i * kThreads * 8), 16, at + i * kStep * static_cast<int>(st) * 2, 0, 0, 0);
+  };
+  const int tiles = ((keys + kTileKeys - 1) / kTileKeys) | 1;
+  int open = vis0 < keys ? vis0 : keys;       // tiles that every row sees whole
+  open = open < 0 ? 0 : open / kTileKeys;
+
+  const int k_x = g ^ k_swz(col);             // piece 2 i + g of row 32 x + col lies at piece (2 i) ^ k_x
+  auto read_k = [&](auto par, int t) KVQ_INLINE {        // operand t of K: channels 16 (t / 2) .., rows 32 (t % 2) ..
+    return *reinterpret_cast<const u32x4*>((decltype(par)::value ? k_odd : k_even) + col * D + ((2 * (t / 2)) ^ k_x) * 8 + 32 * (t % 2) * D);
+  };
+  // 16 tokens a product; this lane's: 16 y + 4 g + e and 16 y + 8 + 4 g + e.  The transposing read of row
+  // 16 y + 8 e + 4 g + tr: channels 32 c + 16 (lane / 16 % 2) + 4 (lane % 4) .. lie at piece (4 c) ^ v_x
+  const int tr = (lane & 15) >> 2, v_x = ((lane >> 4 & 1) * 2 + (lane >> 1 & 1)) ^ v_swz(4 * g + tr);
+  auto read_v = [&](auto par, int t) KVQ_INLINE {        // operand t of V^T: tokens 16 y .., channels 32 c ..
+    const int y = t / (D / 32), c = t % (D / 32);
+    const uint16_t* base = (decltype(par)::value ? v_odd : v_even) + (4 * g + tr) * D + (lane & 1) * 4 + ((4 * c) ^ v_x) * 8 + 16 * y * D;
+    const u32x2 u = read_tr(base), w = read_tr(base + 8 * D);
+    return u32x4{u[0], u[1], w[0], w[1]};
+  };
+  // the softmax of tile j in 18 shares: 0 and 1 find the reference, 2 + i the weights 2 i, 2 i + 1.
+  // register 16 x + 4 b + e of lane half g: token 32 x + 8 b + 4 g + e
+  float top, safe, sum;
+  auto share = [&](auto par, bool masked, int j, auto which) KVQ_INLINE {
+    constexpr int i = decltype(which)::value;
+    auto& t = s[decltype(par)::value];
+    if constexpr (i < 2) {
+      if (masked) {
+        const int lim = visible - j * kTileKeys - 4 * g;
+        each<0, 16>([&](auto e) KVQ_INLINE { t[i][e.value] = 32 * i + 8 * (e.value / 4) + e.value % 4 < lim ? t[i][e.value] : -INFINITY; });
+      }
+      float x = i == 0 ? t[0][0] : fmaxf(top, t[1][0]);
+      each<1, 16>([&](auto e) KVQ_INLINE { x = fmaxf(x, t[i][e.value]); });
+      top = x;
+      if constexpr (i == 1) {
+        // the reference moves only when a score passes it by 2^8: weights up to 256 cost no accuracy, and the
+        // accumulators are hardly ever scaled
+        x = xmax32(x) * a.scale;
+        x = x > m + 8.0f ? x : m;
+        safe = x == -INFINITY ? 0.0f : x;
+        grow = __builtin_amdgcn_exp2f(m - safe);
+        m = x;
+        sum = 0.0f;
+      }
+    } else {
+      constexpr int k = 2 * (i - 2);
+      const float x = __builtin_amdgcn_exp2f(__builtin_fmaf(t[k / 16][k % 16], a.scale, -safe));
+      const float z = __builtin_amdgcn_exp2f(__builtin_fmaf(t[k / 16][k % 16 + 1], a.scale, -safe));
+      sum += x;
+      sum += z;
+      uint32_t w = pack2<BF16>(x, z);
+      asm volatile("" : "+v"(w));             // here, not behind the branch of the rescaling
+      p[decltype(par)::value][k / 8][k % 8 / 2] = w;
+      if constexpr (i == 17) {
+        l = l * grow + sum;
+        asm volatile("" : "+v"(l));
+      }
     }
   };
-  const int tiles = (keys + kTileKeys - 1) / kTileKeys;
-  // tiles that every row sees whole
-  int open = vis0 < keys ? vis0 : keys;
-  open = open < 0 ? 0 : open / kTileKeys;
-  if (tid == 0) flag = 0;
-  if (tiles > 0) load(0);
-
-  for (int j = 0; j < tiles; ++j) {
-    const bool masked = j >= open;
-    __syncthreads();
-    if (masked) {
-      // a value that is hidden from some row may be an infinity or a NaN
-      bool bad = false;
-#pragma unroll
-      for (int i = 0; i < kPer; ++i) {
-        const uint32_t w[4] = {vr[i].x, vr[i].y, vr[i].z, vr[i].w};
-#pragma unroll
-        for (int e = 0; e < 4; ++e) bad |= (w[e] & kInf) == kInf || (w[e] >> 16 & kInf) == kInf;
-      }
-      if (bad) flag = j + 1;
+  constexpr int kV = 4 * (D / 32), kK = 2 * (D / 16);               // steps of the two products
+  constexpr std::integral_constant<int, 0> even{};
+  constexpr std::integral_constant<int, 1> odd{};
+  constexpr std::false_type no{};
+  constexpr std::true_type yes{};
+  auto add_v = [&](auto par, auto t, const u32x4& w) KVQ_INLINE {   // o += V P, operand t
+    constexpr int c = decltype(t)::value % (D / 32), y = decltype(t)::value / (D / 32);
+    o[c] = mfma32<BF16>(w, p[decltype(par)::value][y], o[c]);
+  };
+  // o += V(j-1) P(j-1) (if `with`) beside the softmax of tile j
+  auto values = [&](auto par, bool masked, auto with, int j) KVQ_INLINE {
+    constexpr bool kWith = decltype(with)::value;
+    constexpr std::integral_constant<int, 1 - decltype(par)::value> other{};
+    u32x4 w[3];
+    if constexpr (kWith) {
+      w[0] = read_v(other, 0);
+      w[1] = read_v(other, 1);
     }
+    each<0, kV>([&](auto t) KVQ_INLINE {
+      if constexpr (kWith) {
+        if constexpr (t.value + 2 < kV) w[(t.value + 2) % 3] = read_v(other, t.value + 2);
+        add_v(other, t, w[t.value % 3]);
+      }
+      each<t.value * 18 / kV, (t.value + 1) * 18 / kV>([&](auto i) KVQ_INLINE { share(par, masked, j, i); });
+      __builtin_amdgcn_sched_barrier(0);
+    });
+  };
+  auto products = [&](auto par) KVQ_INLINE {  // S = K Q of the tiles of the other parity
+    constexpr int next = 1 - decltype(par)::value;
+    constexpr std::integral_constant<int, next> other{};
+    u32x4 w[4];
+    each<0, 16>([&](auto e) KVQ_INLINE { s[next][0][e.value] = s[next][1][e.value] = 0.0f; });
+    each<0, 3>([&](auto t) KVQ_INLINE { w[t.value] = read_k(other, t.value); });
+    each<0, kK>([&](auto t) KVQ_INLINE {
+      if constexpr (t.value + 3 < kK) w[(t.value + 3) % 4] = read_k(other, t.value + 3);
+      s[next][t.value % 2] = mfma32<BF16>(w[t.value % 4], q[t.value / 2], s[next][t.value % 2]);
+      __builtin_amdgcn_sched_barrier(0);
+    });
+  };
+  auto rescale = [&]() KVQ_INLINE {
+    if (__builtin_amdgcn_ballot_w64(grow != 1.0f)) each<0, D / 32>([&](auto c) KVQ_INLINE { o[c.value] *= grow; });
+  };
+  // A value that is hidden from some row may be an infinity or a NaN: in LDS it becomes a zero, and the rows that
+  // do see it get it at the end.  A thread looks at the pieces that it fetched itself.
+  auto watch = [&](uint16_t* to, int j) KVQ_INLINE {
 #pragma unroll
     for (int i = 0; i < kPer; ++i) {
-      const int p = tid + i * kThreads, r = p / kRow, c = p % kRow;
-      *reinterpret_cast<uint4*>(ks + r * D + (c ^ (r & kKMask)) * 8) = kr[i];
-      *reinterpret_cast<uint4*>(vs + r * D + (c ^ ((r & kVMask) << 1)) * 8) = vr[i];
+      u32x4* at = reinterpret_cast<u32x4*>(to + (tid + i * kThreads) * 8);
+      u32x4 w = *at;
+      bool bad = false;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const bool b0 = (w[e] & kInf) == kInf, b1 = (w[e] >> 16 & kInf) == kInf;
+        bad |= b0 || b1;
+        w[e] = (b0 ? 0u : w[e] & 0xffffu) | (b1 ? 0u : w[e] & 0xffff0000u);
+      }
+      if (bad) {
+        *at = w;
+        flag[j - open] = 1;
+      }
     }
+  };
+  auto begin = [&](auto par, int j) KVQ_INLINE {
+    fetch(decltype(par)::value ? k_odd : k_even, kb, a.k_st, k_at, j + 2);
+    fetch(decltype(par)::value ? v_odd : v_even, vb, a.v_st, v_at, j);
+    __builtin_amdgcn_sched_barrier(0);
+  };
+  auto end = [&](auto par, int j) KVQ_INLINE {
+    __builtin_amdgcn_s_waitcnt(0x0f70);       // vmcnt(0): this wavefront's pieces are in LDS
+    if (j >= open) watch(decltype(par)::value ? v_odd : v_even, j);
     __syncthreads();
-    const bool bad = masked && flag == j + 1;
-    if (j + 1 < tiles) load(j + 1);
-
-    float t[32];
-#pragma unroll
-    for (int x = 0; x < 2; ++x) {
-      f32x16 s;
-#pragma unroll
-      for (int e = 0; e < 16; ++e) s[e] = 0.0f;
-#pragma unroll
-      for (int i = 0; i < D / 16; ++i) {
-        const uint4 w = *reinterpret_cast<const uint4*>(ks + (32 * x + col) * D + ((2 * i + g) ^ (col & kKMask)) * 8);
-        s = mfma32<BF16>(u32x4{w.x, w.y, w.z, w.w}, q[i], s);
-      }
-#pragma unroll
-      for (int e = 0; e < 16; ++e) t[16 * x + e] = s[e] * a.scale;
+  };
+  auto step = [&](auto par, int j) KVQ_INLINE {
+    __builtin_amdgcn_s_setprio(1);            // the softmax goes before the other wavefront's products
+    values(par, j >= open, yes, j);
+    __builtin_amdgcn_s_setprio(0);
+    begin(par, j);                            // behind the transposing reads: the compiler has those wait for every fetch
+    products(par);
+    rescale();
+    end(par, j);
+  };
+  if (keys > 0) {
+    if (tid < kTiles) flag[tid] = 0;
+    fetch(k_even, kb, a.k_st, k_at, 0);
+    fetch(k_odd, kb, a.k_st, k_at, 1);
+    __builtin_amdgcn_s_waitcnt(0x0f70);
+    __syncthreads();
+    products(odd);
+    __syncthreads();                          // K(2) takes the place of K(0)
+    begin(even, 0);
+    values(even, open == 0, no, 0);
+    products(even);
+    end(even, 0);
+    for (int j = 1; j < tiles; j += 2) {
+      step(odd, j);
+      step(even, j + 1);
     }
-    // register 16 x + 4 b + e of lane half g: token 32 x + 8 b + 4 g + e
-    if (masked) {
-      const int lim = visible - j * kTileKeys - 4 * g;
-#pragma unroll
-      for (int i = 0; i < 32; ++i) t[i] = 32 * (i / 16) + 8 * (i / 4 % 4) + i % 4 < lim ? t[i] : -INFINITY;
-    }
-    float top = t[0];
-#pragma unroll
-    for (int i = 1; i < 32; ++i) top = fmaxf(top, t[i]);
-    top = fmaxf(m, xmax32(top));
-    const float safe = top == -INFINITY ? 0.0f : top, old = __builtin_amdgcn_exp2f(m - safe);
-    float sum = 0.0f;
-#pragma unroll
-    for (int i = 0; i < 32; ++i) {
-      t[i] = __builtin_amdgcn_exp2f(t[i] - safe);
-      sum += t[i];
-    }
-    l = l * old + sum;
-    m = top;
-    if (__builtin_amdgcn_ballot_w64(old != 1.0f)) {
-#pragma unroll
-      for (int c = 0; c < D / 32; ++c) o[c] *= old;
-    }
-    // 16 tokens a product; this lane's: 16 y + 4 g + e and 16 y + 8 + 4 g + e
-    const int tr = (lane & 15) >> 2, tc = (lane >> 4 & 1) * 16 + (lane & 3) * 4;
-#pragma unroll
-    for (int y = 0; y < 4; ++y) {
-      u32x4 p;
-#pragma unroll
-      for (int e = 0; e < 4; ++e) p[e] = pack2<BF16>(t[8 * y + 2 * e], t[8 * y + 2 * e + 1]);
-#pragma unroll
-      for (int c = 0; c < D / 32; ++c) {
-        u32x4 w;
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          const int r = 16 * y + 8 * e + 4 * g + tr, ch = 32 * c + tc;
-          const u32x2 z = read_tr(vs + r * D + ((ch / 8) ^ ((r & kVMask) << 1)) * 8 + ch % 8);
-          w[2 * e] = z[0];
-          w[2 * e + 1] = z[1];
-        }
-        if (bad) {
-#pragma unroll
-          for (int e = 0; e < 4; ++e)
-            w[e] = ((w[e] & kInf) == kInf ? 0u : w[e] & 0xffffu) | ((w[e] >> 16 & kInf) == kInf ? 0u : w[e] & 0xffff0000u);
-        }
-        o[c] = mfma32<BF16>(w, p, o[c]);
-      }
-    }
-    if (bad) {                                // the rows that do see such a value get it
-      for (int r = 0; r < kTileKeys; ++r) {
-        const bool sees = j * kTileKeys + r < visible;
-#pragma unroll
-        for (int c = 0; c < D / 32; ++c)
-#pragma unroll
-          for (int e = 0; e < 16; ++e) {
-            const int ch = 32 * c + 8 * (e / 4) + 4 * g + e % 4;
-            const uint16_t x = vs[r * D + ((ch / 8) ^ ((r & kVMask) << 1)) * 8 + ch % 8];
-            if (sees && (x & kInf) == kInf) o[c][e] += BF16 ? bf16_to_f32(x) : f16_to_f32(x);
-          }
-      }
-    }
+    each<0, kV>([&](auto t) KVQ_INLINE { add_v(even, t, read_v(even, t.value)); });
+    for (int j = open; j < tiles; ++j)
+      if (flag[j - open])
+        for (int r = j * kTileKeys; r < j * kTileKeys + kTileKeys && r < keys; ++r)
+          each<0, D / 32>([&](auto c) KVQ_INLINE {
+            each<0, 16>([&](auto e) KVQ_INLINE {
+              const uint16_t x = vb[r * a.v_st + 32 * c.value + 8 * (e.value / 4) + 4 * g + e.value % 4];
+              if (r < visible && (x & kInf) == kInf) o[c.value][e.value] += BF16 ? bf16_to_f32(x) : f16_to_f32(x);
+            });
+          });
   }
 
   if (!live) return;
   l = xsum32(l);
+  const int piece = it[6];
+  if (piece >= 0) {
+    float* part = a.part + (static_cast<int64_t>(piece) * a.H + h) * (kTileRows * (D + 2));
+    each<0, D / 32>([&](auto c) KVQ_INLINE {
+      each<0, 4>([&](auto e) KVQ_INLINE {
+        const auto& x = o[c.value];
+        *reinterpret_cast<float4*>(part + row * D + 32 * c.value + 8 * e.value + 4 * g) =
+            make_float4(x[4 * e.value], x[4 * e.value + 1], x[4 * e.value + 2], x[4 * e.value + 3]);
+      });
+    });
+    if (g == 0) *reinterpret_cast<float2*>(part + kTileRows * D + 2 * row) = make_float2(m, l);
+    return;
+  }
   const float inv = visible > 0 ? 1.0f / l : 0.0f;                  // a row without a visible key: zeros
   uint16_t* out = a.out + ((row0 + static_cast<int64_t>(tok)) * a.H * a.rep + h * a.rep + hq) * D + 4 * g;
+  each<0, D / 32>([&](auto c) KVQ_INLINE {
+    each<0, 4>([&](auto e) KVQ_INLINE {
+      const auto& x = o[c.value];
+      *reinterpret_cast<uint2*>(out + 32 * c.value + 8 * e.value) =
+          make_uint2(pack2<BF16>(x[4 * e.value] * inv, x[4 * e.value + 1] * inv), pack2<BF16>(x[4 * e.value + 2] * inv, x[4 * e.value + 3] * inv));
+    });
+  });
+}
+
+// One wavefront per row of a tile that was cut: merges[i] = {first part, parts, first row, tokens}.
+template <int D, bool BF16>
+__global__ __launch_bounds__(kThreads) void prompt_merge_kernel(PromptArgs a, const int* __restrict__ merges) {
+  const int* w = merges + 4 * (blockIdx.x / a.H);
+  const int h = blockIdx.x % a.H, lane = threadIdx.x & 63, row = blockIdx.y * (kThreads / 64) + (threadIdx.x >> 6);
+  const int tok = row / a.rep, parts = w[1];
+  if (tok >= w[3]) return;
+  constexpr int64_t kPart = kTileRows * (D + 2);
+  const int64_t stride = a.H * kPart;
+  const float* part = a.part + (static_cast<int64_t>(w[0]) * a.H + h) * kPart;
+  float top = -INFINITY, l = 0.0f, o[D / 64] = {};
+  for (int i0 = 0; i0 < parts; i0 += 64) {
+    const int i = i0 + lane;
+    const float2 st = i < parts ? *reinterpret_cast<const float2*>(part + i * stride + kTileRows * D + 2 * row) : make_float2(-INFINITY, 0.0f);
+    const float m = fmaxf(top, wave_max(st.x)), safe = m == -INFINITY ? 0.0f : m;
+    const float old = __builtin_amdgcn_exp2f(top - safe), f = __builtin_amdgcn_exp2f(st.x - safe);
+    l = l * old + wave_sum(f * st.y);
 #pragma unroll
-  for (int c = 0; c < D / 32; ++c)
+    for (int e = 0; e < D / 64; ++e) o[e] *= old;
+    const int most = parts - i0 < 64 ? parts - i0 : 64;
+    for (int k = 0; k < most; ++k) {
+      const float fk = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(f), k));
+      const float* x = part + (i0 + k) * stride + row * D + lane * (D / 64);
 #pragma unroll
-    for (int e = 0; e < 4; ++e)
-      *reinterpret_cast<uint2*>(out + 32 * c + 8 * e) = make_uint2(pack2<BF16>(o[c][4 * e] * inv, o[c][4 * e + 1] * inv),
-                                                                   pack2<BF16>(o[c][4 * e + 2] * inv, o[c][4 * e + 3] * inv));
+      for (int e = 0; e < D / 64; ++e) o[e] += fk * x[e];
+    }
+    top = m;
+  }
+  const float inv = top == -INFINITY && l == 0.0f ? 0.0f : 1.0f / l;
+  uint16_t* out = a.out + ((w[2] + static_cast<int64_t>(tok)) * a.H * a.rep + h * a.rep + row % a.rep) * D + lane * (D / 64);
+#pragma unroll
+  for (int e = 0; e < D / 64; ++e) out[e] = BF16 ? f32_to_bf16(o[e] * inv) : f32_to_f16(o[e] * inv);
 }
 
 struct Item {
@@ -228,54 +365,109 @@ struct Item {
 
 using namespace kvq;
 
-extern "C" int64_t kvq_prompt_plan(const int64_t* lens_q, const int64_t* lens_k, int64_t n, int64_t rep, int causal, int32_t* items,
-                                   int64_t items_cap) {
-  if (n < 0 || (n && (!lens_q || !lens_k)) || rep < 1 || rep > kTileRows) return -1;
-  const int64_t per = kTileRows / rep;        // tokens of a tile
-  int64_t total = 0, row = 0, key = 0;
-  Item* out = reinterpret_cast<Item*>(items);
+extern "C" int kvq_prompt_plan(const int64_t* lens_q, const int64_t* lens_k, int64_t n, int64_t rep, int64_t H, int causal, int32_t* words,
+                               int64_t words_cap, int64_t* info) {
+  KVQ_REQUIRE(info && n >= 0 && (n == 0 || (lens_q && lens_k)), "kvq_prompt_plan: null pointer");
+  KVQ_REQUIRE(rep >= 1 && rep <= kTileRows && H >= 1, "kvq_prompt_plan: bad head counts");
+  const int64_t per_tile = kTileRows / rep;   // tokens of a tile of rows
+  int64_t rows = 0, keys_all = 0, tiles = 0, work = 0;
+  auto keys_of = [&](int64_t i, int64_t t) {  // keys that the tile from token t of sequence i sees
+    if (!causal) return lens_k[i];
+    const int64_t end = t + per_tile < lens_q[i] ? t + per_tile : lens_q[i], k = lens_k[i] - lens_q[i] + end;
+    return k < 0 ? INT64_C(0) : k;
+  };
   for (int64_t i = 0; i < n; ++i) {
-    const int64_t lq = lens_q[i], lk = lens_k[i];
-    if (lq < 0 || lk < 0 || lq >= INT64_C(1) << 31 || lk >= INT64_C(1) << 31) return -1;
-    for (int64_t t = 0; t < lq; t += per, ++total) {
-      if (!items || total >= items_cap) continue;
-      const int64_t toks = lq - t < per ? lq - t : per, vis0 = causal ? lk - lq + t + 1 : lk;
-      int64_t keys = causal ? vis0 + toks - 1 : lk;
-      keys = keys < 0 ? 0 : keys;
-      out[total] = {static_cast<int32_t>(row + t), static_cast<int32_t>(toks), static_cast<int32_t>(key), static_cast<int32_t>(keys),
-                    static_cast<int32_t>(vis0), causal ? 1 : 0, 0, 0};
+    KVQ_REQUIRE(lens_q[i] >= 0 && lens_k[i] >= 0, "kvq_prompt_plan: lengths must not be negative");
+    rows += lens_q[i];
+    keys_all += lens_k[i];
+    KVQ_REQUIRE(rows < INT64_C(1) << 31 && keys_all < INT64_C(1) << 31, "kvq_prompt_plan: too many rows");
+    for (int64_t t = 0; t < lens_q[i]; t += per_tile, ++tiles) work += (keys_of(i, t) + kTileKeys - 1) / kTileKeys;
+  }
+  // Parts of a tile: no longer than an even share of the work over kSlots workgroups (two on each of 256 CUs), which
+  // is nothing where the tiles fill the chip; 8 key tiles at least, which pay for the part's sums (64 KB).
+  const int64_t even = (work * H + kSlots - 1) / kSlots, most = even > 8 ? even : 8;
+  int64_t items = 0, merges = 0, parts = 0;
+  Item* out = reinterpret_cast<Item*>(words);
+  for (int pass = 0; pass < 2; ++pass) {
+    int64_t row = 0, key = 0, item = 0, part = 0, merge = 0;
+    for (int64_t i = 0; i < n; ++i) {
+      for (int64_t t = 0; t < lens_q[i]; t += per_tile) {
+        const int64_t toks = lens_q[i] - t < per_tile ? lens_q[i] - t : per_tile, keys = keys_of(i, t);
+        const int64_t vis0 = causal ? lens_k[i] - lens_q[i] + t + 1 : keys, steps = (keys + kTileKeys - 1) / kTileKeys;
+        const int64_t cut = (steps + most - 1) / most, count = cut > 1 ? cut : 1;
+        if (pass == 1 && count > 1) {
+          int32_t* w = words + kItemWords * items + 4 * merge;
+          w[0] = static_cast<int32_t>(part);
+          w[1] = static_cast<int32_t>(count);
+          w[2] = static_cast<int32_t>(row + t);
+          w[3] = static_cast<int32_t>(toks);
+        }
+        for (int64_t c = 0; c < count; ++c, ++item) {
+          const int64_t first = steps * c / count * kTileKeys, last = steps * (c + 1) / count * kTileKeys;
+          if (pass == 1)
+            out[item] = {{static_cast<int32_t>(row + t), static_cast<int32_t>(toks), static_cast<int32_t>(key + first),
+                          static_cast<int32_t>((last < keys ? last : keys) - first), static_cast<int32_t>(vis0 - first), causal ? 1 : 0,
+                          count > 1 ? static_cast<int32_t>(part + c) : -1, 0}};
+        }
+        if (count > 1) {
+          part += count;
+          ++merge;
+        }
+      }
+      row += lens_q[i];
+      key += lens_k[i];
     }
-    row += lq;
-    key += lk;
-    if (row >= INT64_C(1) << 31 || key >= INT64_C(1) << 31) return -1;
+    items = item;
+    merges = merge;
+    parts = part;
+    info[0] = items;
+    info[1] = merges;
+    info[2] = parts;
+    if (!words || words_cap < kItemWords * items + 4 * merges) return KVQ_OK;
   }
   // the longest first: the last workgroups to end are short ones
-  if (items && total <= items_cap)
-    std::sort(out, out + total, [](const Item& x, const Item& y) { return x.w[3] != y.w[3] ? x.w[3] > y.w[3] : x.w[0] < y.w[0]; });
-  return total;
+  std::sort(out, out + items, [](const Item& x, const Item& y) { return x.w[3] != y.w[3] ? x.w[3] > y.w[3] : x.w[2] + x.w[0] < y.w[2] + y.w[0]; });
+  return KVQ_OK;
+}
+
+extern "C" int64_t kvq_prompt_workspace(int64_t parts, int64_t H, int64_t D) {
+  return parts < 0 || H < 1 || (D != 64 && D != 128) ? -1 : parts * H * kTileRows * (D + 2);
 }
 
 extern "C" int kvq_prompt_attention(const void* q, int64_t q_st, int64_t q_sh, const void* k, int64_t k_st, int64_t k_sh, const void* v,
                                     int64_t v_st, int64_t v_sh, int dtype, int64_t Hq, int64_t H, int64_t D, float scaling,
-                                    const int32_t* items, int64_t n_items, void* out, void* stream) {
+                                    const int32_t* words, int64_t items, int64_t merges, int64_t parts, void* out, float* workspace,
+                                    int64_t workspace_floats, void* stream) {
   KVQ_REQUIRE(D == 64 || D == 128, "kvq_prompt_attention: head_dim must be 64 or 128 (got %lld)", static_cast<long long>(D));
   KVQ_REQUIRE(dtype == KVQ_F16 || dtype == KVQ_BF16, "kvq_prompt_attention: rows must be fp16 or bf16");
-  KVQ_REQUIRE(H > 0 && Hq > 0 && Hq % H == 0 && Hq / H <= kTileRows && n_items >= 0, "kvq_prompt_attention: bad sizes");
-  if (n_items == 0) return KVQ_OK;
-  KVQ_REQUIRE(q && k && v && items && out, "kvq_prompt_attention: null pointer");
+  KVQ_REQUIRE(H > 0 && Hq > 0 && Hq % H == 0 && Hq / H <= kTileRows && items >= 0 && merges >= 0 && parts >= 0, "kvq_prompt_attention: bad sizes");
+  if (items == 0) return KVQ_OK;
+  KVQ_REQUIRE(q && k && v && words && out, "kvq_prompt_attention: null pointer");
   KVQ_REQUIRE((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v) |
-               reinterpret_cast<uintptr_t>(out)) % 16 == 0 && (q_st | q_sh | k_st | k_sh | v_st | v_sh) % 8 == 0,
+               reinterpret_cast<uintptr_t>(out) | reinterpret_cast<uintptr_t>(workspace)) % 16 == 0 && (q_st | q_sh | k_st | k_sh | v_st | v_sh) % 8 == 0,
               "kvq_prompt_attention: rows and strides must be multiples of 16 bytes");
-  KVQ_REQUIRE(n_items * H < INT64_C(1) << 31, "kvq_prompt_attention: too many rows");
+  KVQ_REQUIRE(items * H < INT64_C(1) << 31, "kvq_prompt_attention: too many rows");
+  KVQ_REQUIRE(k_st >= 0 && v_st >= 0 && k_st < (1 << 24) && v_st < (1 << 24), "kvq_prompt_attention: row strides must be below 2^24 elements");
+  KVQ_REQUIRE(parts == 0 || (workspace && workspace_floats >= kvq_prompt_workspace(parts, H, D)),
+              "kvq_prompt_attention: workspace of %lld floats, %lld needed", static_cast<long long>(workspace_floats),
+              static_cast<long long>(kvq_prompt_workspace(parts, H, D)));
   const PromptArgs a{static_cast<const uint16_t*>(q), static_cast<const uint16_t*>(k), static_cast<const uint16_t*>(v),
-                     q_st, q_sh, k_st, k_sh, v_st, v_sh, items, static_cast<int>(H), static_cast<int>(Hq / H),
-                     scaling * 1.44269504088896341f, static_cast<uint16_t*>(out)};
-  const dim3 grid(static_cast<uint32_t>(n_items * H));
+                     q_st, q_sh, k_st, k_sh, v_st, v_sh, words, static_cast<int>(H), static_cast<int>(Hq / H),
+                     std::fabs(scaling) * 1.44269504088896341f, std::signbit(scaling) ? 0x80008000u : 0u,
+                     static_cast<uint16_t*>(out), workspace};
+  const dim3 grid(static_cast<uint32_t>(items * H)), joins(static_cast<uint32_t>(merges * H), kTileRows * 64 / kThreads);
   hipStream_t s = static_cast<hipStream_t>(stream);
-  if (D == 128 && dtype == KVQ_BF16) hipLaunchKernelGGL((prompt_kernel<128, true>), grid, dim3(kThreads), 0, s, a);
-  else if (D == 128) hipLaunchKernelGGL((prompt_kernel<128, false>), grid, dim3(kThreads), 0, s, a);
-  else if (dtype == KVQ_BF16) hipLaunchKernelGGL((prompt_kernel<64, true>), grid, dim3(kThreads), 0, s, a);
-  else hipLaunchKernelGGL((prompt_kernel<64, false>), grid, dim3(kThreads), 0, s, a);
+  auto run = [&](auto d, auto t) {
+    hipLaunchKernelGGL((prompt_kernel<decltype(d)::value, decltype(t)::value>), grid, dim3(kThreads), 0, s, a);
+    if (merges)
+      hipLaunchKernelGGL((prompt_merge_kernel<decltype(d)::value, decltype(t)::value>), joins, dim3(kThreads), 0, s, a, words + kItemWords * items);
+  };
+  auto by_type = [&](auto d) {
+    if (dtype == KVQ_BF16) run(d, std::true_type{});
+    else run(d, std::false_type{});
+  };
+  if (D == 64) by_type(std::integral_constant<int, 64>{});
+  else by_type(std::integral_constant<int, 128>{});
   KVQ_LAUNCH_CHECK("kvq_prompt_attention");
   return KVQ_OK;
 }

@@ -103,8 +103,10 @@ SIGNATURES = {
     "kvq_quasar_decode": (i32, [vp, i32, i64, i64, i64, i64, i64, i64, f32, vp, vp, i64, i64, vp, vp,
                                 vp, i64, vp, i64, vp, i32, i32, vp, i32, vp, vp, i64, vp, vp, i64, i64, vp, vp,
                                 vp, i32, vp, vp, i64, i32, vp]),
-    "kvq_prompt_plan": (i64, [vp, vp, i64, i64, i32, vp, i64]),
-    "kvq_prompt_attention": (i32, [vp, i64, i64, vp, i64, i64, vp, i64, i64, i32, i64, i64, i64, f32, vp, i64, vp, vp]),
+    "kvq_prompt_plan": (i32, [vp, vp, i64, i64, i64, i32, vp, i64, vp]),
+    "kvq_prompt_workspace": (i64, [i64, i64, i64]),
+    "kvq_prompt_attention": (i32, [vp, i64, i64, vp, i64, i64, vp, i64, i64, i32, i64, i64, i64, f32, vp, i64, i64, i64, vp, vp,
+                                   i64, vp]),
     "kvq_pages_step_words": (i64, [i64, vp, i64]),
     "kvq_pages_extend": (i32, [vp, vp, vp, vp, vp, i64, i64, i64, i64, i64, vp, vp, i64, i64, vp, i64, vp, vp]),
     "kvq_pages_whole": (i32, [vp, vp, i64, i64, vp, i64, vp, i64, vp, vp]),

@@ -15,7 +15,6 @@ import torch
 from . import _lib
 
 MAX_REP = 128                                  # query heads per KV head of a kernel tile
-_WORDS = 8
 
 
 def device_of(device) -> torch.device:
@@ -46,20 +45,22 @@ class PromptPlan:
         self.Hq, self.Hkv, self.causal = int(Hq), int(Hkv), bool(causal)
         self.rows, self.keys = int(lq.sum()), int(lk.sum())
         self.device = device_of(device)
-        rep = self.Hq // self.Hkv
-        lib = _lib.load()
-        args = (lq.ctypes.data, lk.ctypes.data, len(lq), rep, int(self.causal))
-        n = lib.kvq_prompt_plan(*args, None, 0)
-        items = np.empty((max(n, 1), _WORDS), dtype=np.int32)
-        if n < 0 or lib.kvq_prompt_plan(*args, items.ctypes.data, n) != n:
-            raise _lib.KVQError("kvq_prompt_plan rejected the lengths")
-        self.n_items = int(n)
-        self.items = torch.from_numpy(items).to(self.device)
+        info = np.zeros(3, dtype=np.int64)
+        args = (lq.ctypes.data, lk.ctypes.data, len(lq), self.Hq // self.Hkv, self.Hkv, int(self.causal))
+        _lib.call("kvq_prompt_plan", *args, None, 0, info.ctypes.data)
+        words = np.empty(max(8 * info[0] + 4 * info[1], 1), dtype=np.int32)
+        _lib.call("kvq_prompt_plan", *args, words.ctypes.data, words.size, info.ctypes.data)
+        self.items, self.merges, self.parts = info.tolist()
+        self.words = torch.from_numpy(words).to(self.device)
+
+    def workspace_floats(self, d: int) -> int:
+        """Float32 scratch of a call at head_dim ``d``: none where the rows fill the chip without cutting along the keys."""
+        return _lib.load().kvq_prompt_workspace(self.parts, self.Hkv, d)
 
 
 @torch.no_grad()
 def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, scaling: float, plan: PromptPlan, *,
-                     out: Optional[torch.Tensor] = None) -> torch.Tensor:
+                     out: Optional[torch.Tensor] = None, workspace: Optional[torch.Tensor] = None) -> torch.Tensor:
     """Attention of the packed rows q (rows, Hq, d) over k, v (keys, Hkv, d), bf16 or fp16 of one type, head_dim 64
     or 128, any row and head strides of whole 16 bytes (others are copied); returns (rows, Hq, d)."""
     _lib.require_gpu(q, k, v)
@@ -80,14 +81,21 @@ def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, scaling:
     out = _lib.out_or_new(out, (plan.rows, plan.Hq, d), q.dtype, q.device, "prompt_attention")
     if plan.keys == 0:
         return out.zero_()
+    if workspace is None:
+        if plan.parts:
+            workspace = torch.empty((plan.workspace_floats(d),), dtype=torch.float32, device=q.device)
+    elif workspace.dtype != torch.float32 or not workspace.is_contiguous() or workspace.device != q.device:
+        raise ValueError("workspace must be contiguous float32 on the plan's device")
+    ws, floats = (None, 0) if workspace is None else (workspace.data_ptr(), workspace.numel())
     _lib.call_on(q.device, "kvq_prompt_attention", q.data_ptr(), q.stride(0), q.stride(1), k.data_ptr(), k.stride(0), k.stride(1),
                  v.data_ptr(), v.stride(0), v.stride(1), _lib.DTYPE_CODE[q.dtype], plan.Hq, plan.Hkv, d, float(scaling),
-                 plan.items.data_ptr(), plan.n_items, out.data_ptr(), _lib.stream_of(q))
+                 plan.words.data_ptr(), plan.items, plan.merges, plan.parts, out.data_ptr(), ws, floats, _lib.stream_of(q))
     return out
 
 
 def rows16(x: torch.Tensor) -> torch.Tensor:
     """x (rows, heads, d) itself when the kernels can read it in 16-byte pieces, or a copy."""
-    if x.stride(2) != 1 or (x.stride(0) | x.stride(1)) % 8 or x.data_ptr() % 16:
+    st, sh, sd = x.stride()
+    if sd != 1 or (st | sh) % 8 or x.data_ptr() % 16 or not 0 <= st < 1 << 24:
         return x.clone(memory_format=torch.contiguous_format)
     return x

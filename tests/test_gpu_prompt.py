@@ -40,6 +40,8 @@ SHAPES = [
     ([0, 0], [0, 7], 4, 2, 64, True),
     ([2], [300], 128, 1, 64, True),                          # a tile per token
     ([150], [150], 3, 1, 64, False),
+    ([3, 1, 40], [5000, 700, 1300], 4, 1, 128, True),        # few rows: cut along the keys
+    ([1, 2], [6000, 513], 2, 2, 64, False),
 ]
 
 
@@ -97,6 +99,17 @@ def test_values_that_a_row_does_not_see(bad, dtype):
     q, k, v = _inputs(lens, lens, Hq, Hkv, d, dtype, 21)
     plan = kvq.PromptPlan(lens, Hq, Hkv)
     clean = kvq.prompt_attention(q.cuda(), k.cuda(), v.cuda(), d ** -0.5, plan)
+    # the same behind a past that is cut into parts
+    past = [torch.cat([x[:0], torch.randn(3000, Hkv, d).to(dtype), x[:90]]) for x in (k, v)]
+    late = kvq.PromptPlan([90], Hq, Hkv, lens_k=[3090])
+    assert late.parts
+    for s in (0, 1):
+        dirty = [x.clone() for x in past]
+        before = kvq.prompt_attention(q[:90].cuda(), past[0].cuda(), past[1].cuda(), d ** -0.5, late)
+        dirty[s][3000 + at] = bad
+        after = kvq.prompt_attention(q[:90].cuda(), dirty[0].cuda(), dirty[1].cuda(), d ** -0.5, late)
+        assert torch.equal(after[:at], before[:at])
+        assert s == 0 or not torch.isfinite(after[at:].float()).any()
     kb, vb = k.clone(), v.clone()
     kb[at + 5], vb[at, :, 3] = bad, bad
     got = kvq.prompt_attention(q.cuda(), kb.cuda(), vb.cuda(), d ** -0.5, plan)
@@ -137,12 +150,21 @@ def test_replays_and_another_stream():
     gr = torch.cuda.CUDAGraph()
     with torch.cuda.graph(gr):
         kvq.prompt_attention(q, k, v, d ** -0.5, plan, out=out)
+    few = kvq.PromptPlan([2, 3], Hq, Hkv, lens_k=[4000, 900])      # cut along the keys: with scratch of its own
+    assert few.parts
+    k2, v2 = (torch.randn((4900, Hkv, d), dtype=torch.bfloat16, device="cuda") for _ in (0, 1))
+    ws, out2 = torch.empty(few.workspace_floats(d), device="cuda"), torch.empty_like(q[:5])
+    gr2 = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(gr2):
+        kvq.prompt_attention(q[:5], k2, v2, d ** -0.5, few, out=out2, workspace=ws)
     for i in range(3):
         q.copy_(torch.randn_like(q))
         _ = (q.float() * 2).sum()
         torch.cuda.synchronize()
         gr.replay()
+        gr2.replay()
         torch.cuda.synchronize()
+        assert torch.equal(out2, kvq.prompt_attention(q[:5], k2, v2, d ** -0.5, few)), i
         assert torch.equal(out, kvq.prompt_attention(q, k, v, d ** -0.5, plan)), i
 
 

@@ -122,44 +122,75 @@ def test_refusals_change_nothing():
         assert np.array_equal(a, b)
 
 
-def test_prompt_plan_covers_every_row_once():
+def _plan(lib, lq, lk, rep, H, causal):
+    lq, lk, info = np.array(lq, np.int64), np.array(lk, np.int64), np.zeros(3, np.int64)
+    args = (lq.ctypes.data, lk.ctypes.data, len(lq), rep, H, causal)
+    rc = lib.kvq_prompt_plan(*args, None, 0, info.ctypes.data)
+    if rc:
+        return rc, None, None
+    words = np.zeros(max(8 * info[0] + 4 * info[1], 1), np.int32)
+    assert lib.kvq_prompt_plan(*args, words.ctypes.data, words.size, info.ctypes.data) == 0
+    return info, words[:8 * info[0]].reshape(-1, 8), words[8 * info[0]:8 * info[0] + 4 * info[1]].reshape(-1, 4)
+
+
+def test_prompt_plan_covers_every_key_of_every_row_once():
+    """Tiles of rows, cut along the keys where they are few: each visible (row, key) pair in one item, the parts of a
+    tile joined by one merge."""
     from kvq import _lib
     lib = _lib.load()
     rng = random.Random(3)
-    for _ in range(60):
-        n, rep, causal = rng.randint(1, 6), rng.choice([1, 2, 3, 4, 7, 8, 128]), rng.choice([0, 1])
-        lq = np.array([rng.choice([0, 1, 31, 32, rng.randint(0, 300)]) for _ in range(n)], np.int64)
-        lk = np.array([max(0, int(a) + rng.choice([0, 0, 50, -3])) for a in lq], np.int64)
-        count = lib.kvq_prompt_plan(lq.ctypes.data, lk.ctypes.data, n, rep, causal, None, 0)
-        items = np.zeros((max(count, 1), 8), np.int32)
-        assert lib.kvq_prompt_plan(lq.ctypes.data, lk.ctypes.data, n, rep, causal, items.ctypes.data, count) == count
-        seen = np.zeros(int(lq.sum()), np.int64)
+    cut = 0
+    for _ in range(80):
+        n, rep, causal, H = rng.randint(1, 6), rng.choice([1, 2, 3, 4, 7, 8, 128]), rng.choice([0, 1]), rng.choice([1, 2, 8])
+        lq = [rng.choice([0, 1, 31, 32, rng.randint(0, 300)]) for _ in range(n)]
+        lk = [max(0, a + rng.choice([0, 0, 50, -3, rng.randint(0, 9000)])) for a in lq]
+        info, items, merges = _plan(lib, lq, lk, rep, H, causal)
         rows, keys = np.concatenate([[0], np.cumsum(lq)]), np.concatenate([[0], np.cumsum(lk)])
-        for row, toks, key, nk, vis0, step, *_ in items[:count].tolist():
-            seen[row:row + toks] += 1
-            assert 0 < toks * rep <= 128
+        pairs = [np.zeros((a, b), np.int32) for a, b in zip(lq, lk)]
+        parts = {}
+        done = np.zeros(int(rows[-1]), np.int32)
+        for row, toks, key, nk, vis0, step, part, _ in items.tolist():
             s = int(np.searchsorted(rows, row, "right") - 1)
-            assert row + toks <= rows[s + 1] and key == keys[s] and 0 <= nk <= lk[s]
             t = row - rows[s]
-            assert (vis0, step) == ((lk[s] - lq[s] + t + 1, 1) if causal else (lk[s], 0))
-            assert nk == (max(0, vis0 + toks - 1) if causal else lk[s])
-        assert (seen == 1).all()
-    bad = np.array([-1], np.int64)
-    assert lib.kvq_prompt_plan(bad.ctypes.data, bad.ctypes.data, 1, 1, 1, None, 0) == -1
-    one = np.array([1], np.int64)
-    assert lib.kvq_prompt_plan(one.ctypes.data, one.ctypes.data, 1, 129, 1, None, 0) == -1
+            assert 0 < toks * rep <= 128 and row + toks <= rows[s + 1] and nk >= 0 and step == causal
+            first = key - keys[s]
+            assert 0 <= first and first + nk <= lk[s]
+            for i in range(toks):
+                sees = max(0, min(nk, vis0 + step * i))
+                pairs[s][t + i, first:first + sees] += 1
+            if part < 0:
+                done[row:row + toks] += 1
+            else:
+                parts[part] = (row, toks)
+        for part, count, row, toks in merges.tolist():
+            assert count > 1 and all(parts.pop(part + i) == (row, toks) for i in range(count))
+            done[row:row + toks] += 1
+            cut += 1
+        assert not parts and (done == 1).all()
+        assert info[2] == sum(m[1] for m in merges)
+        for a, b, x in zip(lq, lk, pairs):
+            t, j = np.arange(a)[:, None], np.arange(b)[None]
+            assert np.array_equal(x, (j <= t + b - a).astype(np.int32) if causal else np.ones_like(x))
+    assert cut > 20
+    assert _plan(lib, [-1], [1], 1, 1, 1)[0] == 1 and _plan(lib, [1], [-1], 1, 1, 1)[0] == 1
+    assert _plan(lib, [1], [1], 129, 1, 1)[0] == 1 and _plan(lib, [1 << 30] * 2, [1, 1], 1, 1, 1)[0] == 1
 
 
 def test_kernel_entries_refuse_before_any_launch():
     from kvq import _lib
     lib = _lib.load()
     one = ctypes.c_void_p(16)
-    rc = lib.kvq_prompt_attention(one, 64, 64, one, 64, 64, one, 64, 64, 2, 4, 2, 96, 0.1, one, 1, one, None)
+    rc = lib.kvq_prompt_attention(one, 64, 64, one, 64, 64, one, 64, 64, 2, 4, 2, 96, 0.1, one, 1, 0, 0, one, None, 0, None)
     assert rc == 1 and b"head_dim" in lib.kvq_last_error()
-    rc = lib.kvq_prompt_attention(one, 64, 64, one, 64, 64, one, 64, 64, 0, 4, 2, 64, 0.1, one, 1, one, None)
+    rc = lib.kvq_prompt_attention(one, 64, 64, one, 64, 64, one, 64, 64, 0, 4, 2, 64, 0.1, one, 1, 0, 0, one, None, 0, None)
     assert rc == 1 and b"fp16 or bf16" in lib.kvq_last_error()
-    rc = lib.kvq_prompt_attention(one, 64, 60, one, 64, 64, one, 64, 64, 2, 4, 2, 64, 0.1, one, 1, one, None)
+    rc = lib.kvq_prompt_attention(one, 64, 60, one, 64, 64, one, 64, 64, 2, 4, 2, 64, 0.1, one, 1, 0, 0, one, None, 0, None)
     assert rc == 1 and b"16 bytes" in lib.kvq_last_error()
+    assert lib.kvq_prompt_workspace(3, 2, 64) == 3 * 2 * 128 * 66
+    rc = lib.kvq_prompt_attention(one, 64, 64, one, 64, 64, one, 64, 64, 2, 4, 2, 64, 0.1, one, 3, 1, 3, one, one, 3 * 2 * 128 * 66 - 1, None)
+    assert rc == 1 and b"workspace" in lib.kvq_last_error()
+    rc = lib.kvq_prompt_attention(one, 64, 64, one, 1 << 24, 64, one, 64, 64, 2, 4, 2, 64, 0.1, one, 1, 0, 0, one, None, 0, None)
+    assert rc == 1 and b"2^24" in lib.kvq_last_error()
     rc = lib.kvq_pages_append(one, 64, 64, one, 64, 64, 2, one, 1, one, 4, 2, 64, 48, 0, one, one, one, one, one, None)
     assert rc == 1 and b"page" in lib.kvq_last_error()
     rc = lib.kvq_pages_append(one, 64, 64, one, 64, 64, 2, one, 1, one, 4, 2, 64, 64, 3, one, one, one, one, one, None)
