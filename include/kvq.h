@@ -694,9 +694,9 @@ int kvq_prompt_attention(const void* q, int64_t q_st, int64_t q_sh, const void* 
  * full, in order; refused whole ("decode buffer exhausted") when a slot's max_tokens or the free pages do
  * not suffice.  It writes the step's description to `desc` (host, kvq_pages_step_words words) and, by
  * value with launches on `stream`, to desc_device (NULL: host only).  split_cap >= n bounds the decode's split items.
- * kvq_pages_whole describes whole sequences (for kvq_pages_rows; no page list).
  * kvq_pages_append writes one layer's rows k, v (rows, H, D) of the step; running it again writes the same.
- * kvq_pages_rows reads sequences back as dense rows (sum lens, H, D).  items: the description's second word.
+ * kvq_pages_rows reads slots seq[0 .. n) back as dense rows (sum lens, H, D); lens, open and seq are read before it
+ * returns.
  * kvq_pages_fork makes empty slots dst share src's pages and copies the open blocks of all layers (ko,
  * vo of layer 0, layers contiguous; table_device NULL: accounts only).  kvq_pages_free (host only) gives slots back.
  * kvq_pages_move copies pages moves[i] = {from, to} (device) of all layers between pools (the same pool: no
@@ -707,14 +707,13 @@ int kvq_pages_extend(int64_t* lens, int32_t* table, int32_t* refs, uint8_t* open
                      int64_t pages, int64_t max_blocks, int64_t page, int64_t max_tokens, const int64_t* seq,
                      const int64_t* counts, int64_t n, int64_t split_cap, int32_t* desc, int64_t desc_words,
                      int32_t* desc_device, void* stream);
-int kvq_pages_whole(const int64_t* lens, const uint8_t* open, int64_t slots, int64_t page, const int64_t* seq, int64_t n,
-                    int32_t* desc, int64_t desc_words, int32_t* desc_device, void* stream);
 int kvq_pages_append(const void* k, int64_t k_st, int64_t k_sh, const void* v, int64_t v_st, int64_t v_sh, int dtype,
                      const int32_t* step, int64_t items, int32_t* table, int64_t max_blocks, int64_t H, int64_t D,
                      int64_t page, int code, uint8_t* kc, uint8_t* vc, float* sc, void* ko, void* vo, void* stream);
-int kvq_pages_rows(const int32_t* step, int64_t items, const int32_t* table, int64_t max_blocks, int64_t H, int64_t D,
-                   int64_t page, int code, int dtype, const uint8_t* kc, const uint8_t* vc, const float* sc,
-                   const void* ko, const void* vo, void* k_out, void* v_out, void* stream);
+int kvq_pages_rows(const int64_t* lens, const uint8_t* open, int64_t slots, const int64_t* seq, int64_t n,
+                   const int32_t* table, int64_t max_blocks, int64_t H, int64_t D, int64_t page, int code, int dtype,
+                   const uint8_t* kc, const uint8_t* vc, const float* sc, const void* ko, const void* vo, void* k_out,
+                   void* v_out, int64_t out_elements, void* stream);
 int kvq_pages_fork(int64_t* lens, int32_t* table, int32_t* refs, uint8_t* open, int64_t slots, int64_t max_blocks,
                    int64_t page, const int64_t* src, const int64_t* dst, int64_t n, int64_t layers, int64_t H, int64_t D,
                    int32_t* table_device, void* ko, void* vo, void* stream);

@@ -75,7 +75,7 @@ struct DecodeArgs {
   const int* step;
   const int* table;
   int64_t max_blocks;
-  int H, rep, shift;                          // KV heads, query heads per KV head, log2 of the page
+  int H, rep;                                 // KV heads, query heads per KV head
   int pieces;                                 // of 16 rows
   float scale;                                // scaling * log2(e)
   const uint8_t *kc, *vc;
@@ -132,8 +132,8 @@ __device__ __forceinline__ void split_f16(const float (&p)[16], int at, u32x4& h
   }
 }
 
-template <int D, int CODE, bool BF16>
-__global__ __launch_bounds__(kThreads, 2) void paged_split_kernel(DecodeArgs a) {
+template <int D, int P, int CODE, bool BF16>
+__global__ __launch_bounds__(kThreads, 3) void paged_split_kernel(DecodeArgs a) {
   constexpr int kJ = D / 64, kC = D / 16;
   __shared__ float join[kWaves][kRows][D + 4];
   __shared__ float stat[kWaves][kRows][2];
@@ -148,8 +148,8 @@ __global__ __launch_bounds__(kThreads, 2) void paged_split_kernel(DecodeArgs a) 
   const StepSeq s = step_seq(step, b);
   const int rows = a.rep * s.count;
   if (piece * kRows >= rows) return;
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, col = lane & 15, g = lane >> 4;
-  const int P = 1 << a.shift, len = s.pos0 + s.count, full = len >> a.shift << a.shift;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), col = lane & 15, g = lane >> 4;
+  const int len = s.pos0 + s.count, full = len / P * P;
   const int u_full = (full + kUnit - 1) / kUnit, u_all = u_full + (len - full + kUnit - 1) / kUnit;
   const int u0 = (item - s.split0) * per, u1 = u0 + per < u_all ? u0 + per : u_all;
 
@@ -178,34 +178,74 @@ __global__ __launch_bounds__(kThreads, 2) void paged_split_kernel(DecodeArgs a) 
   const int m_tok = 16 * (col >> 2) + (col & 3);                    // + 4 s: the token of S row `col` in tile s
   const int* pages = a.table + s.slot * a.max_blocks;
   const int last = full / P - 1;                                    // last full block
-  int u = u0 + wave;
-  for (; u < u1 && u < u_full; u += kWaves) {
+  const int u_end = u1 < u_full ? u1 : u_full;
+  // The registers of a unit: keys and its scales are read for the next unit once the scores are there, values once
+  // they are added, page numbers a unit further ahead.  With pages of 64 tokens or more a unit lies in one
+  // page: its address and scales are scalars, the lanes' offsets constants.
+  constexpr bool kOne = P >= kUnit;
+  u32x4 kw[4][kJ], vw[kC];
+  float2 z;
+  int pk, pv;                                 // pages of this lane's key rows and value tokens
+  const uint8_t* vp;
+  const uint32_t k_off = m_tok * D + 16 * g, v_off = col * P + 16 * g;
+  auto ids = [&](int u) {
+    if constexpr (kOne) {
+      pk = pages[u * kUnit / P];
+    } else {
+      const int bk = (u * kUnit + m_tok) / P, bv = (u * kUnit + 16 * g) / P;
+      pk = pages[bk < last ? bk : last];      // half a unit may lie behind the last page: masked
+      pv = pages[bv < last ? bv : last];
+    }
+  };
+  auto keys = [&](int u) {
     const int t0 = u * kUnit;
-    int bk = (t0 + m_tok) >> a.shift, bv = (t0 + 16 * g) >> a.shift; // blocks of this lane's key rows and value tokens
-    bk = bk < last ? bk : last;                                     // half a unit may lie behind the last page: masked
-    bv = bv < last ? bv : last;
-    const int64_t pk = static_cast<int64_t>(pages[bk]) * a.H + h, pv = static_cast<int64_t>(pages[bv]) * a.H + h;
-    const uint8_t* kp = a.kc + pk * P * D + ((t0 + m_tok) & (P - 1)) * D + 16 * g;
-    const uint8_t* vp = a.vc + pv * P * D + static_cast<int64_t>(col) * P + ((t0 + 16 * g) & (P - 1));
-    const float2 z = reinterpret_cast<const float2*>(a.sc)[pv];
-    uint4 kw[4][kJ], vw[kC];
+    const uint8_t* kp;
+    if constexpr (kOne) {
+      const int64_t at = static_cast<int64_t>(pk) * a.H + h;
+      kp = a.kc + at * (P * D) + (t0 & (P - 1)) * D;
+      vp = a.vc + at * (P * D) + (t0 & (P - 1));
+      z = reinterpret_cast<const float2*>(a.sc)[at];
+    } else {
+      const int64_t at = static_cast<int64_t>(pv) * a.H + h;
+      kp = a.kc + (static_cast<int64_t>(pk) * a.H + h) * (P * D) + (m_tok & (P - 1)) * D + 16 * g;
+      vp = a.vc + at * (P * D) + col * P + (16 * g & (P - 1));
+      z = reinterpret_cast<const float2*>(a.sc)[at];
+    }
 #pragma unroll
     for (int i = 0; i < 4; ++i)
 #pragma unroll
-      for (int j = 0; j < kJ; ++j) kw[i][j] = *reinterpret_cast<const uint4*>(kp + 4 * i * D + 64 * j);
+      for (int j = 0; j < kJ; ++j) kw[i][j] = *reinterpret_cast<const u32x4*>(kp + (kOne ? k_off + 4 * i * D + 64 * j : 4 * i * D + 64 * j));
+  };
+  auto values = [&]() {
 #pragma unroll
-    for (int c = 0; c < kC; ++c) vw[c] = *reinterpret_cast<const uint4*>(vp + 16 * c * P);
+    for (int c = 0; c < kC; ++c) vw[c] = *reinterpret_cast<const u32x4*>(vp + (kOne ? v_off + 16 * c * P : 16 * c * P));
+  };
+  int u = u0 + wave;
+  if (u < u_end) {
+    ids(u);
+    keys(u);
+    values();
+    if (u + kWaves < u_end) ids(u + kWaves);
+  }
+  for (; u < u_end; u += kWaves) {
+    const int t0 = u * kUnit;
+    const bool more = u + kWaves < u_end;
     float t[16];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       f32x4 acc = {0, 0, 0, 0};
 #pragma unroll
       for (int j = 0; j < kJ; ++j) {
-        acc = mfma16<BF16>(widen8<CODE, BF16>(kw[i][j].x, kw[i][j].y), q[2 * j], acc);
-        acc = mfma16<BF16>(widen8<CODE, BF16>(kw[i][j].z, kw[i][j].w), q[2 * j + 1], acc);
+        acc = mfma16<BF16>(widen8<CODE, BF16>(kw[i][j][0], kw[i][j][1]), q[2 * j], acc);
+        acc = mfma16<BF16>(widen8<CODE, BF16>(kw[i][j][2], kw[i][j][3]), q[2 * j + 1], acc);
       }
 #pragma unroll
       for (int e = 0; e < 4; ++e) t[4 * i + e] = acc[e] * (z.x * a.scale);
+    }
+    const float vz = z.y;
+    if (more) {
+      keys(u + kWaves);
+      if (u + 2 * kWaves < u_end) ids(u + 2 * kWaves);
     }
     const int end = visible < full ? visible : full;
     const bool masked = t0 + kUnit > full || t0 + kUnit > s.pos0 + 1;
@@ -215,7 +255,7 @@ __global__ __launch_bounds__(kThreads, 2) void paged_split_kernel(DecodeArgs a) 
     }
     soft(w, t);
 #pragma unroll
-    for (int i = 0; i < 16; ++i) t[i] *= z.y;
+    for (int i = 0; i < 16; ++i) t[i] *= vz;
     if (masked) {                                                   // a NaN scale of a block that no row sees
 #pragma unroll
       for (int i = 0; i < 16; ++i) t[i] = t0 + 16 * g + i < end ? t[i] : 0.0f;
@@ -225,34 +265,36 @@ __global__ __launch_bounds__(kThreads, 2) void paged_split_kernel(DecodeArgs a) 
     split_bf16(t, 8, hi[1], lo[1]);
 #pragma unroll
     for (int c = 0; c < kC; ++c) {
-      const u32x4 x = widen8<CODE, true>(vw[c].x, vw[c].y), y = widen8<CODE, true>(vw[c].z, vw[c].w);
+      const u32x4 x = widen8<CODE, true>(vw[c][0], vw[c][1]), y = widen8<CODE, true>(vw[c][2], vw[c][3]);
       w.o[c] = mfma16<true>(x, hi[0], w.o[c]);
       w.o[c] = mfma16<true>(y, hi[1], w.o[c]);
       w.o[c] = mfma16<true>(x, lo[0], w.o[c]);
       w.o[c] = mfma16<true>(y, lo[1], w.o[c]);
     }
+    if (more) values();
   }
 
-  // units of the open block
+  // Units of the open block.  32-bit offsets from its scalar base and a few loads at a time: their registers must
+  // not count for the loop above.
   const int64_t open = ((static_cast<int64_t>(s.slot) * 2 + (s.bufs >> 1 & 1)) * a.H + h) * P * D;
+  const uint16_t *ko = a.ko + open, *vo = a.vo + open;
   for (; u < u1; u += kWaves) {
     const int off = (u - u_full) * kUnit, t0 = full + off;
-    const uint16_t* kp = a.ko + open;
-    const uint16_t* vp = a.vo + open + static_cast<int64_t>(col) * P + (off + 16 * g < P ? off + 16 * g : 0);
     float t[16];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const int r = off + m_tok + 4 * i < P ? off + m_tok + 4 * i : P - 1;
+      const int r = off + m_tok + 4 * i < P ? off + m_tok + 4 * i : P - 1;   // behind a page of 32 tokens: masked
       f32x4 acc = {0, 0, 0, 0};
 #pragma unroll
       for (int j = 0; j < kJ; ++j)
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-          const uint4 x = *reinterpret_cast<const uint4*>(kp + r * D + 64 * j + 16 * g + 8 * e);
-          acc = mfma16<BF16>(u32x4{x.x, x.y, x.z, x.w}, q[2 * j + e], acc);
+          const u32x4 x = *reinterpret_cast<const u32x4*>(ko + static_cast<uint32_t>(r * D + 64 * j + 16 * g + 8 * e));
+          acc = mfma16<BF16>(x, q[2 * j + e], acc);
         }
 #pragma unroll
       for (int e = 0; e < 4; ++e) t[4 * i + e] = t0 + 16 * g + 4 * i + e < visible ? acc[e] * a.scale : -INFINITY;
+      __builtin_amdgcn_sched_barrier(0);
     }
     soft(w, t);
     u32x4 hi[2], lo[2];
@@ -264,31 +306,36 @@ __global__ __launch_bounds__(kThreads, 2) void paged_split_kernel(DecodeArgs a) 
     // what lies behind the sequence or is hidden from a row may be an infinity or a NaN: it goes in as zero, and
     // the rows that do see such a value get it afterwards
     constexpr uint32_t kInf = BF16 ? 0x7f80u : 0x7c00u;
-    bool bad = false;
+    const uint32_t at = col * P + (off + 16 * g < P ? off + 16 * g : 0);
+    uint32_t worst = 0;
 #pragma unroll
-    for (int c = 0; c < kC; ++c)
+    for (int c = 0; c < kC; ++c) {
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
-        const uint4 x = *reinterpret_cast<const uint4*>(vp + 16 * c * P + 8 * e);
-        u32x4 v = {x.x, x.y, x.z, x.w};
+        u32x4 v = *reinterpret_cast<const u32x4*>(vo + (at + 16 * c * P + 8 * e));
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          const bool b0 = (v[i] & kInf) == kInf, b1 = (v[i] >> 16 & kInf) == kInf;
-          bad |= b0 || b1;
-          v[i] = (b0 ? 0u : v[i] & 0xffffu) | (b1 ? 0u : v[i] & 0xffff0000u);
+          const uint32_t b0 = v[i] & kInf, b1 = v[i] >> 16 & kInf;
+          worst = b0 > worst ? b0 : worst;
+          worst = b1 > worst ? b1 : worst;
+          v[i] = (b0 == kInf ? 0u : v[i] & 0xffffu) | (b1 == kInf ? 0u : v[i] & 0xffff0000u);
         }
         w.o[c] = mfma16<BF16>(v, hi[e], w.o[c]);
         w.o[c] = mfma16<BF16>(v, lo[e], w.o[c]);
       }
-    if (__builtin_amdgcn_ballot_w64(bad)) {
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    if (__builtin_amdgcn_ballot_w64(worst == kInf)) {
       for (int i = 0; i < kUnit && t0 + i < len; ++i)
 #pragma unroll
-        for (int c = 0; c < kC; ++c)
+        for (int c = 0; c < kC; ++c) {
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
-            const uint16_t x = a.vo[open + static_cast<int64_t>(16 * c + 4 * g + e) * P + off + i];
+            const uint16_t x = vo[static_cast<uint32_t>((16 * c + 4 * g + e) * P + off + i)];
             if ((x & kInf) == kInf && t0 + i < visible) w.o[c][e] += BF16 ? bf16_to_f32(x) : f16_to_f32(x);
           }
+          __builtin_amdgcn_sched_barrier(0);
+        }
     }
   }
 
@@ -408,30 +455,35 @@ extern "C" int kvq_paged_decode(const void* q, int64_t q_st, int64_t q_sh, int d
   KVQ_REQUIRE(workspace_floats >= need, "kvq_paged_decode: workspace of %lld floats, %lld needed", static_cast<long long>(workspace_floats),
               static_cast<long long>(need));
   DecodeArgs a{static_cast<const uint16_t*>(q), q_st, q_sh, step, table, max_blocks, static_cast<int>(H), static_cast<int>(rep),
-               P == 32 ? 5 : P == 64 ? 6 : 7, static_cast<int>(pieces_of(rep, max_count)), scaling * 1.44269504088896341f, kc, vc, sc,
+               static_cast<int>(pieces_of(rep, max_count)), scaling * 1.44269504088896341f, kc, vc, sc,
                static_cast<const uint16_t*>(ko), static_cast<const uint16_t*>(vo), static_cast<uint16_t*>(out), workspace};
   const int64_t blocks = (split_items * H + 7) / 8 * 8 * a.pieces, merges = (rows * Hq + kWaves - 1) / kWaves;
   KVQ_REQUIRE(blocks < INT64_C(1) << 31 && merges < INT64_C(1) << 31, "kvq_paged_decode: too many rows");
-  auto run = [&](auto d, auto c, auto t) {
-    constexpr int D_ = decltype(d)::value, C_ = decltype(c)::value;
+  auto run = [&](auto d, auto p, auto c, auto t) {
+    constexpr int D_ = decltype(d)::value, P_ = decltype(p)::value, C_ = decltype(c)::value;
     constexpr bool T_ = decltype(t)::value != 0;
-    hipLaunchKernelGGL((paged_split_kernel<D_, C_, T_>), dim3(static_cast<uint32_t>(blocks)), dim3(kThreads), 0,
+    hipLaunchKernelGGL((paged_split_kernel<D_, P_, C_, T_>), dim3(static_cast<uint32_t>(blocks)), dim3(kThreads), 0,
                        static_cast<hipStream_t>(stream), a);
     hipLaunchKernelGGL((paged_merge_kernel<D_, T_>), dim3(static_cast<uint32_t>(merges)), dim3(kThreads), 0,
                        static_cast<hipStream_t>(stream), a, rows * Hq);
   };
   using Zero = std::integral_constant<int, 0>;
   using One = std::integral_constant<int, 1>;
-  auto by_type = [&](auto d, auto c) {
-    if (dtype == KVQ_BF16) run(d, c, One{});
-    else run(d, c, Zero{});
+  auto by_type = [&](auto d, auto p, auto c) {
+    if (dtype == KVQ_BF16) run(d, p, c, One{});
+    else run(d, p, c, Zero{});
   };
-  auto by_code = [&](auto d) {
-    if (code == kCodeInt8) by_type(d, Zero{});
-    else by_type(d, One{});
+  auto by_code = [&](auto d, auto p) {
+    if (code == kCodeInt8) by_type(d, p, Zero{});
+    else by_type(d, p, One{});
   };
-  if (D == 64) by_code(std::integral_constant<int, 64>{});
-  else by_code(std::integral_constant<int, 128>{});
+  auto by_page = [&](auto d) {
+    if (P == 32) by_code(d, std::integral_constant<int, 32>{});
+    else if (P == 64) by_code(d, std::integral_constant<int, 64>{});
+    else by_code(d, std::integral_constant<int, 128>{});
+  };
+  if (D == 64) by_page(std::integral_constant<int, 64>{});
+  else by_page(std::integral_constant<int, 128>{});
   KVQ_LAUNCH_CHECK("kvq_paged_decode");
   return KVQ_OK;
 }

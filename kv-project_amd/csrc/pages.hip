@@ -217,10 +217,12 @@ __device__ __forceinline__ uint16_t from_f32(float x) {
   else return f32_to_f16(x);
 }
 
-// One workgroup per (block, KV head): dense rows (rows, H, D) of keys and values.  The description is
-// that of a step that holds the whole sequences.
+// Whole sequences by value with the launch: {slot, tokens, first row, first block, open buffer} of each
+constexpr int kWhole = 5, kMostWhole = kWords / kWhole;
+
+// One workgroup per (block, KV head): dense rows (rows, H, D) of keys and values.
 template <int D, int P, int CODE, bool BF16>
-__global__ __launch_bounds__(kThreads) void rows_kernel(const int* __restrict__ step, const int* __restrict__ table, int64_t max_blocks,
+__global__ __launch_bounds__(kThreads) void rows_kernel(WordBlock whole, int n, const int* __restrict__ table, int64_t max_blocks,
                                                         int H, const uint8_t* __restrict__ kc, const uint8_t* __restrict__ vc,
                                                         const float* __restrict__ sc, const uint16_t* __restrict__ ko,
                                                         const uint16_t* __restrict__ vo, uint16_t* __restrict__ k_out,
@@ -229,19 +231,24 @@ __global__ __launch_bounds__(kThreads) void rows_kernel(const int* __restrict__ 
   constexpr int kPitch = D + 8;
   __shared__ __align__(16) uint16_t turn[P * kPitch];
   const int item = blockIdx.x / H, h = blockIdx.x % H, tid = threadIdx.x;
-  const int n = step[0];
-  if (item >= step[1]) return;
-  const StepSeq s = step_seq(step, step_find(step, n, 4, item));
-  const int j = item - s.item0, first = j * P;
-  const int rows = s.count - first < P ? s.count - first : P;
+  int lo = 0, hi = n - 1;                     // the last sequence whose first block is not behind this one
+  while (lo < hi) {
+    const int mid = (lo + hi + 1) >> 1;
+    if (whole.w[kWhole * mid + 3] <= item) lo = mid;
+    else hi = mid - 1;
+  }
+  const int* s = whole.w + kWhole * lo;
+  const int64_t slot = s[0];
+  const int j = item - s[3], first = j * P;
+  const int rows = s[1] - first < P ? s[1] - first : P;
   const bool open = rows < P;
-  const int64_t out = (static_cast<int64_t>(s.row0 + first) * H + h) * D;
+  const int64_t out = (static_cast<int64_t>(s[2] + first) * H + h) * D;
   int64_t at;
   float2 z = make_float2(1.0f, 1.0f);
   if (open) {
-    at = ((static_cast<int64_t>(s.slot) * 2 + (s.bufs >> 1 & 1)) * H + h) * P * D;
+    at = ((slot * 2 + s[4]) * H + h) * P * D;
   } else {
-    const int64_t page = table[s.slot * max_blocks + j];
+    const int64_t page = table[slot * max_blocks + j];
     at = (page * H + h) * P * D;
     z = reinterpret_cast<const float2*>(sc)[page * H + h];
   }
@@ -354,13 +361,13 @@ int64_t splits_of(const int32_t* e, int64_t page, int64_t per) {    // none for 
 
 // Fills the description from lens (before), counts and open buffers.  Returns the number of items.
 int64_t describe(const int64_t* lens, const uint8_t* open, int64_t page, const int64_t* seq, const int64_t* counts, int64_t n,
-                 int64_t split_cap, bool whole, int32_t* desc) {
+                 int64_t split_cap, int32_t* desc) {
   int64_t row = 0, item = 0, most = 0;
   bool even = true;
   for (int64_t i = 0; i < n; ++i) {
     int32_t* e = desc + kStepHead + kStepSeq * i;
-    const int64_t s = seq[i], len = lens[s], pos0 = whole ? 0 : len, count = whole ? len : counts[i], end = pos0 + count;
-    const int src = open[s] & 1, dst = !whole && pos0 % page && end / page > pos0 / page && end % page ? src ^ 1 : src;
+    const int64_t s = seq[i], len = lens[s], pos0 = len, count = counts[i], end = pos0 + count;
+    const int src = open[s] & 1, dst = pos0 % page && end / page > pos0 / page && end % page ? src ^ 1 : src;
     e[0] = static_cast<int32_t>(s);
     e[1] = static_cast<int32_t>(pos0);
     e[2] = static_cast<int32_t>(count);
@@ -486,7 +493,7 @@ extern "C" int kvq_pages_extend(int64_t* lens, int32_t* table, int32_t* refs, ui
   KVQ_REQUIRE(rows < INT64_C(1) << 31, "kvq_pages_extend: too many rows");
   KVQ_REQUIRE(need <= account[0], "decode buffer exhausted: %lld pages needed, %lld free", static_cast<long long>(need),
               static_cast<long long>(account[0]));
-  describe(lens, open, page, seq, counts, n, split_cap, false, desc);
+  describe(lens, open, page, seq, counts, n, split_cap, desc);
   int32_t* page_of = desc + kStepHead + kStepSeq * (n + 1);
   int64_t low = account[1];
   for (int64_t i = 0; i < n; ++i) {
@@ -512,21 +519,6 @@ extern "C" int kvq_pages_extend(int64_t* lens, int32_t* table, int32_t* refs, ui
   return desc_device ? write_words(desc, words, desc_device, static_cast<hipStream_t>(stream)) : KVQ_OK;
 }
 
-extern "C" int kvq_pages_whole(const int64_t* lens, const uint8_t* open, int64_t slots, int64_t page, const int64_t* seq, int64_t n,
-                               int32_t* desc, int64_t desc_words, int32_t* desc_device, void* stream) {
-  KVQ_REQUIRE(lens && open && desc && desc_device && n > 0 && seq, "kvq_pages_whole: null pointer or no sequence");
-  KVQ_REQUIRE(desc_words >= kStepHead + kStepSeq * (n + 1), "kvq_pages_whole: a short description");
-  int64_t rows = 0;
-  for (int64_t i = 0; i < n; ++i) {
-    KVQ_REQUIRE(seq[i] >= 0 && seq[i] < slots, "kvq_pages_whole: no slot %lld (of %lld)", static_cast<long long>(seq[i]),
-                static_cast<long long>(slots));
-    rows += lens[seq[i]];
-  }
-  KVQ_REQUIRE(rows < INT64_C(1) << 31, "kvq_pages_whole: too many rows");
-  describe(lens, open, page, seq, nullptr, n, n, true, desc);
-  return write_words(desc, kStepHead + kStepSeq * (n + 1), desc_device, static_cast<hipStream_t>(stream));
-}
-
 extern "C" int kvq_pages_append(const void* k, int64_t k_st, int64_t k_sh, const void* v, int64_t v_st, int64_t v_sh, int dtype,
                                 const int32_t* step, int64_t items, int32_t* table, int64_t max_blocks, int64_t H, int64_t D, int64_t P,
                                 int code, uint8_t* kc, uint8_t* vc, float* sc, void* ko, void* vo, void* stream) {
@@ -544,19 +536,45 @@ extern "C" int kvq_pages_append(const void* k, int64_t k_st, int64_t k_sh, const
   return KVQ_OK;
 }
 
-extern "C" int kvq_pages_rows(const int32_t* step, int64_t items, const int32_t* table, int64_t max_blocks, int64_t H, int64_t D, int64_t P,
-                              int code, int dtype, const uint8_t* kc, const uint8_t* vc, const float* sc, const void* ko, const void* vo,
-                              void* k_out, void* v_out, void* stream) {
+extern "C" int kvq_pages_rows(const int64_t* lens, const uint8_t* open, int64_t slots, const int64_t* seq, int64_t n, const int32_t* table,
+                              int64_t max_blocks, int64_t H, int64_t D, int64_t P, int code, int dtype, const uint8_t* kc, const uint8_t* vc,
+                              const float* sc, const void* ko, const void* vo, void* k_out, void* v_out, int64_t out_elements, void* stream) {
   KVQ_PAGES_REQUIRE("kvq_pages_rows")
-  KVQ_REQUIRE(step && table && kc && vc && sc && ko && vo && k_out && v_out, "kvq_pages_rows: null pointer");
+  KVQ_REQUIRE(lens && open && (n == 0 || seq) && table && kc && vc && sc && ko && vo, "kvq_pages_rows: null pointer");
   KVQ_REQUIRE(reinterpret_cast<uintptr_t>(k_out) % 16 == 0 && reinterpret_cast<uintptr_t>(v_out) % 16 == 0,
               "kvq_pages_rows: outputs must be 16-byte aligned");
-  KVQ_REQUIRE(items >= 0 && items * H < INT64_C(1) << 31, "kvq_pages_rows: too many blocks");
-  if (items == 0) return KVQ_OK;
-  KVQ_PAGES_DISPATCH(hipLaunchKernelGGL((rows_kernel<D_, P_, C_, T_>), dim3(static_cast<uint32_t>(items * H)), dim3(kThreads), 0,
-                                        static_cast<hipStream_t>(stream), step, table, max_blocks, static_cast<int>(H), kc, vc, sc,
-                                        static_cast<const uint16_t*>(ko), static_cast<const uint16_t*>(vo), static_cast<uint16_t*>(k_out),
-                                        static_cast<uint16_t*>(v_out)))
+  int64_t rows = 0, blocks = 0;
+  for (int64_t i = 0; i < n; ++i) {
+    KVQ_REQUIRE(seq[i] >= 0 && seq[i] < slots, "kvq_pages_rows: no slot %lld (of %lld)", static_cast<long long>(seq[i]),
+                static_cast<long long>(slots));
+    rows += lens[seq[i]];
+    blocks += (lens[seq[i]] + P - 1) / P;
+  }
+  KVQ_REQUIRE(rows < INT64_C(1) << 31 && blocks * H < INT64_C(1) << 31, "kvq_pages_rows: too many rows");
+  KVQ_REQUIRE(out_elements >= rows * H * D && (rows == 0 || (k_out && v_out)), "kvq_pages_rows: outputs of %lld elements, %lld needed",
+              static_cast<long long>(out_elements), static_cast<long long>(rows * H * D));
+  int64_t row = 0;
+  for (int64_t at = 0; at < n; at += kMostWhole) {
+    WordBlock w;
+    const int64_t m = n - at < kMostWhole ? n - at : kMostWhole;
+    int64_t block = 0;
+    for (int64_t i = 0; i < m; ++i) {
+      const int64_t s = seq[at + i];
+      int* e = w.w + kWhole * i;
+      e[0] = static_cast<int>(s);
+      e[1] = static_cast<int>(lens[s]);
+      e[2] = static_cast<int>(row);
+      e[3] = static_cast<int>(block);
+      e[4] = open[s] & 1;
+      row += lens[s];
+      block += (lens[s] + P - 1) / P;
+    }
+    if (block == 0) continue;
+    KVQ_PAGES_DISPATCH(hipLaunchKernelGGL((rows_kernel<D_, P_, C_, T_>), dim3(static_cast<uint32_t>(block * H)), dim3(kThreads), 0,
+                                          static_cast<hipStream_t>(stream), w, static_cast<int>(m), table, max_blocks, static_cast<int>(H), kc,
+                                          vc, sc, static_cast<const uint16_t*>(ko), static_cast<const uint16_t*>(vo),
+                                          static_cast<uint16_t*>(k_out), static_cast<uint16_t*>(v_out)))
+  }
   KVQ_LAUNCH_CHECK("kvq_pages_rows");
   return KVQ_OK;
 }

@@ -37,7 +37,7 @@ def _ints(x, what: str) -> np.ndarray:
 class Step:
     """New tokens of some slots: ``rows`` packed rows, slot by slot.  Made by ``PagedCache.extend``."""
 
-    __slots__ = ("slots", "counts", "ends", "rows", "items", "splits", "max_count", "desc", "host", "generation")
+    __slots__ = ("slots", "counts", "ends", "rows", "items", "splits", "max_count", "desc", "host", "generation", "stamp")
 
 
 class PagedCache:
@@ -67,12 +67,14 @@ class PagedCache:
         self._table = np.zeros((self.slots, self.max_blocks), dtype=np.int32)
         self._open = np.zeros(self.slots, dtype=np.uint8)
         self._set_refs(np.zeros(self.pages, dtype=np.int32))
-        self._generation = 0
+        self._generation = 0                   # of the pools
+        self._stamp = 0                        # of the slots' lengths
         self.table = torch.zeros((self.slots, self.max_blocks), dtype=torch.int32, device=self.device)
         self.kc, self.vc, self.sc = self._pool(self.pages)
         rows = (self.layers, self.slots, 2, self.Hkv, self.page * self.d)
         self.k_open = torch.zeros(rows, dtype=dtype, device=self.device)     # token major, as a page's keys
         self.v_open = torch.zeros(rows, dtype=dtype, device=self.device)     # channel major, as a page's values
+        self._set_addresses()
 
     def _pool(self, pages: int):
         new = lambda *s, dt=torch.int8: torch.empty((self.layers, pages, self.Hkv, *s), dtype=dt, device=self.device)
@@ -83,6 +85,11 @@ class PagedCache:
         self._refs = refs
         self._account = np.array([free.size, free[0] if free.size else refs.size], dtype=np.int64)
         self._host = tuple(x.ctypes.data for x in (self._lens, self._table, self._refs, self._open, self._account))
+
+    def _set_addresses(self) -> None:
+        """Of each layer's codes, scales and open blocks."""
+        parts = [(x.data_ptr(), x.stride(0) * x.element_size()) for x in (self.kc, self.vc, self.sc, self.k_open, self.v_open)]
+        self._at = [tuple(p + l * step for p, step in parts) for l in range(self.layers)]
 
     # ---- what is held ------------------------------------------------------------------------
 
@@ -139,19 +146,20 @@ class PagedCache:
             st.splits = max(1, int(st.host[2]))         # what later steps written into this one keep to
             st.items = st.host.size - 8 * (n + 2)
             st.rows, st.max_count = int(c.sum()), int(c.max())
-        st.slots, st.counts, st.ends, st.generation = s, c, self._lens[s], self._generation
+        self._stamp += 1
+        st.slots, st.counts, st.ends, st.generation, st.stamp = s, c, self._lens[s], self._generation, self._stamp
         return st
 
     def check_step(self, step: Step, what: str) -> None:
         """A step describes its slots only until they take more tokens or are freed."""
-        if not (self._lens[step.slots] == step.ends).all():
-            raise ValueError(f"{what}: the step's slots have changed since it was made")
+        if step.stamp != self._stamp:
+            if not (self._lens[step.slots] == step.ends).all():
+                raise ValueError(f"{what}: the step's slots have changed since it was made")
+            step.stamp = self._stamp           # what changed were other slots
 
-    @torch.no_grad()
     def append(self, layer: int, k: torch.Tensor, v: torch.Tensor, step: Step) -> None:
         """The step's new rows k, v (rows, Hkv, d) of one layer, slot by slot: full blocks to codes, the rest to the open
         blocks.  Running it again writes the same."""
-        _lib.require_gpu(k, v)
         self._layer(layer)
         shape = (step.rows, self.Hkv, self.d)
         if k.shape != shape or v.shape != shape:
@@ -159,6 +167,7 @@ class PagedCache:
         if k.dtype != self.dtype or v.dtype != self.dtype:
             raise TypeError("appended rows must have the cache's dtype")
         if k.device != self.device or v.device != self.device:
+            _lib.require_gpu(k, v)
             raise ValueError(f"append: the cache is on {self.device}")
         self.check_step(step, "append")
         if step.generation != self._generation:
@@ -168,35 +177,24 @@ class PagedCache:
         k, v = rows16(k), rows16(v)
         _lib.call_on(self.device, "kvq_pages_append", k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(), v.stride(0), v.stride(1),
                      _lib.DTYPE_CODE[self.dtype], step.desc.data_ptr(), step.items, self.table.data_ptr(), self.max_blocks,
-                     self.Hkv, self.d, self.page, CODES[self.code], *self._at(layer), _lib.stream_of(k))
+                     self.Hkv, self.d, self.page, CODES[self.code], *self._at[layer], _lib.stream_of(k))
 
     def _layer(self, layer: int) -> None:
         if not 0 <= layer < self.layers:
             raise IndexError(f"no layer {layer} (of {self.layers})")
 
-    def _at(self, layer: int):
-        """Addresses of a layer's codes, scales and open blocks."""
-        return tuple(x.data_ptr() + layer * x.stride(0) * x.element_size()
-                     for x in (self.kc, self.vc, self.sc, self.k_open, self.v_open))
-
-    @torch.no_grad()
     def rows(self, layer: int, slots: Sequence[int]) -> Tuple[torch.Tensor, torch.Tensor]:
         """All tokens of the slots, one behind the other, as dense rows k, v (tokens, Hkv, d): code times scale, rounded
         once, and the open blocks as they are.  With prompt_attention this is the attention of many new tokens."""
         self._layer(layer)
         s = _ints(slots, "slots")
-        n = s.size
-        host = np.empty(8 * (n + 2), dtype=np.int32)
-        desc = torch.empty(host.size, dtype=torch.int32, device=self.device)
-        stream = _lib.stream_of(desc)
-        _lib.call_on(self.device, "kvq_pages_whole", self._host[0], self._host[3], self.slots, self.page, s.ctypes.data, n,
-                     host.ctypes.data, host.size, desc.data_ptr(), stream)
-        total = int(self._lens[s].sum())
-        k, v = (torch.empty((total, self.Hkv, self.d), dtype=self.dtype, device=self.device) for _ in (0, 1))
-        if total:
-            _lib.call_on(self.device, "kvq_pages_rows", desc.data_ptr(), int(host[1]), self.table.data_ptr(), self.max_blocks, self.Hkv,
-                         self.d, self.page, CODES[self.code], _lib.DTYPE_CODE[self.dtype], *self._at(layer), k.data_ptr(),
-                         v.data_ptr(), stream)
+        if s.min() < 0 or s.max() >= self.slots:
+            raise _lib.KVQError(f"rows: no slot {s.min() if s.min() < 0 else s.max()} (of {self.slots})")
+        out = torch.empty((2, int(self._lens[s].sum()), self.Hkv, self.d), dtype=self.dtype, device=self.device)
+        k, v = out.unbind(0)
+        _lib.call_on(self.device, "kvq_pages_rows", self._host[0], self._host[3], self.slots, s.ctypes.data, s.size, self.table.data_ptr(),
+                     self.max_blocks, self.Hkv, self.d, self.page, CODES[self.code], _lib.DTYPE_CODE[self.dtype], *self._at[layer],
+                     k.data_ptr(), v.data_ptr(), k.numel(), _lib.stream_of(out))
         return k, v
 
     # ---- sequences and pages -----------------------------------------------------------------
@@ -210,11 +208,13 @@ class PagedCache:
         _lib.call_on(self.device, "kvq_pages_fork", *self._host[:4], self.slots, self.max_blocks, self.page, s.ctypes.data, t.ctypes.data,
                      s.size, self.layers, self.Hkv, self.d, self.table.data_ptr(), self.k_open.data_ptr(), self.v_open.data_ptr(),
                      _lib.stream_of(self.table))
+        self._stamp += 1
 
     def free(self, slots: Sequence[int]) -> None:
         """Empty the slots; pages that no other sequence shares become free."""
         s = _ints(slots, "slots")
         _lib.call("kvq_pages_free", *self._host, self.slots, self.max_blocks, self.page, s.ctypes.data, s.size)
+        self._stamp += 1
 
     def compact(self) -> int:
         """Move the pages at the end of the pool to the free places below, in order, so that the pages in use are the
@@ -234,6 +234,7 @@ class PagedCache:
         pool = self._pool(pages)
         self._move(pages, pool)
         (self.kc, self.vc, self.sc), self.pages = pool, pages
+        self._set_addresses()
 
     def _move(self, end: int, pool) -> None:
         live = np.flatnonzero(self._refs)
@@ -266,13 +267,11 @@ def paged_workspace_floats(step: Step, Hq: int, Hkv: int, d: int) -> int:
     return n
 
 
-@torch.no_grad()
 def paged_decode(q: torch.Tensor, scaling: float, cache: PagedCache, layer: int, step: Step, *,
                  out: Optional[torch.Tensor] = None, workspace: Optional[torch.Tensor] = None) -> torch.Tensor:
     """Attention of the step's query rows q (rows, Hq, d), slot by slot, over the cache; returns (rows, Hq, d).  Query i of
     a slot's new tokens sees every token up to its own.  Meant for a few tokens per slot (16 rows = query
     heads of a KV head times tokens go over the keys together); for many, ``cache.rows`` and prompt_attention."""
-    _lib.require_gpu(q)
     cache._layer(layer)
     if q.dim() != 3 or q.shape[0] != step.rows or q.shape[2] != cache.d or q.shape[1] < 1 or q.shape[1] % cache.Hkv:
         raise ValueError(f"paged_decode: q {tuple(q.shape)} does not match the step ({step.rows} rows) and the cache "
@@ -280,6 +279,7 @@ def paged_decode(q: torch.Tensor, scaling: float, cache: PagedCache, layer: int,
     if q.dtype != cache.dtype:
         raise TypeError("q must have the cache's dtype")
     if q.device != cache.device:
+        _lib.require_gpu(q)
         raise ValueError(f"paged_decode: the cache is on {cache.device}")
     cache.check_step(step, "paged_decode")
     q = rows16(q)
@@ -293,6 +293,6 @@ def paged_decode(q: torch.Tensor, scaling: float, cache: PagedCache, layer: int,
         raise ValueError("workspace must be contiguous float32 on the cache's device")
     _lib.call_on(q.device, "kvq_paged_decode", q.data_ptr(), q.stride(0), q.stride(1), _lib.DTYPE_CODE[q.dtype], step.rows, Hq, cache.Hkv,
                  cache.d, float(scaling), step.desc.data_ptr(), step.splits, step.max_count, cache.table.data_ptr(),
-                 cache.max_blocks, cache.page, CODES[cache.code], *cache._at(layer), out.data_ptr(), workspace.data_ptr(),
+                 cache.max_blocks, cache.page, CODES[cache.code], *cache._at[layer], out.data_ptr(), workspace.data_ptr(),
                  workspace.numel(), _lib.stream_of(q))
     return out

@@ -58,12 +58,10 @@ class PromptPlan:
         return _lib.load().kvq_prompt_workspace(self.parts, self.Hkv, d)
 
 
-@torch.no_grad()
 def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, scaling: float, plan: PromptPlan, *,
                      out: Optional[torch.Tensor] = None, workspace: Optional[torch.Tensor] = None) -> torch.Tensor:
     """Attention of the packed rows q (rows, Hq, d) over k, v (keys, Hkv, d), bf16 or fp16 of one type, head_dim 64
     or 128, any row and head strides of whole 16 bytes (others are copied); returns (rows, Hq, d)."""
-    _lib.require_gpu(q, k, v)
     if q.dim() != 3 or k.dim() != 3 or v.shape != k.shape:
         raise ValueError(f"prompt_attention takes q (rows, Hq, d) and k, v (keys, Hkv, d), got {tuple(q.shape)}, "
                          f"{tuple(k.shape)}, {tuple(v.shape)}")
@@ -76,6 +74,7 @@ def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, scaling:
     if d not in (64, 128):
         raise _lib.KVQError(f"prompt_attention: head_dim must be 64 or 128 (got {d})")
     if q.device != plan.device or k.device != plan.device or v.device != plan.device:
+        _lib.require_gpu(q, k, v)
         raise ValueError(f"prompt_attention: the plan is for {plan.device}")
     q, k, v = (rows16(x) for x in (q, k, v))
     out = _lib.out_or_new(out, (plan.rows, plan.Hq, d), q.dtype, q.device, "prompt_attention")
@@ -97,5 +96,5 @@ def rows16(x: torch.Tensor) -> torch.Tensor:
     """x (rows, heads, d) itself when the kernels can read it in 16-byte pieces, or a copy."""
     st, sh, sd = x.stride()
     if sd != 1 or (st | sh) % 8 or x.data_ptr() % 16 or not 0 <= st < 1 << 24:
-        return x.clone(memory_format=torch.contiguous_format)
+        return x.detach().clone(memory_format=torch.contiguous_format)
     return x

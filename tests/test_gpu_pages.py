@@ -210,6 +210,17 @@ def test_random_life():
             m.check(f"step {i}")
 
 
+def test_many_slots():
+    """More sequences than go with one launch by value."""
+    n = 300
+    m = Mirror(slots=2 * n, pages=700, max_tokens=100, Hkv=1, d=64, page=32, seed=14)
+    m.push(list(range(n)), [1 + (7 * i) % 90 for i in range(n)])
+    m.fork(list(range(n)), list(range(n, 2 * n)))
+    step = m.push(list(range(2 * n)), [1] * (2 * n))
+    m.check("many")
+    m.decode(step, 2, what="many")
+
+
 def test_append_again_writes_the_same():
     """A step that fills a block and opens the next one, appended twice."""
     m = Mirror(seed=6, page=32)
@@ -375,6 +386,8 @@ def test_gpu_refusals():
         kvq.paged_decode(q.half(), 0.1, c, 0, step)
     with pytest.raises(kvq.KVQError, match="workspace"):
         kvq.paged_decode(q, 0.1, c, 0, step, workspace=torch.empty(10, device="cuda"))
+    with pytest.raises(kvq.KVQError, match="no slot"):
+        c.rows(0, [0, 3])
     with pytest.raises(ValueError, match="same counts"):
         c.extend([0, 1], [1, 1], into=step)
     c.extend([1], [1])
