@@ -728,12 +728,16 @@ int kvq_pages_move(const uint8_t* kc, const uint8_t* vc, const float* sc, int64_
  * i of a sequence with `count` new tokens sees all tokens up to its own.  split_items >= the description's
  * third word and max_count >= every count give the grid.  out (rows, Hq, D) contiguous.  workspace:
  * kvq_paged_decode_workspace floats, no clearing; calls that share one must not overlap in time.
+ * tickets: NULL, or (slots, H, 4) int32 zeros, which a call leaves as zeros: sequences of several split items are
+ * then joined within the one launch, by the workgroup that comes last (in the items' order: the result is the
+ * same), where a sequence has at most 64 rows per KV head.  Calls over one slot of one layer must not overlap.
  * ---------------------------------------------------------------------------------------- */
 int64_t kvq_paged_decode_workspace(int64_t split_items, int64_t H, int64_t rep, int64_t max_count, int64_t D);
 int kvq_paged_decode(const void* q, int64_t q_st, int64_t q_sh, int dtype, int64_t rows, int64_t Hq, int64_t H, int64_t D,
                      float scaling, const int32_t* step, int64_t split_items, int64_t max_count, const int32_t* table,
                      int64_t max_blocks, int64_t page, int code, const uint8_t* kc, const uint8_t* vc, const float* sc,
-                     const void* ko, const void* vo, void* out, float* workspace, int64_t workspace_floats, void* stream);
+                     const void* ko, const void* vo, void* out, float* workspace, int64_t workspace_floats,
+                     int32_t* tickets, void* stream);
 
 #ifdef __cplusplus
 }

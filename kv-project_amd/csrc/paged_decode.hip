@@ -10,8 +10,9 @@
 // 16-bit numbers exactly.  Probabilities times scale keep 16 bits as a pair of bfloat16 (the range of a
 // scale is float32's), so they round at 2^-17.
 //
-// Workgroups take the units of one split item, their wavefronts in turn, and join in LDS; a sequence
-// of several items is joined by merge_kernel in the items' order.
+// Workgroups take the units of one split item, their wavefronts in turn, and join in LDS.  A sequence of
+// several items is joined in the items' order: by the workgroup that comes last, where tickets are given, or
+// by paged_merge_kernel, which spreads long joins over the chip.
 #include <type_traits>
 
 #include "mfma_common.hpp"
@@ -83,13 +84,60 @@ struct DecodeArgs {
   const uint16_t *ko, *vo;
   uint16_t* out;                              // (rows, Hq, D)
   float* part;                                // (items, H, pieces): 16 x D sums, then 16 x {max, sum}
+  int* tickets;                               // (slots, H, kTickets) zeros, or none: joins by a launch of its own
 };
+constexpr int kTickets = 4;                   // pieces of a sequence that the last workgroup may join
 
 template <int D, bool BF16>
 struct Wave {                                 // one wavefront's running softmax: column lane % 16
   f32x4 o[D / 16];                            // channels 16 c + 4 g + i
   float m, l;                                 // base-2 maximum (of all groups), this lane's part of the sum
 };
+
+// Values that workgroups on other dies read in this launch: stores and loads at the level that the dies share, past
+// their own caches (a release fence writes a whole cache back: 50 us where 768 workgroups have one each)
+__device__ __forceinline__ void put_shared(float* p, float x) { __hip_atomic_store(p, x, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
+template <bool SHARED>
+__device__ __forceinline__ float get(const float* p) {
+  if constexpr (SHARED) return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  else return *p;
+}
+
+// Row r of `items` partial results, 64 maxima at a time, by one wavefront
+template <int D, bool BF16, bool SHARED>
+__device__ __forceinline__ void join_row(const float* part, int64_t stride, int items, int r, uint16_t* out) {
+  const int lane = threadIdx.x & 63;
+  float top = -INFINITY, l = 0.0f, o[D / 64] = {};
+  for (int i0 = 0; i0 < items; i0 += 64) {
+    const int i = i0 + lane;
+    float2 st = make_float2(-INFINITY, 0.0f);
+    if (i < items) st = make_float2(get<SHARED>(part + i * stride + kRows * D + 2 * r), get<SHARED>(part + i * stride + kRows * D + 2 * r + 1));
+    const float m = fmaxf(top, wave_max(st.x)), safe = m == -INFINITY ? 0.0f : m;
+    const float old = __builtin_amdgcn_exp2f(top - safe), f = __builtin_amdgcn_exp2f(st.x - safe);
+    l = l * old + wave_sum(f * st.y);
+#pragma unroll
+    for (int e = 0; e < D / 64; ++e) o[e] *= old;
+    const int most = items - i0 < 64 ? items - i0 : 64;
+    const float* p = part + i0 * stride + r * D + lane * (D / 64);
+    for (int k0 = 0; k0 < most; k0 += 8) {                          // eight loads on their way; behind the last: it again, times zero
+      float x[8][D / 64];
+#pragma unroll
+      for (int k = 0; k < 8; ++k)
+#pragma unroll
+        for (int e = 0; e < D / 64; ++e) x[k][e] = get<SHARED>(p + (k0 + k < most ? k0 + k : most - 1) * stride + e);
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        const float fk = k0 + k < most ? __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(f), k0 + k)) : 0.0f;
+#pragma unroll
+        for (int e = 0; e < D / 64; ++e) o[e] += k0 + k < most ? fk * x[k][e] : 0.0f;
+      }
+    }
+    top = m;
+  }
+  const float inv = 1.0f / l;
+#pragma unroll
+  for (int e = 0; e < D / 64; ++e) out[lane * (D / 64) + e] = BF16 ? f32_to_bf16(o[e] * inv) : f32_to_f16(o[e] * inv);
+}
 
 // Scores t (16 tokens of this lane, masked ones -inf) -> probabilities in t, o and l brought to the new maximum
 template <int D, bool BF16>
@@ -364,10 +412,11 @@ __global__ __launch_bounds__(kThreads, 3) void paged_split_kernel(DecodeArgs a) 
     for (int e = 0; e < kPer; ++e) o[e] += f * join[i][r][c0 + e];
   }
   const int R = piece * kRows + r;
-  if (R >= rows) return;
+  const int64_t Hq = static_cast<int64_t>(a.H) * a.rep;
   if (single) {
+    if (R >= rows) return;
     const float inv = 1.0f / l;
-    uint16_t* out = a.out + ((static_cast<int64_t>(s.row0) + R / a.rep) * a.H * a.rep + h * a.rep + R % a.rep) * D + c0;
+    uint16_t* out = a.out + ((static_cast<int64_t>(s.row0) + R / a.rep) * Hq + h * a.rep + R % a.rep) * D + c0;
     uint32_t p[kPer / 2];
 #pragma unroll
     for (int e = 0; e < kPer / 2; ++e)
@@ -377,13 +426,41 @@ __global__ __launch_bounds__(kThreads, 3) void paged_split_kernel(DecodeArgs a) 
     for (int e = 0; e < kPer / 4; ++e) *reinterpret_cast<uint2*>(out + 4 * e) = make_uint2(p[2 * e], p[2 * e + 1]);
     return;
   }
-  float* part = a.part + (ih * a.pieces + piece) * (kRows * (D + 2));
+  constexpr int64_t kPart = kRows * (D + 2);
+  float* part = a.part + (ih * a.pieces + piece) * kPart;
+  if (!a.tickets) {
+    if (R >= rows) return;
 #pragma unroll
-  for (int e = 0; e < kPer / 4; ++e)
-    *reinterpret_cast<float4*>(part + r * D + c0 + 4 * e) = make_float4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
-  if (c0 == 0) {
-    part[kRows * D + 2 * r] = top;
-    part[kRows * D + 2 * r + 1] = l;
+    for (int e = 0; e < kPer / 4; ++e)
+      *reinterpret_cast<float4*>(part + r * D + c0 + 4 * e) = make_float4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
+    if (c0 == 0) *reinterpret_cast<float2*>(part + kRows * D + 2 * r) = make_float2(top, l);
+    return;
+  }
+  if (R < rows) {
+#pragma unroll
+    for (int e = 0; e < kPer; ++e) put_shared(part + r * D + c0 + e, o[e]);
+    if (c0 == 0) {
+      put_shared(part + kRows * D + 2 * r, top);
+      put_shared(part + kRows * D + 2 * r + 1, l);
+    }
+  }
+  // The last workgroup of the sequence's items joins them.  Each one's partial results are visible on every die
+  // before its ticket is counted; the ticket is a zero again afterwards.
+  __shared__ int last_one;
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  __syncthreads();
+  const int items = next - s.split0;
+  if (threadIdx.x == 0) {
+    int* ticket = a.tickets + (static_cast<int64_t>(s.slot) * a.H + h) * kTickets + piece;
+    last_one = __hip_atomic_fetch_add(ticket, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == items - 1;
+    if (last_one) __hip_atomic_store(ticket, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  }
+  __syncthreads();
+  if (!last_one) return;
+  const float* first = a.part + ((static_cast<int64_t>(s.split0) * a.H + h) * a.pieces + piece) * kPart;
+  for (int i = wave; i < kRows && piece * kRows + i < rows; i += kWaves) {
+    const int Ri = piece * kRows + i;
+    join_row<D, BF16, true>(first, a.H * a.pieces * kPart, items, i, a.out + ((static_cast<int64_t>(s.row0) + Ri / a.rep) * Hq + h * a.rep + Ri % a.rep) * D);
   }
 }
 
@@ -401,29 +478,7 @@ __global__ __launch_bounds__(kThreads) void paged_merge_kernel(DecodeArgs a, int
   const int R = (n - s.row0) * a.rep + head % a.rep, piece = R / kRows, r = R % kRows;
   constexpr int64_t kPart = kRows * (D + 2);
   const int64_t stride = static_cast<int64_t>(a.H) * a.pieces * kPart;
-  const float* part = a.part + (static_cast<int64_t>(s.split0) * a.H + h) * a.pieces * kPart + piece * kPart;
-  float top = -INFINITY, l = 0.0f, o[D / 64] = {};
-  for (int i0 = 0; i0 < items; i0 += 64) {
-    const int i = i0 + lane;
-    const float2 st = i < items ? *reinterpret_cast<const float2*>(part + i * stride + kRows * D + 2 * r) : make_float2(-INFINITY, 0.0f);
-    const float m = fmaxf(top, wave_max(st.x)), safe = m == -INFINITY ? 0.0f : m;
-    const float old = __builtin_amdgcn_exp2f(top - safe), f = __builtin_amdgcn_exp2f(st.x - safe);
-    l = l * old + wave_sum(f * st.y);
-#pragma unroll
-    for (int e = 0; e < D / 64; ++e) o[e] *= old;
-    const int most = items - i0 < 64 ? items - i0 : 64;
-    for (int k = 0; k < most; ++k) {
-      const float fk = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(f), k));
-      const float* p = part + (i0 + k) * stride + r * D + lane * (D / 64);
-#pragma unroll
-      for (int e = 0; e < D / 64; ++e) o[e] += fk * p[e];
-    }
-    top = m;
-  }
-  const float inv = 1.0f / l;
-  uint16_t* out = a.out + at * D + lane * (D / 64);
-#pragma unroll
-  for (int e = 0; e < D / 64; ++e) out[e] = BF16 ? f32_to_bf16(o[e] * inv) : f32_to_f16(o[e] * inv);
+  join_row<D, BF16, false>(a.part + (static_cast<int64_t>(s.split0) * a.H + h) * a.pieces * kPart + piece * kPart, stride, items, r, a.out + at * D);
 }
 
 int64_t pieces_of(int64_t rep, int64_t most) { return (rep * most + kRows - 1) / kRows; }
@@ -441,7 +496,8 @@ extern "C" int64_t kvq_paged_decode_workspace(int64_t split_items, int64_t H, in
 extern "C" int kvq_paged_decode(const void* q, int64_t q_st, int64_t q_sh, int dtype, int64_t rows, int64_t Hq, int64_t H, int64_t D,
                                 float scaling, const int32_t* step, int64_t split_items, int64_t max_count, const int32_t* table,
                                 int64_t max_blocks, int64_t P, int code, const uint8_t* kc, const uint8_t* vc, const float* sc,
-                                const void* ko, const void* vo, void* out, float* workspace, int64_t workspace_floats, void* stream) {
+                                const void* ko, const void* vo, void* out, float* workspace, int64_t workspace_floats, int32_t* tickets,
+                                void* stream) {
   KVQ_REQUIRE(D == 64 || D == 128, "kvq_paged_decode: head_dim must be 64 or 128 (got %lld)", static_cast<long long>(D));
   KVQ_REQUIRE(P == 32 || P == 64 || P == 128, "kvq_paged_decode: pages hold 32, 64 or 128 tokens");
   KVQ_REQUIRE(dtype == KVQ_F16 || dtype == KVQ_BF16, "kvq_paged_decode: queries must be fp16 or bf16");
@@ -456,7 +512,10 @@ extern "C" int kvq_paged_decode(const void* q, int64_t q_st, int64_t q_sh, int d
               static_cast<long long>(need));
   DecodeArgs a{static_cast<const uint16_t*>(q), q_st, q_sh, step, table, max_blocks, static_cast<int>(H), static_cast<int>(rep),
                static_cast<int>(pieces_of(rep, max_count)), scaling * 1.44269504088896341f, kc, vc, sc,
-               static_cast<const uint16_t*>(ko), static_cast<const uint16_t*>(vo), static_cast<uint16_t*>(out), workspace};
+               static_cast<const uint16_t*>(ko), static_cast<const uint16_t*>(vo), static_cast<uint16_t*>(out), workspace,
+               pieces_of(rep, max_count) <= kTickets && split_items * H * pieces_of(rep, max_count) <= 256 ? tickets : nullptr};
+  // Joining in the launch: 128 workgroups 14.2 -> 10.3 us, 768 of them 23.9 -> 26.1 (their stores past the caches
+  // and the wait for the last one); so only where every workgroup has a CU of its own.
   const int64_t blocks = (split_items * H + 7) / 8 * 8 * a.pieces, merges = (rows * Hq + kWaves - 1) / kWaves;
   KVQ_REQUIRE(blocks < INT64_C(1) << 31 && merges < INT64_C(1) << 31, "kvq_paged_decode: too many rows");
   auto run = [&](auto d, auto p, auto c, auto t) {
@@ -464,7 +523,7 @@ extern "C" int kvq_paged_decode(const void* q, int64_t q_st, int64_t q_sh, int d
     constexpr bool T_ = decltype(t)::value != 0;
     hipLaunchKernelGGL((paged_split_kernel<D_, P_, C_, T_>), dim3(static_cast<uint32_t>(blocks)), dim3(kThreads), 0,
                        static_cast<hipStream_t>(stream), a);
-    hipLaunchKernelGGL((paged_merge_kernel<D_, T_>), dim3(static_cast<uint32_t>(merges)), dim3(kThreads), 0,
+    if (!a.tickets) hipLaunchKernelGGL((paged_merge_kernel<D_, T_>), dim3(static_cast<uint32_t>(merges)), dim3(kThreads), 0,
                        static_cast<hipStream_t>(stream), a, rows * Hq);
   };
   using Zero = std::integral_constant<int, 0>;

@@ -24,7 +24,9 @@ from .prompt import device_of, rows16
 
 CODES = {"int8": 0, "e4m3": 1}
 PAGES = (32, 64, 128)
-SPLIT_BLOCKS = 768                             # workgroups a decode is split into at most: three on each of 256 CUs
+# workgroups a decode is split into at most, by head_dim: two and three on each of 256 CUs.  16 sequences at 32k,
+# head_dim 128: 197 us with 512, 202 with 768; 48 ragged ones, head_dim 64: 40 with 512, 33 with 768, 34 with 1024.
+SPLIT_BLOCKS = {128: 512, 64: 768}
 
 
 def _ints(x, what: str) -> np.ndarray:
@@ -37,7 +39,7 @@ def _ints(x, what: str) -> np.ndarray:
 class Step:
     """New tokens of some slots: ``rows`` packed rows, slot by slot.  Made by ``PagedCache.extend``."""
 
-    __slots__ = ("slots", "counts", "ends", "rows", "items", "splits", "max_count", "desc", "host", "generation", "stamp")
+    __slots__ = ("slots", "counts", "ends", "rows", "items", "splits", "max_count", "desc", "ptr", "host", "generation", "stamp")
 
 
 class PagedCache:
@@ -74,6 +76,9 @@ class PagedCache:
         rows = (self.layers, self.slots, 2, self.Hkv, self.page * self.d)
         self.k_open = torch.zeros(rows, dtype=dtype, device=self.device)     # token major, as a page's keys
         self.v_open = torch.zeros(rows, dtype=dtype, device=self.device)     # channel major, as a page's values
+        # counters of the decodes that join their parts in one launch: zeros between calls
+        self._counters = torch.zeros((self.layers, self.slots, self.Hkv, 4), dtype=torch.int32, device=self.device)
+        self._tickets = [self._counters[l].data_ptr() for l in range(self.layers)]
         self._set_addresses()
 
     def _pool(self, pages: int):
@@ -87,7 +92,9 @@ class PagedCache:
         self._host = tuple(x.ctypes.data for x in (self._lens, self._table, self._refs, self._open, self._account))
 
     def _set_addresses(self) -> None:
-        """Of each layer's codes, scales and open blocks."""
+        """Of each layer's codes, scales and open blocks; what every call passes."""
+        self._index, self._type = self.device.index, _lib.DTYPE_CODE[self.dtype]
+        self._fixed = (self.table.data_ptr(), self.max_blocks, self.Hkv, self.d, self.page, CODES[self.code])
         parts = [(x.data_ptr(), x.stride(0) * x.element_size()) for x in (self.kc, self.vc, self.sc, self.k_open, self.v_open)]
         self._at = [tuple(p + l * step for p, step in parts) for l in range(self.layers)]
 
@@ -134,14 +141,15 @@ class PagedCache:
             st = Step()
             st.host = np.empty(words, dtype=np.int32)
             st.desc = torch.empty(words, dtype=torch.int32, device=self.device)
-            st.splits = max(n, -(-SPLIT_BLOCKS // self.Hkv))
+            st.ptr = st.desc.data_ptr()
+            st.splits = max(n, -(-SPLIT_BLOCKS[self.d] // self.Hkv))
         else:
             st = into
             if not np.array_equal(st.counts, c):
                 raise ValueError("a step is rewritten for the same counts only")
         _lib.call_on(self.device, "kvq_pages_extend", *self._host, self.slots, self.pages, self.max_blocks, self.page,
                      self.max_tokens, s.ctypes.data, c.ctypes.data, n, st.splits, st.host.ctypes.data, st.host.size,
-                     st.desc.data_ptr(), _lib.stream_of(st.desc))
+                     st.ptr, _lib.stream_of(st.desc))
         if into is None:
             st.splits = max(1, int(st.host[2]))         # what later steps written into this one keep to
             st.items = st.host.size - 8 * (n + 2)
@@ -160,40 +168,38 @@ class PagedCache:
     def append(self, layer: int, k: torch.Tensor, v: torch.Tensor, step: Step) -> None:
         """The step's new rows k, v (rows, Hkv, d) of one layer, slot by slot: full blocks to codes, the rest to the open
         blocks.  Running it again writes the same."""
-        self._layer(layer)
+        if not 0 <= layer < self.layers:
+            raise IndexError(f"no layer {layer} (of {self.layers})")
         shape = (step.rows, self.Hkv, self.d)
         if k.shape != shape or v.shape != shape:
             raise ValueError(f"append: k {tuple(k.shape)} and v {tuple(v.shape)} must be {shape}")
         if k.dtype != self.dtype or v.dtype != self.dtype:
             raise TypeError("appended rows must have the cache's dtype")
-        if k.device != self.device or v.device != self.device:
+        if k.get_device() != self._index or v.get_device() != self._index:
             _lib.require_gpu(k, v)
             raise ValueError(f"append: the cache is on {self.device}")
-        self.check_step(step, "append")
+        if step.stamp != self._stamp:
+            self.check_step(step, "append")
         if step.generation != self._generation:
             raise ValueError("append: the pages have moved since the step was made")
         if step.rows == 0:
             return
-        k, v = rows16(k), rows16(v)
-        _lib.call_on(self.device, "kvq_pages_append", k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(), v.stride(0), v.stride(1),
-                     _lib.DTYPE_CODE[self.dtype], step.desc.data_ptr(), step.items, self.table.data_ptr(), self.max_blocks,
-                     self.Hkv, self.d, self.page, CODES[self.code], *self._at[layer], _lib.stream_of(k))
-
-    def _layer(self, layer: int) -> None:
-        if not 0 <= layer < self.layers:
-            raise IndexError(f"no layer {layer} (of {self.layers})")
+        k, kt, kh = rows16(k)
+        v, vt, vh = rows16(v)
+        _lib.call_on(self.device, "kvq_pages_append", k.data_ptr(), kt, kh, v.data_ptr(), vt, vh, self._type, step.ptr, step.items,
+                     *self._fixed, *self._at[layer], _lib.stream_of(k))
 
     def rows(self, layer: int, slots: Sequence[int]) -> Tuple[torch.Tensor, torch.Tensor]:
         """All tokens of the slots, one behind the other, as dense rows k, v (tokens, Hkv, d): code times scale, rounded
         once, and the open blocks as they are.  With prompt_attention this is the attention of many new tokens."""
-        self._layer(layer)
+        if not 0 <= layer < self.layers:
+            raise IndexError(f"no layer {layer} (of {self.layers})")
         s = _ints(slots, "slots")
         if s.min() < 0 or s.max() >= self.slots:
             raise _lib.KVQError(f"rows: no slot {s.min() if s.min() < 0 else s.max()} (of {self.slots})")
         out = torch.empty((2, int(self._lens[s].sum()), self.Hkv, self.d), dtype=self.dtype, device=self.device)
         k, v = out.unbind(0)
-        _lib.call_on(self.device, "kvq_pages_rows", self._host[0], self._host[3], self.slots, s.ctypes.data, s.size, self.table.data_ptr(),
-                     self.max_blocks, self.Hkv, self.d, self.page, CODES[self.code], _lib.DTYPE_CODE[self.dtype], *self._at[layer],
+        _lib.call_on(self.device, "kvq_pages_rows", self._host[0], self._host[3], self.slots, s.ctypes.data, s.size, *self._fixed, self._type, *self._at[layer],
                      k.data_ptr(), v.data_ptr(), k.numel(), _lib.stream_of(out))
         return k, v
 
@@ -272,27 +278,30 @@ def paged_decode(q: torch.Tensor, scaling: float, cache: PagedCache, layer: int,
     """Attention of the step's query rows q (rows, Hq, d), slot by slot, over the cache; returns (rows, Hq, d).  Query i of
     a slot's new tokens sees every token up to its own.  Meant for a few tokens per slot (16 rows = query
     heads of a KV head times tokens go over the keys together); for many, ``cache.rows`` and prompt_attention."""
-    cache._layer(layer)
-    if q.dim() != 3 or q.shape[0] != step.rows or q.shape[2] != cache.d or q.shape[1] < 1 or q.shape[1] % cache.Hkv:
-        raise ValueError(f"paged_decode: q {tuple(q.shape)} does not match the step ({step.rows} rows) and the cache "
-                         f"({cache.Hkv} KV heads, head_dim {cache.d})")
+    if not 0 <= layer < cache.layers:
+        raise IndexError(f"no layer {layer} (of {cache.layers})")
+    shape, Hkv, d = q.shape, cache.Hkv, cache.d
+    if len(shape) != 3 or shape[0] != step.rows or shape[2] != d or shape[1] < 1 or shape[1] % Hkv:
+        raise ValueError(f"paged_decode: q {tuple(shape)} does not match the step ({step.rows} rows) and the cache "
+                         f"({Hkv} KV heads, head_dim {d})")
     if q.dtype != cache.dtype:
         raise TypeError("q must have the cache's dtype")
-    if q.device != cache.device:
+    if q.get_device() != cache._index:
         _lib.require_gpu(q)
         raise ValueError(f"paged_decode: the cache is on {cache.device}")
-    cache.check_step(step, "paged_decode")
-    q = rows16(q)
-    Hq = q.shape[1]
-    out = _lib.out_or_new(out, (step.rows, Hq, cache.d), q.dtype, q.device, "paged_decode")
+    if step.stamp != cache._stamp:
+        cache.check_step(step, "paged_decode")
+    q, qt, qh = rows16(q)
+    Hq, device = shape[1], cache.device
+    out = torch.empty(shape, dtype=cache.dtype, device=device) if out is None else _lib.out_or_new(out, shape, cache.dtype, device, "paged_decode")
     if step.rows == 0:
         return out
     if workspace is None:
-        workspace = torch.empty((paged_workspace_floats(step, Hq, cache.Hkv, cache.d),), dtype=torch.float32, device=q.device)
-    elif workspace.dtype != torch.float32 or not workspace.is_contiguous() or workspace.device != q.device:
+        workspace = torch.empty((paged_workspace_floats(step, Hq, Hkv, d),), dtype=torch.float32, device=device)
+    elif workspace.dtype != torch.float32 or not workspace.is_contiguous() or workspace.device != device:
         raise ValueError("workspace must be contiguous float32 on the cache's device")
-    _lib.call_on(q.device, "kvq_paged_decode", q.data_ptr(), q.stride(0), q.stride(1), _lib.DTYPE_CODE[q.dtype], step.rows, Hq, cache.Hkv,
-                 cache.d, float(scaling), step.desc.data_ptr(), step.splits, step.max_count, cache.table.data_ptr(),
-                 cache.max_blocks, cache.page, CODES[cache.code], *cache._at[layer], out.data_ptr(), workspace.data_ptr(),
-                 workspace.numel(), _lib.stream_of(q))
+    table, max_blocks, _, _, page, code = cache._fixed
+    _lib.call_on(device, "kvq_paged_decode", q.data_ptr(), qt, qh, cache._type, step.rows, Hq, Hkv, d, float(scaling), step.ptr,
+                 step.splits, step.max_count, table, max_blocks, page, code, *cache._at[layer], out.data_ptr(), workspace.data_ptr(),
+                 workspace.numel(), cache._tickets[layer], _lib.stream_of(q))
     return out

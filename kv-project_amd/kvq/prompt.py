@@ -76,25 +76,28 @@ def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, scaling:
     if q.device != plan.device or k.device != plan.device or v.device != plan.device:
         _lib.require_gpu(q, k, v)
         raise ValueError(f"prompt_attention: the plan is for {plan.device}")
-    q, k, v = (rows16(x) for x in (q, k, v))
     out = _lib.out_or_new(out, (plan.rows, plan.Hq, d), q.dtype, q.device, "prompt_attention")
     if plan.keys == 0:
         return out.zero_()
-    if workspace is None:
-        if plan.parts:
-            workspace = torch.empty((plan.workspace_floats(d),), dtype=torch.float32, device=q.device)
-    elif workspace.dtype != torch.float32 or not workspace.is_contiguous() or workspace.device != q.device:
-        raise ValueError("workspace must be contiguous float32 on the plan's device")
-    ws, floats = (None, 0) if workspace is None else (workspace.data_ptr(), workspace.numel())
-    _lib.call_on(q.device, "kvq_prompt_attention", q.data_ptr(), q.stride(0), q.stride(1), k.data_ptr(), k.stride(0), k.stride(1),
-                 v.data_ptr(), v.stride(0), v.stride(1), _lib.DTYPE_CODE[q.dtype], plan.Hq, plan.Hkv, d, float(scaling),
-                 plan.words.data_ptr(), plan.items, plan.merges, plan.parts, out.data_ptr(), ws, floats, _lib.stream_of(q))
+    (q, qt, qh), (k, kt, kh), (v, vt, vh) = rows16(q), rows16(k), rows16(v)
+    ws, floats = None, 0
+    if workspace is not None:
+        if workspace.dtype != torch.float32 or not workspace.is_contiguous() or workspace.device != q.device:
+            raise ValueError("workspace must be contiguous float32 on the plan's device")
+    elif plan.parts:
+        workspace = torch.empty((plan.workspace_floats(d),), dtype=torch.float32, device=q.device)
+    if workspace is not None:
+        ws, floats = workspace.data_ptr(), workspace.numel()
+    _lib.call_on(plan.device, "kvq_prompt_attention", q.data_ptr(), qt, qh, k.data_ptr(), kt, kh, v.data_ptr(), vt, vh,
+                 _lib.DTYPE_CODE[q.dtype], plan.Hq, plan.Hkv, d, float(scaling), plan.words.data_ptr(), plan.items, plan.merges, plan.parts,
+                 out.data_ptr(), ws, floats, _lib.stream_of(q))
     return out
 
 
-def rows16(x: torch.Tensor) -> torch.Tensor:
-    """x (rows, heads, d) itself when the kernels can read it in 16-byte pieces, or a copy."""
+def rows16(x: torch.Tensor):
+    """x (rows, heads, d) with its row and head strides, or a copy where the kernels cannot read it in 16-byte pieces."""
     st, sh, sd = x.stride()
     if sd != 1 or (st | sh) % 8 or x.data_ptr() % 16 or not 0 <= st < 1 << 24:
-        return x.detach().clone(memory_format=torch.contiguous_format)
-    return x
+        x = x.detach().clone(memory_format=torch.contiguous_format)
+        st, sh, _ = x.stride()
+    return x, st, sh

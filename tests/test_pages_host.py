@@ -197,6 +197,6 @@ def test_kernel_entries_refuse_before_any_launch():
     assert rc == 1 and b"code" in lib.kvq_last_error()
     need = lib.kvq_paged_decode_workspace(4, 2, 2, 1, 64)
     assert need == 4 * 2 * 16 * 66
-    rc = lib.kvq_paged_decode(one, 256, 64, 2, 1, 4, 2, 64, 0.1, one, 4, 1, one, 4, 64, 0, one, one, one, one, one, one, one, need - 1, None)
+    rc = lib.kvq_paged_decode(one, 256, 64, 2, 1, 4, 2, 64, 0.1, one, 4, 1, one, 4, 64, 0, one, one, one, one, one, one, one, need - 1, None, None)
     assert rc == 1 and b"workspace" in lib.kvq_last_error()
     assert lib.kvq_paged_decode_workspace(4, 2, 2, 1, 96) == -1
