@@ -699,8 +699,10 @@ int kvq_prompt_attention(const void* q, int64_t q_st, int64_t q_sh, const void* 
  * returns.
  * kvq_pages_fork makes empty slots dst share src's pages and copies the open blocks of all layers (ko,
  * vo of layer 0, layers contiguous; table_device NULL: accounts only).  kvq_pages_free (host only) gives slots back.
- * kvq_pages_move copies pages moves[i] = {from, to} (device) of all layers between pools (the same pool: no
- * page both read and written) and maps the table's page numbers through place (device, `pages` entries).
+ * kvq_pages_move moves every page in use from `end` on to the lowest free place, in order, and the others
+ * nowhere: within one pool (pages_to = pages, refs_to = refs, the same kc, vc, sc), or into another of pages_to >=
+ * end pages, all of those in use.  place: host scratch of `pages` int32.  The accounts (refs_to for the new pool) and
+ * the table on the host and the device follow (table_device NULL: host only).
  * ---------------------------------------------------------------------------------------- */
 int64_t kvq_pages_step_words(int64_t page, const int64_t* counts, int64_t n);
 int kvq_pages_extend(int64_t* lens, int32_t* table, int32_t* refs, uint8_t* open, int64_t* account, int64_t slots,
@@ -719,9 +721,10 @@ int kvq_pages_fork(int64_t* lens, int32_t* table, int32_t* refs, uint8_t* open, 
                    int32_t* table_device, void* ko, void* vo, void* stream);
 int kvq_pages_free(int64_t* lens, const int32_t* table, int32_t* refs, uint8_t* open, int64_t* account, int64_t slots,
                    int64_t max_blocks, int64_t page, const int64_t* seq, int64_t n);
-int kvq_pages_move(const uint8_t* kc, const uint8_t* vc, const float* sc, int64_t pages, uint8_t* kc_to, uint8_t* vc_to,
-                   float* sc_to, int64_t pages_to, int64_t layers, int64_t H, int64_t D, int64_t page,
-                   const int32_t* moves, int64_t n, const int32_t* place, int32_t* table, int64_t entries, void* stream);
+int kvq_pages_move(const int64_t* lens, int32_t* table, const int32_t* refs, int32_t* refs_to, int64_t* account,
+                   int64_t slots, int64_t pages, int64_t pages_to, int64_t end, int64_t max_blocks, int64_t page,
+                   int32_t* place, int64_t layers, int64_t H, int64_t D, const uint8_t* kc, const uint8_t* vc,
+                   const float* sc, uint8_t* kc_to, uint8_t* vc_to, float* sc_to, int32_t* table_device, void* stream);
 
 /* ------------------------------------------------------------------------------------------
  * Attention of a step's query rows over the paged cache: q (rows, Hq, D), the step's rows in order; query

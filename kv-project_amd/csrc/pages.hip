@@ -58,12 +58,15 @@ __device__ __forceinline__ uint32_t abs_max2(uint32_t m, uint32_t w) {
   return m > b ? m : b;
 }
 
+// Four values of at most the type's top as codes, rounded to nearest even.  int8: 1.5 2^23 + x is a float32 whose
+// low byte is the rounded x.
 template <int CODE>
 __device__ __forceinline__ uint32_t encode4(float a, float b, float c, float d) {
+#pragma clang fp contract(off)
   if constexpr (CODE == kCodeInt8) {
-    const int x = static_cast<int>(__builtin_rintf(a)), y = static_cast<int>(__builtin_rintf(b));
-    const int z = static_cast<int>(__builtin_rintf(c)), w = static_cast<int>(__builtin_rintf(d));
-    return (x & 255) | (y & 255) << 8 | (z & 255) << 16 | static_cast<uint32_t>(w) << 24;
+    const uint32_t x = __float_as_uint(a + 12582912.0f), y = __float_as_uint(b + 12582912.0f);
+    const uint32_t z = __float_as_uint(c + 12582912.0f), w = __float_as_uint(d + 12582912.0f);
+    return __builtin_amdgcn_perm(__builtin_amdgcn_perm(w, z, 0x0c0c0400u), __builtin_amdgcn_perm(y, x, 0x0c0c0400u), 0x05040100u);
   } else {
     int r = __builtin_amdgcn_cvt_pk_fp8_f32(a, b, 0, false);
     return static_cast<uint32_t>(__builtin_amdgcn_cvt_pk_fp8_f32(c, d, r, true));
@@ -94,8 +97,10 @@ __global__ __launch_bounds__(kThreads) void append_kernel(Rows16 k, Rows16 v, co
                                                           uint16_t* __restrict__ ko, uint16_t* __restrict__ vo) {
   constexpr int kChunks = P * D / 8, kPer = kChunks / kThreads;      // pieces of 8 elements, per thread
   constexpr int kRow = D / 8;                                       // pieces of a token
-  constexpr int kPitch = P + 8;                                     // 16-bit elements of a channel in LDS
-  __shared__ uint16_t turn[D * kPitch];
+  // values turn to channel-major order in LDS: channel c's tokens 8 u .. at piece u ^ (c / 8) of its row, so that
+  // the channels of a wavefront's writes (8 apart) do not meet in the same banks
+  __shared__ __align__(16) uint16_t turn[D * P];
+  auto place = [](int c, int t) { return c * P + (((t >> 3) ^ (c >> 3)) & (P / 8 - 1)) * 8 + (t & 7); };
   __shared__ uint32_t top[8];
   const int item = blockIdx.x / H, h = blockIdx.x % H, tid = threadIdx.x;
   const int n = step[0];
@@ -141,23 +146,41 @@ __global__ __launch_bounds__(kThreads) void append_kernel(Rows16 k, Rows16 v, co
     kmax = abs_max2(abs_max2(abs_max2(abs_max2(kmax, kw[i].x), kw[i].y), kw[i].z), kw[i].w);
   }
   const int old = from - first;                                     // tokens that lie in the open buffer
+  if (old == 0) {
 #pragma unroll
-  for (int i = 0; i < kPer; ++i) {
-    const int q = tid + i * kThreads, t = q / kRow, c = q % kRow * 8;
-    if (t >= old) {
+    for (int i = 0; i < (kPer + 1) / 2; ++i) {                      // two tokens at a time: words of a channel's pair
+      const int q = tid + i * kThreads, t = q / kRow * 2, c = q % kRow * 8;
+      if (kPer % 2 && q >= kChunks / 2) break;
+      const uint16_t* at = vn + (row0 + first + t) * v.st + c;
+      const uint4 x = *reinterpret_cast<const uint4*>(at), y = *reinterpret_cast<const uint4*>(at + v.st);
+      const uint32_t xs[4] = {x.x, x.y, x.z, x.w}, ys[4] = {y.x, y.y, y.z, y.w};
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        *reinterpret_cast<uint32_t*>(turn + place(c + e, t)) = __builtin_amdgcn_perm(ys[e >> 1], xs[e >> 1], e & 1 ? 0x07060302u : 0x05040100u);
+    }
+  } else {
+    for (int i = tid; i < (P - old) * kRow; i += kThreads) {
+      const int t = old + i / kRow, c = i % kRow * 8;
       const uint4 w = *reinterpret_cast<const uint4*>(vn + (row0 + first + t) * v.st + c);
       const uint32_t ws[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
-      for (int e = 0; e < 8; ++e) turn[(c + e) * kPitch + t] = static_cast<uint16_t>(ws[e >> 1] >> (16 * (e & 1)));
+      for (int e = 0; e < 8; ++e) turn[place(c + e, t)] = static_cast<uint16_t>(ws[e >> 1] >> (16 * (e & 1)));
+    }
+    for (int i = tid; i < D * (P / 8); i += kThreads) {             // pieces of 8 tokens, the last one in part
+      const int c = i / (P / 8), t = i % (P / 8) * 8;
+      if (t + 8 <= old) {
+        *reinterpret_cast<uint4*>(turn + place(c, t)) = *reinterpret_cast<const uint4*>(vb + c * P + t);
+      } else {
+        for (int e = 0; e < 8 && t + e < old; ++e) turn[place(c, t + e)] = vb[c * P + t + e];
+      }
     }
   }
-  for (int i = tid; i < D * old; i += kThreads) turn[i / old * kPitch + i % old] = vb[i / old * P + i % old];
   __syncthreads();
   uint4 vw[kPer];                                                   // pieces of 8 tokens of a channel
 #pragma unroll
   for (int i = 0; i < kPer; ++i) {
     const int q = tid + i * kThreads, c = q / (P / 8), t = q % (P / 8) * 8;
-    vw[i] = *reinterpret_cast<const uint4*>(turn + c * kPitch + t);
+    vw[i] = *reinterpret_cast<const uint4*>(turn + place(c, t));
     vmax = abs_max2(abs_max2(abs_max2(abs_max2(vmax, vw[i].x), vw[i].y), vw[i].z), vw[i].w);
   }
   for (int o = 32; o; o >>= 1) {
@@ -184,6 +207,7 @@ __global__ __launch_bounds__(kThreads) void append_kernel(Rows16 k, Rows16 v, co
     if (h == 0) table[s.slot * max_blocks + j] = page;
   }
   auto put = [&](uint8_t* dst, const uint4& w, const Scale& z) {
+#pragma clang fp contract(off)                                      // the product is rounded before it is rounded to a code
     const bool bad = z.inv == 0.0f;                                 // 0 * inf would be a NaN code
     const uint32_t ws[4] = {bad ? 0 : w.x, bad ? 0 : w.y, bad ? 0 : w.z, bad ? 0 : w.w};
     float x[8];
@@ -324,10 +348,14 @@ struct Pool {
   float* sc;
 };
 
-// Workgroup (move, layer): one page with all its heads.  moves: {from, to} pairs on the device.
-__global__ __launch_bounds__(kThreads) void move_kernel(Pool s, Pool d, int64_t s_pages, int64_t d_pages, const int* __restrict__ moves, int H,
-                                                        int64_t page_bytes) {
-  const int64_t layer = blockIdx.y, from = layer * s_pages + moves[2 * blockIdx.x], to = layer * d_pages + moves[2 * blockIdx.x + 1];
+// {from, to} of each page
+struct Moves {
+  int w[kWords];
+};
+
+// Workgroup (move, layer): one page with all its heads.
+__global__ __launch_bounds__(kThreads) void move_kernel(Moves m, Pool s, Pool d, int64_t s_pages, int64_t d_pages, int H, int64_t page_bytes) {
+  const int64_t layer = blockIdx.y, from = layer * s_pages + m.w[2 * blockIdx.x], to = layer * d_pages + m.w[2 * blockIdx.x + 1];
   const uint4* a = reinterpret_cast<const uint4*>(s.kc + from * page_bytes);
   const uint4* b = reinterpret_cast<const uint4*>(s.vc + from * page_bytes);
   uint4* x = reinterpret_cast<uint4*>(d.kc + to * page_bytes);
@@ -339,12 +367,18 @@ __global__ __launch_bounds__(kThreads) void move_kernel(Pool s, Pool d, int64_t 
   for (int i = threadIdx.x; i < 2 * H; i += kThreads) d.sc[to * 2 * H + i] = s.sc[from * 2 * H + i];
 }
 
-// every page number of the table through place (dead pages: any number in range)
-__global__ __launch_bounds__(kThreads) void remap_kernel(int* __restrict__ table, int64_t n, const int* __restrict__ place, int pages) {
+// entries of the table that name a page behind the new end: those in use are written again by patch_kernel
+__global__ __launch_bounds__(kThreads) void clip_kernel(int* __restrict__ table, int64_t n, int pages) {
   const int64_t i = static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x;
-  if (i >= n) return;
-  const int p = table[i];
-  table[i] = p >= 0 && p < pages ? place[p] : 0;
+  if (i < n && table[i] >= pages) table[i] = 0;
+}
+
+// {slot, block, page}
+struct Patches {
+  int w[kWords];
+};
+__global__ __launch_bounds__(kThreads) void patch_kernel(Patches p, int n, int* __restrict__ table, int64_t max_blocks) {
+  for (int i = threadIdx.x; i < n; i += kThreads) table[p.w[3 * i] * max_blocks + p.w[3 * i + 1]] = p.w[3 * i + 2];
 }
 
 // ---- the accounts (host) ----------------------------------------------------------------------
@@ -362,7 +396,7 @@ int64_t splits_of(const int32_t* e, int64_t page, int64_t per) {    // none for 
 // Fills the description from lens (before), counts and open buffers.  Returns the number of items.
 int64_t describe(const int64_t* lens, const uint8_t* open, int64_t page, const int64_t* seq, const int64_t* counts, int64_t n,
                  int64_t split_cap, int32_t* desc) {
-  int64_t row = 0, item = 0, most = 0;
+  int64_t row = 0, item = 0, most = 0, longest = 0;
   bool even = true;
   for (int64_t i = 0; i < n; ++i) {
     int32_t* e = desc + kStepHead + kStepSeq * i;
@@ -376,6 +410,7 @@ int64_t describe(const int64_t* lens, const uint8_t* open, int64_t page, const i
     e[6] = src | dst << 1;
     e[7] = 0;
     row += count;
+    longest = count > longest ? count : longest;
     item += count ? (end - 1) / page - pos0 / page + 1 : 0;
     even = even && item == i + 1;
     const int64_t u = units_of(end, page);
@@ -409,6 +444,7 @@ int64_t describe(const int64_t* lens, const uint8_t* open, int64_t page, const i
   desc[2] = static_cast<int32_t>(split);
   desc[3] = static_cast<int32_t>(lo);
   desc[4] = even;
+  desc[5] = static_cast<int32_t>(longest);
   return item;
 }
 
@@ -649,20 +685,78 @@ extern "C" int kvq_pages_free(int64_t* lens, const int32_t* table, int32_t* refs
   return KVQ_OK;
 }
 
-extern "C" int kvq_pages_move(const uint8_t* kc, const uint8_t* vc, const float* sc, int64_t pages, uint8_t* kc_to, uint8_t* vc_to,
-                              float* sc_to, int64_t pages_to, int64_t layers, int64_t H, int64_t D, int64_t page, const int32_t* moves,
-                              int64_t n, const int32_t* place, int32_t* table, int64_t entries, void* stream) {
-  KVQ_REQUIRE(page_ok(page, D) && H > 0 && layers > 0 && layers < 65536 && n >= 0 && entries >= 0, "kvq_pages_move: bad sizes");
-  KVQ_REQUIRE((n == 0 || (kc && vc && sc && kc_to && vc_to && sc_to && moves)) && (entries == 0 || (place && table)),
-              "kvq_pages_move: null pointer");
-  KVQ_REQUIRE(n < INT64_C(1) << 31 && pages < INT64_C(1) << 31 && entries / kThreads < INT64_C(1) << 30, "kvq_pages_move: too many pages");
-  const Pool s{const_cast<uint8_t*>(kc), const_cast<uint8_t*>(vc), const_cast<float*>(sc)}, d{kc_to, vc_to, sc_to};
-  if (n)
-    hipLaunchKernelGGL(move_kernel, dim3(static_cast<uint32_t>(n), static_cast<uint32_t>(layers)), dim3(kThreads), 0,
-                       static_cast<hipStream_t>(stream), s, d, pages, pages_to, moves, static_cast<int>(H), H * D * page);
-  if (entries)
-    hipLaunchKernelGGL(remap_kernel, dim3(static_cast<uint32_t>((entries + kThreads - 1) / kThreads)), dim3(kThreads), 0,
-                       static_cast<hipStream_t>(stream), table, entries, place, static_cast<int>(pages));
-  KVQ_LAUNCH_CHECK("kvq_pages_move");
+extern "C" int kvq_pages_move(const int64_t* lens, int32_t* table, const int32_t* refs, int32_t* refs_to, int64_t* account, int64_t slots,
+                              int64_t pages, int64_t pages_to, int64_t end, int64_t max_blocks, int64_t page, int32_t* place, int64_t layers,
+                              int64_t H, int64_t D, const uint8_t* kc, const uint8_t* vc, const float* sc, uint8_t* kc_to, uint8_t* vc_to,
+                              float* sc_to, int32_t* table_device, void* stream) {
+  KVQ_REQUIRE(lens && table && refs && refs_to && account && place, "kvq_pages_move: null pointer");
+  KVQ_REQUIRE(page_ok(page, D) && H > 0 && layers > 0 && layers < 65536 && pages < INT64_C(1) << 31 && pages_to < INT64_C(1) << 31 &&
+                  end >= 0 && end <= pages_to,
+              "kvq_pages_move: bad sizes");
+  KVQ_REQUIRE(!table_device || (kc && vc && sc && kc_to && vc_to && sc_to), "kvq_pages_move: null pointer");
+  const bool same = kc == kc_to;
+  KVQ_REQUIRE(!same || (pages == pages_to && refs == refs_to), "kvq_pages_move: one pool has one size");
+  int64_t used = 0;
+  for (int64_t p = 0; p < pages; ++p) used += refs[p] != 0;
+  KVQ_REQUIRE(used <= end, "kvq_pages_move: %lld pages are in use", static_cast<long long>(used));
+  // pages from `end` on to the lowest free places, in order
+  int64_t hole = 0;
+  for (int64_t p = 0; p < pages; ++p) {
+    place[p] = static_cast<int32_t>(p);
+    if (refs[p] && p >= end) {
+      while (hole < pages && refs[hole]) ++hole;
+      place[p] = static_cast<int32_t>(hole++);
+    }
+  }
+  hipStream_t st = static_cast<hipStream_t>(stream);
+  if (table_device) {
+    const Pool s{const_cast<uint8_t*>(kc), const_cast<uint8_t*>(vc), const_cast<float*>(sc)}, d{kc_to, vc_to, sc_to};
+    Moves m;
+    int n = 0;
+    auto flush = [&] {
+      if (n) hipLaunchKernelGGL(move_kernel, dim3(n, static_cast<uint32_t>(layers)), dim3(kThreads), 0, st, m, s, d, pages, pages_to,
+                                static_cast<int>(H), H * D * page);
+      n = 0;
+    };
+    for (int64_t p = 0; p < pages; ++p) {
+      if (!refs[p] || (same && place[p] == p)) continue;
+      m.w[2 * n] = static_cast<int>(p);
+      m.w[2 * n + 1] = place[p];
+      if (++n == kWords / 2) flush();
+    }
+    flush();
+    if (pages_to < pages) {
+      const int64_t entries = slots * max_blocks;
+      KVQ_REQUIRE(entries / kThreads < INT64_C(1) << 30, "kvq_pages_move: the table is too large");
+      hipLaunchKernelGGL(clip_kernel, dim3(static_cast<uint32_t>((entries + kThreads - 1) / kThreads)), dim3(kThreads), 0, st, table_device,
+                         entries, static_cast<int>(pages_to));
+    }
+  }
+  Patches c;
+  int n = 0;
+  auto flush = [&] {
+    if (n && table_device) hipLaunchKernelGGL(patch_kernel, dim3(1), dim3(kThreads), 0, st, c, n, table_device, max_blocks);
+    n = 0;
+  };
+  for (int64_t i = 0; i < slots; ++i)
+    for (int64_t j = 0; j < lens[i] / page; ++j) {
+      int32_t& p = table[i * max_blocks + j];
+      if (place[p] == p) continue;
+      p = place[p];
+      c.w[3 * n] = static_cast<int>(i);
+      c.w[3 * n + 1] = static_cast<int>(j);
+      c.w[3 * n + 2] = p;
+      if (++n == kWords / 3) flush();
+    }
+  flush();
+  if (!same) memset(refs_to, 0, sizeof(int32_t) * pages_to);
+  for (int64_t p = 0; p < pages; ++p) {
+    if (!refs[p] || (same && place[p] == p)) continue;
+    refs_to[place[p]] = refs[p];                                    // in place: to a page that was free
+    if (same) refs_to[p] = 0;
+  }
+  account[0] = pages_to - used;
+  account[1] = 0;
+  if (table_device) KVQ_LAUNCH_CHECK("kvq_pages_move");
   return KVQ_OK;
 }

@@ -12,7 +12,8 @@
 //   table (slots, max_blocks) int32: the page of each full block
 //
 // A step's description (int32 words on the device): a header of 8 words {sequences, items, split items,
-// units per split, whether every sequence has one item}, then 8 words per sequence {slot, tokens before, new tokens, first packed row, first
+// units per split, whether every sequence has one item, the most new
+// tokens of one}, then 8 words per sequence {slot, tokens before, new tokens, first packed row, first
 // item, first split item, open buffer before | after << 1} and one entry behind the last with the
 // totals, then the page of every item.  An item is a block that the step's tokens touch.
 #pragma once

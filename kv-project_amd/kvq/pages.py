@@ -68,7 +68,8 @@ class PagedCache:
         self._lens = np.zeros(self.slots, dtype=np.int64)
         self._table = np.zeros((self.slots, self.max_blocks), dtype=np.int32)
         self._open = np.zeros(self.slots, dtype=np.uint8)
-        self._set_refs(np.zeros(self.pages, dtype=np.int32))
+        self._refs = np.zeros(self.pages, dtype=np.int32)
+        self._account = np.array([self.pages, 0], dtype=np.int64)   # free pages, none of them below
         self._generation = 0                   # of the pools
         self._stamp = 0                        # of the slots' lengths
         self.table = torch.zeros((self.slots, self.max_blocks), dtype=torch.int32, device=self.device)
@@ -85,14 +86,9 @@ class PagedCache:
         new = lambda *s, dt=torch.int8: torch.empty((self.layers, pages, self.Hkv, *s), dtype=dt, device=self.device)
         return new(self.page, self.d), new(self.d, self.page), new(2, dt=torch.float32)
 
-    def _set_refs(self, refs: np.ndarray) -> None:
-        free = np.flatnonzero(refs == 0)
-        self._refs = refs
-        self._account = np.array([free.size, free[0] if free.size else refs.size], dtype=np.int64)
-        self._host = tuple(x.ctypes.data for x in (self._lens, self._table, self._refs, self._open, self._account))
-
     def _set_addresses(self) -> None:
         """Of each layer's codes, scales and open blocks; what every call passes."""
+        self._host = tuple(x.ctypes.data for x in (self._lens, self._table, self._refs, self._open, self._account))
         self._index, self._type = self.device.index, _lib.DTYPE_CODE[self.dtype]
         self._fixed = (self.table.data_ptr(), self.max_blocks, self.Hkv, self.d, self.page, CODES[self.code])
         parts = [(x.data_ptr(), x.stride(0) * x.element_size()) for x in (self.kc, self.vc, self.sc, self.k_open, self.v_open)]
@@ -153,7 +149,7 @@ class PagedCache:
         if into is None:
             st.splits = max(1, int(st.host[2]))         # what later steps written into this one keep to
             st.items = st.host.size - 8 * (n + 2)
-            st.rows, st.max_count = int(c.sum()), int(c.max())
+            st.rows, st.max_count = int(st.host[8 * n + 11]), int(st.host[5])
         self._stamp += 1
         st.slots, st.counts, st.ends, st.generation, st.stamp = s, c, self._lens[s], self._generation, self._stamp
         return st
@@ -195,9 +191,8 @@ class PagedCache:
         if not 0 <= layer < self.layers:
             raise IndexError(f"no layer {layer} (of {self.layers})")
         s = _ints(slots, "slots")
-        if s.min() < 0 or s.max() >= self.slots:
-            raise _lib.KVQError(f"rows: no slot {s.min() if s.min() < 0 else s.max()} (of {self.slots})")
-        out = torch.empty((2, int(self._lens[s].sum()), self.Hkv, self.d), dtype=self.dtype, device=self.device)
+        total = int(np.add.reduce(self._lens.take(s, mode="clip")))
+        out = torch.empty((2, total, self.Hkv, self.d), dtype=self.dtype, device=self.device)
         k, v = out.unbind(0)
         _lib.call_on(self.device, "kvq_pages_rows", self._host[0], self._host[3], self.slots, s.ctypes.data, s.size, *self._fixed, self._type, *self._at[layer],
                      k.data_ptr(), v.data_ptr(), k.numel(), _lib.stream_of(out))
@@ -237,32 +232,21 @@ class PagedCache:
             raise ValueError(f"{self.pages - self.free_pages} pages are in use")
         if pages >= 1 << 31:
             raise ValueError("too many pages")
-        pool = self._pool(pages)
-        self._move(pages, pool)
-        (self.kc, self.vc, self.sc), self.pages = pool, pages
-        self._set_addresses()
+        self._move(pages, self._pool(pages))
 
     def _move(self, end: int, pool) -> None:
-        live = np.flatnonzero(self._refs)
-        high = live[live >= end]
-        place = np.zeros(self.pages, dtype=np.int32)
-        place[live] = live
-        place[high] = np.flatnonzero(self._refs[:end] == 0)[:high.size]
-        if pool is None and not high.size:
-            return
-        moved = live if pool is not None else high
-        moves = np.stack([moved, place[moved]], 1).astype(np.int32).reshape(-1)
-        # pinned, so that the copy is ordered on the stream without a wait here
-        words = torch.from_numpy(np.concatenate([moves, place])).pin_memory().to(self.device, non_blocking=True)
-        to = (self.kc, self.vc, self.sc) if pool is None else pool
-        _lib.call_on(self.device, "kvq_pages_move", self.kc.data_ptr(), self.vc.data_ptr(), self.sc.data_ptr(), self.pages,
-                     to[0].data_ptr(), to[1].data_ptr(), to[2].data_ptr(), self.pages if pool is None else end, self.layers, self.Hkv,
-                     self.d, self.page, words.data_ptr(), moved.size, words.data_ptr() + 4 * moves.size, self.table.data_ptr(),
-                     self.table.numel(), _lib.stream_of(self.table))
-        refs = np.zeros(self.pages if pool is None else end, dtype=np.int32)
-        refs[place[live]] = self._refs[live]
-        self._table[:] = place[self._table]
-        self._set_refs(refs)
+        """Pages from ``end`` on to the lowest free places; with ``pool``, every page in use into that one of ``end`` pages."""
+        pages = self.pages if pool is None else end
+        refs = self._refs if pool is None else np.empty(pages, dtype=np.int32)
+        place = np.empty(self.pages, dtype=np.int32)
+        src = (self.kc, self.vc, self.sc)
+        _lib.call_on(self.device, "kvq_pages_move", self._host[0], self._host[1], self._host[2], refs.ctypes.data, self._host[4], self.slots,
+                     self.pages, pages, end, self.max_blocks, self.page, place.ctypes.data, self.layers, self.Hkv, self.d,
+                     *[x.data_ptr() for x in src], *[x.data_ptr() for x in (src if pool is None else pool)], self._fixed[0],
+                     _lib.stream_of(self.table))
+        if pool is not None:
+            (self.kc, self.vc, self.sc), self.pages, self._refs = pool, pages, refs
+            self._set_addresses()
         self._generation += 1
 
 

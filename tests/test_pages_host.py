@@ -39,6 +39,16 @@ class Host:
         s = np.array(slots, np.int64)
         return self.lib.kvq_pages_free(*self.p, self.slots, self.blocks, self.page, s.ctypes.data, len(s))
 
+    def move(self, end, pages, same):
+        refs = self.refs if same else np.zeros(pages, np.int32)
+        place = np.zeros(len(self.refs), np.int32)
+        rc = self.lib.kvq_pages_move(*self.p[:3], refs.ctypes.data, self.p[4], self.slots, self.pages, pages, end, self.blocks, self.page,
+                                     place.ctypes.data, 1, 1, 64, 16, 16, 16, *([16] * 3 if same else [32] * 3), None, None)
+        if rc == 0:
+            self.refs, self.pages = refs, pages
+            self.p[2] = refs.ctypes.data
+        return rc
+
     def error(self):
         return self.lib.kvq_last_error()
 
@@ -55,7 +65,7 @@ def test_accounts_follow_the_model(page):
     rng = random.Random(page)
     host, model = Host(9, 40, 20 * page, page), Accounts(9, 40, page)
     for _ in range(300):
-        op = rng.choice(["extend", "extend", "extend", "fork", "free"])
+        op = rng.choice(["extend", "extend", "extend", "extend", "fork", "free", "move"])
         if op == "extend":
             slots = rng.sample(range(9), rng.randint(1, 4))
             counts = [rng.choice([0, 1, 2, page - 1, page, rng.randint(1, 3 * page)]) for _ in slots]
@@ -77,6 +87,11 @@ def test_accounts_follow_the_model(page):
             src = [rng.choice(held) for _ in dst]
             assert host.fork(src, dst) == 0
             model.fork(src, dst)
+        elif op == "move":
+            used, same = host.pages - int(host.account[0]), rng.random() < 0.5
+            end = rng.randint(used, host.pages) if same else max(1, used, rng.randint(20, 50))
+            assert host.move(end, host.pages if same else end, same) == 0
+            model.move(end, host.pages)
         else:
             slots = rng.sample(range(9), rng.randint(1, 3))
             assert host.free(slots + slots[:1]) == 0              # a slot named twice is empty the second time
@@ -117,6 +132,7 @@ def test_refusals_change_nothing():
     for src, dst, message in (([0], [1], b"in use"), ([0, 0], [2, 2], b"twice"), ([0], [4], b"no slot"), ([-1], [2], b"no slot"),
                               ([0], [0], b"in use"), ([2], [2], b"both"), ([0, 2], [2, 3], b"both")):
         assert host.fork(src, dst) == 1 and message in host.error(), (src, dst, host.error())
+    assert host.move(1, 1, False) == 1 and b"in use" in host.error()
     assert host.free([0, 9]) == 1 and b"no slot" in host.error()
     for a, b in zip(before, (host.lens, host.table, host.refs, host.open, host.account)):
         assert np.array_equal(a, b)
