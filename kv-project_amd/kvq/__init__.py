@@ -24,6 +24,7 @@ from .coverage import coverage_groups, coverage_plan, coverage_stats
 from .strata_compress import StrataCompressor, rotation_matrix
 from .prompt import PromptPlan, prompt_attention
 from .pages import PagedCache, paged_decode, paged_workspace_floats
+from .paged_ctl import PagedCtl
 
 __all__ = [
     "KVQError", "load_library", "kivi_quant", "kivi_quant_stored", "pack_codes", "unpack_codes", "pack_rows", "unpack_rows",
@@ -39,5 +40,5 @@ __all__ = [
     "StrataCompressor", "rotation_matrix", "chunk_share", "fake_quant_tokens", "finalize_chunk", "gather_rows",
     "EvictedState", "MTLPState", "mtlp_budget", "mtlp_select", "snapkv_keep", "streaming_keep", "PackedState",
     "exact_rows_cache", "quasar_scores", "quasar_values", "retained_decode",
-    "retained_workspace_floats", "PromptPlan", "prompt_attention", "PagedCache", "paged_decode", "paged_workspace_floats",
+    "retained_workspace_floats", "PromptPlan", "prompt_attention", "PagedCache", "paged_decode", "paged_workspace_floats", "PagedCtl",
 ]

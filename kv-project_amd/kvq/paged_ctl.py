@@ -1,0 +1,82 @@
+"""The attention router's controller over a ``PagedCache``: prompts and steps of a batch of sequences.
+
+``with routed(PagedCtl(cache, slots)) as ctl: ctl.begin(counts); model(...)`` runs a model whose attention is
+registered under ``kvq.register()`` (STRATA_KV.py:495-523) on the slots of the cache: each layer's new keys
+and values are appended to its pages, and its queries attend
+
+* over the prompt itself (prompt_attention, exact keys and values) where all of the sequences begin,
+* over the cache by ``paged_decode`` in steps of a few tokens,
+* over the cache's rows by ``rows`` and prompt_attention in steps of many tokens (a further question, a chunk of
+  a prompt): the same attention as paged_decode's, with the rows read back once rather than once per 16 query rows.
+
+Layer ``module.layer_idx`` of the model is layer ``layer_idx`` of the cache.
+"""
+from __future__ import annotations
+
+from typing import Sequence, Union
+
+import torch
+
+from .pages import PagedCache, paged_decode
+from .prompt import PromptPlan, prompt_attention
+
+# query rows per KV head of a sequence (query heads times new tokens) from which on the rows are read back
+MANY_ROWS = 64
+
+
+class PagedCtl:
+    """Sequences in ``slots`` of ``cache``, the rows of the model's batch in that order."""
+
+    def __init__(self, cache: PagedCache, slots: Sequence[int]):
+        self.cache, self.slots = cache, [int(s) for s in slots]
+        self.step = None
+
+    def begin(self, counts: Union[int, Sequence[int]]) -> None:
+        """Claim the next step: ``counts`` new tokens of every sequence, or of each one (in a batch padded on the left:
+        the last counts[b] tokens of row b are its own).  Once per forward pass, before it."""
+        n = [int(counts)] * len(self.slots) if isinstance(counts, int) else [int(c) for c in counts]
+        if len(n) != len(self.slots):
+            raise ValueError("counts must be one number or one per sequence")
+        before = [self.cache.length(s) for s in self.slots]
+        self.step = self.cache.extend(self.slots, n)
+        self.counts, self.lens, self.fresh = n, [a + b for a, b in zip(before, n)], not any(before)
+        self.plan = self.index = None
+
+    def _plan(self, Hq: int, lens_k) -> PromptPlan:
+        if self.plan is None or self.plan.Hq != Hq:           # one for all layers of the step
+            self.plan = PromptPlan(self.counts, Hq, self.cache.Hkv, lens_k=lens_k, device=self.cache.device)
+        return self.plan
+
+    def _packed(self, x: torch.Tensor, T: int) -> torch.Tensor:
+        """(B, H, T, d) -> the sequences' own rows (rows, H, d)."""
+        x = x.transpose(1, 2).reshape(-1, x.shape[1], x.shape[3])
+        return x if self.index is None else x.index_select(0, self.index)
+
+    def attend(self, module, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, mask, kwargs):
+        """One layer of the step (the controller's part of router_attention): q (B, Hq, T, d), k, v (B, Hkv, T, d) ->
+        ((B, T, Hq, d), None).  Rows of padding come out as zeros."""
+        if self.step is None:
+            raise RuntimeError("PagedCtl: begin() claims the step before the forward pass")
+        B, Hq, T, d = q.shape
+        if B != len(self.slots) or k.shape[2] != T or T < max(self.counts):
+            raise ValueError(f"PagedCtl: a batch of {B} rows of {T} tokens for {len(self.slots)} sequences of up to "
+                             f"{max(self.counts)} new tokens")
+        if self.index is None and min(self.counts) < T:
+            own = torch.arange(T)[None] >= T - torch.tensor(self.counts)[:, None]
+            self.index = own.reshape(-1).nonzero()[:, 0].to(q.device)
+        scaling = kwargs.get("scaling")
+        scaling = module.scaling if scaling is None else scaling
+        layer, cache = module.layer_idx, self.cache
+        qp, kp, vp = (self._packed(x, T) for x in (q, k, v))
+        cache.append(layer, kp, vp, self.step)
+        if self.fresh:
+            out = prompt_attention(qp, kp, vp, scaling, self._plan(Hq, None))
+        elif Hq // cache.Hkv * max(self.counts) < MANY_ROWS:
+            out = paged_decode(qp, scaling, cache, layer, self.step)
+        else:
+            out = prompt_attention(qp, *cache.rows(layer, self.slots), scaling, self._plan(Hq, self.lens))
+        if self.index is None:
+            return out.view(B, T, Hq, d), None
+        whole = torch.zeros((B * T, Hq, d), dtype=out.dtype, device=out.device)
+        whole.index_copy_(0, self.index, out)
+        return whole.view(B, T, Hq, d), None

@@ -101,6 +101,12 @@ class PagedCache:
         """Tokens of each slot."""
         return self._lens.tolist()
 
+    def length(self, slot: int) -> int:
+        """Tokens of one slot."""
+        if not 0 <= slot < self.slots:
+            raise IndexError(f"no slot {slot} (of {self.slots})")
+        return int(self._lens[slot])
+
     @property
     def free_pages(self) -> int:
         return int(self._account[0])
