@@ -121,15 +121,22 @@ __global__ __launch_bounds__(kThreads, 2) void prompt_kernel(PromptArgs a) {
   const int k_at = (xr * static_cast<int>(a.k_st) + (xc ^ k_swz(xr)) * 8) * 2;
   const int v_at = (xr * static_cast<int>(a.v_st) + (xc ^ v_swz(xr)) * 8) * 2;
   const int wave0 = __builtin_amdgcn_readfirstlane(wave) * 512;     // elements
+  // Straight to LDS, 16 bytes a lane, written down here so that it can run beside the transposing reads (the compiler
+  // has those wait for every load to LDS).  No register is written; end() waits for it.
   auto fetch = [&](uint16_t* to, const uint16_t* base, int64_t st, int at, int j) KVQ_INLINE {
     // rows behind the last one read as zeros: the buffer ends with the last row
     const int64_t left = keys - static_cast<int64_t>(j) * kTileKeys;
     const int64_t bytes = left > 0 ? ((left - 1) * st + D) * 2 : 0;
-    const auto rsrc = make_rsrc(base + (left > 0 ? static_cast<int64_t>(j) * kTileKeys * st : 0),
-                                static_cast<uint32_t>(bytes < 0x7fffffff ? bytes : 0x7fffffff));
+    const uint64_t from = reinterpret_cast<uint64_t>(base + (left > 0 ? static_cast<int64_t>(j) * kTileKeys * st : 0));
+    const u32x4 rsrc = {static_cast<uint32_t>(from), static_cast<uint32_t>(from >> 32) & 0xffffu,
+                        static_cast<uint32_t>(bytes < 0x7fffffff ? bytes : 0x7fffffff), 0x00020000u};
+    const uint32_t lds = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((lds_void*)(to + wave0)));
 #pragma unroll
     for (int i = 0; i < kPer; ++i)
-      __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (lds_void*)(to + wave0 + i * kThreads * 8), 16, at + i * kStep * static_cast<int>(st) * 2, 0, 0, 0);
+      asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
+                   :
+                   : "s"(lds + i * kThreads * 16), "v"(at + i * kStep * static_cast<int>(st) * 2), "s"(rsrc)
+                   : "memory", "m0");
   };
   const int tiles = ((keys + kTileKeys - 1) / kTileKeys) | 1;
   int open = vis0 < keys ? vis0 : keys;       // tiles that every row sees whole
@@ -255,15 +262,15 @@ __global__ __launch_bounds__(kThreads, 2) void prompt_kernel(PromptArgs a) {
     __builtin_amdgcn_sched_barrier(0);
   };
   auto end = [&](auto par, int j) KVQ_INLINE {
-    __builtin_amdgcn_s_waitcnt(0x0f70);       // vmcnt(0): this wavefront's pieces are in LDS
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");                // this wavefront's pieces are in LDS
     if (j >= open) watch(decltype(par)::value ? v_odd : v_even, j);
     __syncthreads();
   };
   auto step = [&](auto par, int j) KVQ_INLINE {
+    begin(par, j);
     __builtin_amdgcn_s_setprio(1);            // the softmax goes before the other wavefront's products
     values(par, j >= open, yes, j);
     __builtin_amdgcn_s_setprio(0);
-    begin(par, j);                            // behind the transposing reads: the compiler has those wait for every fetch
     products(par);
     rescale();
     end(par, j);
@@ -272,7 +279,7 @@ __global__ __launch_bounds__(kThreads, 2) void prompt_kernel(PromptArgs a) {
     if (tid < kTiles) flag[tid] = 0;
     fetch(k_even, kb, a.k_st, k_at, 0);
     fetch(k_odd, kb, a.k_st, k_at, 1);
-    __builtin_amdgcn_s_waitcnt(0x0f70);
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     __syncthreads();
     products(odd);
     __syncthreads();                          // K(2) takes the place of K(0)
