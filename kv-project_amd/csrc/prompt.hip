@@ -122,7 +122,7 @@ __global__ __launch_bounds__(kThreads, 2) void prompt_kernel(PromptArgs a) {
   const int v_at = (xr * static_cast<int>(a.v_st) + (xc ^ v_swz(xr)) * 8) * 2;
   const int wave0 = __builtin_amdgcn_readfirstlane(wave) * 512;     // elements
   // Straight to LDS, 16 bytes a lane, written down here so that it can run beside the transposing reads (the compiler
-  // has those wait for every load to LDS).  No register is written; end() waits for it.
+  // has those wait for every load to LDS).  No register is written but m0, which nothing else here uses; end() waits.
   auto fetch = [&](uint16_t* to, const uint16_t* base, int64_t st, int at, int j) KVQ_INLINE {
     // rows behind the last one read as zeros: the buffer ends with the last row
     const int64_t left = keys - static_cast<int64_t>(j) * kTileKeys;
@@ -136,7 +136,7 @@ __global__ __launch_bounds__(kThreads, 2) void prompt_kernel(PromptArgs a) {
       asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
                    :
                    : "s"(lds + i * kThreads * 16), "v"(at + i * kStep * static_cast<int>(st) * 2), "s"(rsrc)
-                   : "memory", "m0");
+                   : "memory");
   };
   const int tiles = ((keys + kTileKeys - 1) / kTileKeys) | 1;
   int open = vis0 < keys ? vis0 : keys;       // tiles that every row sees whole
@@ -277,16 +277,23 @@ __global__ __launch_bounds__(kThreads, 2) void prompt_kernel(PromptArgs a) {
   };
   if (keys > 0) {
     if (tid < kTiles) flag[tid] = 0;
-    fetch(k_even, kb, a.k_st, k_at, 0);
-    fetch(k_odd, kb, a.k_st, k_at, 1);
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     __syncthreads();
-    products(odd);
-    __syncthreads();                          // K(2) takes the place of K(0)
-    begin(even, 0);
-    values(even, open == 0, no, 0);
-    products(even);
+    fetch(k_even, kb, a.k_st, k_at, 0);
+    fetch(v_even, vb, a.v_st, v_at, 0);
+    if (tiles > 1) fetch(k_odd, kb, a.k_st, k_at, 1);
     end(even, 0);
+    products(odd);
+    if (tiles > 1) {
+      __syncthreads();                        // K(2) takes the place of K(0)
+      fetch(k_even, kb, a.k_st, k_at, 2);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    values(even, open == 0, no, 0);
+    if (tiles > 1) {
+      products(even);
+      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+      __syncthreads();
+    }
     for (int j = 1; j < tiles; j += 2) {
       step(odd, j);
       step(even, j + 1);
