@@ -38,6 +38,16 @@ int write_words(const int32_t* src, int64_t n, int32_t* dst, hipStream_t stream)
   return KVQ_OK;
 }
 
+// The heads of one block on one of the 8 dies: their rows lie next to each other in memory.
+struct BlockHead {
+  int item, h;
+};
+__device__ __forceinline__ BlockHead block_head(int H) {
+  const int i = blockIdx.x / 8;
+  return {i / H * 8 + static_cast<int>(blockIdx.x % 8), i % H};
+}
+int64_t block_grid(int64_t items, int64_t H) { return (items + 7) / 8 * 8 * H; }
+
 // ---- filling ----------------------------------------------------------------------------------
 
 struct Rows16 {                               // packed rows (n, H, D) of 16-bit elements
@@ -102,7 +112,8 @@ __global__ __launch_bounds__(kThreads) void append_kernel(Rows16 k, Rows16 v, co
   __shared__ __align__(16) uint16_t turn[D * P];
   auto place = [](int c, int t) { return c * P + (((t >> 3) ^ (c >> 3)) & (P / 8 - 1)) * 8 + (t & 7); };
   __shared__ uint32_t top[8];
-  const int item = blockIdx.x / H, h = blockIdx.x % H, tid = threadIdx.x;
+  const BlockHead bh = block_head(H);
+  const int item = bh.item, h = bh.h, tid = threadIdx.x;
   const int n = step[0];
   if (item >= step[1]) return;
   const StepSeq s = step_seq(step, step[4] ? item : step_find(step, n, 4, item));
@@ -143,16 +154,26 @@ __global__ __launch_bounds__(kThreads) void append_kernel(Rows16 k, Rows16 v, co
     const int q = tid + i * kThreads, t = q / kRow, c = q % kRow * 8;
     const bool fresh = first + t >= from;
     kw[i] = *reinterpret_cast<const uint4*>(fresh ? kn + (row0 + first + t) * k.st + c : kb + t * D + c);
-    kmax = abs_max2(abs_max2(abs_max2(abs_max2(kmax, kw[i].x), kw[i].y), kw[i].z), kw[i].w);
   }
   const int old = from - first;                                     // tokens that lie in the open buffer
   if (old == 0) {
+    constexpr int kPairs = (kPer + 1) / 2;                          // two tokens at a time: words of a channel's pair
+    uint4 vx[kPairs], vy[kPairs];
 #pragma unroll
-    for (int i = 0; i < (kPer + 1) / 2; ++i) {                      // two tokens at a time: words of a channel's pair
+    for (int i = 0; i < kPairs; ++i) {                              // all on their way before the first is used, the keys too
+      const int q = tid + i * kThreads, t = q / kRow * 2, c = q % kRow * 8;
+      const uint16_t* at = vn + (row0 + first + t) * v.st + c;
+      if (kPer % 2 == 0 || q < kChunks / 2) {
+        vx[i] = *reinterpret_cast<const uint4*>(at);
+        vy[i] = *reinterpret_cast<const uint4*>(at + v.st);
+      }
+    }
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int i = 0; i < kPairs; ++i) {
       const int q = tid + i * kThreads, t = q / kRow * 2, c = q % kRow * 8;
       if (kPer % 2 && q >= kChunks / 2) break;
-      const uint16_t* at = vn + (row0 + first + t) * v.st + c;
-      const uint4 x = *reinterpret_cast<const uint4*>(at), y = *reinterpret_cast<const uint4*>(at + v.st);
+      const uint4 x = vx[i], y = vy[i];
       const uint32_t xs[4] = {x.x, x.y, x.z, x.w}, ys[4] = {y.x, y.y, y.z, y.w};
 #pragma unroll
       for (int e = 0; e < 8; ++e)
@@ -175,6 +196,8 @@ __global__ __launch_bounds__(kThreads) void append_kernel(Rows16 k, Rows16 v, co
       }
     }
   }
+#pragma unroll
+  for (int i = 0; i < kPer; ++i) kmax = abs_max2(abs_max2(abs_max2(abs_max2(kmax, kw[i].x), kw[i].y), kw[i].z), kw[i].w);
   __syncthreads();
   uint4 vw[kPer];                                                   // pieces of 8 tokens of a channel
 #pragma unroll
@@ -246,7 +269,7 @@ constexpr int kWhole = 5, kMostWhole = kWords / kWhole;
 
 // One workgroup per (block, KV head): dense rows (rows, H, D) of keys and values.
 template <int D, int P, int CODE, bool BF16>
-__global__ __launch_bounds__(kThreads) void rows_kernel(WordBlock whole, int n, const int* __restrict__ table, int64_t max_blocks,
+__global__ __launch_bounds__(kThreads) void rows_kernel(WordBlock whole, int n, int blocks, const int* __restrict__ table, int64_t max_blocks,
                                                         int H, const uint8_t* __restrict__ kc, const uint8_t* __restrict__ vc,
                                                         const float* __restrict__ sc, const uint16_t* __restrict__ ko,
                                                         const uint16_t* __restrict__ vo, uint16_t* __restrict__ k_out,
@@ -254,13 +277,10 @@ __global__ __launch_bounds__(kThreads) void rows_kernel(WordBlock whole, int n, 
   constexpr int kChunks = P * D / 8, kPer = kChunks / kThreads, kRow = D / 8;
   constexpr int kPitch = D + 8;
   __shared__ __align__(16) uint16_t turn[P * kPitch];
-  const int item = blockIdx.x / H, h = blockIdx.x % H, tid = threadIdx.x;
-  int lo = 0, hi = n - 1;                     // the last sequence whose first block is not behind this one
-  while (lo < hi) {
-    const int mid = (lo + hi + 1) >> 1;
-    if (whole.w[kWhole * mid + 3] <= item) lo = mid;
-    else hi = mid - 1;
-  }
+  const BlockHead bh = block_head(H);
+  const int item = bh.item, h = bh.h, tid = threadIdx.x;
+  if (item >= blocks) return;
+  const int lo = __builtin_amdgcn_readfirstlane(last_not_above(whole.w + 3, kWhole, n, item));
   const int* s = whole.w + kWhole * lo;
   const int64_t slot = s[0];
   const int j = item - s[3], first = j * P;
@@ -562,10 +582,10 @@ extern "C" int kvq_pages_append(const void* k, int64_t k_st, int64_t k_sh, const
   KVQ_REQUIRE(k && v && step && table && kc && vc && sc && ko && vo, "kvq_pages_append: null pointer");
   KVQ_REQUIRE(reinterpret_cast<uintptr_t>(k) % 16 == 0 && reinterpret_cast<uintptr_t>(v) % 16 == 0 && (k_st | k_sh | v_st | v_sh) % 8 == 0,
               "kvq_pages_append: rows and strides must be multiples of 16 bytes");
-  KVQ_REQUIRE(items >= 0 && items * H < INT64_C(1) << 31, "kvq_pages_append: too many blocks");
+  KVQ_REQUIRE(items >= 0 && block_grid(items, H) < INT64_C(1) << 31, "kvq_pages_append: too many blocks");
   if (items == 0) return KVQ_OK;
   const Rows16 kr{static_cast<const uint16_t*>(k), k_st, k_sh}, vr{static_cast<const uint16_t*>(v), v_st, v_sh};
-  KVQ_PAGES_DISPATCH(hipLaunchKernelGGL((append_kernel<D_, P_, C_, T_>), dim3(static_cast<uint32_t>(items * H)), dim3(kThreads), 0,
+  KVQ_PAGES_DISPATCH(hipLaunchKernelGGL((append_kernel<D_, P_, C_, T_>), dim3(static_cast<uint32_t>(block_grid(items, H))), dim3(kThreads), 0,
                                         static_cast<hipStream_t>(stream), kr, vr, step, table, max_blocks, static_cast<int>(H), kc, vc, sc,
                                         static_cast<uint16_t*>(ko), static_cast<uint16_t*>(vo)))
   KVQ_LAUNCH_CHECK("kvq_pages_append");
@@ -586,7 +606,7 @@ extern "C" int kvq_pages_rows(const int64_t* lens, const uint8_t* open, int64_t 
     rows += lens[seq[i]];
     blocks += (lens[seq[i]] + P - 1) / P;
   }
-  KVQ_REQUIRE(rows < INT64_C(1) << 31 && blocks * H < INT64_C(1) << 31, "kvq_pages_rows: too many rows");
+  KVQ_REQUIRE(rows < INT64_C(1) << 31 && block_grid(blocks, H) < INT64_C(1) << 31, "kvq_pages_rows: too many rows");
   KVQ_REQUIRE(out_elements >= rows * H * D && (rows == 0 || (k_out && v_out)), "kvq_pages_rows: outputs of %lld elements, %lld needed",
               static_cast<long long>(out_elements), static_cast<long long>(rows * H * D));
   int64_t row = 0;
@@ -606,8 +626,8 @@ extern "C" int kvq_pages_rows(const int64_t* lens, const uint8_t* open, int64_t 
       block += (lens[s] + P - 1) / P;
     }
     if (block == 0) continue;
-    KVQ_PAGES_DISPATCH(hipLaunchKernelGGL((rows_kernel<D_, P_, C_, T_>), dim3(static_cast<uint32_t>(block * H)), dim3(kThreads), 0,
-                                          static_cast<hipStream_t>(stream), w, static_cast<int>(m), table, max_blocks, static_cast<int>(H), kc,
+    KVQ_PAGES_DISPATCH(hipLaunchKernelGGL((rows_kernel<D_, P_, C_, T_>), dim3(static_cast<uint32_t>(block_grid(block, H))), dim3(kThreads), 0,
+                                          static_cast<hipStream_t>(stream), w, static_cast<int>(m), static_cast<int>(block), table, max_blocks, static_cast<int>(H), kc,
                                           vc, sc, static_cast<const uint16_t*>(ko), static_cast<const uint16_t*>(vo),
                                           static_cast<uint16_t*>(k_out), static_cast<uint16_t*>(v_out)))
   }

@@ -35,15 +35,23 @@ __device__ __forceinline__ StepSeq step_seq(const int* step, int b) {
   return {e[0], e[1], e[2], e[3], e[4], e[5], e[6]};
 }
 
+// The last of n sequences whose word (at first[i * stride]) is not above `value`: 64 at a time, one memory round trip
+// each instead of one per halving.  By whole wavefronts, `value` the same in all lanes.
+__device__ __forceinline__ int last_not_above(const int* first, int stride, int n, int value) {
+  const int lane = threadIdx.x & 63;
+  int count = 0;
+  for (int i = 0; i < n; i += 64) {
+    const int x = i + lane < n ? first[(i + lane) * stride] : 0x7fffffff;
+    const int c = __popcll(__builtin_amdgcn_ballot_w64(x <= value));
+    count += c;
+    if (c < 64) break;
+  }
+  return count - 1;
+}
+
 // The sequence whose range [first, next first) of word `w` holds i (ranges may be empty).
 __device__ __forceinline__ int step_find(const int* step, int n, int w, int i) {
-  int lo = 0, hi = n - 1;                     // the last b with first(b) <= i
-  while (lo < hi) {
-    const int mid = (lo + hi + 1) >> 1;
-    if (step[kStepHead + kStepSeq * mid + w] <= i) lo = mid;
-    else hi = mid - 1;
-  }
-  return lo;
+  return __builtin_amdgcn_readfirstlane(last_not_above(step + kStepHead + w, kStepSeq, n, i));
 }
 
 }  // namespace kvq
