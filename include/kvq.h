@@ -694,6 +694,8 @@ int kvq_prompt_attention(const void* q, int64_t q_st, int64_t q_sh, const void* 
  * full, in order; refused whole ("decode buffer exhausted") when a slot's max_tokens or the free pages do
  * not suffice.  It writes the step's description to `desc` (host, kvq_pages_step_words words) and, by
  * value with launches on `stream`, to desc_device (NULL: host only).  split_cap >= n bounds the decode's split items.
+ * Pages that neighbouring sequences of the step share in front are read once for all of them where the description
+ * stays within most_run tokens of a run (its seventh word) and most_tokens of all split items (its eighth).
  * kvq_pages_append writes one layer's rows k, v (rows, H, D) of the step; running it again writes the same.
  * kvq_pages_rows reads slots seq[0 .. n) back as dense rows (sum lens, H, D); lens, open and seq are read before it
  * returns.
@@ -707,8 +709,8 @@ int kvq_prompt_attention(const void* q, int64_t q_st, int64_t q_sh, const void* 
 int64_t kvq_pages_step_words(int64_t page, const int64_t* counts, int64_t n);
 int kvq_pages_extend(int64_t* lens, int32_t* table, int32_t* refs, uint8_t* open, int64_t* account, int64_t slots,
                      int64_t pages, int64_t max_blocks, int64_t page, int64_t max_tokens, const int64_t* seq,
-                     const int64_t* counts, int64_t n, int64_t split_cap, int32_t* desc, int64_t desc_words,
-                     int32_t* desc_device, void* stream);
+                     const int64_t* counts, int64_t n, int64_t split_cap, int64_t most_run, int64_t most_tokens,
+                     int32_t* desc, int64_t desc_words, int32_t* desc_device, void* stream);
 int kvq_pages_append(const void* k, int64_t k_st, int64_t k_sh, const void* v, int64_t v_st, int64_t v_sh, int dtype,
                      const int32_t* step, int64_t items, int32_t* table, int64_t max_blocks, int64_t H, int64_t D,
                      int64_t page, int code, uint8_t* kc, uint8_t* vc, float* sc, void* ko, void* vo, void* stream);
@@ -728,16 +730,19 @@ int kvq_pages_move(const int64_t* lens, int32_t* table, const int32_t* refs, int
 
 /* ------------------------------------------------------------------------------------------
  * Attention of a step's query rows over the paged cache: q (rows, Hq, D), the step's rows in order; query
- * i of a sequence with `count` new tokens sees all tokens up to its own.  split_items >= the description's
- * third word and max_count >= every count give the grid.  out (rows, Hq, D) contiguous.  workspace:
- * kvq_paged_decode_workspace floats, no clearing; calls that share one must not overlap in time.
+ * i of a sequence with `count` new tokens sees all tokens up to its own.  split_items, run_tokens and split_tokens: at
+ * least the description's third, seventh and eighth word; they give the grid and the workspace.  out (rows, Hq, D)
+ * contiguous.  workspace: kvq_paged_decode_workspace floats, no clearing; calls that share one must not
+ * overlap in time.
  * tickets: NULL, or (slots, H, 4) int32 zeros, which a call leaves as zeros: sequences of several split items are
  * then joined within the one launch, by the workgroup that comes last (in the items' order: the result is the
- * same), where a sequence has at most 64 rows per KV head.  Calls over one slot of one layer must not overlap.
+ * same), where a sequence has at most 64 rows per KV head.  Not for a step with shared fronts.  Calls over one slot of one
+ * layer must not overlap.
  * ---------------------------------------------------------------------------------------- */
-int64_t kvq_paged_decode_workspace(int64_t split_items, int64_t H, int64_t rep, int64_t max_count, int64_t D);
+int64_t kvq_paged_decode_workspace(int64_t split_tokens, int64_t H, int64_t rep, int64_t D);
 int kvq_paged_decode(const void* q, int64_t q_st, int64_t q_sh, int dtype, int64_t rows, int64_t Hq, int64_t H, int64_t D,
-                     float scaling, const int32_t* step, int64_t split_items, int64_t max_count, const int32_t* table,
+                     float scaling, const int32_t* step, int64_t split_items, int64_t run_tokens, int64_t split_tokens,
+                     const int32_t* table,
                      int64_t max_blocks, int64_t page, int code, const uint8_t* kc, const uint8_t* vc, const float* sc,
                      const void* ko, const void* vo, void* out, float* workspace, int64_t workspace_floats,
                      int32_t* tickets, void* stream);

@@ -77,13 +77,14 @@ struct DecodeArgs {
   const int* table;
   int64_t max_blocks;
   int H, rep;                                 // KV heads, query heads per KV head
-  int pieces;                                 // of 16 rows
+  int pieces;                                 // of 16 rows, of the widest run
   float scale;                                // scaling * log2(e)
   const uint8_t *kc, *vc;
   const float* sc;
   const uint16_t *ko, *vo;
   uint16_t* out;                              // (rows, Hq, D)
-  float* part;                                // (items, H, pieces): 16 x D sums, then 16 x {max, sum}
+  float* part;                                // (part_rows, H): D sums; behind them {max, sum} each
+  int64_t part_rows;                          // rows of all split items
   int* tickets;                               // (slots, H, kTickets) zeros, or none: joins by a launch of its own
 };
 constexpr int kTickets = 4;                   // pieces of a sequence that the last workgroup may join
@@ -103,41 +104,49 @@ __device__ __forceinline__ float get(const float* p) {
   else return *p;
 }
 
-// Row r of `items` partial results, 64 maxima at a time, by one wavefront
-template <int D, bool BF16, bool SHARED>
-__device__ __forceinline__ void join_row(const float* part, int64_t stride, int items, int r, uint16_t* out) {
-  const int lane = threadIdx.x & 63;
+// A row joined by one wavefront: the maximum, the sum, its channels of the weighted sums
+template <int D, bool SHARED>
+struct Join {
   float top = -INFINITY, l = 0.0f, o[D / 64] = {};
-  for (int i0 = 0; i0 < items; i0 += 64) {
-    const int i = i0 + lane;
-    float2 st = make_float2(-INFINITY, 0.0f);
-    if (i < items) st = make_float2(get<SHARED>(part + i * stride + kRows * D + 2 * r), get<SHARED>(part + i * stride + kRows * D + 2 * r + 1));
-    const float m = fmaxf(top, wave_max(st.x)), safe = m == -INFINITY ? 0.0f : m;
-    const float old = __builtin_amdgcn_exp2f(top - safe), f = __builtin_amdgcn_exp2f(st.x - safe);
-    l = l * old + wave_sum(f * st.y);
+  // row R of each of a run's split items, 64 maxima at a time
+  __device__ __forceinline__ void add(const DecodeArgs& a, const StepRun& run, int items, int R, int h) {
+    const int lane = threadIdx.x & 63;
+    const int64_t first = (static_cast<int64_t>(a.rep) * run.base + R) * a.H + h, stride = static_cast<int64_t>(a.rep) * run.tokens * a.H;
+    const float* stat = a.part + a.part_rows * a.H * D;
+    for (int i0 = 0; i0 < items; i0 += 64) {
+      const int i = i0 + lane;
+      float2 st = make_float2(-INFINITY, 0.0f);
+      if (i < items) st = make_float2(get<SHARED>(stat + 2 * (first + i * stride)), get<SHARED>(stat + 2 * (first + i * stride) + 1));
+      const float m = fmaxf(top, wave_max(st.x)), safe = m == -INFINITY ? 0.0f : m;
+      const float old = __builtin_amdgcn_exp2f(top - safe), f = __builtin_amdgcn_exp2f(st.x - safe);
+      l = l * old + wave_sum(f * st.y);
 #pragma unroll
-    for (int e = 0; e < D / 64; ++e) o[e] *= old;
-    const int most = items - i0 < 64 ? items - i0 : 64;
-    const float* p = part + i0 * stride + r * D + lane * (D / 64);
-    for (int k0 = 0; k0 < most; k0 += 8) {                          // eight loads on their way; behind the last: it again, times zero
-      float x[8][D / 64];
+      for (int e = 0; e < D / 64; ++e) o[e] *= old;
+      const int most = items - i0 < 64 ? items - i0 : 64;
+      const float* p = a.part + (first + i0 * stride) * D + lane * (D / 64);
+      for (int k0 = 0; k0 < most; k0 += 8) {                        // eight loads on their way; behind the last: it again, unused
+        float x[8][D / 64];
 #pragma unroll
-      for (int k = 0; k < 8; ++k)
+        for (int k = 0; k < 8; ++k)
 #pragma unroll
-        for (int e = 0; e < D / 64; ++e) x[k][e] = get<SHARED>(p + (k0 + k < most ? k0 + k : most - 1) * stride + e);
+          for (int e = 0; e < D / 64; ++e) x[k][e] = get<SHARED>(p + (k0 + k < most ? k0 + k : most - 1) * stride * D + e);
 #pragma unroll
-      for (int k = 0; k < 8; ++k) {
-        const float fk = k0 + k < most ? __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(f), k0 + k)) : 0.0f;
+        for (int k = 0; k < 8; ++k) {
+          const float fk = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(f), k0 + k < most ? k0 + k : 0));
 #pragma unroll
-        for (int e = 0; e < D / 64; ++e) o[e] += k0 + k < most ? fk * x[k][e] : 0.0f;
+          for (int e = 0; e < D / 64; ++e) o[e] += k0 + k < most ? fk * x[k][e] : 0.0f;
+        }
       }
+      top = m;
     }
-    top = m;
   }
-  const float inv = 1.0f / l;
+  template <bool BF16>
+  __device__ __forceinline__ void put(uint16_t* out) const {
+    const float inv = 1.0f / l;
 #pragma unroll
-  for (int e = 0; e < D / 64; ++e) out[lane * (D / 64) + e] = BF16 ? f32_to_bf16(o[e] * inv) : f32_to_f16(o[e] * inv);
-}
+    for (int e = 0; e < D / 64; ++e) out[(threadIdx.x & 63) * (D / 64) + e] = BF16 ? f32_to_bf16(o[e] * inv) : f32_to_f16(o[e] * inv);
+  }
+};
 
 // Scores t (16 tokens of this lane, masked ones -inf) -> probabilities in t, o and l brought to the new maximum
 template <int D, bool BF16>
@@ -192,22 +201,25 @@ __global__ __launch_bounds__(kThreads, 3) void paged_split_kernel(DecodeArgs a) 
   const int64_t ih = static_cast<int64_t>(group) * 8 + within % 8;
   const int piece = within / 8, item = static_cast<int>(ih / a.H), h = static_cast<int>(ih % a.H);
   if (item >= step[2]) return;
-  const int b = step_find(step, n, 5, item);
-  const StepSeq s = step_seq(step, b);
-  const int rows = a.rep * s.count;
+  const int* runs = step_runs(step, n);
+  const int ri = __builtin_amdgcn_readfirstlane(last_not_above(runs + 5, kStepRun, step[kStepHead + kStepSeq * n + 5], item));
+  const StepRun run = step_run(runs, ri);
+  const int rows = a.rep * run.tokens;
   if (piece * kRows >= rows) return;
+  const bool own = run.seq >= 0;              // or a shared front: whole pages that every row sees
+  const StepSeq s = step_seq(step, own ? run.seq : 0);
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), col = lane & 15, g = lane >> 4;
-  const int len = s.pos0 + s.count, full = len / P * P;
-  const int u_full = (full + kUnit - 1) / kUnit, u_all = u_full + (len - full + kUnit - 1) / kUnit;
-  const int u0 = (item - s.split0) * per, u1 = u0 + per < u_all ? u0 + per : u_all;
+  const int pos0 = own ? s.pos0 : run.u1 * kUnit, len = own ? s.pos0 + s.count : run.u1 * kUnit, full = len / P * P;
+  const int u_full = (full + kUnit - 1) / kUnit;
+  const int u0 = run.u0 + (item - run.split0) * per, u1 = u0 + per < run.u1 ? u0 + per : run.u1;
 
   // the query rows: column col of B, channels 64 j + 16 g + 8 e ..
   const int row = piece * kRows + col, tok = row / a.rep, hq = row % a.rep;
   const bool live = row < rows;
-  const int visible = live ? s.pos0 + tok + 1 : 0;
+  const int visible = live ? pos0 + tok + 1 : 0;
   u32x4 q[2 * kJ];
   {
-    const uint16_t* qp = a.q + (s.row0 + (live ? tok : 0)) * a.q_st + (static_cast<int64_t>(h) * a.rep + (live ? hq : 0)) * a.q_sh;
+    const uint16_t* qp = a.q + (run.row0 + (live ? tok : 0)) * a.q_st + (static_cast<int64_t>(h) * a.rep + (live ? hq : 0)) * a.q_sh;
 #pragma unroll
     for (int j = 0; j < kJ; ++j)
 #pragma unroll
@@ -224,7 +236,7 @@ __global__ __launch_bounds__(kThreads, 3) void paged_split_kernel(DecodeArgs a) 
   w.l = 0.0f;
 
   const int m_tok = 16 * (col >> 2) + (col & 3);                    // + 4 s: the token of S row `col` in tile s
-  const int* pages = a.table + s.slot * a.max_blocks;
+  const int* pages = a.table + run.slot * a.max_blocks;
   const int last = full / P - 1;                                    // last full block
   const int u_end = u1 < u_full ? u1 : u_full;
   // The registers of a unit: keys and its scales are read for the next unit once the scores are there, values once
@@ -296,7 +308,7 @@ __global__ __launch_bounds__(kThreads, 3) void paged_split_kernel(DecodeArgs a) 
       if (u + 2 * kWaves < u_end) ids(u + 2 * kWaves);
     }
     const int end = visible < full ? visible : full;
-    const bool masked = t0 + kUnit > full || t0 + kUnit > s.pos0 + 1;
+    const bool masked = t0 + kUnit > full || t0 + kUnit > pos0 + 1;
     if (masked) {
 #pragma unroll
       for (int i = 0; i < 16; ++i) t[i] = t0 + 16 * g + i < end ? t[i] : -INFINITY;
@@ -395,8 +407,8 @@ __global__ __launch_bounds__(kThreads, 3) void paged_split_kernel(DecodeArgs a) 
     stat[wave][col][1] = w.l;
   }
   __syncthreads();
-  const int next = step[kStepHead + kStepSeq * (b + 1) + 5];
-  const bool single = next - s.split0 == 1;
+  const int items = runs[kStepRun * (ri + 1) + 5] - run.split0;
+  const bool single = own && items == 1 && s.front == 0;
   constexpr int kPer = kRows * D / kThreads;                        // channels of a row per thread
   const int r = threadIdx.x / (D / kPer), c0 = threadIdx.x % (D / kPer) * kPer;
   float top = stat[0][r][0];
@@ -416,7 +428,7 @@ __global__ __launch_bounds__(kThreads, 3) void paged_split_kernel(DecodeArgs a) 
   if (single) {
     if (R >= rows) return;
     const float inv = 1.0f / l;
-    uint16_t* out = a.out + ((static_cast<int64_t>(s.row0) + R / a.rep) * Hq + h * a.rep + R % a.rep) * D + c0;
+    uint16_t* out = a.out + ((static_cast<int64_t>(run.row0) + R / a.rep) * Hq + h * a.rep + R % a.rep) * D + c0;
     uint32_t p[kPer / 2];
 #pragma unroll
     for (int e = 0; e < kPer / 2; ++e)
@@ -426,30 +438,29 @@ __global__ __launch_bounds__(kThreads, 3) void paged_split_kernel(DecodeArgs a) 
     for (int e = 0; e < kPer / 4; ++e) *reinterpret_cast<uint2*>(out + 4 * e) = make_uint2(p[2 * e], p[2 * e + 1]);
     return;
   }
-  constexpr int64_t kPart = kRows * (D + 2);
-  float* part = a.part + (ih * a.pieces + piece) * kPart;
+  const int64_t at = (static_cast<int64_t>(a.rep) * (run.base + static_cast<int64_t>(item - run.split0) * run.tokens) + R) * a.H + h;
+  float *part = a.part + at * D, *st = a.part + a.part_rows * a.H * D + 2 * at;
   if (!a.tickets) {
     if (R >= rows) return;
 #pragma unroll
     for (int e = 0; e < kPer / 4; ++e)
-      *reinterpret_cast<float4*>(part + r * D + c0 + 4 * e) = make_float4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
-    if (c0 == 0) *reinterpret_cast<float2*>(part + kRows * D + 2 * r) = make_float2(top, l);
+      *reinterpret_cast<float4*>(part + c0 + 4 * e) = make_float4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
+    if (c0 == 0) *reinterpret_cast<float2*>(st) = make_float2(top, l);
     return;
   }
   if (R < rows) {
 #pragma unroll
-    for (int e = 0; e < kPer; ++e) put_shared(part + r * D + c0 + e, o[e]);
+    for (int e = 0; e < kPer; ++e) put_shared(part + c0 + e, o[e]);
     if (c0 == 0) {
-      put_shared(part + kRows * D + 2 * r, top);
-      put_shared(part + kRows * D + 2 * r + 1, l);
+      put_shared(st, top);
+      put_shared(st + 1, l);
     }
   }
-  // The last workgroup of the sequence's items joins them.  Each one's partial results are visible on every die
-  // before its ticket is counted; the ticket is a zero again afterwards.
+  // The last workgroup of the sequence's items joins them (no tickets where there are shared fronts).  Each one's
+  // partial results are visible on every die before its ticket is counted; the ticket is a zero again afterwards.
   __shared__ int last_one;
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
   __syncthreads();
-  const int items = next - s.split0;
   if (threadIdx.x == 0) {
     int* ticket = a.tickets + (static_cast<int64_t>(s.slot) * a.H + h) * kTickets + piece;
     last_one = __hip_atomic_fetch_add(ticket, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == items - 1;
@@ -457,44 +468,50 @@ __global__ __launch_bounds__(kThreads, 3) void paged_split_kernel(DecodeArgs a) 
   }
   __syncthreads();
   if (!last_one) return;
-  const float* first = a.part + ((static_cast<int64_t>(s.split0) * a.H + h) * a.pieces + piece) * kPart;
   for (int i = wave; i < kRows && piece * kRows + i < rows; i += kWaves) {
     const int Ri = piece * kRows + i;
-    join_row<D, BF16, true>(first, a.H * a.pieces * kPart, items, i, a.out + ((static_cast<int64_t>(s.row0) + Ri / a.rep) * Hq + h * a.rep + Ri % a.rep) * D);
+    Join<D, true> j;
+    j.add(a, run, items, Ri, h);
+    j.template put<BF16>(a.out + ((static_cast<int64_t>(run.row0) + Ri / a.rep) * Hq + h * a.rep + Ri % a.rep) * D);
   }
 }
 
-// One wavefront per (packed row, query head): the items of its sequence, 64 maxima at a time.
+// One wavefront per (packed row, query head): the items of its sequence's shared front, then its own.
 template <int D, bool BF16>
 __global__ __launch_bounds__(kThreads) void paged_merge_kernel(DecodeArgs a, int64_t total) {
   const int64_t at = static_cast<int64_t>(blockIdx.x) * kWaves + (threadIdx.x >> 6);
   if (at >= total) return;
-  const int Hq = a.H * a.rep, lane = threadIdx.x & 63;
+  const int Hq = a.H * a.rep;
   const int n = static_cast<int>(at / Hq), head = static_cast<int>(at % Hq), h = head / a.rep;
-  const int b = step_find(a.step, a.step[0], 3, n);
-  const StepSeq s = step_seq(a.step, b);
-  const int items = a.step[kStepHead + kStepSeq * (b + 1) + 5] - s.split0;
-  if (n >= s.row0 + s.count || items < 2) return;
-  const int R = (n - s.row0) * a.rep + head % a.rep, piece = R / kRows, r = R % kRows;
-  constexpr int64_t kPart = kRows * (D + 2);
-  const int64_t stride = static_cast<int64_t>(a.H) * a.pieces * kPart;
-  join_row<D, BF16, false>(a.part + (static_cast<int64_t>(s.split0) * a.H + h) * a.pieces * kPart + piece * kPart, stride, items, r, a.out + at * D);
+  const StepSeq s = step_seq(a.step, step_find(a.step, a.step[0], 3, n));
+  if (n >= s.row0 + s.count) return;
+  const int* runs = step_runs(a.step, a.step[0]);
+  const StepRun own = step_run(runs, s.run);
+  const int items = runs[kStepRun * (s.run + 1) + 5] - own.split0;
+  if (items < 2 && !s.front) return;          // its workgroup has written the result
+  Join<D, false> j;
+  if (s.front) {
+    const StepRun front = step_run(runs, s.front - 1);
+    j.add(a, front, runs[kStepRun * s.front + 5] - front.split0, (n - front.row0) * a.rep + head % a.rep, h);
+  }
+  j.add(a, own, items, (n - s.row0) * a.rep + head % a.rep, h);
+  j.template put<BF16>(a.out + at * D);
 }
 
-int64_t pieces_of(int64_t rep, int64_t most) { return (rep * most + kRows - 1) / kRows; }
+int64_t pieces_of(int64_t rep, int64_t tokens) { return (rep * tokens + kRows - 1) / kRows; }
 
 }  // namespace
 }  // namespace kvq
 
 using namespace kvq;
 
-extern "C" int64_t kvq_paged_decode_workspace(int64_t split_items, int64_t H, int64_t rep, int64_t max_count, int64_t D) {
-  if (split_items < 1 || H < 1 || rep < 1 || max_count < 1 || (D != 64 && D != 128)) return -1;
-  return split_items * H * pieces_of(rep, max_count) * kRows * (D + 2);
+extern "C" int64_t kvq_paged_decode_workspace(int64_t split_tokens, int64_t H, int64_t rep, int64_t D) {
+  if (split_tokens < 0 || split_tokens >= INT64_C(1) << 31 || H < 1 || rep < 1 || (D != 64 && D != 128)) return -1;
+  return split_tokens * rep * H * (D + 2);
 }
 
 extern "C" int kvq_paged_decode(const void* q, int64_t q_st, int64_t q_sh, int dtype, int64_t rows, int64_t Hq, int64_t H, int64_t D,
-                                float scaling, const int32_t* step, int64_t split_items, int64_t max_count, const int32_t* table,
+                                float scaling, const int32_t* step, int64_t split_items, int64_t run_tokens, int64_t split_tokens, const int32_t* table,
                                 int64_t max_blocks, int64_t P, int code, const uint8_t* kc, const uint8_t* vc, const float* sc,
                                 const void* ko, const void* vo, void* out, float* workspace, int64_t workspace_floats, int32_t* tickets,
                                 void* stream) {
@@ -502,18 +519,19 @@ extern "C" int kvq_paged_decode(const void* q, int64_t q_st, int64_t q_sh, int d
   KVQ_REQUIRE(P == 32 || P == 64 || P == 128, "kvq_paged_decode: pages hold 32, 64 or 128 tokens");
   KVQ_REQUIRE(dtype == KVQ_F16 || dtype == KVQ_BF16, "kvq_paged_decode: queries must be fp16 or bf16");
   KVQ_REQUIRE(code == kCodeInt8 || code == kCodeE4M3, "kvq_paged_decode: unknown code %d", code);
-  KVQ_REQUIRE(H > 0 && Hq > 0 && Hq % H == 0 && rows > 0 && max_count > 0 && split_items > 0, "kvq_paged_decode: bad sizes");
+  KVQ_REQUIRE(H > 0 && Hq > 0 && Hq % H == 0 && rows > 0 && run_tokens > 0 && split_items > 0, "kvq_paged_decode: bad sizes");
   KVQ_REQUIRE(q && step && table && kc && vc && sc && ko && vo && out && workspace, "kvq_paged_decode: null pointer");
   KVQ_REQUIRE(reinterpret_cast<uintptr_t>(q) % 16 == 0 && (q_st | q_sh) % 8 == 0 && reinterpret_cast<uintptr_t>(out) % 16 == 0 &&
                   reinterpret_cast<uintptr_t>(workspace) % 16 == 0,
               "kvq_paged_decode: rows and strides must be multiples of 16 bytes");
-  const int64_t rep = Hq / H, need = kvq_paged_decode_workspace(split_items, H, rep, max_count, D);
+  const int64_t rep = Hq / H, need = kvq_paged_decode_workspace(split_tokens, H, rep, D), pieces = pieces_of(rep, run_tokens);
+  KVQ_REQUIRE(need >= 0, "kvq_paged_decode: too many split tokens (%lld)", static_cast<long long>(split_tokens));
   KVQ_REQUIRE(workspace_floats >= need, "kvq_paged_decode: workspace of %lld floats, %lld needed", static_cast<long long>(workspace_floats),
               static_cast<long long>(need));
   DecodeArgs a{static_cast<const uint16_t*>(q), q_st, q_sh, step, table, max_blocks, static_cast<int>(H), static_cast<int>(rep),
-               static_cast<int>(pieces_of(rep, max_count)), scaling * 1.44269504088896341f, kc, vc, sc,
+               static_cast<int>(pieces), scaling * 1.44269504088896341f, kc, vc, sc,
                static_cast<const uint16_t*>(ko), static_cast<const uint16_t*>(vo), static_cast<uint16_t*>(out), workspace,
-               pieces_of(rep, max_count) <= kTickets && split_items * H * pieces_of(rep, max_count) <= 256 ? tickets : nullptr};
+               split_tokens * rep, pieces <= kTickets && split_items * H * pieces <= 256 ? tickets : nullptr};
   // Joining in the launch: 128 workgroups 14.2 -> 10.3 us, 768 of them 23.9 -> 26.1 (their stores past the caches
   // and the wait for the last one); so only where every workgroup has a CU of its own.
   const int64_t blocks = (split_items * H + 7) / 8 * 8 * a.pieces, merges = (rows * Hq + kWaves - 1) / kWaves;

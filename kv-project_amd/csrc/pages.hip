@@ -222,7 +222,7 @@ __global__ __launch_bounds__(kThreads) void append_kernel(Rows16 k, Rows16 v, co
     vmax = vmax > top[4 + i] ? vmax : top[4 + i];
   }
   const Scale ks = block_scale<CODE, BF16>(kmax), vs = block_scale<CODE, BF16>(vmax);
-  const int page = step[kStepHead + kStepSeq * (n + 1) + item];
+  const int page = step_pages(step, n)[item];
   const int64_t at = (static_cast<int64_t>(page) * H + h) * P * D;
   if (tid == 0) {
     float2* p = reinterpret_cast<float2*>(sc) + static_cast<int64_t>(page) * H + h;
@@ -409,18 +409,26 @@ int64_t units_of(int64_t len, int64_t page) {
   return (full + kUnit - 1) / kUnit + (len - full + kUnit - 1) / kUnit;
 }
 
-int64_t splits_of(const int32_t* e, int64_t page, int64_t per) {    // none for a sequence without new tokens
-  return e[2] ? (units_of(static_cast<int64_t>(e[1]) + e[2], page) + per - 1) / per : 0;
+// Pages in front that slots a and b share, of the first `most`
+int64_t shared(const int32_t* table, int64_t max_blocks, int64_t a, int64_t b, int64_t most) {
+  int64_t i = 0;
+  while (i < most && table[a * max_blocks + i] == table[b * max_blocks + i]) ++i;
+  return i;
 }
 
-// Fills the description from lens (before), counts and open buffers.  Returns the number of items.
-int64_t describe(const int64_t* lens, const uint8_t* open, int64_t page, const int64_t* seq, const int64_t* counts, int64_t n,
-                 int64_t split_cap, int32_t* desc) {
-  int64_t row = 0, item = 0, most = 0, longest = 0;
+// A front is worth a run of its own from this many units on: one for each wavefront of a workgroup.
+constexpr int64_t kFront = 4;
+
+// Fills the description from lens (before), counts and open buffers; pages are written by the caller.  split_cap bounds
+// the split items (those of a front weighted by the workgroups that its rows take at four query heads per KV head).
+// most_run, most_tokens: where the step has to fit a launch that was captured; fronts that do not are left out.
+void describe(const int64_t* lens, const uint8_t* open, const int32_t* table, int64_t max_blocks, int64_t page, const int64_t* seq,
+              const int64_t* counts, int64_t n, int64_t split_cap, int64_t most_run, int64_t most_tokens, int32_t* desc) {
+  int64_t row = 0, item = 0, longest = 0;
   bool even = true;
   for (int64_t i = 0; i < n; ++i) {
     int32_t* e = desc + kStepHead + kStepSeq * i;
-    const int64_t s = seq[i], len = lens[s], pos0 = len, count = counts[i], end = pos0 + count;
+    const int64_t s = seq[i], pos0 = lens[s], count = counts[i], end = pos0 + count;
     const int src = open[s] & 1, dst = pos0 % page && end / page > pos0 / page && end % page ? src ^ 1 : src;
     e[0] = static_cast<int32_t>(s);
     e[1] = static_cast<int32_t>(pos0);
@@ -428,44 +436,86 @@ int64_t describe(const int64_t* lens, const uint8_t* open, int64_t page, const i
     e[3] = static_cast<int32_t>(row);
     e[4] = static_cast<int32_t>(item);
     e[6] = src | dst << 1;
-    e[7] = 0;
     row += count;
     longest = count > longest ? count : longest;
     item += count ? (end - 1) / page - pos0 / page + 1 : 0;
     even = even && item == i + 1;
-    const int64_t u = units_of(end, page);
-    most = u > most ? u : most;
   }
-  int64_t lo = 4, hi = most > 4 ? most : 4;                         // a wavefront takes a unit at least
-  while (lo < hi) {
-    const int64_t mid = (lo + hi) / 2;
-    int64_t items = 0;
-    for (int64_t i = 0; i < n; ++i) {
-      const int32_t* e = desc + kStepHead + kStepSeq * i;
-      items += splits_of(e, page, mid);
+  int32_t* last = desc + kStepHead + kStepSeq * n;
+  memset(last, 0, sizeof(int32_t) * kStepSeq);
+  last[3] = static_cast<int32_t>(row);
+  last[4] = static_cast<int32_t>(item);
+  int32_t* runs = desc + kStepHead + kStepSeq * (n + 1) + item;
+  for (int fronts = 1; fronts >= 0; --fronts) {
+    int64_t nr = 0, widest = longest;
+    auto add = [&](int64_t slot, int64_t row0, int64_t tokens, int64_t u0, int64_t u1, int64_t b) {
+      int32_t* r = runs + kStepRun * nr++;
+      r[0] = static_cast<int32_t>(slot);
+      r[1] = static_cast<int32_t>(row0);
+      r[2] = static_cast<int32_t>(tokens);
+      r[3] = static_cast<int32_t>(u0);
+      r[4] = static_cast<int32_t>(tokens ? u1 : u0);
+      r[7] = static_cast<int32_t>(b);
+    };
+    for (int64_t i = 0; i < n;) {
+      int64_t j = i + 1, common = 0, tokens = counts[i];
+      for (; fronts && counts[i] && j < n && counts[j]; ++j) {
+        const int64_t a = lens[seq[i]] / page, b = lens[seq[j]] / page, most = a < b ? a : b;
+        const int64_t c = shared(table, max_blocks, seq[i], seq[j], j > i + 1 && common < most ? common : most);
+        if (c * page < kFront * kUnit || 2 * c < common) break;
+        common = c;
+        tokens += counts[j];
+      }
+      const int64_t front = j > i + 1 ? common * page / kUnit : 0;
+      if (front) add(seq[i], desc[kStepHead + kStepSeq * i + 3], tokens, 0, front, -1);
+      widest = front && tokens > widest ? tokens : widest;
+      const int64_t of = front ? nr : 0;      // 1 + its index
+      for (int64_t b = i; b < j; ++b) {
+        int32_t* e = desc + kStepHead + kStepSeq * b;
+        e[5] = static_cast<int32_t>(nr);
+        e[7] = static_cast<int32_t>(of);
+        add(seq[b], e[3], counts[b], front, units_of(lens[seq[b]] + counts[b], page), b);
+      }
+      i = j;
     }
-    if (items <= split_cap) hi = mid;
-    else lo = mid + 1;
+    int64_t most = 4;                         // a wavefront takes a unit at least
+    for (int64_t i = 0; i < nr; ++i) most = runs[kStepRun * i + 4] - runs[kStepRun * i + 3] > most ? runs[kStepRun * i + 4] - runs[kStepRun * i + 3] : most;
+    auto splits = [&](int64_t i, int64_t per) { return (runs[kStepRun * i + 4] - runs[kStepRun * i + 3] + per - 1) / per; };
+    auto weighted = [&](int64_t per) {
+      int64_t w = 0;
+      for (int64_t i = 0; i < nr; ++i) w += splits(i, per) * (runs[kStepRun * i + 7] < 0 ? (runs[kStepRun * i + 2] + 3) / 4 : 1);
+      return w;
+    };
+    int64_t lo = 4, hi = most;
+    while (lo < hi) {
+      const int64_t mid = (lo + hi) / 2;
+      if (weighted(mid) <= split_cap) hi = mid;
+      else lo = mid + 1;
+    }
+    int64_t split = 0, base = 0;
+    for (int64_t i = 0; i < nr; ++i) {
+      int32_t* r = runs + kStepRun * i;
+      r[5] = static_cast<int32_t>(split);
+      r[6] = static_cast<int32_t>(base);
+      split += splits(i, lo);
+      base += splits(i, lo) * r[2];
+    }
+    if (fronts && nr > n && (weighted(lo) > split_cap || widest > most_run || base > most_tokens)) continue;
+    int32_t* r = runs + kStepRun * nr;
+    memset(r, 0, sizeof(int32_t) * kStepRun);
+    r[5] = static_cast<int32_t>(split);
+    r[6] = static_cast<int32_t>(base);
+    desc[0] = static_cast<int32_t>(n);
+    desc[1] = static_cast<int32_t>(item);
+    desc[2] = static_cast<int32_t>(split);
+    desc[3] = static_cast<int32_t>(lo);
+    desc[4] = even;
+    desc[5] = static_cast<int32_t>(longest);
+    desc[6] = static_cast<int32_t>(widest);
+    desc[7] = base < INT64_C(1) << 31 ? static_cast<int32_t>(base) : -1;
+    last[5] = static_cast<int32_t>(nr);
+    return;
   }
-  int64_t split = 0;
-  for (int64_t i = 0; i < n; ++i) {
-    int32_t* e = desc + kStepHead + kStepSeq * i;
-    e[5] = static_cast<int32_t>(split);
-    split += splits_of(e, page, lo);
-  }
-  int32_t* e = desc + kStepHead + kStepSeq * n;
-  memset(e, 0, sizeof(int32_t) * kStepSeq);
-  e[3] = static_cast<int32_t>(row);
-  e[4] = static_cast<int32_t>(item);
-  e[5] = static_cast<int32_t>(split);
-  memset(desc, 0, sizeof(int32_t) * kStepHead);
-  desc[0] = static_cast<int32_t>(n);
-  desc[1] = static_cast<int32_t>(item);
-  desc[2] = static_cast<int32_t>(split);
-  desc[3] = static_cast<int32_t>(lo);
-  desc[4] = even;
-  desc[5] = static_cast<int32_t>(longest);
-  return item;
 }
 
 int64_t item_cap(int64_t page, const int64_t* counts, int64_t n) {
@@ -514,18 +564,20 @@ extern "C" int64_t kvq_pages_step_words(int64_t page, const int64_t* counts, int
   if (n < 0 || (n && !counts) || (page != 32 && page != 64 && page != 128)) return -1;
   for (int64_t i = 0; i < n; ++i)
     if (counts[i] < 0 || counts[i] >= INT64_C(1) << 31) return -1;
-  return kStepHead + kStepSeq * (n + 1) + item_cap(page, counts, n);
+  return kStepHead + kStepSeq * (n + 1) + item_cap(page, counts, n) + kStepRun * (2 * n + 1);
 }
 
 extern "C" int kvq_pages_extend(int64_t* lens, int32_t* table, int32_t* refs, uint8_t* open, int64_t* account, int64_t slots,
                                 int64_t pages, int64_t max_blocks, int64_t page, int64_t max_tokens, const int64_t* seq,
-                                const int64_t* counts, int64_t n, int64_t split_cap, int32_t* desc, int64_t desc_words,
-                                int32_t* desc_device, void* stream) {
+                                const int64_t* counts, int64_t n, int64_t split_cap, int64_t most_run, int64_t most_tokens,
+                                int32_t* desc, int64_t desc_words, int32_t* desc_device, void* stream) {
   KVQ_REQUIRE(lens && table && refs && open && account && desc && n > 0 && seq && counts,
               "kvq_pages_extend: null pointer or no sequence");
   const int64_t need_words = kvq_pages_step_words(page, counts, n);
   KVQ_REQUIRE(need_words >= 0 && need_words <= desc_words, "kvq_pages_extend: bad counts or a short description");
-  KVQ_REQUIRE(split_cap >= n, "kvq_pages_extend: at least one split item per sequence is needed");
+  int64_t active = 0;
+  for (int64_t i = 0; i < n; ++i) active += counts[i] > 0;
+  KVQ_REQUIRE(split_cap >= active, "kvq_pages_extend: at least one split item per sequence is needed");
   // every check first: nothing is changed by a call that is refused
   int64_t need = 0, rows = 0, bad = -1, twice = -1;
   int64_t checked = 0;
@@ -549,7 +601,7 @@ extern "C" int kvq_pages_extend(int64_t* lens, int32_t* table, int32_t* refs, ui
   KVQ_REQUIRE(rows < INT64_C(1) << 31, "kvq_pages_extend: too many rows");
   KVQ_REQUIRE(need <= account[0], "decode buffer exhausted: %lld pages needed, %lld free", static_cast<long long>(need),
               static_cast<long long>(account[0]));
-  describe(lens, open, page, seq, counts, n, split_cap, desc);
+  describe(lens, open, table, max_blocks, page, seq, counts, n, split_cap, most_run, most_tokens, desc);
   int32_t* page_of = desc + kStepHead + kStepSeq * (n + 1);
   int64_t low = account[1];
   for (int64_t i = 0; i < n; ++i) {
@@ -571,7 +623,7 @@ extern "C" int kvq_pages_extend(int64_t* lens, int32_t* table, int32_t* refs, ui
   }
   account[0] -= need;
   account[1] = low;
-  const int64_t words = kStepHead + kStepSeq * (n + 1) + desc[1];
+  const int64_t words = kStepHead + kStepSeq * (n + 1) + desc[1] + kStepRun * (desc[kStepHead + kStepSeq * n + 5] + 1);
   return desc_device ? write_words(desc, words, desc_device, static_cast<hipStream_t>(stream)) : KVQ_OK;
 }
 

@@ -39,7 +39,7 @@ def _ints(x, what: str) -> np.ndarray:
 class Step:
     """New tokens of some slots: ``rows`` packed rows, slot by slot.  Made by ``PagedCache.extend``."""
 
-    __slots__ = ("slots", "counts", "ends", "rows", "items", "splits", "max_count", "desc", "ptr", "host", "generation", "stamp")
+    __slots__ = ("slots", "counts", "ends", "rows", "items", "splits", "run_tokens", "split_tokens", "fronts", "desc", "ptr", "host", "generation", "stamp")
 
 
 class PagedCache:
@@ -145,17 +145,21 @@ class PagedCache:
             st.desc = torch.empty(words, dtype=torch.int32, device=self.device)
             st.ptr = st.desc.data_ptr()
             st.splits = max(n, -(-SPLIT_BLOCKS[self.d] // self.Hkv))
+            st.run_tokens = st.split_tokens = 1 << 31
         else:
             st = into
             if not np.array_equal(st.counts, c):
                 raise ValueError("a step is rewritten for the same counts only")
         _lib.call_on(self.device, "kvq_pages_extend", *self._host, self.slots, self.pages, self.max_blocks, self.page,
-                     self.max_tokens, s.ctypes.data, c.ctypes.data, n, st.splits, st.host.ctypes.data, st.host.size,
+                     self.max_tokens, s.ctypes.data, c.ctypes.data, n, st.splits, st.run_tokens, st.split_tokens, st.host.ctypes.data, st.host.size,
                      st.ptr, _lib.stream_of(st.desc))
+        head = st.host[:8].tolist()
         if into is None:
-            st.splits = max(1, int(st.host[2]))         # what later steps written into this one keep to
-            st.items = st.host.size - 8 * (n + 2)
-            st.rows, st.max_count = int(st.host[8 * n + 11]), int(st.host[5])
+            # what later steps written into this one keep to: without shared fronts any of them does
+            st.splits, st.run_tokens = max(1, head[2]), head[6]
+            st.split_tokens = max(head[7], st.splits * head[5])
+            st.items, st.rows = st.host.size - 24 * n - 24, int(st.host[8 * n + 11])
+        st.fronts = int(st.host[8 * n + 13]) > n
         self._stamp += 1
         st.slots, st.counts, st.ends, st.generation, st.stamp = s, c, self._lens[s], self._generation, self._stamp
         return st
@@ -257,7 +261,7 @@ class PagedCache:
 
 
 def paged_workspace_floats(step: Step, Hq: int, Hkv: int, d: int) -> int:
-    n = _lib.load().kvq_paged_decode_workspace(step.splits, Hkv, Hq // Hkv, step.max_count, d)
+    n = _lib.load().kvq_paged_decode_workspace(step.split_tokens, Hkv, Hq // Hkv, d)
     if n < 0:
         raise _lib.KVQError("kvq_paged_decode_workspace rejected the shape")
     return n
@@ -266,7 +270,8 @@ def paged_workspace_floats(step: Step, Hq: int, Hkv: int, d: int) -> int:
 def paged_decode(q: torch.Tensor, scaling: float, cache: PagedCache, layer: int, step: Step, *,
                  out: Optional[torch.Tensor] = None, workspace: Optional[torch.Tensor] = None) -> torch.Tensor:
     """Attention of the step's query rows q (rows, Hq, d), slot by slot, over the cache; returns (rows, Hq, d).  Query i of
-    a slot's new tokens sees every token up to its own.  Meant for a few tokens per slot (16 rows = query
+    a slot's new tokens sees every token up to its own.  Pages that neighbouring slots of the step share (forks of one
+    sequence, named side by side) are read once for all of them.  Meant for a few tokens per slot (16 rows = query
     heads of a KV head times tokens go over the keys together); for many, ``cache.rows`` and prompt_attention."""
     if not 0 <= layer < cache.layers:
         raise IndexError(f"no layer {layer} (of {cache.layers})")
@@ -292,6 +297,6 @@ def paged_decode(q: torch.Tensor, scaling: float, cache: PagedCache, layer: int,
         raise ValueError("workspace must be contiguous float32 on the cache's device")
     table, max_blocks, _, _, page, code = cache._fixed
     _lib.call_on(device, "kvq_paged_decode", q.data_ptr(), qt, qh, cache._type, step.rows, Hq, Hkv, d, float(scaling), step.ptr,
-                 step.splits, step.max_count, table, max_blocks, page, code, *cache._at[layer], out.data_ptr(), workspace.data_ptr(),
-                 workspace.numel(), cache._tickets[layer], _lib.stream_of(q))
+                 step.splits, step.run_tokens, step.split_tokens, table, max_blocks, page, code, *cache._at[layer], out.data_ptr(), workspace.data_ptr(),
+                 workspace.numel(), None if step.fronts else cache._tickets[layer], _lib.stream_of(q))
     return out

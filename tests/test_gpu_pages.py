@@ -177,6 +177,43 @@ def test_fork_free_and_moves():
     assert m.cache.free_pages == 1
 
 
+@pytest.mark.parametrize("page,d,Hkv,rep", [(32, 64, 2, 4), (64, 128, 1, 3), (128, 64, 1, 8)])
+def test_shared_fronts(page, d, Hkv, rep):
+    """Forks side by side read their shared pages once: uneven drafts, growth over block borders, and others between."""
+    import kvq
+    m = Mirror(slots=12, pages=200, max_tokens=2500, Hkv=Hkv, d=d, page=page, seed=page)
+    m.push([0, 1, 2], [1500, 700, 40])
+    m.fork([0, 0, 0, 1, 2, 0], [3, 4, 5, 6, 7, 8])
+    step = m.push([0, 3, 4, 1, 6, 2, 7, 5], [1, 3, 1, 2, 1, 1, 1, 1])
+    assert step.fronts
+    m.decode(step, rep * Hkv, what="forks")
+    step = m.push([8, 3, 4], [page + 5, 1, 2 * page])
+    q, out = m.decode(step, rep * Hkv, what="apart")
+    assert step.fronts and torch.equal(out, kvq.paged_decode(q.cuda(), d ** -0.5, m.cache, 0, step))
+    step = m.push([3, 2, 4], [1, 1, 1])                             # not side by side
+    assert not step.fronts
+    m.decode(step, rep * Hkv, what="between")
+    m.free([0, 8])
+    step = m.push([4, 3], [1, 2])
+    assert step.fronts
+    m.decode(step, rep * Hkv, what="freed")
+
+
+def test_a_step_written_over_one_without_forks():
+    """A captured decode of two sequences runs a later step whose slots have come to share pages."""
+    import kvq
+    m = Mirror(slots=4, pages=90, max_tokens=1300, Hkv=1, d=64, page=32, seed=17)
+    m.push([0, 1], [600, 300])
+    step = m.push([0, 1], [2, 1])
+    floats = kvq.paged_workspace_floats(step, 4, 1, 64)
+    m.free([1])
+    m.fork([0], [1])
+    step, [(k, v)] = m.extend([0, 1], [2, 1], into=step)
+    m.cache.append(0, k.cuda(), v.cuda(), step)
+    assert kvq.paged_workspace_floats(step, 4, 1, 64) == floats
+    m.decode(step, 4, what="rewritten")
+
+
 def test_random_life():
     """A few hundred random steps, forks, frees and moves."""
     rng = random.Random(11)
@@ -362,6 +399,7 @@ def test_gpu_refusals():
     with pytest.raises(ValueError):
         c.extend([], [])
     none = c.extend([0, 2], [0, 0])
+    c.extend([0, 2], [0, 0], into=none)
     empty = torch.empty((0, 2, 64), dtype=torch.bfloat16, device="cuda")
     c.append(1, empty, empty, none)
     assert kvq.paged_decode(torch.empty((0, 4, 64), dtype=torch.bfloat16, device="cuda"), 0.1, c, 0, none).shape == (0, 4, 64)

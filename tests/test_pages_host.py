@@ -23,12 +23,12 @@ class Host:
         self.account = np.array([pages, 0], np.int64)
         self.p = [x.ctypes.data for x in (self.lens, self.table, self.refs, self.open, self.account)]
 
-    def extend(self, slots, counts, cap=64, words=None):
+    def extend(self, slots, counts, cap=64, words=None, run=1 << 31, tokens=1 << 31):
         s, c = np.array(slots, np.int64), np.array(counts, np.int64)
         n = self.lib.kvq_pages_step_words(self.page, c.ctypes.data, len(c)) if words is None else words
         self.desc = np.zeros(max(n, 1), np.int32)
         return self.lib.kvq_pages_extend(*self.p, self.slots, self.pages, self.blocks, self.page, self.max_tokens, s.ctypes.data,
-                                         c.ctypes.data, len(s), cap, self.desc.ctypes.data, n, None, None)
+                                         c.ctypes.data, len(s), cap, run, tokens, self.desc.ctypes.data, n, None, None)
 
     def fork(self, src, dst):
         s, d = np.array(src, np.int64), np.array(dst, np.int64)
@@ -100,24 +100,61 @@ def test_accounts_follow_the_model(page):
 
 
 def _description(host, slots, counts):
-    """Rows, items, split items and the pages of what gets full."""
+    """Rows, items, the pages of what gets full; runs: every unit of every sequence in one, shared ones only in front."""
     n, d, page = len(slots), host.desc, host.page
     seq = d[8:8 + 8 * (n + 1)].reshape(n + 1, 8)
-    row = item = split = 0
+    pages, items, nr = d[8 + 8 * (n + 1):], int(d[1]), int(seq[n, 5])
+    runs = pages[items:items + 8 * (nr + 1)].reshape(nr + 1, 8)
+    row = item = 0
     for i, (s, c) in enumerate(zip(slots, counts)):
         end = int(host.lens[s])
         pos0 = end - c
-        assert seq[i, :6].tolist() == [s, pos0, c, row, item, split]
+        assert seq[i, :5].tolist() == [s, pos0, c, row, item]
         for j in range(pos0 // page, (end - 1) // page + 1 if c else 0):
             want = host.table[s, j] if (j + 1) * page <= end else -1
-            assert d[8 + 8 * (n + 1) + item] == want
+            assert pages[item] == want
             item += 1
-        row += c
         full = end // page * page
         units = -(-full // 64) + -(-(end - full) // 64)
-        split += -(-units // int(d[3])) if c else 0
+        own, front = runs[seq[i, 5]], seq[i, 7]
+        assert own[[0, 1, 2, 7]].tolist() == [s, row, c, i] and own[4] == (units if c else own[3])
+        assert own[3] == (runs[front - 1, 4] if front else 0)
+        if front:
+            f = runs[front - 1]
+            assert c and f[3] == 0 and f[4] >= 4 and f[7] == -1 and f[1] <= row and row + c <= f[1] + f[2]
+            blocks = f[4] * 64 // page
+            assert f[4] * 64 <= pos0 // page * page
+            assert np.array_equal(host.table[s, :blocks], host.table[f[0], :blocks])
+        row += c
+    split = base = 0
+    for r in runs[:nr]:
+        assert r[5] == split and r[6] == base
+        k = -(-(r[4] - r[3]) // int(d[3]))
+        split, base = split + k, base + k * r[2]
+    assert runs[nr, 5:7].tolist() == [split, base]
     assert d[4] == all(b - a == 1 for a, b in zip(seq[:, 4], seq[1:, 4]))
-    assert seq[n, 3:6].tolist() == [row, item, split] and d[:3].tolist() == [n, item, split] and split <= 64
+    assert seq[n, 3:5].tolist() == [row, item] and d[:3].tolist() == [n, item, split] and split <= 64
+    assert d[5:8].tolist() == [max(counts), max(max(counts), *(int(r[2]) for r in runs[:nr])), base]
+
+
+def test_fronts_of_forks():
+    """Forks named side by side share a run in front; where the step has to fit an older one they do not."""
+    host = Host(8, 60, 60 * 64, 64)
+    assert host.extend([0], [64 * 9 + 5]) == 0 and host.extend([1], [64 * 6]) == 0
+    assert host.fork([0, 0, 0, 1], [2, 3, 4, 5]) == 0
+    slots, counts = [2, 3, 0, 4, 1, 5, 6], [1, 2, 1, 64, 1, 1, 3]
+    assert host.extend(slots, counts) == 0
+    _description(host, slots, counts)
+    seq = host.desc[8:8 + 8 * 8].reshape(8, 8)
+    assert seq[:7, 7].tolist() == [1, 1, 1, 1, 6, 6, 0] and seq[7, 5] == 9
+    host.free(range(8))
+    assert host.extend([0], [64 * 9]) == 0 and host.fork([0], [1]) == 0
+    for limit in (dict(run=1), dict(tokens=2), dict(cap=2)):
+        assert host.extend([0, 1], [1, 1], **limit) == 0
+        assert int(host.desc[8 + 16 + 5]) == 2
+    assert host.extend([0, 1], [1, 1], run=2, tokens=64, cap=64) == 0
+    assert int(host.desc[8 + 16 + 5]) == 3
+    assert host.extend([0, 1], [1, 0]) == 0 and int(host.desc[8 + 16 + 5]) == 2      # nobody to share with
 
 
 def test_refusals_change_nothing():
@@ -211,8 +248,8 @@ def test_kernel_entries_refuse_before_any_launch():
     assert rc == 1 and b"page" in lib.kvq_last_error()
     rc = lib.kvq_pages_append(one, 64, 64, one, 64, 64, 2, one, 1, one, 4, 2, 64, 64, 3, one, one, one, one, one, None)
     assert rc == 1 and b"code" in lib.kvq_last_error()
-    need = lib.kvq_paged_decode_workspace(4, 2, 2, 1, 64)
-    assert need == 4 * 2 * 16 * 66
-    rc = lib.kvq_paged_decode(one, 256, 64, 2, 1, 4, 2, 64, 0.1, one, 4, 1, one, 4, 64, 0, one, one, one, one, one, one, one, need - 1, None, None)
+    need = lib.kvq_paged_decode_workspace(4, 2, 2, 64)
+    assert need == 4 * 2 * 2 * 66
+    rc = lib.kvq_paged_decode(one, 256, 64, 2, 1, 4, 2, 64, 0.1, one, 4, 1, 4, one, 4, 64, 0, one, one, one, one, one, one, one, need - 1, None, None)
     assert rc == 1 and b"workspace" in lib.kvq_last_error()
-    assert lib.kvq_paged_decode_workspace(4, 2, 2, 1, 96) == -1
+    assert lib.kvq_paged_decode_workspace(4, 2, 2, 96) == -1
