@@ -693,7 +693,8 @@ int kvq_prompt_attention(const void* q, int64_t q_st, int64_t q_sh, const void* 
  * kvq_pages_extend claims counts[i] >= 0 tokens for slot seq[i]: the lowest free page for each block that gets
  * full, in order; refused whole ("decode buffer exhausted") when a slot's max_tokens or the free pages do
  * not suffice.  It writes the step's description to `desc` (host, kvq_pages_step_words words) and, by
- * value with launches on `stream`, to desc_device (NULL: host only).  split_cap >= n bounds the decode's split items.
+ * value with launches on `stream`, to desc_device (NULL: host only).  split_cap >= n bounds the decode's split items; a step
+ * of at most few_units units (64 tokens of a sequence) takes about few_cap of them.
  * Pages that neighbouring sequences of the step share in front are read once for all of them where the description
  * stays within most_run tokens of a run (its seventh word) and most_tokens of all split items (its eighth).
  * kvq_pages_append writes one layer's rows k, v (rows, H, D) of the step; running it again writes the same.
@@ -709,8 +710,8 @@ int kvq_prompt_attention(const void* q, int64_t q_st, int64_t q_sh, const void* 
 int64_t kvq_pages_step_words(int64_t page, const int64_t* counts, int64_t n);
 int kvq_pages_extend(int64_t* lens, int32_t* table, int32_t* refs, uint8_t* open, int64_t* account, int64_t slots,
                      int64_t pages, int64_t max_blocks, int64_t page, int64_t max_tokens, const int64_t* seq,
-                     const int64_t* counts, int64_t n, int64_t split_cap, int64_t most_run, int64_t most_tokens,
-                     int32_t* desc, int64_t desc_words, int32_t* desc_device, void* stream);
+                     const int64_t* counts, int64_t n, int64_t split_cap, int64_t few_cap, int64_t few_units,
+                     int64_t most_run, int64_t most_tokens, int32_t* desc, int64_t desc_words, int32_t* desc_device, void* stream);
 int kvq_pages_append(const void* k, int64_t k_st, int64_t k_sh, const void* v, int64_t v_st, int64_t v_sh, int dtype,
                      const int32_t* step, int64_t items, int32_t* table, int64_t max_blocks, int64_t H, int64_t D,
                      int64_t page, int code, uint8_t* kc, uint8_t* vc, float* sc, void* ko, void* vo, void* stream);

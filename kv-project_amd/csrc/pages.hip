@@ -420,10 +420,13 @@ int64_t shared(const int32_t* table, int64_t max_blocks, int64_t a, int64_t b, i
 constexpr int64_t kFront = 4;
 
 // Fills the description from lens (before), counts and open buffers; pages are written by the caller.  split_cap bounds
-// the split items (those of a front weighted by the workgroups that its rows take at four query heads per KV head).
+// the split items (those of a front weighted by the workgroups that its rows take at four query heads per KV head);
+// of no more than few_units units there are few_cap items, unless that makes the longest one more than twice an
+// even share.
 // most_run, most_tokens: where the step has to fit a launch that was captured; fronts that do not are left out.
 void describe(const int64_t* lens, const uint8_t* open, const int32_t* table, int64_t max_blocks, int64_t page, const int64_t* seq,
-              const int64_t* counts, int64_t n, int64_t split_cap, int64_t most_run, int64_t most_tokens, int32_t* desc) {
+              const int64_t* counts, int64_t n, int64_t split_cap, int64_t few_cap, int64_t few_units, int64_t most_run, int64_t most_tokens,
+              int32_t* desc) {
   int64_t row = 0, item = 0, longest = 0;
   bool even = true;
   for (int64_t i = 0; i < n; ++i) {
@@ -486,11 +489,20 @@ void describe(const int64_t* lens, const uint8_t* open, const int32_t* table, in
       for (int64_t i = 0; i < nr; ++i) w += splits(i, per) * (runs[kStepRun * i + 7] < 0 ? (runs[kStepRun * i + 2] + 3) / 4 : 1);
       return w;
     };
-    int64_t lo = 4, hi = most;
-    while (lo < hi) {
-      const int64_t mid = (lo + hi) / 2;
-      if (weighted(mid) <= split_cap) hi = mid;
-      else lo = mid + 1;
+    auto units = [&](int64_t cap) {           // of an item, so that there are at most `cap` items
+      int64_t lo = 4, hi = most;
+      while (lo < hi) {
+        const int64_t mid = (lo + hi) / 2;
+        if (weighted(mid) <= cap) hi = mid;
+        else lo = mid + 1;
+      }
+      return lo;
+    };
+    int64_t lo = units(split_cap);
+    const int64_t all = weighted(1);
+    if (few_cap > 0 && few_cap < split_cap && all <= few_units) {
+      const int64_t few = units(few_cap), even = (all + few_cap - 1) / few_cap;
+      if (few <= 2 * (even > 4 ? even : 4)) lo = few;
     }
     int64_t split = 0, base = 0;
     for (int64_t i = 0; i < nr; ++i) {
@@ -569,8 +581,8 @@ extern "C" int64_t kvq_pages_step_words(int64_t page, const int64_t* counts, int
 
 extern "C" int kvq_pages_extend(int64_t* lens, int32_t* table, int32_t* refs, uint8_t* open, int64_t* account, int64_t slots,
                                 int64_t pages, int64_t max_blocks, int64_t page, int64_t max_tokens, const int64_t* seq,
-                                const int64_t* counts, int64_t n, int64_t split_cap, int64_t most_run, int64_t most_tokens,
-                                int32_t* desc, int64_t desc_words, int32_t* desc_device, void* stream) {
+                                const int64_t* counts, int64_t n, int64_t split_cap, int64_t few_cap, int64_t few_units, int64_t most_run,
+                                int64_t most_tokens, int32_t* desc, int64_t desc_words, int32_t* desc_device, void* stream) {
   KVQ_REQUIRE(lens && table && refs && open && account && desc && n > 0 && seq && counts,
               "kvq_pages_extend: null pointer or no sequence");
   const int64_t need_words = kvq_pages_step_words(page, counts, n);
@@ -601,7 +613,7 @@ extern "C" int kvq_pages_extend(int64_t* lens, int32_t* table, int32_t* refs, ui
   KVQ_REQUIRE(rows < INT64_C(1) << 31, "kvq_pages_extend: too many rows");
   KVQ_REQUIRE(need <= account[0], "decode buffer exhausted: %lld pages needed, %lld free", static_cast<long long>(need),
               static_cast<long long>(account[0]));
-  describe(lens, open, table, max_blocks, page, seq, counts, n, split_cap, most_run, most_tokens, desc);
+  describe(lens, open, table, max_blocks, page, seq, counts, n, split_cap, few_cap, few_units, most_run, most_tokens, desc);
   int32_t* page_of = desc + kStepHead + kStepSeq * (n + 1);
   int64_t low = account[1];
   for (int64_t i = 0; i < n; ++i) {

@@ -108,7 +108,7 @@ SIGNATURES = {
     "kvq_prompt_attention": (i32, [vp, i64, i64, vp, i64, i64, vp, i64, i64, i32, i64, i64, i64, f32, vp, i64, i64, i64, vp, vp,
                                    i64, vp]),
     "kvq_pages_step_words": (i64, [i64, vp, i64]),
-    "kvq_pages_extend": (i32, [vp, vp, vp, vp, vp, i64, i64, i64, i64, i64, vp, vp, i64, i64, i64, i64, vp, i64, vp, vp]),
+    "kvq_pages_extend": (i32, [vp, vp, vp, vp, vp, i64, i64, i64, i64, i64, vp, vp, i64, i64, i64, i64, i64, i64, vp, i64, vp, vp]),
     "kvq_pages_append": (i32, [vp, i64, i64, vp, i64, i64, i32, vp, i64, vp, i64, i64, i64, i64, i32, vp, vp, vp, vp, vp, vp]),
     "kvq_pages_rows": (i32, [vp, vp, i64, vp, i64, vp, i64, i64, i64, i64, i32, i32, vp, vp, vp, vp, vp, vp, vp, i64, vp]),
     "kvq_pages_fork": (i32, [vp, vp, vp, vp, i64, i64, i64, vp, vp, i64, i64, i64, i64, vp, vp, vp, vp]),

@@ -24,9 +24,13 @@ from .prompt import device_of, rows16
 
 CODES = {"int8": 0, "e4m3": 1}
 PAGES = (32, 64, 128)
-# workgroups a decode is split into at most, by head_dim: two and three on each of 256 CUs.  16 sequences at 32k,
+# Workgroups a decode is split into at most, by head_dim: two and three on each of 256 CUs.  16 sequences at 32k,
 # head_dim 128: 197 us with 512, 202 with 768; 48 ragged ones, head_dim 64: 40 with 512, 33 with 768, 34 with 1024.
 SPLIT_BLOCKS = {128: 512, 64: 768}
+# One on each CU where there are few units of 64 tokens (times KV heads), joined in the same launch: with 256 and with
+# 512, at head_dim 128, 2048 of them 13.5 and 18.4 us, 8192 29.4 and 34.8, 16384 55.9 and 55.8.
+FEW_BLOCKS, FEW_UNITS = 256, 16384
+
 
 
 def _ints(x, what: str) -> np.ndarray:
@@ -146,12 +150,14 @@ class PagedCache:
             st.ptr = st.desc.data_ptr()
             st.splits = max(n, -(-SPLIT_BLOCKS[self.d] // self.Hkv))
             st.run_tokens = st.split_tokens = 1 << 31
+            few = (-(-FEW_BLOCKS // self.Hkv), FEW_UNITS // self.Hkv)
         else:
             st = into
             if not np.array_equal(st.counts, c):
                 raise ValueError("a step is rewritten for the same counts only")
+            few = (0, 0)
         _lib.call_on(self.device, "kvq_pages_extend", *self._host, self.slots, self.pages, self.max_blocks, self.page,
-                     self.max_tokens, s.ctypes.data, c.ctypes.data, n, st.splits, st.run_tokens, st.split_tokens, st.host.ctypes.data, st.host.size,
+                     self.max_tokens, s.ctypes.data, c.ctypes.data, n, st.splits, *few, st.run_tokens, st.split_tokens, st.host.ctypes.data, st.host.size,
                      st.ptr, _lib.stream_of(st.desc))
         head = st.host[:8].tolist()
         if into is None:

@@ -23,12 +23,12 @@ class Host:
         self.account = np.array([pages, 0], np.int64)
         self.p = [x.ctypes.data for x in (self.lens, self.table, self.refs, self.open, self.account)]
 
-    def extend(self, slots, counts, cap=64, words=None, run=1 << 31, tokens=1 << 31):
+    def extend(self, slots, counts, cap=64, words=None, run=1 << 31, tokens=1 << 31, few=(0, 0)):
         s, c = np.array(slots, np.int64), np.array(counts, np.int64)
         n = self.lib.kvq_pages_step_words(self.page, c.ctypes.data, len(c)) if words is None else words
         self.desc = np.zeros(max(n, 1), np.int32)
         return self.lib.kvq_pages_extend(*self.p, self.slots, self.pages, self.blocks, self.page, self.max_tokens, s.ctypes.data,
-                                         c.ctypes.data, len(s), cap, run, tokens, self.desc.ctypes.data, n, None, None)
+                                         c.ctypes.data, len(s), cap, *few, run, tokens, self.desc.ctypes.data, n, None, None)
 
     def fork(self, src, dst):
         s, d = np.array(src, np.int64), np.array(dst, np.int64)
@@ -135,6 +135,15 @@ def _description(host, slots, counts):
     assert d[4] == all(b - a == 1 for a, b in zip(seq[:, 4], seq[1:, 4]))
     assert seq[n, 3:5].tolist() == [row, item] and d[:3].tolist() == [n, item, split] and split <= 64
     assert d[5:8].tolist() == [max(counts), max(max(counts), *(int(r[2]) for r in runs[:nr])), base]
+
+
+def test_few_units_take_few_items():
+    host = Host(6, 2000, 64 * 400, 64)
+    for slots, counts, few, want in (([0], [64 * 64], (16, 100), 16), ([1], [64 * 64], (16, 63), 16), ([2], [64 * 300], (16, 400), 16),
+                                     ([3, 4, 5], [64 * 300, 64, 64], (3, 400), 64)):       # the last: one would hold nearly all
+        assert host.extend(slots, counts, cap=64, few=few) == 0
+        _description(host, slots, counts)
+        assert want // 2 < int(host.desc[2]) <= want
 
 
 def test_fronts_of_forks():
