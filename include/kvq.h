@@ -731,7 +731,7 @@ int kvq_pages_move(const int64_t* lens, int32_t* table, const int32_t* refs, int
 
 /* ------------------------------------------------------------------------------------------
  * Attention of a step's query rows over the paged cache: q (rows, Hq, D), the step's rows in order; query
- * i of a sequence with `count` new tokens sees all tokens up to its own.  split_items, run_tokens and split_tokens: at
+ * i of a sequence with `count` new tokens sees all tokens up to its own.  sequences: of the step; split_items, run_tokens and split_tokens: at
  * least the description's third, seventh and eighth word; they give the grid and the workspace.  out (rows, Hq, D)
  * contiguous.  workspace: kvq_paged_decode_workspace floats, no clearing; calls that share one must not
  * overlap in time.
@@ -742,8 +742,8 @@ int kvq_pages_move(const int64_t* lens, int32_t* table, const int32_t* refs, int
  * ---------------------------------------------------------------------------------------- */
 int64_t kvq_paged_decode_workspace(int64_t split_tokens, int64_t H, int64_t rep, int64_t D);
 int kvq_paged_decode(const void* q, int64_t q_st, int64_t q_sh, int dtype, int64_t rows, int64_t Hq, int64_t H, int64_t D,
-                     float scaling, const int32_t* step, int64_t split_items, int64_t run_tokens, int64_t split_tokens,
-                     const int32_t* table,
+                     float scaling, const int32_t* step, int64_t sequences, int64_t split_items, int64_t run_tokens,
+                     int64_t split_tokens, const int32_t* table,
                      int64_t max_blocks, int64_t page, int code, const uint8_t* kc, const uint8_t* vc, const float* sc,
                      const void* ko, const void* vo, void* out, float* workspace, int64_t workspace_floats,
                      int32_t* tickets, void* stream);

@@ -74,6 +74,7 @@ struct DecodeArgs {
   const uint16_t* q;
   int64_t q_st, q_sh;
   const int* step;
+  int n;                                      // sequences of the step
   const int* table;
   int64_t max_blocks;
   int H, rep;                                 // KV heads, query heads per KV head
@@ -109,8 +110,8 @@ template <int D, bool SHARED>
 struct Join {
   float top = -INFINITY, l = 0.0f, o[D / 64] = {};
   // row R of each of a run's split items, 64 maxima at a time
-  __device__ __forceinline__ void add(const DecodeArgs& a, const StepRun& run, int items, int R, int h) {
-    const int lane = threadIdx.x & 63;
+  __device__ __forceinline__ void add(const DecodeArgs& a, const StepRun& run, int R, int h) {
+    const int lane = threadIdx.x & 63, items = run.items;
     const int64_t first = (static_cast<int64_t>(a.rep) * run.base + R) * a.H + h, stride = static_cast<int64_t>(a.rep) * run.tokens * a.H;
     const float* stat = a.part + a.part_rows * a.H * D;
     for (int i0 = 0; i0 < items; i0 += 64) {
@@ -195,21 +196,21 @@ __global__ __launch_bounds__(kThreads, 3) void paged_split_kernel(DecodeArgs a) 
   __shared__ float join[kWaves][kRows][D + 4];
   __shared__ float stat[kWaves][kRows][2];
   const int* step = a.step;
-  const int n = step[0], per = step[3];
+  const int per = step[3];
   // pieces of one item and head on one of the 8 dies, next to each other: they read the same pages
   const int group = blockIdx.x / (8 * a.pieces), within = blockIdx.x % (8 * a.pieces);
   const int64_t ih = static_cast<int64_t>(group) * 8 + within % 8;
   const int piece = within / 8, item = static_cast<int>(ih / a.H), h = static_cast<int>(ih % a.H);
   if (item >= step[2]) return;
-  const int* runs = step_runs(step, n);
-  const int ri = __builtin_amdgcn_readfirstlane(last_not_above(runs + 5, kStepRun, step[kStepHead + kStepSeq * n + 5], item));
+  const int* runs = step_runs(step, a.n);
+  // one sequence is one run: no look before it
+  const int ri = a.n == 1 ? 0 : __builtin_amdgcn_readfirstlane(last_not_above(runs + 5, kStepRun, step[8], item));
   const StepRun run = step_run(runs, ri);
   const int rows = a.rep * run.tokens;
   if (piece * kRows >= rows) return;
   const bool own = run.seq >= 0;              // or a shared front: whole pages that every row sees
-  const StepSeq s = step_seq(step, own ? run.seq : 0);
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), col = lane & 15, g = lane >> 4;
-  const int pos0 = own ? s.pos0 : run.u1 * kUnit, len = own ? s.pos0 + s.count : run.u1 * kUnit, full = len / P * P;
+  const int pos0 = own ? run.pos0 : run.u1 * kUnit, len = own ? run.pos0 + run.tokens : run.u1 * kUnit, full = len / P * P;
   const int u_full = (full + kUnit - 1) / kUnit;
   const int u0 = run.u0 + (item - run.split0) * per, u1 = u0 + per < run.u1 ? u0 + per : run.u1;
 
@@ -336,7 +337,7 @@ __global__ __launch_bounds__(kThreads, 3) void paged_split_kernel(DecodeArgs a) 
 
   // Units of the open block.  32-bit offsets from its scalar base and a few loads at a time: their registers must
   // not count for the loop above.
-  const int64_t open = ((static_cast<int64_t>(s.slot) * 2 + (s.bufs >> 1 & 1)) * a.H + h) * P * D;
+  const int64_t open = ((static_cast<int64_t>(run.slot) * 2 + run.open) * a.H + h) * P * D;
   const uint16_t *ko = a.ko + open, *vo = a.vo + open;
   for (; u < u1; u += kWaves) {
     const int off = (u - u_full) * kUnit, t0 = full + off;
@@ -407,8 +408,7 @@ __global__ __launch_bounds__(kThreads, 3) void paged_split_kernel(DecodeArgs a) 
     stat[wave][col][1] = w.l;
   }
   __syncthreads();
-  const int items = runs[kStepRun * (ri + 1) + 5] - run.split0;
-  const bool single = own && items == 1 && s.front == 0;
+  const bool single = own && run.items == 1 && run.front == 0;
   constexpr int kPer = kRows * D / kThreads;                        // channels of a row per thread
   const int r = threadIdx.x / (D / kPer), c0 = threadIdx.x % (D / kPer) * kPer;
   float top = stat[0][r][0];
@@ -462,8 +462,8 @@ __global__ __launch_bounds__(kThreads, 3) void paged_split_kernel(DecodeArgs a) 
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
   __syncthreads();
   if (threadIdx.x == 0) {
-    int* ticket = a.tickets + (static_cast<int64_t>(s.slot) * a.H + h) * kTickets + piece;
-    last_one = __hip_atomic_fetch_add(ticket, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == items - 1;
+    int* ticket = a.tickets + (static_cast<int64_t>(run.slot) * a.H + h) * kTickets + piece;
+    last_one = __hip_atomic_fetch_add(ticket, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == run.items - 1;
     if (last_one) __hip_atomic_store(ticket, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
   }
   __syncthreads();
@@ -471,7 +471,7 @@ __global__ __launch_bounds__(kThreads, 3) void paged_split_kernel(DecodeArgs a) 
   for (int i = wave; i < kRows && piece * kRows + i < rows; i += kWaves) {
     const int Ri = piece * kRows + i;
     Join<D, true> j;
-    j.add(a, run, items, Ri, h);
+    j.add(a, run, Ri, h);
     j.template put<BF16>(a.out + ((static_cast<int64_t>(run.row0) + Ri / a.rep) * Hq + h * a.rep + Ri % a.rep) * D);
   }
 }
@@ -483,18 +483,17 @@ __global__ __launch_bounds__(kThreads) void paged_merge_kernel(DecodeArgs a, int
   if (at >= total) return;
   const int Hq = a.H * a.rep;
   const int n = static_cast<int>(at / Hq), head = static_cast<int>(at % Hq), h = head / a.rep;
-  const StepSeq s = step_seq(a.step, step_find(a.step, a.step[0], 3, n));
+  const StepSeq s = step_seq(a.step, a.n == 1 ? 0 : step_find(a.step, a.n, 3, n));
   if (n >= s.row0 + s.count) return;
-  const int* runs = step_runs(a.step, a.step[0]);
+  const int* runs = step_runs(a.step, a.n);
   const StepRun own = step_run(runs, s.run);
-  const int items = runs[kStepRun * (s.run + 1) + 5] - own.split0;
-  if (items < 2 && !s.front) return;          // its workgroup has written the result
+  if (own.items < 2 && !s.front) return;      // its workgroup has written the result
   Join<D, false> j;
   if (s.front) {
     const StepRun front = step_run(runs, s.front - 1);
-    j.add(a, front, runs[kStepRun * s.front + 5] - front.split0, (n - front.row0) * a.rep + head % a.rep, h);
+    j.add(a, front, (n - front.row0) * a.rep + head % a.rep, h);
   }
-  j.add(a, own, items, (n - s.row0) * a.rep + head % a.rep, h);
+  j.add(a, own, (n - s.row0) * a.rep + head % a.rep, h);
   j.template put<BF16>(a.out + at * D);
 }
 
@@ -511,7 +510,7 @@ extern "C" int64_t kvq_paged_decode_workspace(int64_t split_tokens, int64_t H, i
 }
 
 extern "C" int kvq_paged_decode(const void* q, int64_t q_st, int64_t q_sh, int dtype, int64_t rows, int64_t Hq, int64_t H, int64_t D,
-                                float scaling, const int32_t* step, int64_t split_items, int64_t run_tokens, int64_t split_tokens, const int32_t* table,
+                                float scaling, const int32_t* step, int64_t sequences, int64_t split_items, int64_t run_tokens, int64_t split_tokens, const int32_t* table,
                                 int64_t max_blocks, int64_t P, int code, const uint8_t* kc, const uint8_t* vc, const float* sc,
                                 const void* ko, const void* vo, void* out, float* workspace, int64_t workspace_floats, int32_t* tickets,
                                 void* stream) {
@@ -519,7 +518,7 @@ extern "C" int kvq_paged_decode(const void* q, int64_t q_st, int64_t q_sh, int d
   KVQ_REQUIRE(P == 32 || P == 64 || P == 128, "kvq_paged_decode: pages hold 32, 64 or 128 tokens");
   KVQ_REQUIRE(dtype == KVQ_F16 || dtype == KVQ_BF16, "kvq_paged_decode: queries must be fp16 or bf16");
   KVQ_REQUIRE(code == kCodeInt8 || code == kCodeE4M3, "kvq_paged_decode: unknown code %d", code);
-  KVQ_REQUIRE(H > 0 && Hq > 0 && Hq % H == 0 && rows > 0 && run_tokens > 0 && split_items > 0, "kvq_paged_decode: bad sizes");
+  KVQ_REQUIRE(H > 0 && Hq > 0 && Hq % H == 0 && rows > 0 && run_tokens > 0 && split_items > 0 && sequences > 0, "kvq_paged_decode: bad sizes");
   KVQ_REQUIRE(q && step && table && kc && vc && sc && ko && vo && out && workspace, "kvq_paged_decode: null pointer");
   KVQ_REQUIRE(reinterpret_cast<uintptr_t>(q) % 16 == 0 && (q_st | q_sh) % 8 == 0 && reinterpret_cast<uintptr_t>(out) % 16 == 0 &&
                   reinterpret_cast<uintptr_t>(workspace) % 16 == 0,
@@ -528,7 +527,7 @@ extern "C" int kvq_paged_decode(const void* q, int64_t q_st, int64_t q_sh, int d
   KVQ_REQUIRE(need >= 0, "kvq_paged_decode: too many split tokens (%lld)", static_cast<long long>(split_tokens));
   KVQ_REQUIRE(workspace_floats >= need, "kvq_paged_decode: workspace of %lld floats, %lld needed", static_cast<long long>(workspace_floats),
               static_cast<long long>(need));
-  DecodeArgs a{static_cast<const uint16_t*>(q), q_st, q_sh, step, table, max_blocks, static_cast<int>(H), static_cast<int>(rep),
+  DecodeArgs a{static_cast<const uint16_t*>(q), q_st, q_sh, step, static_cast<int>(sequences), table, max_blocks, static_cast<int>(H), static_cast<int>(rep),
                static_cast<int>(pieces), scaling * 1.44269504088896341f, kc, vc, sc,
                static_cast<const uint16_t*>(ko), static_cast<const uint16_t*>(vo), static_cast<uint16_t*>(out), workspace,
                split_tokens * rep, pieces <= kTickets && split_items * H * pieces <= 256 ? tickets : nullptr};

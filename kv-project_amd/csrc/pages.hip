@@ -222,7 +222,7 @@ __global__ __launch_bounds__(kThreads) void append_kernel(Rows16 k, Rows16 v, co
     vmax = vmax > top[4 + i] ? vmax : top[4 + i];
   }
   const Scale ks = block_scale<CODE, BF16>(kmax), vs = block_scale<CODE, BF16>(vmax);
-  const int page = step_pages(step, n)[item];
+  const int page = step[step[9] + item];
   const int64_t at = (static_cast<int64_t>(page) * H + h) * P * D;
   if (tid == 0) {
     float2* p = reinterpret_cast<float2*>(sc) + static_cast<int64_t>(page) * H + h;
@@ -448,7 +448,7 @@ void describe(const int64_t* lens, const uint8_t* open, const int32_t* table, in
   memset(last, 0, sizeof(int32_t) * kStepSeq);
   last[3] = static_cast<int32_t>(row);
   last[4] = static_cast<int32_t>(item);
-  int32_t* runs = desc + kStepHead + kStepSeq * (n + 1) + item;
+  int32_t* runs = desc + kStepHead + kStepSeq * (n + 1);
   for (int fronts = 1; fronts >= 0; --fronts) {
     int64_t nr = 0, widest = longest;
     auto add = [&](int64_t slot, int64_t row0, int64_t tokens, int64_t u0, int64_t u1, int64_t b) {
@@ -459,6 +459,10 @@ void describe(const int64_t* lens, const uint8_t* open, const int32_t* table, in
       r[3] = static_cast<int32_t>(u0);
       r[4] = static_cast<int32_t>(tokens ? u1 : u0);
       r[7] = static_cast<int32_t>(b);
+      const int32_t* e = desc + kStepHead + kStepSeq * (b < 0 ? 0 : b);
+      r[8] = b < 0 ? 0 : e[1];
+      r[9] = b < 0 ? 0 : e[6] >> 1;
+      r[10] = b < 0 ? 0 : e[7];
     };
     for (int64_t i = 0; i < n;) {
       int64_t j = i + 1, common = 0, tokens = counts[i];
@@ -509,6 +513,7 @@ void describe(const int64_t* lens, const uint8_t* open, const int32_t* table, in
       int32_t* r = runs + kStepRun * i;
       r[5] = static_cast<int32_t>(split);
       r[6] = static_cast<int32_t>(base);
+      r[11] = static_cast<int32_t>(splits(i, lo));
       split += splits(i, lo);
       base += splits(i, lo) * r[2];
     }
@@ -525,6 +530,9 @@ void describe(const int64_t* lens, const uint8_t* open, const int32_t* table, in
     desc[5] = static_cast<int32_t>(longest);
     desc[6] = static_cast<int32_t>(widest);
     desc[7] = base < INT64_C(1) << 31 ? static_cast<int32_t>(base) : -1;
+    desc[8] = static_cast<int32_t>(nr);
+    desc[9] = static_cast<int32_t>(kStepHead + kStepSeq * (n + 1) + kStepRun * (nr + 1));
+    desc[10] = desc[11] = 0;
     last[5] = static_cast<int32_t>(nr);
     return;
   }
@@ -614,7 +622,7 @@ extern "C" int kvq_pages_extend(int64_t* lens, int32_t* table, int32_t* refs, ui
   KVQ_REQUIRE(need <= account[0], "decode buffer exhausted: %lld pages needed, %lld free", static_cast<long long>(need),
               static_cast<long long>(account[0]));
   describe(lens, open, table, max_blocks, page, seq, counts, n, split_cap, few_cap, few_units, most_run, most_tokens, desc);
-  int32_t* page_of = desc + kStepHead + kStepSeq * (n + 1);
+  int32_t* page_of = desc + desc[9];
   int64_t low = account[1];
   for (int64_t i = 0; i < n; ++i) {
     const int32_t* e = desc + kStepHead + kStepSeq * i;
@@ -635,7 +643,7 @@ extern "C" int kvq_pages_extend(int64_t* lens, int32_t* table, int32_t* refs, ui
   }
   account[0] -= need;
   account[1] = low;
-  const int64_t words = kStepHead + kStepSeq * (n + 1) + desc[1] + kStepRun * (desc[kStepHead + kStepSeq * n + 5] + 1);
+  const int64_t words = desc[9] + desc[1];
   return desc_device ? write_words(desc, words, desc_device, static_cast<hipStream_t>(stream)) : KVQ_OK;
 }
 

@@ -11,23 +11,24 @@
 //   ko (slots, 2, H, P, D)      vo (slots, 2, H, D, P)      16-bit elements of the model's type
 //   table (slots, max_blocks) int32: the page of each full block
 //
-// A step's description (int32 words on the device): a header of 8 words {sequences, items, split items,
+// A step's description (int32 words on the device): a header of 12 words {sequences, items, split items,
 // units per split, whether every sequence has one item, the most new tokens of one, the most of a run, the
-// tokens of all split items}, then 8 words per sequence {slot, tokens before, new tokens, first packed row,
-// first item, its run, open buffer before | after << 1, 1 + the run of its shared front or 0} and one entry
-// behind the last with the totals, then the page of every item, then the runs.  An item is a block that the
-// step's tokens touch.
+// tokens of all split items, runs, first word of the items' pages}, then 8 words per sequence {slot, tokens
+// before, new tokens, first packed row, first item, its run, open buffer before | after << 1, 1 + the run of its
+// shared front or 0} and one entry behind the last with the totals, then the runs, then the page of every item.
+// An item is a block that the step's tokens touch.
 //
 // A run is what a decode reads once for a range of packed rows, in split items of so many units: a sequence
 // (or what is its own of it), or the pages that neighbouring sequences of the step share in front, for the rows of
-// all of them.  8 words: {slot whose table row names the pages, first packed row, tokens, first unit, end,
-// first split item, tokens of the split items before, sequence or -1}, and an entry behind the last.
+// all of them.  12 words: {slot whose table row names the pages, first packed row, tokens, first unit, end,
+// first split item, tokens of the split items before, sequence or -1, and of a sequence its tokens before, its
+// open buffer, 1 + the run of its shared front or 0; split items}, and an entry behind the last.
 #pragma once
 #include "common.hpp"
 
 namespace kvq {
 
-constexpr int kStepHead = 8, kStepSeq = 8, kStepRun = 8;
+constexpr int kStepHead = 12, kStepSeq = 8, kStepRun = 12;
 constexpr int kUnit = 64;                     // tokens of one decode unit
 
 enum { kCodeInt8 = 0, kCodeE4M3 = 1 };
@@ -36,18 +37,17 @@ struct StepSeq {
   int slot, pos0, count, row0, item0, run, bufs, front;
 };
 struct StepRun {
-  int slot, row0, tokens, u0, u1, split0, base, seq;
+  int slot, row0, tokens, u0, u1, split0, base, seq, pos0, open, front, items;
 };
 
 __device__ __forceinline__ StepSeq step_seq(const int* step, int b) {
   const int* e = step + kStepHead + kStepSeq * b;
   return {e[0], e[1], e[2], e[3], e[4], e[5], e[6], e[7]};
 }
-__device__ __forceinline__ const int* step_pages(const int* step, int n) { return step + kStepHead + kStepSeq * (n + 1); }
-__device__ __forceinline__ const int* step_runs(const int* step, int n) { return step_pages(step, n) + step[1]; }
+__device__ __forceinline__ const int* step_runs(const int* step, int n) { return step + kStepHead + kStepSeq * (n + 1); }
 __device__ __forceinline__ StepRun step_run(const int* runs, int i) {
   const int* e = runs + kStepRun * i;
-  return {e[0], e[1], e[2], e[3], e[4], e[5], e[6], e[7]};
+  return {e[0], e[1], e[2], e[3], e[4], e[5], e[6], e[7], e[8], e[9], e[10], e[11]};
 }
 
 // The last of n sequences whose word (at first[i * stride]) is not above `value`: 64 at a time, one memory round trip

@@ -159,13 +159,13 @@ class PagedCache:
         _lib.call_on(self.device, "kvq_pages_extend", *self._host, self.slots, self.pages, self.max_blocks, self.page,
                      self.max_tokens, s.ctypes.data, c.ctypes.data, n, st.splits, *few, st.run_tokens, st.split_tokens, st.host.ctypes.data, st.host.size,
                      st.ptr, _lib.stream_of(st.desc))
-        head = st.host[:8].tolist()
+        head = st.host[:9].tolist()
         if into is None:
             # what later steps written into this one keep to: without shared fronts any of them does
             st.splits, st.run_tokens = max(1, head[2]), head[6]
             st.split_tokens = max(head[7], st.splits * head[5])
-            st.items, st.rows = st.host.size - 24 * n - 24, int(st.host[8 * n + 11])
-        st.fronts = int(st.host[8 * n + 13]) > n
+            st.items, st.rows = st.host.size - 32 * n - 32, int(st.host[8 * n + 15])
+        st.fronts = head[8] > n
         self._stamp += 1
         st.slots, st.counts, st.ends, st.generation, st.stamp = s, c, self._lens[s], self._generation, self._stamp
         return st
@@ -303,6 +303,6 @@ def paged_decode(q: torch.Tensor, scaling: float, cache: PagedCache, layer: int,
         raise ValueError("workspace must be contiguous float32 on the cache's device")
     table, max_blocks, _, _, page, code = cache._fixed
     _lib.call_on(device, "kvq_paged_decode", q.data_ptr(), qt, qh, cache._type, step.rows, Hq, Hkv, d, float(scaling), step.ptr,
-                 step.splits, step.run_tokens, step.split_tokens, table, max_blocks, page, code, *cache._at[layer], out.data_ptr(), workspace.data_ptr(),
+                 step.slots.size, step.splits, step.run_tokens, step.split_tokens, table, max_blocks, page, code, *cache._at[layer], out.data_ptr(), workspace.data_ptr(),
                  workspace.numel(), None if step.fronts else cache._tickets[layer], _lib.stream_of(q))
     return out

@@ -102,9 +102,10 @@ def test_accounts_follow_the_model(page):
 def _description(host, slots, counts):
     """Rows, items, the pages of what gets full; runs: every unit of every sequence in one, shared ones only in front."""
     n, d, page = len(slots), host.desc, host.page
-    seq = d[8:8 + 8 * (n + 1)].reshape(n + 1, 8)
-    pages, items, nr = d[8 + 8 * (n + 1):], int(d[1]), int(seq[n, 5])
-    runs = pages[items:items + 8 * (nr + 1)].reshape(nr + 1, 8)
+    seq, nr = d[12:12 + 8 * (n + 1)].reshape(n + 1, 8), int(d[8])
+    runs = d[12 + 8 * (n + 1):][:12 * (nr + 1)].reshape(nr + 1, 12)
+    pages = d[int(d[9]):]
+    assert seq[n, 5] == nr and d[9] == 12 + 8 * (n + 1) + 12 * (nr + 1)
     row = item = 0
     for i, (s, c) in enumerate(zip(slots, counts)):
         end = int(host.lens[s])
@@ -118,7 +119,7 @@ def _description(host, slots, counts):
         units = -(-full // 64) + -(-(end - full) // 64)
         own, front = runs[seq[i, 5]], seq[i, 7]
         assert own[[0, 1, 2, 7]].tolist() == [s, row, c, i] and own[4] == (units if c else own[3])
-        assert own[3] == (runs[front - 1, 4] if front else 0)
+        assert own[3] == (runs[front - 1, 4] if front else 0) and own[8:11].tolist() == [pos0, seq[i, 6] >> 1, front]
         if front:
             f = runs[front - 1]
             assert c and f[3] == 0 and f[4] >= 4 and f[7] == -1 and f[1] <= row and row + c <= f[1] + f[2]
@@ -130,6 +131,7 @@ def _description(host, slots, counts):
     for r in runs[:nr]:
         assert r[5] == split and r[6] == base
         k = -(-(r[4] - r[3]) // int(d[3]))
+        assert r[11] == k
         split, base = split + k, base + k * r[2]
     assert runs[nr, 5:7].tolist() == [split, base]
     assert d[4] == all(b - a == 1 for a, b in zip(seq[:, 4], seq[1:, 4]))
@@ -154,16 +156,16 @@ def test_fronts_of_forks():
     slots, counts = [2, 3, 0, 4, 1, 5, 6], [1, 2, 1, 64, 1, 1, 3]
     assert host.extend(slots, counts) == 0
     _description(host, slots, counts)
-    seq = host.desc[8:8 + 8 * 8].reshape(8, 8)
+    seq = host.desc[12:12 + 8 * 8].reshape(8, 8)
     assert seq[:7, 7].tolist() == [1, 1, 1, 1, 6, 6, 0] and seq[7, 5] == 9
     host.free(range(8))
     assert host.extend([0], [64 * 9]) == 0 and host.fork([0], [1]) == 0
     for limit in (dict(run=1), dict(tokens=2), dict(cap=2)):
         assert host.extend([0, 1], [1, 1], **limit) == 0
-        assert int(host.desc[8 + 16 + 5]) == 2
+        assert int(host.desc[8]) == 2
     assert host.extend([0, 1], [1, 1], run=2, tokens=64, cap=64) == 0
-    assert int(host.desc[8 + 16 + 5]) == 3
-    assert host.extend([0, 1], [1, 0]) == 0 and int(host.desc[8 + 16 + 5]) == 2      # nobody to share with
+    assert int(host.desc[8]) == 3
+    assert host.extend([0, 1], [1, 0]) == 0 and int(host.desc[8]) == 2      # nobody to share with
 
 
 def test_refusals_change_nothing():
@@ -259,6 +261,6 @@ def test_kernel_entries_refuse_before_any_launch():
     assert rc == 1 and b"code" in lib.kvq_last_error()
     need = lib.kvq_paged_decode_workspace(4, 2, 2, 64)
     assert need == 4 * 2 * 2 * 66
-    rc = lib.kvq_paged_decode(one, 256, 64, 2, 1, 4, 2, 64, 0.1, one, 4, 1, 4, one, 4, 64, 0, one, one, one, one, one, one, one, need - 1, None, None)
+    rc = lib.kvq_paged_decode(one, 256, 64, 2, 1, 4, 2, 64, 0.1, one, 1, 4, 1, 4, one, 4, 64, 0, one, one, one, one, one, one, one, need - 1, None, None)
     assert rc == 1 and b"workspace" in lib.kvq_last_error()
     assert lib.kvq_paged_decode_workspace(4, 2, 2, 96) == -1
