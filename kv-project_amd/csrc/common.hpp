@@ -152,6 +152,9 @@ __device__ __forceinline__ void copy_exact_unit(const ExactRows& p, int64_t u) {
   (keys ? p.k.dst : p.v.dst)[u] = w;
 }
 
+// A launch counts its threads in 32 bits: the most workgroups of 256
+constexpr int64_t kMaxGrid = (INT64_C(1) << 24) - 1;
+
 inline bool valid_dtype(int dt) { return dt == KVQ_F32 || dt == KVQ_F16 || dt == KVQ_BF16; }
 
 }  // namespace kvq

@@ -534,7 +534,7 @@ extern "C" int kvq_paged_decode(const void* q, int64_t q_st, int64_t q_sh, int d
   // Joining in the launch: 128 workgroups 14.2 -> 10.3 us, 768 of them 23.9 -> 26.1 (their stores past the caches
   // and the wait for the last one); so only where every workgroup has a CU of its own.
   const int64_t blocks = (split_items * H + 7) / 8 * 8 * a.pieces, merges = (rows * Hq + kWaves - 1) / kWaves;
-  KVQ_REQUIRE(blocks < INT64_C(1) << 31 && merges < INT64_C(1) << 31, "kvq_paged_decode: too many rows");
+  KVQ_REQUIRE(blocks <= kMaxGrid && merges <= kMaxGrid, "kvq_paged_decode: too many rows");
   auto run = [&](auto d, auto p, auto c, auto t) {
     constexpr int D_ = decltype(d)::value, P_ = decltype(p)::value, C_ = decltype(c)::value;
     constexpr bool T_ = decltype(t)::value != 0;

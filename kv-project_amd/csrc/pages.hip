@@ -654,7 +654,7 @@ extern "C" int kvq_pages_append(const void* k, int64_t k_st, int64_t k_sh, const
   KVQ_REQUIRE(k && v && step && table && kc && vc && sc && ko && vo, "kvq_pages_append: null pointer");
   KVQ_REQUIRE(reinterpret_cast<uintptr_t>(k) % 16 == 0 && reinterpret_cast<uintptr_t>(v) % 16 == 0 && (k_st | k_sh | v_st | v_sh) % 8 == 0,
               "kvq_pages_append: rows and strides must be multiples of 16 bytes");
-  KVQ_REQUIRE(items >= 0 && block_grid(items, H) < INT64_C(1) << 31, "kvq_pages_append: too many blocks");
+  KVQ_REQUIRE(items >= 0 && block_grid(items, H) <= kMaxGrid, "kvq_pages_append: too many blocks");
   if (items == 0) return KVQ_OK;
   const Rows16 kr{static_cast<const uint16_t*>(k), k_st, k_sh}, vr{static_cast<const uint16_t*>(v), v_st, v_sh};
   KVQ_PAGES_DISPATCH(hipLaunchKernelGGL((append_kernel<D_, P_, C_, T_>), dim3(static_cast<uint32_t>(block_grid(items, H))), dim3(kThreads), 0,
@@ -678,7 +678,7 @@ extern "C" int kvq_pages_rows(const int64_t* lens, const uint8_t* open, int64_t 
     rows += lens[seq[i]];
     blocks += (lens[seq[i]] + P - 1) / P;
   }
-  KVQ_REQUIRE(rows < INT64_C(1) << 31 && block_grid(blocks, H) < INT64_C(1) << 31, "kvq_pages_rows: too many rows");
+  KVQ_REQUIRE(rows < INT64_C(1) << 31 && block_grid(blocks, H) <= kMaxGrid, "kvq_pages_rows: too many rows");
   KVQ_REQUIRE(out_elements >= rows * H * D && (rows == 0 || (k_out && v_out)), "kvq_pages_rows: outputs of %lld elements, %lld needed",
               static_cast<long long>(out_elements), static_cast<long long>(rows * H * D));
   int64_t row = 0;
@@ -819,7 +819,7 @@ extern "C" int kvq_pages_move(const int64_t* lens, int32_t* table, const int32_t
     flush();
     if (pages_to < pages) {
       const int64_t entries = slots * max_blocks;
-      KVQ_REQUIRE(entries / kThreads < INT64_C(1) << 30, "kvq_pages_move: the table is too large");
+      KVQ_REQUIRE(entries / kThreads < kMaxGrid, "kvq_pages_move: the table is too large");
       hipLaunchKernelGGL(clip_kernel, dim3(static_cast<uint32_t>((entries + kThreads - 1) / kThreads)), dim3(kThreads), 0, st, table_device,
                          entries, static_cast<int>(pages_to));
     }

@@ -440,7 +440,7 @@ extern "C" int kvq_prompt_plan(const int64_t* lens_q, const int64_t* lens_k, int
     if (!words || words_cap < kItemWords * items + 4 * merges) return KVQ_OK;
   }
   // the longest first: the last workgroups to end are short ones
-  std::sort(out, out + items, [](const Item& x, const Item& y) { return x.w[3] != y.w[3] ? x.w[3] > y.w[3] : x.w[2] + x.w[0] < y.w[2] + y.w[0]; });
+  std::sort(out, out + items, [](const Item& x, const Item& y) { return x.w[3] != y.w[3] ? x.w[3] > y.w[3] : x.w[2] != y.w[2] ? x.w[2] < y.w[2] : x.w[0] < y.w[0]; });
   return KVQ_OK;
 }
 
@@ -460,7 +460,7 @@ extern "C" int kvq_prompt_attention(const void* q, int64_t q_st, int64_t q_sh, c
   KVQ_REQUIRE((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v) |
                reinterpret_cast<uintptr_t>(out) | reinterpret_cast<uintptr_t>(workspace)) % 16 == 0 && (q_st | q_sh | k_st | k_sh | v_st | v_sh) % 8 == 0,
               "kvq_prompt_attention: rows and strides must be multiples of 16 bytes");
-  KVQ_REQUIRE(items * H < INT64_C(1) << 31, "kvq_prompt_attention: too many rows");
+  KVQ_REQUIRE(items * H <= kMaxGrid && merges * H <= kMaxGrid, "kvq_prompt_attention: too many rows");
   KVQ_REQUIRE(k_st >= 0 && v_st >= 0 && k_st < (1 << 24) && v_st < (1 << 24), "kvq_prompt_attention: row strides must be below 2^24 elements");
   KVQ_REQUIRE(parts == 0 || (workspace && workspace_floats >= kvq_prompt_workspace(parts, H, D)),
               "kvq_prompt_attention: workspace of %lld floats, %lld needed", static_cast<long long>(workspace_floats),

@@ -120,6 +120,18 @@ def test_values_that_a_row_does_not_see(bad, dtype):
     assert torch.equal(seen[:, :, 4:], clean[at:at + 5, :, 4:].float())
 
 
+def test_expanded_rows_and_a_negative_scaling():
+    import kvq
+    lens, Hq, Hkv, d = [90, 3], 4, 2, 128
+    q, k, v = _inputs(lens, lens, Hq, Hkv, d, torch.float16, 51)
+    plan = kvq.PromptPlan(lens, Hq, Hkv)
+    one = k[:1].cuda().expand(93, -1, -1)
+    assert torch.equal(kvq.prompt_attention(q.cuda(), one, v.cuda(), 0.1, plan),
+                       kvq.prompt_attention(q.cuda(), one.contiguous(), v.cuda(), 0.1, plan))
+    assert torch.equal(kvq.prompt_attention(q.cuda(), k.cuda(), v.cuda(), -0.1, plan),
+                       kvq.prompt_attention(-q.cuda(), k.cuda(), v.cuda(), 0.1, plan))
+
+
 def test_offsets_past_32_bits():
     """Rows whose offsets pass 2^32 bytes and 2^31 elements."""
     import kvq
