@@ -43,7 +43,8 @@ def _ints(x, what: str) -> np.ndarray:
 class Step:
     """New tokens of some slots: ``rows`` packed rows, slot by slot.  Made by ``PagedCache.extend``."""
 
-    __slots__ = ("slots", "counts", "ends", "rows", "items", "splits", "run_tokens", "split_tokens", "fronts", "desc", "ptr", "host", "generation", "stamp")
+    __slots__ = ("slots", "counts", "ends", "rows", "items", "splits", "run_tokens", "split_tokens", "fronts", "shares",
+                 "desc", "ptr", "host", "generation", "stamp")
 
 
 class PagedCache:
@@ -131,8 +132,8 @@ class PagedCache:
     # ---- steps -------------------------------------------------------------------------------
 
     def extend(self, slots: Sequence[int], counts: Sequence[int], *, into: Optional[Step] = None) -> Step:
-        """Claim room for counts[i] more tokens (or none) of slots[i] (each slot once): the lowest free page for each block that
-        gets full.  Raises KVQError ("decode buffer exhausted") and changes nothing when a slot or the pool is
+        """Claim room for counts[i] more tokens (or none) of slots[i] (each slot once): the lowest free page for each
+        block that gets full.  Raises KVQError ("decode buffer exhausted") and changes nothing when a slot or the pool is
         full.  ``into``: a step of the same counts whose description is rewritten in place, so that a
         captured graph of its append and decode runs the new step when it is replayed."""
         s, c = _ints(slots, "slots"), _ints(counts, "counts")
@@ -156,9 +157,11 @@ class PagedCache:
             if not np.array_equal(st.counts, c):
                 raise ValueError("a step is rewritten for the same counts only")
             few = (0, 0)
+        # a captured decode joins shared fronts only if it was captured with some
+        run_tokens = st.run_tokens if into is None or st.shares else 0
         _lib.call_on(self.device, "kvq_pages_extend", *self._host, self.slots, self.pages, self.max_blocks, self.page,
-                     self.max_tokens, s.ctypes.data, c.ctypes.data, n, st.splits, *few, st.run_tokens, st.split_tokens, st.host.ctypes.data, st.host.size,
-                     st.ptr, _lib.stream_of(st.desc))
+                     self.max_tokens, s.ctypes.data, c.ctypes.data, n, st.splits, *few, run_tokens, st.split_tokens,
+                     st.host.ctypes.data, st.host.size, st.ptr, _lib.stream_of(st.desc))
         head = st.host[:9].tolist()
         if into is None:
             # what later steps written into this one keep to: without shared fronts any of them does
@@ -166,6 +169,8 @@ class PagedCache:
             st.split_tokens = max(head[7], st.splits * head[5])
             st.items, st.rows = st.host.size - 32 * n - 32, int(st.host[8 * n + 15])
         st.fronts = head[8] > n
+        if into is None:
+            st.shares = st.fronts
         self._stamp += 1
         st.slots, st.counts, st.ends, st.generation, st.stamp = s, c, self._lens[s], self._generation, self._stamp
         return st
@@ -210,8 +215,8 @@ class PagedCache:
         total = int(np.add.reduce(self._lens.take(s, mode="clip")))
         out = torch.empty((2, total, self.Hkv, self.d), dtype=self.dtype, device=self.device)
         k, v = out.unbind(0)
-        _lib.call_on(self.device, "kvq_pages_rows", self._host[0], self._host[3], self.slots, s.ctypes.data, s.size, *self._fixed, self._type, *self._at[layer],
-                     k.data_ptr(), v.data_ptr(), k.numel(), _lib.stream_of(out))
+        _lib.call_on(self.device, "kvq_pages_rows", self._host[0], self._host[3], self.slots, s.ctypes.data, s.size,
+                     *self._fixed, self._type, *self._at[layer], k.data_ptr(), v.data_ptr(), k.numel(), _lib.stream_of(out))
         return k, v
 
     # ---- sequences and pages -----------------------------------------------------------------
@@ -261,6 +266,9 @@ class PagedCache:
                      *[x.data_ptr() for x in src], *[x.data_ptr() for x in (src if pool is None else pool)], self._fixed[0],
                      _lib.stream_of(self.table))
         if pool is not None:
+            stream = torch.cuda.current_stream(self.device)
+            for x in src:                      # may be another stream than the pools': they are read until it gets there
+                x.record_stream(stream)
             (self.kc, self.vc, self.sc), self.pages, self._refs = pool, pages, refs
             self._set_addresses()
         self._generation += 1
@@ -303,6 +311,7 @@ def paged_decode(q: torch.Tensor, scaling: float, cache: PagedCache, layer: int,
         raise ValueError("workspace must be contiguous float32 on the cache's device")
     table, max_blocks, _, _, page, code = cache._fixed
     _lib.call_on(device, "kvq_paged_decode", q.data_ptr(), qt, qh, cache._type, step.rows, Hq, Hkv, d, float(scaling), step.ptr,
-                 step.slots.size, step.splits, step.run_tokens, step.split_tokens, table, max_blocks, page, code, *cache._at[layer], out.data_ptr(), workspace.data_ptr(),
-                 workspace.numel(), None if step.fronts else cache._tickets[layer], _lib.stream_of(q))
+                 step.slots.size, step.splits, step.run_tokens, step.split_tokens, table, max_blocks, page, code,
+                 *cache._at[layer], out.data_ptr(), workspace.data_ptr(), workspace.numel(),
+                 None if step.shares else cache._tickets[layer], _lib.stream_of(q))
     return out

@@ -214,6 +214,82 @@ def test_a_step_written_over_one_without_forks():
     m.decode(step, 4, what="rewritten")
 
 
+def test_a_captured_step_without_fronts_keeps_to_none():
+    """Three sequences of three, one and one new tokens, captured when nothing was shared: a later step over forks side by
+    side runs in the same graph, which joins no shared fronts."""
+    import kvq
+    m = Mirror(slots=3, pages=90, max_tokens=1300, Hkv=1, d=64, page=32, seed=18)
+    m.push([0, 1, 2], [400, 600, 500])
+    step, [(k, v)] = m.extend([0, 1, 2], [3, 1, 1])
+    kd, vd, q = k.cuda(), v.cuda(), m.rand(5, 4).cuda()
+    out, ws = torch.empty_like(q), torch.empty(kvq.paged_workspace_floats(step, 4, 1, 64), device="cuda")
+    m.cache.append(0, kd, vd, step)
+    torch.cuda.synchronize()
+    gr = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(gr):
+        m.cache.append(0, kd, vd, step)
+        kvq.paged_decode(q, 0.125, m.cache, 0, step, out=out, workspace=ws)
+    m.free([2])
+    m.fork([1], [2])
+    for i in range(3):
+        step, [(k, v)] = m.extend([0, 1, 2], [3, 1, 1], into=step)
+        kd.copy_(k)
+        vd.copy_(v)
+        _ = (q.float() * 2).sum()
+        gr.replay()
+        torch.cuda.synchronize()
+        a = 0
+        for s, n in ((0, 3), (1, 1), (2, 1)):
+            kk, vv = cached(m.k[0][s], 32, "int8"), cached(m.v[0][s], 32, "int8")
+            check(out[a:a + n], attend(q[a:a + n].cpu(), kk, vv, 0.125), float(vv.abs().max()), kk.shape[0], 64, torch.bfloat16, PAIR,
+                  f"replay {i}, slot {s}")
+            a += n
+    # a new step of the same slots shares
+    assert m.push([0, 1, 2], [3, 1, 1]).fronts
+
+
+def test_another_stream_and_expanded_rows():
+    """Steps on a side stream; one token's rows expanded over a step (strides of zero)."""
+    import kvq
+    m = Mirror(slots=2, Hkv=2, d=64, page=32, seed=19)
+    m.push([0], [70])
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step = m.push([0, 1], [3, 40])
+        q = m.rand(1, 4)
+        out = kvq.paged_decode(q.cuda().expand(43, -1, -1), 0.125, m.cache, 0, step)
+    torch.cuda.current_stream().wait_stream(side)
+    assert torch.equal(out, kvq.paged_decode(q.expand(43, -1, -1).contiguous().cuda(), 0.125, m.cache, 0, step))
+    m.check("side stream")
+    step, _ = m.extend([1], [50])
+    k = m.rand(1, 2)
+    m.k[0][1] = torch.cat([m.k[0][1][:-50], k.expand(50, -1, -1)])
+    m.v[0][1] = torch.cat([m.v[0][1][:-50], k.expand(50, -1, -1)])
+    kd = k.cuda().expand(50, -1, -1)
+    m.cache.append(0, kd, kd, step)
+    m.check("expanded")
+
+
+def test_resize_on_another_stream():
+    """The old pools are read by a stream that is busy; what the pools' own stream allocates next is other memory."""
+    m = Mirror(slots=2, pages=40, max_tokens=1000, Hkv=2, d=64, page=32, seed=21)
+    m.push([0, 1], [600, 300])
+    x = torch.ones(4096, 4096, device="cuda")
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        for _ in range(20):
+            x = x @ x * 1e-4
+        m.cache.resize(60)
+    m.model.move(60, 60)
+    size = 40 * 2 * 32 * 64
+    held = [torch.full((size,), 77, dtype=torch.int8, device="cuda") for _ in range(4)]
+    torch.cuda.current_stream().wait_stream(side)
+    m.check("resized")
+    assert all(bool((h == 77).all()) for h in held)
+
+
 def test_random_life():
     """A few hundred random steps, forks, frees and moves."""
     rng = random.Random(11)
@@ -347,7 +423,7 @@ def test_hidden_nan_block():
 
 def test_extreme_magnitudes():
     """Blocks of tiny and of the largest values, and of zeros, beside ordinary ones."""
-    for dtype, big in ((torch.bfloat16, 1e30), (torch.float16, 6e4)):
+    for dtype, big in ((torch.bfloat16, 1e30), (torch.bfloat16, 3.3e38), (torch.float16, 6e4)):
         m = Mirror(slots=1, Hkv=1, d=64, page=32, dtype=dtype, seed=9)
         for scale in (1.0, 1e-30, 0.0, big):
             step, [(k, v)] = m.extend([0], [32])
