@@ -7,7 +7,7 @@ and values are appended to its pages, and its queries attend
 * over the prompt itself (prompt_attention, exact keys and values) where all of the sequences begin,
 * over the cache by ``paged_decode`` in steps of a few tokens,
 * over the cache's rows by ``rows`` and prompt_attention in steps of many tokens (a further question, a chunk of
-  a prompt): the same attention as paged_decode's, with the rows read back once rather than once per 16 query rows.
+  a prompt): the same attention as paged_decode's, with the codes read once rather than once per 16 query rows.
 
 Layer ``module.layer_idx`` of the model is layer ``layer_idx`` of the cache.
 """
@@ -20,8 +20,11 @@ import torch
 from .pages import PagedCache, paged_decode
 from .prompt import PromptPlan, prompt_attention
 
-# query rows per KV head of a sequence (query heads times new tokens) from which on the rows are read back
-MANY_ROWS = 64
+# Query rows per KV head of a sequence (query heads times new tokens) from which on the rows are read back.  Both ways,
+# decode / read back, on an MI355X with 8 KV heads of 128, at 128 and at 256 rows: 16 sequences of 16384 tokens 422 / 525
+# and 781 / 587 us, 8 of 2048 49 / 48 and 80 / 57, one of 8192 33 / 38 and 49 / 41 (head_dim 64: 230 / 281 and 444 / 322,
+# 27 / 32 and 46 / 37, 20 / 30 and 30 / 32).
+MANY_ROWS = 192
 
 
 class PagedCtl:
@@ -38,6 +41,7 @@ class PagedCtl:
         if len(n) != len(self.slots):
             raise ValueError("counts must be one number or one per sequence")
         before = [self.cache.length(s) for s in self.slots]
+        self.step = None                       # none is left if this one does not fit
         self.step = self.cache.extend(self.slots, n)
         self.counts, self.lens, self.fresh = n, [a + b for a, b in zip(before, n)], not any(before)
         self.plan = self.index = None

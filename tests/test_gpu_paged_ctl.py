@@ -24,6 +24,7 @@ class Served:
 
     def step(self, counts, T=None, what=""):
         import kvq
+        from kvq.paged_ctl import MANY_ROWS
         n = self.ctl.slots
         c = [counts] * len(n) if isinstance(counts, int) else counts
         T = max(c) if T is None else T
@@ -45,7 +46,7 @@ class Served:
                     if not fresh:
                         kk, vv = (cached(x, self.cache.page, self.cache.code) for x in (kk, vv))
                     # read back for prompt_attention the cache's rows are rounded once more: u of each key and value
-                    many = not fresh and self.Hq // self.cache.Hkv * max(c) >= 64
+                    many = not fresh and self.Hq // self.cache.Hkv * max(c) >= MANY_ROWS
                     if many:
                         kk, vv = kk.to(self.dtype), vv.to(self.dtype)
                     ref = attend(q[b].transpose(0, 1)[T - m:], kk, vv, self.d ** -0.5)
@@ -61,6 +62,7 @@ def test_a_batch_through_the_router(dtype):
     s.step(3, what="drafts")
     s.step([1, 0, 2], T=4, what="uneven")
     s.step(33, what="question")
+    s.step([60, 49, 1], what="long question")
     s.step(1, what="token")
 
 
@@ -76,6 +78,10 @@ def test_refusals():
         ctl.begin([1])
     ctl.begin(4)
     with pytest.raises(ValueError, match="new tokens"):
+        ctl.attend(m, q, k, k, None, {})
+    with pytest.raises(kvq.KVQError, match="exhausted"):
+        ctl.begin(400)
+    with pytest.raises(RuntimeError, match="begin"):
         ctl.attend(m, q, k, k, None, {})
     with pytest.raises(IndexError):
         kvq.PagedCtl(cache, [5]).begin(1)
