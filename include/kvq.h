@@ -663,8 +663,8 @@ int kvq_selftest_mfma_layout(const uint16_t* a, const uint16_t* b, float* out, v
  * Attention over whole prompts (the reference leaves it to SDPA: STRATA_KV.py:499-504).
  * Packed rows of n sequences: q (sum lens_q, Hq, D), k, v (sum lens_k, Hq / rep, D) of one 16-bit dtype,
  * element strides per row and head, channels contiguous, pointers and strides multiples of 16 bytes; D 64
- * or 128, rep <= 128, row strides below 2^24.  Query t of a sequence sees keys 0 .. t + len_k - len_q (causal), or all of them; one
- * that sees none gets zeros.  out (sum lens_q, Hq, D), contiguous.
+ * or 128, rep <= 128, row strides below 2^24.  Query t of a sequence sees keys 0 .. t + len_k - len_q (causal), or
+ * all of them; one that sees none gets zeros.  out (sum lens_q, Hq, D), contiguous.
  * kvq_prompt_plan (host memory): fills `words` for a call over such sequences and H KV heads; info[3] = {items,
  * merges, parts}.  8 items + 4 merges words are needed: with less room only info is set.  The words go to the
  * device as they are; they bound what kvq_prompt_attention reads.  workspace: kvq_prompt_workspace floats
@@ -688,13 +688,14 @@ int kvq_prompt_attention(const void* q, int64_t q_st, int64_t q_sh, const void* 
  *   lens (slots) int64, table (slots, max_blocks) int32, refs (pages) int32 users of each page,
  *   open (slots) uint8 the current open buffer, account[2] = {free pages, no free page below this one}.
  * code: 0 int8, 1 e4m3.  a = max(|x|, 2^-100) over a block of one head, scale = a * (1 / top),
- * code = rne(x * ((1 / a) * top)), top 127 or 448, each operation in float32; a block with an infinity or a NaN has the scale NaN.
+ * code = rne(x * ((1 / a) * top)), top 127 or 448, each operation in float32; a block with an infinity or a NaN has
+ * the scale NaN.
  *
  * kvq_pages_extend claims counts[i] >= 0 tokens for slot seq[i]: the lowest free page for each block that gets
  * full, in order; refused whole ("decode buffer exhausted") when a slot's max_tokens or the free pages do
  * not suffice.  It writes the step's description to `desc` (host, kvq_pages_step_words words) and, by
- * value with launches on `stream`, to desc_device (NULL: host only).  split_cap >= n bounds the decode's split items; a step
- * of at most few_units units (64 tokens of a sequence) takes about few_cap of them.
+ * value with launches on `stream`, to desc_device (NULL: host only).  split_cap >= n bounds the decode's split
+ * items; a step of at most few_units units (64 tokens of a sequence) takes about few_cap of them.
  * Pages that neighbouring sequences of the step share in front are read once for all of them where the description
  * stays within most_run tokens of a run (its seventh word) and most_tokens of all split items (its eighth).
  * kvq_pages_append writes one layer's rows k, v (rows, H, D) of the step; running it again writes the same.
@@ -731,10 +732,10 @@ int kvq_pages_move(const int64_t* lens, int32_t* table, const int32_t* refs, int
 
 /* ------------------------------------------------------------------------------------------
  * Attention of a step's query rows over the paged cache: q (rows, Hq, D), the step's rows in order; query
- * i of a sequence with `count` new tokens sees all tokens up to its own.  sequences: of the step; split_items, run_tokens and split_tokens: at
- * least the description's third, seventh and eighth word; they give the grid and the workspace.  out (rows, Hq, D)
- * contiguous.  workspace: kvq_paged_decode_workspace floats, no clearing; calls that share one must not
- * overlap in time.
+ * i of a sequence with `count` new tokens sees all tokens up to its own.  sequences: of the step; split_items,
+ * run_tokens and split_tokens: at least the description's third, seventh and eighth word; they give the grid and the
+ * workspace.  out (rows, Hq, D) contiguous.  workspace: kvq_paged_decode_workspace floats, no clearing; calls that
+ * share one must not overlap in time.
  * tickets: NULL, or (slots, H, 4) int32 zeros, which a call leaves as zeros: sequences of several split items are
  * then joined within the one launch, by the workgroup that comes last (in the items' order: the result is the
  * same), where a sequence has at most 64 rows per KV head.  Not for a step with shared fronts.  Calls over one slot of one
@@ -743,10 +744,9 @@ int kvq_pages_move(const int64_t* lens, int32_t* table, const int32_t* refs, int
 int64_t kvq_paged_decode_workspace(int64_t split_tokens, int64_t H, int64_t rep, int64_t D);
 int kvq_paged_decode(const void* q, int64_t q_st, int64_t q_sh, int dtype, int64_t rows, int64_t Hq, int64_t H, int64_t D,
                      float scaling, const int32_t* step, int64_t sequences, int64_t split_items, int64_t run_tokens,
-                     int64_t split_tokens, const int32_t* table,
-                     int64_t max_blocks, int64_t page, int code, const uint8_t* kc, const uint8_t* vc, const float* sc,
-                     const void* ko, const void* vo, void* out, float* workspace, int64_t workspace_floats,
-                     int32_t* tickets, void* stream);
+                     int64_t split_tokens, const int32_t* table, int64_t max_blocks, int64_t page, int code, const uint8_t* kc,
+                     const uint8_t* vc, const float* sc, const void* ko, const void* vo, void* out, float* workspace,
+                     int64_t workspace_floats, int32_t* tickets, void* stream);
 
 #ifdef __cplusplus
 }

@@ -13,6 +13,12 @@
 // Workgroups take the units of one split item, their wavefronts in turn, and join in LDS.  A sequence of
 // several items is joined in the items' order: by the workgroup that comes last, where tickets are given, or
 // by paged_merge_kernel, which spreads long joins over the chip.
+//
+// What bounds it: long caches, the codes' way from memory: 16 sequences of 32768 tokens, 8 KV heads of 128, 186-201 us
+// for 1.07 GB (5.4-5.8 TB/s, 88-94% of the 6.1 TB/s of a read-only stream; the matrix cores are busy 10% of the time, the
+// vector unit, which widens the codes, 33%), and 4.7 us of joins.  One sequence of 4096 tokens, 128 workgroups: 9.2 us,
+// the round trips of one unit: description, page number, codes, join.  Registers for two workgroups a CU instead
+// of three were no faster.
 #include <type_traits>
 
 #include "mfma_common.hpp"
@@ -476,7 +482,8 @@ __global__ __launch_bounds__(kThreads, 3) void paged_split_kernel(DecodeArgs a) 
   }
 }
 
-// One wavefront per (packed row, query head): the items of its sequence's shared front, then its own.
+// One wavefront per (packed row, query head): the items of its sequence's shared front, then its own.  4-5 us: a launch
+// and two round trips.
 template <int D, bool BF16>
 __global__ __launch_bounds__(kThreads) void paged_merge_kernel(DecodeArgs a, int64_t total) {
   const int64_t at = static_cast<int64_t>(blockIdx.x) * kWaves + (threadIdx.x >> 6);
@@ -510,8 +517,8 @@ extern "C" int64_t kvq_paged_decode_workspace(int64_t split_tokens, int64_t H, i
 }
 
 extern "C" int kvq_paged_decode(const void* q, int64_t q_st, int64_t q_sh, int dtype, int64_t rows, int64_t Hq, int64_t H, int64_t D,
-                                float scaling, const int32_t* step, int64_t sequences, int64_t split_items, int64_t run_tokens, int64_t split_tokens, const int32_t* table,
-                                int64_t max_blocks, int64_t P, int code, const uint8_t* kc, const uint8_t* vc, const float* sc,
+                                float scaling, const int32_t* step, int64_t sequences, int64_t split_items, int64_t run_tokens,
+                                int64_t split_tokens, const int32_t* table, int64_t max_blocks, int64_t P, int code, const uint8_t* kc, const uint8_t* vc, const float* sc,
                                 const void* ko, const void* vo, void* out, float* workspace, int64_t workspace_floats, int32_t* tickets,
                                 void* stream) {
   KVQ_REQUIRE(D == 64 || D == 128, "kvq_paged_decode: head_dim must be 64 or 128 (got %lld)", static_cast<long long>(D));
@@ -527,8 +534,8 @@ extern "C" int kvq_paged_decode(const void* q, int64_t q_st, int64_t q_sh, int d
   KVQ_REQUIRE(need >= 0, "kvq_paged_decode: too many split tokens (%lld)", static_cast<long long>(split_tokens));
   KVQ_REQUIRE(workspace_floats >= need, "kvq_paged_decode: workspace of %lld floats, %lld needed", static_cast<long long>(workspace_floats),
               static_cast<long long>(need));
-  DecodeArgs a{static_cast<const uint16_t*>(q), q_st, q_sh, step, static_cast<int>(sequences), table, max_blocks, static_cast<int>(H), static_cast<int>(rep),
-               static_cast<int>(pieces), scaling * 1.44269504088896341f, kc, vc, sc,
+  DecodeArgs a{static_cast<const uint16_t*>(q), q_st, q_sh, step, static_cast<int>(sequences), table, max_blocks,
+               static_cast<int>(H), static_cast<int>(rep), static_cast<int>(pieces), scaling * 1.44269504088896341f, kc, vc, sc,
                static_cast<const uint16_t*>(ko), static_cast<const uint16_t*>(vo), static_cast<uint16_t*>(out), workspace,
                split_tokens * rep, pieces <= kTickets && split_items * H * pieces <= 256 ? tickets : nullptr};
   // Joining in the launch: 128 workgroups 14.2 -> 10.3 us, 768 of them 23.9 -> 26.1 (their stores past the caches

@@ -3,10 +3,12 @@
 // A block is coded once, when its last token comes: a = max(|x|, 2^-100) over the P x D values of one KV
 // head, scale = a * (1 / top), code = rne(x * ((1 / a) * top)), top = 127 (int8) or 448 (e4m3), each
 // operation rounded to float32 (as torch divides by a number, and a number by a tensor, on this device;
-// bf16 values meet exact ties often enough for the last bit to count).  The codes of a block therefore do not depend on how its tokens arrived.  A block
-// that holds an infinity or a NaN gets the scale NaN: its tokens read as NaN.
+// bf16 values meet exact ties often enough for the last bit to count).  The codes of a block therefore do not depend
+// on how its tokens arrived.  A block that holds an infinity or a NaN gets the scale NaN: its tokens read as NaN.
 //
-// All of these kernels move bytes: filling reads 4 D and writes 2 D bytes per token and KV head.
+// All of these kernels move bytes: filling reads 4 D and writes 2 D bytes per token and KV head, reading back the
+// reverse.  16 prompts of 6001 to 8200 tokens, 8 KV heads of 128: filling 129-144 us for 694 MB (4.8-5.4 TB/s), reading
+// back 116-123 (5.6-6.0); a large copy reaches 4.9.  A few tokens: 2-5 us each, a launch and its round trips.
 #include <cmath>
 #include <cstring>
 
@@ -373,7 +375,8 @@ struct Moves {
   int w[kWords];
 };
 
-// Workgroup (move, layer): one page with all its heads.
+// Workgroup (move, layer): one page with all its heads, which lie behind one another (keys and values 64 KB each at 8
+// heads of 128 and 64 tokens).  The pages of 12 sequences in 32 layers, 3.8 GB read and written: 727-740 us, 5.2 TB/s.
 __global__ __launch_bounds__(kThreads) void move_kernel(Moves m, Pool s, Pool d, int64_t s_pages, int64_t d_pages, int H, int64_t page_bytes) {
   const int64_t layer = blockIdx.y, from = layer * s_pages + m.w[2 * blockIdx.x], to = layer * d_pages + m.w[2 * blockIdx.x + 1];
   const uint4* a = reinterpret_cast<const uint4*>(s.kc + from * page_bytes);
@@ -403,7 +406,7 @@ __global__ __launch_bounds__(kThreads) void patch_kernel(Patches p, int n, int* 
 
 // ---- the accounts (host) ----------------------------------------------------------------------
 
-// Split items: each sequence's units in runs of `per` units, per as small as `cap` items allow.
+// Units of a sequence: those of its full blocks, and those of its open one
 int64_t units_of(int64_t len, int64_t page) {
   const int64_t full = len / page * page;
   return (full + kUnit - 1) / kUnit + (len - full + kUnit - 1) / kUnit;

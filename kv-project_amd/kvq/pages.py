@@ -50,7 +50,12 @@ class Step:
 class PagedCache:
     """``layers`` layers of ``pages`` pages for ``slots`` sequences of at most ``max_tokens`` tokens: ``Hkv`` KV heads of
     head_dim ``d`` (64 or 128), blocks of ``page`` tokens (32, 64 or 128) held as ``code`` ("int8" or "e4m3"), rows of
-    ``dtype`` (bf16 or fp16)."""
+    ``dtype`` (bf16 or fp16).
+
+    Calls on one cache run in the order in which they are made: on one stream, or on streams that wait for each other
+    (the accounts of slots and pages are on the host and change at once; not thread-safe).  append and paged_decode may be
+    captured in a graph, for steps that ``extend(..., into=step)`` writes in front of each replay; the calls that change
+    slots or pages may not."""
 
     def __init__(self, layers: int, slots: int, pages: int, max_tokens: int, Hkv: int, d: int, *, page: int = 64,
                  code: str = "int8", dtype: torch.dtype = torch.bfloat16, device="cuda"):
@@ -184,7 +189,7 @@ class PagedCache:
 
     def append(self, layer: int, k: torch.Tensor, v: torch.Tensor, step: Step) -> None:
         """The step's new rows k, v (rows, Hkv, d) of one layer, slot by slot: full blocks to codes, the rest to the open
-        blocks.  Running it again writes the same."""
+        blocks.  Every layer appends every step, before the slots take the next one.  Running it again writes the same."""
         if not 0 <= layer < self.layers:
             raise IndexError(f"no layer {layer} (of {self.layers})")
         shape = (step.rows, self.Hkv, self.d)
