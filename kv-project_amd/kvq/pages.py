@@ -14,6 +14,7 @@ this one has no counterpart there.
 """
 from __future__ import annotations
 
+import ctypes as C
 from typing import List, Optional, Sequence, Tuple
 
 import numpy as np
@@ -38,6 +39,14 @@ def _ints(x, what: str) -> np.ndarray:
     if a.size == 0:
         raise ValueError(f"{what} must not be empty")
     return a
+
+
+_Start = C.c_char * 0
+
+
+def _address(a: np.ndarray) -> int:
+    """The address of an array that may be written (a third of the time that ``a.ctypes.data`` takes)."""
+    return C.addressof(_Start.from_buffer(a))
 
 
 class Step:
@@ -144,10 +153,10 @@ class PagedCache:
         s, c = _ints(slots, "slots"), _ints(counts, "counts")
         if s.shape != c.shape:
             raise ValueError("slots and counts must have the same length")
-        n = s.size
+        n, pc = s.size, _address(c)
         lib = _lib.load()
         if into is None:
-            words = lib.kvq_pages_step_words(self.page, c.ctypes.data, n)
+            words = lib.kvq_pages_step_words(self.page, pc, n)
             if words < 0:
                 raise ValueError("counts must not be negative, and below 2^31")
             st = Step()
@@ -165,8 +174,8 @@ class PagedCache:
         # a captured decode joins shared fronts only if it was captured with some
         run_tokens = st.run_tokens if into is None or st.shares else 0
         _lib.call_on(self.device, "kvq_pages_extend", *self._host, self.slots, self.pages, self.max_blocks, self.page,
-                     self.max_tokens, s.ctypes.data, c.ctypes.data, n, st.splits, *few, run_tokens, st.split_tokens,
-                     st.host.ctypes.data, st.host.size, st.ptr, _lib.stream_of(st.desc))
+                     self.max_tokens, _address(s), pc, n, st.splits, *few, run_tokens, st.split_tokens,
+                     _address(st.host), st.host.size, st.ptr, _lib.stream_of(st.desc))
         head = st.host[:9].tolist()
         if into is None:
             # what later steps written into this one keep to: without shared fronts any of them does
@@ -217,10 +226,10 @@ class PagedCache:
         if not 0 <= layer < self.layers:
             raise IndexError(f"no layer {layer} (of {self.layers})")
         s = _ints(slots, "slots")
-        total = int(np.add.reduce(self._lens.take(s, mode="clip")))
+        total = sum(self._lens.take(s, mode="clip").tolist())
         out = torch.empty((2, total, self.Hkv, self.d), dtype=self.dtype, device=self.device)
         k, v = out.unbind(0)
-        _lib.call_on(self.device, "kvq_pages_rows", self._host[0], self._host[3], self.slots, s.ctypes.data, s.size,
+        _lib.call_on(self.device, "kvq_pages_rows", self._host[0], self._host[3], self.slots, _address(s), s.size,
                      *self._fixed, self._type, *self._at[layer], k.data_ptr(), v.data_ptr(), k.numel(), _lib.stream_of(out))
         return k, v
 
@@ -232,15 +241,15 @@ class PagedCache:
         s, t = _ints(src, "src"), _ints(dst, "dst")
         if s.shape != t.shape:
             raise ValueError("src and dst must have the same length")
-        _lib.call_on(self.device, "kvq_pages_fork", *self._host[:4], self.slots, self.max_blocks, self.page, s.ctypes.data, t.ctypes.data,
-                     s.size, self.layers, self.Hkv, self.d, self.table.data_ptr(), self.k_open.data_ptr(), self.v_open.data_ptr(),
+        _lib.call_on(self.device, "kvq_pages_fork", *self._host[:4], self.slots, self.max_blocks, self.page, _address(s),
+                     _address(t), s.size, self.layers, self.Hkv, self.d, self.table.data_ptr(), self.k_open.data_ptr(), self.v_open.data_ptr(),
                      _lib.stream_of(self.table))
         self._stamp += 1
 
     def free(self, slots: Sequence[int]) -> None:
         """Empty the slots; pages that no other sequence shares become free."""
         s = _ints(slots, "slots")
-        _lib.call("kvq_pages_free", *self._host, self.slots, self.max_blocks, self.page, s.ctypes.data, s.size)
+        _lib.call("kvq_pages_free", *self._host, self.slots, self.max_blocks, self.page, _address(s), s.size)
         self._stamp += 1
 
     def compact(self) -> int:
@@ -266,8 +275,8 @@ class PagedCache:
         refs = self._refs if pool is None else np.empty(pages, dtype=np.int32)
         place = np.empty(self.pages, dtype=np.int32)
         src = (self.kc, self.vc, self.sc)
-        _lib.call_on(self.device, "kvq_pages_move", self._host[0], self._host[1], self._host[2], refs.ctypes.data, self._host[4], self.slots,
-                     self.pages, pages, end, self.max_blocks, self.page, place.ctypes.data, self.layers, self.Hkv, self.d,
+        _lib.call_on(self.device, "kvq_pages_move", *self._host[:3], _address(refs), self._host[4], self.slots, self.pages,
+                     pages, end, self.max_blocks, self.page, _address(place), self.layers, self.Hkv, self.d,
                      *[x.data_ptr() for x in src], *[x.data_ptr() for x in (src if pool is None else pool)], self._fixed[0],
                      _lib.stream_of(self.table))
         if pool is not None:

@@ -62,34 +62,39 @@ def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, scaling:
                      out: Optional[torch.Tensor] = None, workspace: Optional[torch.Tensor] = None) -> torch.Tensor:
     """Attention of the packed rows q (rows, Hq, d) over k, v (keys, Hkv, d), bf16 or fp16 of one type, head_dim 64
     or 128, any row and head strides of whole 16 bytes (others are copied); returns (rows, Hq, d)."""
-    if q.dim() != 3 or k.dim() != 3 or v.shape != k.shape:
-        raise ValueError(f"prompt_attention takes q (rows, Hq, d) and k, v (keys, Hkv, d), got {tuple(q.shape)}, "
-                         f"{tuple(k.shape)}, {tuple(v.shape)}")
-    d = q.shape[2]
-    if q.shape[:2] != (plan.rows, plan.Hq) or k.shape != (plan.keys, plan.Hkv, d):
-        raise ValueError(f"prompt_attention: q {tuple(q.shape)} and k {tuple(k.shape)} do not match the plan "
+    qs, ks = q.shape, k.shape
+    if len(qs) != 3 or len(ks) != 3 or v.shape != ks:
+        raise ValueError(f"prompt_attention takes q (rows, Hq, d) and k, v (keys, Hkv, d), got {tuple(qs)}, "
+                         f"{tuple(ks)}, {tuple(v.shape)}")
+    d, dtype = qs[2], q.dtype
+    if qs[0] != plan.rows or qs[1] != plan.Hq or ks != (plan.keys, plan.Hkv, d):
+        raise ValueError(f"prompt_attention: q {tuple(qs)} and k {tuple(ks)} do not match the plan "
                          f"({plan.rows} rows of {plan.Hq} heads, {plan.keys} keys of {plan.Hkv})")
-    if q.dtype not in (torch.bfloat16, torch.float16) or k.dtype != q.dtype or v.dtype != q.dtype:
+    if dtype not in (torch.bfloat16, torch.float16) or k.dtype != dtype or v.dtype != dtype:
         raise TypeError("prompt_attention takes bf16 or fp16 rows of one type")
     if d not in (64, 128):
         raise _lib.KVQError(f"prompt_attention: head_dim must be 64 or 128 (got {d})")
-    if q.device != plan.device or k.device != plan.device or v.device != plan.device:
+    device, index = plan.device, plan.device.index
+    if q.get_device() != index or k.get_device() != index or v.get_device() != index:
         _lib.require_gpu(q, k, v)
-        raise ValueError(f"prompt_attention: the plan is for {plan.device}")
-    out = _lib.out_or_new(out, (plan.rows, plan.Hq, d), q.dtype, q.device, "prompt_attention")
+        raise ValueError(f"prompt_attention: the plan is for {device}")
+    if out is None:
+        out = torch.empty(qs, dtype=dtype, device=device)
+    else:
+        _lib.out_or_new(out, qs, dtype, device, "prompt_attention")
     if plan.keys == 0:
         return out.zero_()
     (q, qt, qh), (k, kt, kh), (v, vt, vh) = rows16(q), rows16(k), rows16(v)
     ws, floats = None, 0
     if workspace is not None:
-        if workspace.dtype != torch.float32 or not workspace.is_contiguous() or workspace.device != q.device:
+        if workspace.dtype != torch.float32 or not workspace.is_contiguous() or workspace.device != device:
             raise ValueError("workspace must be contiguous float32 on the plan's device")
     elif plan.parts:
-        workspace = torch.empty((plan.workspace_floats(d),), dtype=torch.float32, device=q.device)
+        workspace = torch.empty((plan.workspace_floats(d),), dtype=torch.float32, device=device)
     if workspace is not None:
         ws, floats = workspace.data_ptr(), workspace.numel()
-    _lib.call_on(plan.device, "kvq_prompt_attention", q.data_ptr(), qt, qh, k.data_ptr(), kt, kh, v.data_ptr(), vt, vh,
-                 _lib.DTYPE_CODE[q.dtype], plan.Hq, plan.Hkv, d, float(scaling), plan.words.data_ptr(), plan.items, plan.merges, plan.parts,
+    _lib.call_on(device, "kvq_prompt_attention", q.data_ptr(), qt, qh, k.data_ptr(), kt, kh, v.data_ptr(), vt, vh,
+                 _lib.DTYPE_CODE[dtype], plan.Hq, plan.Hkv, d, float(scaling), plan.words.data_ptr(), plan.items, plan.merges, plan.parts,
                  out.data_ptr(), ws, floats, _lib.stream_of(q))
     return out
 
