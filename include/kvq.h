@@ -736,10 +736,10 @@ int kvq_pages_move(const int64_t* lens, int32_t* table, const int32_t* refs, int
  * run_tokens and split_tokens: at least the description's third, seventh and eighth word; they give the grid and the
  * workspace.  out (rows, Hq, D) contiguous.  workspace: kvq_paged_decode_workspace floats, no clearing; calls that
  * share one must not overlap in time.
- * tickets: NULL, or (slots, H, 4) int32 zeros, which a call leaves as zeros: sequences of several split items are
- * then joined within the one launch, by the workgroup that comes last (in the items' order: the result is the
- * same), where a sequence has at most 64 rows per KV head.  Not for a step with shared fronts.  Calls over one slot of one
- * layer must not overlap.
+ * tickets: NULL, or (slots, H, 32) int32 zeros, which a call leaves as zeros: a sequence's split items are then joined
+ * within the one launch, by the workgroup that comes last (in the items' order: the result is the same), where
+ * that is the faster way: at most 4 rows per KV head and 256 workgroups.  Not for a step with shared fronts.  Calls over
+ * one slot of one layer must not overlap.
  * ---------------------------------------------------------------------------------------- */
 int64_t kvq_paged_decode_workspace(int64_t split_tokens, int64_t H, int64_t rep, int64_t D);
 int kvq_paged_decode(const void* q, int64_t q_st, int64_t q_sh, int dtype, int64_t rows, int64_t Hq, int64_t H, int64_t D,

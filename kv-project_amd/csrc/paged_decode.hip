@@ -92,9 +92,9 @@ struct DecodeArgs {
   uint16_t* out;                              // (rows, Hq, D)
   float* part;                                // (part_rows, H): D sums; behind them {max, sum} each
   int64_t part_rows;                          // rows of all split items
-  int* tickets;                               // (slots, H, kTickets) zeros, or none: joins by a launch of its own
+  int* tickets;                               // (slots, H, kApart) zeros, or none: joins by a launch of its own
 };
-constexpr int kTickets = 4;                   // pieces of a sequence that the last workgroup may join
+constexpr int kApart = 32;                    // a cache line for each ticket: 208 workgroups 10.7 us, 12.2 with them side by side
 
 template <int D, bool BF16>
 struct Wave {                                 // one wavefront's running softmax: column lane % 16
@@ -462,24 +462,22 @@ __global__ __launch_bounds__(kThreads, 3) void paged_split_kernel(DecodeArgs a) 
       put_shared(st + 1, l);
     }
   }
-  // The last workgroup of the sequence's items joins them (no tickets where there are shared fronts).  Each one's
+  // The last workgroup of the sequence's items joins them, a row for each wavefront (tickets are given where a sequence
+  // has no more rows, which are one piece, and where there are no shared fronts).  Each one's
   // partial results are visible on every die before its ticket is counted; the ticket is a zero again afterwards.
   __shared__ int last_one;
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
   __syncthreads();
   if (threadIdx.x == 0) {
-    int* ticket = a.tickets + (static_cast<int64_t>(run.slot) * a.H + h) * kTickets + piece;
+    int* ticket = a.tickets + (static_cast<int64_t>(run.slot) * a.H + h) * kApart;
     last_one = __hip_atomic_fetch_add(ticket, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == run.items - 1;
     if (last_one) __hip_atomic_store(ticket, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
   }
   __syncthreads();
-  if (!last_one) return;
-  for (int i = wave; i < kRows && piece * kRows + i < rows; i += kWaves) {
-    const int Ri = piece * kRows + i;
-    Join<D, true> j;
-    j.add(a, run, Ri, h);
-    j.template put<BF16>(a.out + ((static_cast<int64_t>(run.row0) + Ri / a.rep) * Hq + h * a.rep + Ri % a.rep) * D);
-  }
+  if (!last_one || wave >= rows) return;
+  Join<D, true> j;
+  j.add(a, run, wave, h);
+  j.template put<BF16>(a.out + ((static_cast<int64_t>(run.row0) + wave / a.rep) * Hq + h * a.rep + wave % a.rep) * D);
 }
 
 // One wavefront per (packed row, query head): the items of its sequence's shared front, then its own.  4-5 us: a launch
@@ -537,9 +535,11 @@ extern "C" int kvq_paged_decode(const void* q, int64_t q_st, int64_t q_sh, int d
   DecodeArgs a{static_cast<const uint16_t*>(q), q_st, q_sh, step, static_cast<int>(sequences), table, max_blocks,
                static_cast<int>(H), static_cast<int>(rep), static_cast<int>(pieces), scaling * 1.44269504088896341f, kc, vc, sc,
                static_cast<const uint16_t*>(ko), static_cast<const uint16_t*>(vo), static_cast<uint16_t*>(out), workspace,
-               split_tokens * rep, pieces <= kTickets && split_items * H * pieces <= 256 ? tickets : nullptr};
-  // Joining in the launch: 128 workgroups 14.2 -> 10.3 us, 768 of them 23.9 -> 26.1 (their stores past the caches
-  // and the wait for the last one); so only where every workgroup has a CU of its own.
+               split_tokens * rep, rep * run_tokens <= kWaves && split_items * H <= 256 ? tickets : nullptr};
+  // Joining in the launch, against a launch for it.  One sequence of 4096 tokens, 8 KV heads of 128, 136 workgroups: with
+  // one row 9.4 / 11.9 us, four 10.3 / 11.7, eight 13.0 / 11.9, sixteen 18.6 / 12.1 (rows one after the other in a wavefront,
+  // loads past the caches); 768 workgroups with four rows 26.1 / 23.9 (their stores and the wait for the last one).  So
+  // where a wavefront has one row at most and every workgroup a CU of its own.
   const int64_t blocks = (split_items * H + 7) / 8 * 8 * a.pieces, merges = (rows * Hq + kWaves - 1) / kWaves;
   KVQ_REQUIRE(blocks <= kMaxGrid && merges <= kMaxGrid, "kvq_paged_decode: too many rows");
   auto run = [&](auto d, auto p, auto c, auto t) {

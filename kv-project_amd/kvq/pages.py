@@ -97,7 +97,7 @@ class PagedCache:
         self.k_open = torch.zeros(rows, dtype=dtype, device=self.device)     # token major, as a page's keys
         self.v_open = torch.zeros(rows, dtype=dtype, device=self.device)     # channel major, as a page's values
         # counters of the decodes that join their parts in one launch: zeros between calls
-        self._counters = torch.zeros((self.layers, self.slots, self.Hkv, 4), dtype=torch.int32, device=self.device)
+        self._counters = torch.zeros((self.layers, self.slots, self.Hkv, 32), dtype=torch.int32, device=self.device)
         self._tickets = [self._counters[l].data_ptr() for l in range(self.layers)]
         self._set_addresses()
 

@@ -290,6 +290,21 @@ def test_resize_on_another_stream():
     assert all(bool((h == 77).all()) for h in held)
 
 
+@pytest.mark.parametrize("rep,T", [(1, 1), (2, 2), (4, 1), (3, 1), (5, 1), (8, 2)])
+def test_joins_within_the_launch(rep, T):
+    """A step's items joined by the last workgroup, where it has few rows, or by a launch: the same; counters are zeros again."""
+    import kvq
+    m = Mirror(slots=3, pages=200, max_tokens=7000, Hkv=2, d=128, page=64, seed=22)
+    m.push([0, 1, 2], [6000, 900, 1])
+    step = m.push([0, 1, 2], [T] * 3)
+    q, out = m.decode(step, 2 * rep, what="joined")
+    for _ in range(3):
+        assert torch.equal(out, kvq.paged_decode(q.cuda(), 128 ** -0.5, m.cache, 0, step))
+    assert not m.cache._counters.any()
+    m.cache._tickets = [None]
+    assert torch.equal(out, kvq.paged_decode(q.cuda(), 128 ** -0.5, m.cache, 0, step))
+
+
 def test_random_life():
     """A few hundred random steps, forks, frees and moves."""
     rng = random.Random(11)
