@@ -32,7 +32,7 @@
 namespace kvq {
 namespace {
 
-constexpr int kThreads = 256, kTileRows = 128, kTileKeys = 64, kItemWords = 8, kSlots = 512;
+constexpr int kThreads = 256, kTileRows = 128, kTileKeys = 64, kItemWords = 8, kSlots = 512, kMinPart = 8;
 
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
@@ -394,22 +394,34 @@ extern "C" int kvq_prompt_plan(const int64_t* lens_q, const int64_t* lens_k, int
   KVQ_REQUIRE(info && n >= 0 && (n == 0 || (lens_q && lens_k)), "kvq_prompt_plan: null pointer");
   KVQ_REQUIRE(rep >= 1 && rep <= kTileRows && H >= 1, "kvq_prompt_plan: bad head counts");
   const int64_t per_tile = kTileRows / rep;   // tokens of a tile of rows
-  int64_t rows = 0, keys_all = 0, tiles = 0, work = 0;
+  int64_t rows = 0, keys_all = 0, tiles = 0, longest = 0;
   auto keys_of = [&](int64_t i, int64_t t) {  // keys that the tile from token t of sequence i sees
     if (!causal) return lens_k[i];
     const int64_t end = t + per_tile < lens_q[i] ? t + per_tile : lens_q[i], k = lens_k[i] - lens_q[i] + end;
     return k < 0 ? INT64_C(0) : k;
   };
+  auto steps_of = [&](int64_t i, int64_t t) { return (keys_of(i, t) + kTileKeys - 1) / kTileKeys; };
   for (int64_t i = 0; i < n; ++i) {
     KVQ_REQUIRE(lens_q[i] >= 0 && lens_k[i] >= 0, "kvq_prompt_plan: lengths must not be negative");
     rows += lens_q[i];
     keys_all += lens_k[i];
     KVQ_REQUIRE(rows < INT64_C(1) << 31 && keys_all < INT64_C(1) << 31, "kvq_prompt_plan: too many rows");
-    for (int64_t t = 0; t < lens_q[i]; t += per_tile, ++tiles) work += (keys_of(i, t) + kTileKeys - 1) / kTileKeys;
+    for (int64_t t = 0; t < lens_q[i]; t += per_tile, ++tiles) longest = steps_of(i, t) > longest ? steps_of(i, t) : longest;
   }
-  // Parts of a tile: no longer than an even share of the work over kSlots workgroups (two on each of 256 CUs), which
-  // is nothing where the tiles fill the chip; 8 key tiles at least, which pay for the part's sums (64 KB).
-  const int64_t even = (work * H + kSlots - 1) / kSlots, most = even > 8 ? even : 8;
+  // Where the tiles of rows do not fill kSlots places (two on each of 256 CUs), they are cut into the shortest parts that
+  // fit: 8 key tiles at least, which pay for the part's sums (64 KB).  Parts beyond the places start a second round, which
+  // costs more than uneven ones: 8 sequences of 1024 tokens, 8 heads of 128, 512 tiles whole 36 us, 768 parts of an even
+  // share at most 53; 24 of 16 tokens behind 32768, 384 parts 605, 576 of them 723.
+  int64_t most = kMinPart, high = longest > kMinPart ? longest : kMinPart;
+  if (tiles * H > kSlots) most = high;
+  while (most < high) {
+    const int64_t mid = (most + high) / 2;
+    int64_t count = 0;
+    for (int64_t i = 0; i < n; ++i)
+      for (int64_t t = 0; t < lens_q[i]; t += per_tile) count += steps_of(i, t) > mid ? (steps_of(i, t) + mid - 1) / mid : 1;
+    if (count * H <= kSlots) high = mid;
+    else most = mid + 1;
+  }
   int64_t items = 0, merges = 0, parts = 0;
   Item* out = reinterpret_cast<Item*>(words);
   for (int pass = 0; pass < 2; ++pass) {
@@ -417,7 +429,7 @@ extern "C" int kvq_prompt_plan(const int64_t* lens_q, const int64_t* lens_k, int
     for (int64_t i = 0; i < n; ++i) {
       for (int64_t t = 0; t < lens_q[i]; t += per_tile) {
         const int64_t toks = lens_q[i] - t < per_tile ? lens_q[i] - t : per_tile, keys = keys_of(i, t);
-        const int64_t vis0 = causal ? lens_k[i] - lens_q[i] + t + 1 : keys, steps = (keys + kTileKeys - 1) / kTileKeys;
+        const int64_t vis0 = causal ? lens_k[i] - lens_q[i] + t + 1 : keys, steps = steps_of(i, t);
         const int64_t cut = (steps + most - 1) / most, count = cut > 1 ? cut : 1;
         if (pass == 1 && count > 1) {
           int32_t* w = words + kItemWords * items + 4 * merge;
