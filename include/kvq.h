@@ -695,7 +695,8 @@ int kvq_prompt_attention(const void* q, int64_t q_st, int64_t q_sh, const void* 
  * full, in order; refused whole ("decode buffer exhausted") when a slot's max_tokens or the free pages do
  * not suffice.  It writes the step's description to `desc` (host, kvq_pages_step_words words) and, by
  * value with launches on `stream`, to desc_device (NULL: host only).  split_cap >= n bounds the decode's split
- * items; a step of at most few_units units (64 tokens of a sequence) takes about few_cap of them.
+ * items.  With few_cap > 0, a step of at most few_units units (64 tokens of a sequence) takes about few_cap of them,
+ * and one of uneven sequences up to 2 split_cap.
  * Pages that neighbouring sequences of the step share in front are read once for all of them where the description
  * stays within most_run tokens of a run (its seventh word) and most_tokens of all split items (its eighth).
  * kvq_pages_append writes one layer's rows k, v (rows, H, D) of the step; running it again writes the same.
@@ -734,19 +735,20 @@ int kvq_pages_move(const int64_t* lens, int32_t* table, const int32_t* refs, int
  * Attention of a step's query rows over the paged cache: q (rows, Hq, D), the step's rows in order; query
  * i of a sequence with `count` new tokens sees all tokens up to its own.  sequences: of the step; split_items,
  * run_tokens and split_tokens: at least the description's third, seventh and eighth word; they give the grid and the
- * workspace.  out (rows, Hq, D) contiguous.  workspace: kvq_paged_decode_workspace floats, no clearing; calls that
- * share one must not overlap in time.
+ * workspace.  joins: its eleventh word, or 1 (a launch joins the results of several split items).  out (rows, Hq, D)
+ * contiguous.  workspace: kvq_paged_decode_workspace floats, no clearing; calls that share one must not overlap in
+ * time.
  * tickets: NULL, or (slots, H, 32) int32 zeros, which a call leaves as zeros: a sequence's split items are then joined
- * within the one launch, by the workgroup that comes last (in the items' order: the result is the same), where
- * that is the faster way: at most 4 rows per KV head and 256 workgroups.  Not for a step with shared fronts.  Calls over
- * one slot of one layer must not overlap.
+ * within the one launch, by the workgroup that comes last (always in the items' order), where that is the faster way:
+ * few rows, items and workgroups.  Not for a step with shared fronts.  Calls over one slot of one layer must not
+ * overlap.
  * ---------------------------------------------------------------------------------------- */
 int64_t kvq_paged_decode_workspace(int64_t split_tokens, int64_t H, int64_t rep, int64_t D);
 int kvq_paged_decode(const void* q, int64_t q_st, int64_t q_sh, int dtype, int64_t rows, int64_t Hq, int64_t H, int64_t D,
                      float scaling, const int32_t* step, int64_t sequences, int64_t split_items, int64_t run_tokens,
-                     int64_t split_tokens, const int32_t* table, int64_t max_blocks, int64_t page, int code, const uint8_t* kc,
-                     const uint8_t* vc, const float* sc, const void* ko, const void* vo, void* out, float* workspace,
-                     int64_t workspace_floats, int32_t* tickets, void* stream);
+                     int64_t split_tokens, int joins, const int32_t* table, int64_t max_blocks, int64_t page, int code,
+                     const uint8_t* kc, const uint8_t* vc, const float* sc, const void* ko, const void* vo, void* out,
+                     float* workspace, int64_t workspace_floats, int32_t* tickets, void* stream);
 
 #ifdef __cplusplus
 }

@@ -111,49 +111,92 @@ __device__ __forceinline__ float get(const float* p) {
   else return *p;
 }
 
-// A row joined by one wavefront: the maximum, the sum, its channels of the weighted sums
-template <int D, bool SHARED>
+// N rows joined by one wavefront: the maxima, the sums, its channels of the weighted sums
+template <int D, bool SHARED, int N>
 struct Join {
-  float top = -INFINITY, l = 0.0f, o[D / 64] = {};
-  // row R of each of a run's split items, 64 maxima at a time
-  __device__ __forceinline__ void add(const DecodeArgs& a, const StepRun& run, int R, int h) {
-    const int lane = threadIdx.x & 63, items = run.items;
-    const int64_t first = (static_cast<int64_t>(a.rep) * run.base + R) * a.H + h, stride = static_cast<int64_t>(a.rep) * run.tokens * a.H;
-    const float* stat = a.part + a.part_rows * a.H * D;
-    for (int i0 = 0; i0 < items; i0 += 64) {
-      const int i = i0 + lane;
-      float2 st = make_float2(-INFINITY, 0.0f);
-      if (i < items) st = make_float2(get<SHARED>(stat + 2 * (first + i * stride)), get<SHARED>(stat + 2 * (first + i * stride) + 1));
-      const float m = fmaxf(top, wave_max(st.x)), safe = m == -INFINITY ? 0.0f : m;
-      const float old = __builtin_amdgcn_exp2f(top - safe), f = __builtin_amdgcn_exp2f(st.x - safe);
-      l = l * old + wave_sum(f * st.y);
+  float top[N], l[N], o[N][D / 64];
+  __device__ __forceinline__ Join() {
 #pragma unroll
-      for (int e = 0; e < D / 64; ++e) o[e] *= old;
-      const int most = items - i0 < 64 ? items - i0 : 64;
-      const float* p = a.part + (first + i0 * stride) * D + lane * (D / 64);
-      for (int k0 = 0; k0 < most; k0 += 8) {                        // eight loads on their way; behind the last: it again, unused
-        float x[8][D / 64];
+    for (int n = 0; n < N; ++n) {
+      top[n] = -INFINITY;
+      l[n] = 0.0f;
 #pragma unroll
-        for (int k = 0; k < 8; ++k)
+      for (int e = 0; e < D / 64; ++e) o[n][e] = 0.0f;
+    }
+  }
+  // DEEP items of every row on their way at once; behind the last: it again, unused
+  template <int DEEP>
+  __device__ __forceinline__ void some(const float* const (&p)[N], int64_t stride, int k0, int most, const float (&f)[N]) {
+    float x[N][DEEP][D / 64];
 #pragma unroll
-          for (int e = 0; e < D / 64; ++e) x[k][e] = get<SHARED>(p + (k0 + k < most ? k0 + k : most - 1) * stride * D + e);
+    for (int n = 0; n < N; ++n)
 #pragma unroll
-        for (int k = 0; k < 8; ++k) {
-          const float fk = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(f), k0 + k < most ? k0 + k : 0));
+      for (int k = 0; k < DEEP; ++k)
 #pragma unroll
-          for (int e = 0; e < D / 64; ++e) o[e] += k0 + k < most ? fk * x[k][e] : 0.0f;
-        }
+        for (int e = 0; e < D / 64; ++e) x[n][k][e] = get<SHARED>(p[n] + (k0 + k < most ? k0 + k : most - 1) * stride * D + e);
+#pragma unroll
+    for (int n = 0; n < N; ++n)
+#pragma unroll
+      for (int k = 0; k < DEEP; ++k) {
+        const float fk = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(f[n]), k0 + k < most ? k0 + k : 0));
+#pragma unroll
+        for (int e = 0; e < D / 64; ++e) o[n][e] += k0 + k < most ? fk * x[n][k][e] : 0.0f;
       }
-      top = m;
+  }
+  // rows R of a run's split items from .. to - 1, 64 maxima at a time
+  __device__ __forceinline__ void add(const DecodeArgs& a, const StepRun& run, const int (&R)[N], int h, int from, int to) {
+    const int lane = threadIdx.x & 63;
+    const int64_t stride = static_cast<int64_t>(a.rep) * run.tokens * a.H;
+    const float* stat = a.part + a.part_rows * a.H * D;
+    for (int i0 = from; i0 < to; i0 += 64) {
+      const int i = i0 + lane, most = to - i0 < 64 ? to - i0 : 64;
+      float2 st[N];
+      const float* p[N];
+#pragma unroll
+      for (int n = 0; n < N; ++n) {
+        const int64_t first = (static_cast<int64_t>(a.rep) * run.base + R[n]) * a.H + h;
+        p[n] = a.part + (first + i0 * stride) * D + lane * (D / 64);
+        st[n] = make_float2(-INFINITY, 0.0f);
+        if (i < to) st[n] = make_float2(get<SHARED>(stat + 2 * (first + i * stride)), get<SHARED>(stat + 2 * (first + i * stride) + 1));
+      }
+      float f[N];
+#pragma unroll
+      for (int n = 0; n < N; ++n) {
+        const float m = fmaxf(top[n], wave_max(st[n].x)), safe = m == -INFINITY ? 0.0f : m;
+        const float old = __builtin_amdgcn_exp2f(top[n] - safe);
+        f[n] = __builtin_amdgcn_exp2f(st[n].x - safe);
+        l[n] = l[n] * old + wave_sum(f[n] * st[n].y);
+#pragma unroll
+        for (int e = 0; e < D / 64; ++e) o[n][e] *= old;
+        top[n] = m;
+      }
+      int k0 = 0;
+      if constexpr (!SHARED)
+        for (; k0 + 32 <= most; k0 += 32) some<32>(p, stride, k0, most, f);
+      for (; k0 < most; k0 += 8) some<8>(p, stride, k0, most, f);
     }
   }
   template <bool BF16>
-  __device__ __forceinline__ void put(uint16_t* out) const {
-    const float inv = 1.0f / l;
+  __device__ __forceinline__ void put(int n, uint16_t* out) const {
+    const float inv = 1.0f / l[n];
 #pragma unroll
-    for (int e = 0; e < D / 64; ++e) out[(threadIdx.x & 63) * (D / 64) + e] = BF16 ? f32_to_bf16(o[e] * inv) : f32_to_f16(o[e] * inv);
+    for (int e = 0; e < D / 64; ++e) out[(threadIdx.x & 63) * (D / 64) + e] = BF16 ? f32_to_bf16(o[n][e] * inv) : f32_to_f16(o[n][e] * inv);
   }
 };
+
+// Rows wave, wave + kWaves, .. of a sequence (N of them at most) out of its split items, within the launch that made them
+template <int D, bool BF16, int N>
+__device__ __forceinline__ void join_rows(const DecodeArgs& a, const StepRun& run, int wave, int rows, int h) {
+  int R[N];
+#pragma unroll
+  for (int n = 0; n < N; ++n) R[n] = wave + n * kWaves < rows ? wave + n * kWaves : rows - 1;
+  Join<D, true, N> j;
+  j.add(a, run, R, h, 0, run.items);
+#pragma unroll
+  for (int n = 0; n < N; ++n)
+    if (wave + n * kWaves < rows)
+      j.template put<BF16>(n, a.out + ((static_cast<int64_t>(run.row0) + R[n] / a.rep) * a.H * a.rep + h * a.rep + R[n] % a.rep) * D);
+}
 
 // Scores t (16 tokens of this lane, masked ones -inf) -> probabilities in t, o and l brought to the new maximum
 template <int D, bool BF16>
@@ -209,8 +252,8 @@ __global__ __launch_bounds__(kThreads, 3) void paged_split_kernel(DecodeArgs a) 
   const int piece = within / 8, item = static_cast<int>(ih / a.H), h = static_cast<int>(ih % a.H);
   if (item >= step[2]) return;
   const int* runs = step_runs(step, a.n);
-  // one sequence is one run: no look before it
-  const int ri = a.n == 1 ? 0 : __builtin_amdgcn_readfirstlane(last_not_above(runs + 5, kStepRun, step[8], item));
+  // no look where a run is one item, or one sequence the only run
+  const int ri = step[11] ? item : a.n == 1 ? 0 : __builtin_amdgcn_readfirstlane(last_not_above(runs + 5, kStepRun, step[8], item));
   const StepRun run = step_run(runs, ri);
   const int rows = a.rep * run.tokens;
   if (piece * kRows >= rows) return;
@@ -462,8 +505,8 @@ __global__ __launch_bounds__(kThreads, 3) void paged_split_kernel(DecodeArgs a) 
       put_shared(st + 1, l);
     }
   }
-  // The last workgroup of the sequence's items joins them, a row for each wavefront (tickets are given where a sequence
-  // has no more rows, which are one piece, and where there are no shared fronts).  Each one's
+  // The last workgroup of the sequence's items joins them, a row or two for each wavefront (tickets are given where a
+  // sequence has no more rows, which are one piece, and where there are no shared fronts).  Each one's
   // partial results are visible on every die before its ticket is counted; the ticket is a zero again afterwards.
   __shared__ int last_one;
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
@@ -475,16 +518,19 @@ __global__ __launch_bounds__(kThreads, 3) void paged_split_kernel(DecodeArgs a) 
   }
   __syncthreads();
   if (!last_one || wave >= rows) return;
-  Join<D, true> j;
-  j.add(a, run, wave, h);
-  j.template put<BF16>(a.out + ((static_cast<int64_t>(run.row0) + wave / a.rep) * Hq + h * a.rep + wave % a.rep) * D);
+  if (D > 64 || rows <= kWaves) {
+    join_rows<D, BF16, 1>(a, run, wave, rows, h);
+  } else if constexpr (D == 64) {
+    join_rows<D, BF16, 2>(a, run, wave, rows, h);
+  }
 }
 
-// One wavefront per (packed row, query head): the items of its sequence's shared front, then its own.  4-5 us: a launch
+// WAVES wavefronts per (packed row, query head): the items of its sequence's shared front, then its own.  4-5 us: a launch
 // and two round trips.
-template <int D, bool BF16>
+template <int D, bool BF16, int WAVES>
 __global__ __launch_bounds__(kThreads) void paged_merge_kernel(DecodeArgs a, int64_t total) {
-  const int64_t at = static_cast<int64_t>(blockIdx.x) * kWaves + (threadIdx.x >> 6);
+  const int wave = threadIdx.x >> 6, part = wave % WAVES, lane = threadIdx.x & 63;
+  const int64_t at = static_cast<int64_t>(blockIdx.x) * (kWaves / WAVES) + wave / WAVES;
   if (at >= total) return;
   const int Hq = a.H * a.rep;
   const int n = static_cast<int>(at / Hq), head = static_cast<int>(at % Hq), h = head / a.rep;
@@ -493,13 +539,38 @@ __global__ __launch_bounds__(kThreads) void paged_merge_kernel(DecodeArgs a, int
   const int* runs = step_runs(a.step, a.n);
   const StepRun own = step_run(runs, s.run);
   if (own.items < 2 && !s.front) return;      // its workgroup has written the result
-  Join<D, false> j;
+  Join<D, false, 1> j;
   if (s.front) {
     const StepRun front = step_run(runs, s.front - 1);
-    j.add(a, front, (n - front.row0) * a.rep + head % a.rep, h);
+    const int R[1] = {(n - front.row0) * a.rep + head % a.rep};
+    j.add(a, front, R, h, front.items * part / WAVES, front.items * (part + 1) / WAVES);
   }
-  j.add(a, own, (n - s.row0) * a.rep + head % a.rep, h);
-  j.template put<BF16>(a.out + at * D);
+  const int R[1] = {(n - s.row0) * a.rep + head % a.rep};
+  j.add(a, own, R, h, own.items * part / WAVES, own.items * (part + 1) / WAVES);
+  if constexpr (WAVES > 1) {
+    __shared__ float sums[kWaves][D], stats[kWaves][2];
+#pragma unroll
+    for (int e = 0; e < D / 64; ++e) sums[wave][lane * (D / 64) + e] = j.o[0][e];
+    if (lane == 0) {
+      stats[wave][0] = j.top[0];
+      stats[wave][1] = j.l[0];
+    }
+    __syncthreads();                          // a workgroup is one row: all or none get here
+    if (part) return;
+    float top = stats[0][0];
+#pragma unroll
+    for (int i = 1; i < WAVES; ++i) top = fmaxf(top, stats[i][0]);
+    const float safe = top == -INFINITY ? 0.0f : top;
+    j = Join<D, false, 1>();
+#pragma unroll
+    for (int i = 0; i < WAVES; ++i) {
+      const float f = __builtin_amdgcn_exp2f(stats[i][0] - safe);
+      j.l[0] += f * stats[i][1];
+#pragma unroll
+      for (int e = 0; e < D / 64; ++e) j.o[0][e] += f * sums[i][lane * (D / 64) + e];
+    }
+  }
+  j.template put<BF16>(0, a.out + at * D);
 }
 
 int64_t pieces_of(int64_t rep, int64_t tokens) { return (rep * tokens + kRows - 1) / kRows; }
@@ -516,7 +587,7 @@ extern "C" int64_t kvq_paged_decode_workspace(int64_t split_tokens, int64_t H, i
 
 extern "C" int kvq_paged_decode(const void* q, int64_t q_st, int64_t q_sh, int dtype, int64_t rows, int64_t Hq, int64_t H, int64_t D,
                                 float scaling, const int32_t* step, int64_t sequences, int64_t split_items, int64_t run_tokens,
-                                int64_t split_tokens, const int32_t* table, int64_t max_blocks, int64_t P, int code, const uint8_t* kc, const uint8_t* vc, const float* sc,
+                                int64_t split_tokens, int joins, const int32_t* table, int64_t max_blocks, int64_t P, int code, const uint8_t* kc, const uint8_t* vc, const float* sc,
                                 const void* ko, const void* vo, void* out, float* workspace, int64_t workspace_floats, int32_t* tickets,
                                 void* stream) {
   KVQ_REQUIRE(D == 64 || D == 128, "kvq_paged_decode: head_dim must be 64 or 128 (got %lld)", static_cast<long long>(D));
@@ -535,20 +606,30 @@ extern "C" int kvq_paged_decode(const void* q, int64_t q_st, int64_t q_sh, int d
   DecodeArgs a{static_cast<const uint16_t*>(q), q_st, q_sh, step, static_cast<int>(sequences), table, max_blocks,
                static_cast<int>(H), static_cast<int>(rep), static_cast<int>(pieces), scaling * 1.44269504088896341f, kc, vc, sc,
                static_cast<const uint16_t*>(ko), static_cast<const uint16_t*>(vo), static_cast<uint16_t*>(out), workspace,
-               split_tokens * rep, rep * run_tokens <= kWaves && split_items * H <= 256 ? tickets : nullptr};
-  // Joining in the launch, against a launch for it.  One sequence of 4096 tokens, 8 KV heads of 128, 136 workgroups: with
-  // one row 9.4 / 11.9 us, four 10.3 / 11.7, eight 13.0 / 11.9, sixteen 18.6 / 12.1 (rows one after the other in a wavefront,
-  // loads past the caches); 768 workgroups with four rows 26.1 / 23.9 (their stores and the wait for the last one).  So
-  // where a wavefront has one row at most and every workgroup a CU of its own.
-  const int64_t blocks = (split_items * H + 7) / 8 * 8 * a.pieces, merges = (rows * Hq + kWaves - 1) / kWaves;
+               split_tokens * rep, rep * run_tokens * D <= kWaves * 128 && split_items * H <= 256 && split_items <= 64 * sequences ? tickets : nullptr};
+  // Joining in the launch, against a launch for it, in us.  One sequence, 8 KV heads: of 128 and 4096 tokens, 136 workgroups,
+  // with one row 9.5 / 11.1, four 10.4 / 11.2, eight 12.6 / 11.2 (a wavefront's rows share its loads past the caches); of 64, four
+  // rows 8.0 / 10.2, eight 8.7 / 10.2.  768 workgroups 26.1 / 23.9 (their stores and the wait for the last one); 2 KV heads, 30000
+  // tokens, 118 items of one sequence 17.1 / 12.5.
+  // The launch takes a workgroup for each row, a quarter of the items to a wavefront, where sequences have many items and
+  // the rows are few: those 118 items 22.5 -> 12.5; otherwise a wavefront for each row: 16 sequences of 5 items, 896 rows,
+  // 13.9 against 15.0.
+  const int64_t blocks = (split_items * H + 7) / 8 * 8 * a.pieces,
+                waves = rows * Hq <= 1024 && split_items >= 16 * sequences ? kWaves : 1,
+                merges = (rows * Hq * waves + kWaves - 1) / kWaves;
   KVQ_REQUIRE(blocks <= kMaxGrid && merges <= kMaxGrid, "kvq_paged_decode: too many rows");
   auto run = [&](auto d, auto p, auto c, auto t) {
     constexpr int D_ = decltype(d)::value, P_ = decltype(p)::value, C_ = decltype(c)::value;
     constexpr bool T_ = decltype(t)::value != 0;
     hipLaunchKernelGGL((paged_split_kernel<D_, P_, C_, T_>), dim3(static_cast<uint32_t>(blocks)), dim3(kThreads), 0,
                        static_cast<hipStream_t>(stream), a);
-    if (!a.tickets) hipLaunchKernelGGL((paged_merge_kernel<D_, T_>), dim3(static_cast<uint32_t>(merges)), dim3(kThreads), 0,
-                       static_cast<hipStream_t>(stream), a, rows * Hq);
+    if (a.tickets || !joins) return;
+    auto join = [&](auto w) {
+      hipLaunchKernelGGL((paged_merge_kernel<D_, T_, decltype(w)::value>), dim3(static_cast<uint32_t>(merges)), dim3(kThreads), 0,
+                         static_cast<hipStream_t>(stream), a, rows * Hq);
+    };
+    if (waves == kWaves) join(std::integral_constant<int, kWaves>{});
+    else join(std::integral_constant<int, 1>{});
   };
   using Zero = std::integral_constant<int, 0>;
   using One = std::integral_constant<int, 1>;

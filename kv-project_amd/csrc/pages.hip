@@ -9,6 +9,7 @@
 // All of these kernels move bytes: filling reads 4 D and writes 2 D bytes per token and KV head, reading back the
 // reverse.  16 prompts of 6001 to 8200 tokens, 8 KV heads of 128: filling 129-144 us for 694 MB (4.8-5.4 TB/s), reading
 // back 116-123 (5.6-6.0); a large copy reaches 4.9.  A few tokens: 2-5 us each, a launch and its round trips.
+#include <algorithm>
 #include <cmath>
 #include <cstring>
 
@@ -421,11 +422,14 @@ int64_t shared(const int32_t* table, int64_t max_blocks, int64_t a, int64_t b, i
 
 // A front is worth a run of its own from this many units on: one for each wavefront of a workgroup.
 constexpr int64_t kFront = 4;
+constexpr int64_t kUneven = 16;
 
 // Fills the description from lens (before), counts and open buffers; pages are written by the caller.  split_cap bounds
-// the split items (those of a front weighted by the workgroups that its rows take at four query heads per KV head);
-// of no more than few_units units there are few_cap items, unless that makes the longest one more than twice an
-// even share.
+// the split items (those of a front weighted by the workgroups that its rows take at four query heads per KV head).
+// With few_cap, the workgroups that have a CU each: of no more than few_units units there are few_cap items, unless that
+// makes the longest one more than twice an even share, or there are more sequences and long ones among them; and up to twice split_cap where the longest item is kUneven units
+// and 1.5 times an even share at least, and all sequences start at once (8 KV heads of 128: 64 sequences of 100 to 4000
+// tokens 61 -> 54 us, but 64 of 3000 to 4000 94 -> 98, and 256 of 16 to 3000 with 16 rows each 187 -> 209).
 // most_run, most_tokens: where the step has to fit a launch that was captured; fronts that do not are left out.
 void describe(const int64_t* lens, const uint8_t* open, const int32_t* table, int64_t max_blocks, int64_t page, const int64_t* seq,
               const int64_t* counts, int64_t n, int64_t split_cap, int64_t few_cap, int64_t few_units, int64_t most_run, int64_t most_tokens,
@@ -505,13 +509,18 @@ void describe(const int64_t* lens, const uint8_t* open, const int32_t* table, in
       }
       return lo;
     };
-    int64_t lo = units(split_cap);
-    const int64_t all = weighted(1);
-    if (few_cap > 0 && few_cap < split_cap && all <= few_units) {
-      const int64_t few = units(few_cap), even = (all + few_cap - 1) / few_cap;
-      if (few <= 2 * (even > 4 ? even : 4)) lo = few;
+    int64_t lo = units(split_cap), cap = split_cap;
+    const int64_t all = weighted(1), active = std::count_if(counts, counts + n, [](int64_t c) { return c > 0; });
+    auto even_share = [&](int64_t items) { const int64_t x = (all + items - 1) / items; return x > 4 ? x : 4; };
+    const int64_t few = few_cap > 0 && few_cap < split_cap && all <= few_units ? units(few_cap) : 0;
+    if (few && few <= 2 * even_share(few_cap) && (few < kUneven || weighted(few) <= few_cap)) {
+      lo = few;
+    } else if (lo >= kUneven && active <= 2 * few_cap && 2 * lo > 3 * even_share(split_cap)) {
+      cap = 2 * split_cap;
+      lo = units(cap);
     }
     int64_t split = 0, base = 0;
+    bool ones = true, joins = nr > n;
     for (int64_t i = 0; i < nr; ++i) {
       int32_t* r = runs + kStepRun * i;
       r[5] = static_cast<int32_t>(split);
@@ -519,8 +528,10 @@ void describe(const int64_t* lens, const uint8_t* open, const int32_t* table, in
       r[11] = static_cast<int32_t>(splits(i, lo));
       split += splits(i, lo);
       base += splits(i, lo) * r[2];
+      ones = ones && splits(i, lo) == 1;
+      joins = joins || splits(i, lo) > 1;
     }
-    if (fronts && nr > n && (weighted(lo) > split_cap || widest > most_run || base > most_tokens)) continue;
+    if (fronts && nr > n && (weighted(lo) > cap || widest > most_run || base > most_tokens)) continue;
     int32_t* r = runs + kStepRun * nr;
     memset(r, 0, sizeof(int32_t) * kStepRun);
     r[5] = static_cast<int32_t>(split);
@@ -535,7 +546,8 @@ void describe(const int64_t* lens, const uint8_t* open, const int32_t* table, in
     desc[7] = base < INT64_C(1) << 31 ? static_cast<int32_t>(base) : -1;
     desc[8] = static_cast<int32_t>(nr);
     desc[9] = static_cast<int32_t>(kStepHead + kStepSeq * (n + 1) + kStepRun * (nr + 1));
-    desc[10] = desc[11] = 0;
+    desc[10] = joins;
+    desc[11] = ones;
     last[5] = static_cast<int32_t>(nr);
     return;
   }

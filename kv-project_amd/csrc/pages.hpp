@@ -13,7 +13,8 @@
 //
 // A step's description (int32 words on the device): a header of 12 words {sequences, items, split items,
 // units per split, whether every sequence has one item, the most new tokens of one, the most of a run, the
-// tokens of all split items, runs, first word of the items' pages}, then 8 words per sequence {slot, tokens
+// tokens of all split items, runs, first word of the items' pages, whether results are joined of several items,
+// whether every run is one item}, then 8 words per sequence {slot, tokens
 // before, new tokens, first packed row, first item, its run, open buffer before | after << 1, 1 + the run of its
 // shared front or 0} and one entry behind the last with the totals, then the runs, then the page of every item.
 // An item is a block that the step's tokens touch.
@@ -50,16 +51,21 @@ __device__ __forceinline__ StepRun step_run(const int* runs, int i) {
   return {e[0], e[1], e[2], e[3], e[4], e[5], e[6], e[7], e[8], e[9], e[10], e[11]};
 }
 
-// The last of n sequences whose word (at first[i * stride]) is not above `value`: 64 at a time, one memory round trip
+// The last of n sequences whose word (at first[i * stride]) is not above `value`: 256 at a time, one memory round trip
 // each instead of one per halving.  By whole wavefronts, `value` the same in all lanes.
 __device__ __forceinline__ int last_not_above(const int* first, int stride, int n, int value) {
   const int lane = threadIdx.x & 63;
   int count = 0;
-  for (int i = 0; i < n; i += 64) {
-    const int x = i + lane < n ? first[(i + lane) * stride] : 0x7fffffff;
-    const int c = __popcll(__builtin_amdgcn_ballot_w64(x <= value));
-    count += c;
-    if (c < 64) break;
+  for (int i = 0; i < n; i += 256) {
+    int x[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const int at = i + 64 * k + lane;
+      x[k] = first[(at < n ? at : n - 1) * stride];
+    }
+#pragma unroll
+    for (int k = 0; k < 4; ++k) count += __popcll(__builtin_amdgcn_ballot_w64(i + 64 * k + lane < n && x[k] <= value));
+    if (count < i + 256) break;
   }
   return count - 1;
 }

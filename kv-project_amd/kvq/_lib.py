@@ -115,8 +115,8 @@ SIGNATURES = {
     "kvq_pages_free": (i32, [vp, vp, vp, vp, vp, i64, i64, i64, vp, i64]),
     "kvq_pages_move": (i32, [vp, vp, vp, vp, vp, i64, i64, i64, i64, i64, i64, vp, i64, i64, i64, vp, vp, vp, vp, vp, vp, vp, vp]),
     "kvq_paged_decode_workspace": (i64, [i64, i64, i64, i64]),
-    "kvq_paged_decode": (i32, [vp, i64, i64, i32, i64, i64, i64, i64, f32, vp, i64, i64, i64, i64, vp, i64, i64, i32, vp, vp, vp, vp, vp,
-                               vp, vp, i64, vp, vp]),
+    "kvq_paged_decode": (i32, [vp, i64, i64, i32, i64, i64, i64, i64, f32, vp, i64, i64, i64, i64, i32, vp, i64, i64, i32, vp, vp, vp,
+                               vp, vp, vp, vp, i64, vp, vp]),
 }
 
 

@@ -52,7 +52,7 @@ def _address(a: np.ndarray) -> int:
 class Step:
     """New tokens of some slots: ``rows`` packed rows, slot by slot.  Made by ``PagedCache.extend``."""
 
-    __slots__ = ("slots", "counts", "ends", "rows", "items", "splits", "run_tokens", "split_tokens", "fronts", "shares",
+    __slots__ = ("slots", "counts", "ends", "rows", "items", "splits", "run_tokens", "split_tokens", "joins", "fronts", "shares",
                  "desc", "ptr", "host", "generation", "stamp")
 
 
@@ -176,10 +176,10 @@ class PagedCache:
         _lib.call_on(self.device, "kvq_pages_extend", *self._host, self.slots, self.pages, self.max_blocks, self.page,
                      self.max_tokens, _address(s), pc, n, st.splits, *few, run_tokens, st.split_tokens,
                      _address(st.host), st.host.size, st.ptr, _lib.stream_of(st.desc))
-        head = st.host[:9].tolist()
+        head = st.host[:11].tolist()
         if into is None:
             # what later steps written into this one keep to: without shared fronts any of them does
-            st.splits, st.run_tokens = max(1, head[2]), head[6]
+            st.splits, st.run_tokens, st.joins = max(1, head[2]), head[6], head[10]
             st.split_tokens = max(head[7], st.splits * head[5])
             st.items, st.rows = st.host.size - 32 * n - 32, int(st.host[8 * n + 15])
         st.fronts = head[8] > n
@@ -325,7 +325,7 @@ def paged_decode(q: torch.Tensor, scaling: float, cache: PagedCache, layer: int,
         raise ValueError("workspace must be contiguous float32 on the cache's device")
     table, max_blocks, _, _, page, code = cache._fixed
     _lib.call_on(device, "kvq_paged_decode", q.data_ptr(), qt, qh, cache._type, step.rows, Hq, Hkv, d, float(scaling), step.ptr,
-                 step.slots.size, step.splits, step.run_tokens, step.split_tokens, table, max_blocks, page, code,
-                 *cache._at[layer], out.data_ptr(), workspace.data_ptr(), workspace.numel(),
+                 step.slots.size, step.splits, step.run_tokens, step.split_tokens, step.joins, table, max_blocks, page,
+                 code, *cache._at[layer], out.data_ptr(), workspace.data_ptr(), workspace.numel(),
                  None if step.shares else cache._tickets[layer], _lib.stream_of(q))
     return out

@@ -290,9 +290,9 @@ def test_resize_on_another_stream():
     assert all(bool((h == 77).all()) for h in held)
 
 
-@pytest.mark.parametrize("rep,T", [(1, 1), (2, 2), (4, 1), (3, 1), (5, 1), (8, 2)])
+@pytest.mark.parametrize("rep,T", [(1, 1), (2, 2), (4, 1), (3, 1), (5, 1), (7, 1), (4, 2), (8, 2)])
 def test_joins_within_the_launch(rep, T):
-    """A step's items joined by the last workgroup, where it has few rows, or by a launch: the same; counters are zeros again."""
+    """A step's items joined by the last workgroup, where it has few rows, and by a launch; counters are zeros again."""
     import kvq
     m = Mirror(slots=3, pages=200, max_tokens=7000, Hkv=2, d=128, page=64, seed=22)
     m.push([0, 1, 2], [6000, 900, 1])
@@ -302,7 +302,53 @@ def test_joins_within_the_launch(rep, T):
         assert torch.equal(out, kvq.paged_decode(q.cuda(), 128 ** -0.5, m.cache, 0, step))
     assert not m.cache._counters.any()
     m.cache._tickets = [None]
-    assert torch.equal(out, kvq.paged_decode(q.cuda(), 128 ** -0.5, m.cache, 0, step))
+    m.decode(step, 2 * rep, what="joined by a launch")
+
+
+def test_a_captured_step_without_joins():
+    """As many sequences as there are places: an item each and no launch for joins, in later steps of the graph neither, however
+    long some of them have grown; nothing new for one sequence."""
+    import kvq
+    n = 66
+    m = Mirror(slots=n, pages=900, max_tokens=1200, Hkv=8, d=64, page=32, seed=23)
+    m.push(list(range(n)), [1 + 5 * i % 90 for i in range(n)])
+    counts = [0 if i == 7 else 1 for i in range(n)]
+    # 96 places at head_dim 64: short sequences take one item all the same
+    step, [(k, v)] = m.extend(list(range(n)), counts)
+    assert step.joins == 0 and step.splits == n - 1
+    kd, vd, q = k.cuda(), v.cuda(), m.rand(n - 1, 16).cuda()
+    out, ws = torch.empty_like(q), torch.empty(kvq.paged_workspace_floats(step, 16, 8, 64), device="cuda")
+    m.cache.append(0, kd, vd, step)
+    torch.cuda.synchronize()
+    gr = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(gr):
+        m.cache.append(0, kd, vd, step)
+        kvq.paged_decode(q, 0.125, m.cache, 0, step, out=out, workspace=ws)
+    for i in range(3):
+        m.push([3, 40], [300, 33])
+        step, [(k, v)] = m.extend(list(range(n)), counts, into=step)
+        kd.copy_(k)
+        vd.copy_(v)
+        _ = (q.float() * 2).sum()
+        gr.replay()
+        torch.cuda.synchronize()
+        a = 0
+        for s, c in enumerate(counts):
+            if c:
+                kk, vv = cached(m.k[0][s], 32, "int8"), cached(m.v[0][s], 32, "int8")
+                check(out[a:a + 1], attend(q[a:a + 1].cpu(), kk, vv, 0.125), float(vv.abs().max()), kk.shape[0], 64, torch.bfloat16,
+                      PAIR, f"replay {i}, slot {s}")
+                a += 1
+
+
+def test_uneven_sequences():
+    """A step of sequences that are cut finer than the places, and of long ones whose joins take a workgroup each."""
+    m = Mirror(slots=66, pages=1200, max_tokens=9000, Hkv=8, d=64, page=64, seed=24)
+    m.push(list(range(60)), [3 + 41 * i % 1500 for i in range(60)])
+    m.decode(m.push(list(range(60)), [1 + i % 2 for i in range(60)]), 16, what="uneven")
+    m.push([64], [8500])
+    m.decode(m.push([64], [2]), 40, what="one long")
+    m.decode(m.push([64, 65], [1, 3]), 16, what="long and short")
 
 
 def test_random_life():

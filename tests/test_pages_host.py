@@ -99,7 +99,7 @@ def test_accounts_follow_the_model(page):
         host.same(model)
 
 
-def _description(host, slots, counts):
+def _description(host, slots, counts, most=64):
     """Rows, items, the pages of what gets full; runs: every unit of every sequence in one, shared ones only in front."""
     n, d, page = len(slots), host.desc, host.page
     seq, nr = d[12:12 + 8 * (n + 1)].reshape(n + 1, 8), int(d[8])
@@ -128,6 +128,7 @@ def _description(host, slots, counts):
             assert np.array_equal(host.table[s, :blocks], host.table[f[0], :blocks])
         row += c
     split = base = 0
+    assert d[10] == (nr > n or (runs[:nr, 11] > 1).any()) and d[11] == (runs[:nr, 11] == 1).all()
     for r in runs[:nr]:
         assert r[5] == split and r[6] == base
         k = -(-(r[4] - r[3]) // int(d[3]))
@@ -135,7 +136,7 @@ def _description(host, slots, counts):
         split, base = split + k, base + k * r[2]
     assert runs[nr, 5:7].tolist() == [split, base]
     assert d[4] == all(b - a == 1 for a, b in zip(seq[:, 4], seq[1:, 4]))
-    assert seq[n, 3:5].tolist() == [row, item] and d[:3].tolist() == [n, item, split] and split <= 64
+    assert seq[n, 3:5].tolist() == [row, item] and d[:3].tolist() == [n, item, split] and split <= most
     assert d[5:8].tolist() == [max(counts), max(max(counts), *(int(r[2]) for r in runs[:nr])), base]
 
 
@@ -146,6 +147,23 @@ def test_few_units_take_few_items():
         assert host.extend(slots, counts, cap=64, few=few) == 0
         _description(host, slots, counts)
         assert want // 2 < int(host.desc[2]) <= want
+
+
+def test_uneven_sequences_take_more_items():
+    """64 sequences with a place each, the longest twice an even share: up to twice as many items; not for even ones, short
+    ones, more sequences than places, or a step that has to fit an older one."""
+    slots = list(range(64))
+    uneven = [64 * (1 + i % 60) for i in slots]
+    for counts, few, more in ((uneven, (32, 1), True), (uneven, (0, 0), False), (uneven, (31, 1), False),
+                              ([64 * (50 + i % 10) for i in slots], (32, 1), False), ([64 * (1 + i % 14) for i in slots], (32, 1), False)):
+        host = Host(64, 64 * 64, 64 * 64, 64)
+        assert host.extend(slots, counts, cap=64, few=few) == 0
+        _description(host, slots, counts, most=128)
+        assert (int(host.desc[2]) > 64) == more
+    host = Host(64, 64 * 64, 64 * 64, 64)      # few units, but not one item for each: the same
+    assert host.extend(slots, uneven, cap=64, few=(32, 10000)) == 0 and int(host.desc[2]) > 64
+    host = Host(64, 64 * 64, 64 * 64, 64)
+    assert host.extend(slots, [64 * 10] * 64, cap=96, few=(32, 10000)) == 0 and int(host.desc[2]) == 64 and not host.desc[10]
 
 
 def test_fronts_of_forks():
@@ -261,6 +279,6 @@ def test_kernel_entries_refuse_before_any_launch():
     assert rc == 1 and b"code" in lib.kvq_last_error()
     need = lib.kvq_paged_decode_workspace(4, 2, 2, 64)
     assert need == 4 * 2 * 2 * 66
-    rc = lib.kvq_paged_decode(one, 256, 64, 2, 1, 4, 2, 64, 0.1, one, 1, 4, 1, 4, one, 4, 64, 0, one, one, one, one, one, one, one, need - 1, None, None)
+    rc = lib.kvq_paged_decode(one, 256, 64, 2, 1, 4, 2, 64, 0.1, one, 1, 4, 1, 4, 1, one, 4, 64, 0, one, one, one, one, one, one, one, need - 1, None, None)
     assert rc == 1 and b"workspace" in lib.kvq_last_error()
     assert lib.kvq_paged_decode_workspace(4, 2, 2, 96) == -1
