@@ -735,9 +735,9 @@ int kvq_pages_move(const int64_t* lens, int32_t* table, const int32_t* refs, int
  * Attention of a step's query rows over the paged cache: q (rows, Hq, D), the step's rows in order; query
  * i of a sequence with `count` new tokens sees all tokens up to its own.  sequences: of the step; split_items,
  * run_tokens and split_tokens: at least the description's third, seventh and eighth word; they give the grid and the
- * workspace.  joins: its eleventh word, or 1 (a launch joins the results of several split items).  out (rows, Hq, D)
- * contiguous.  workspace: kvq_paged_decode_workspace floats, no clearing; calls that share one must not overlap in
- * time.
+ * workspace.  joins: its eleventh word, or 1: results of several split items are joined; without, no workspace is
+ * needed.  out (rows, Hq, D) contiguous.  workspace: kvq_paged_decode_workspace floats, no clearing; calls that share
+ * one must not overlap in time.
  * tickets: NULL, or (slots, H, 32) int32 zeros, which a call leaves as zeros: a sequence's split items are then joined
  * within the one launch, by the workgroup that comes last (always in the items' order), where that is the faster way:
  * few rows, items and workgroups.  Not for a step with shared fronts.  Calls over one slot of one layer must not

@@ -595,11 +595,11 @@ extern "C" int kvq_paged_decode(const void* q, int64_t q_st, int64_t q_sh, int d
   KVQ_REQUIRE(dtype == KVQ_F16 || dtype == KVQ_BF16, "kvq_paged_decode: queries must be fp16 or bf16");
   KVQ_REQUIRE(code == kCodeInt8 || code == kCodeE4M3, "kvq_paged_decode: unknown code %d", code);
   KVQ_REQUIRE(H > 0 && Hq > 0 && Hq % H == 0 && rows > 0 && run_tokens > 0 && split_items > 0 && sequences > 0, "kvq_paged_decode: bad sizes");
-  KVQ_REQUIRE(q && step && table && kc && vc && sc && ko && vo && out && workspace, "kvq_paged_decode: null pointer");
+  KVQ_REQUIRE(q && step && table && kc && vc && sc && ko && vo && out && (workspace || !joins), "kvq_paged_decode: null pointer");
   KVQ_REQUIRE(reinterpret_cast<uintptr_t>(q) % 16 == 0 && (q_st | q_sh) % 8 == 0 && reinterpret_cast<uintptr_t>(out) % 16 == 0 &&
                   reinterpret_cast<uintptr_t>(workspace) % 16 == 0,
               "kvq_paged_decode: rows and strides must be multiples of 16 bytes");
-  const int64_t rep = Hq / H, need = kvq_paged_decode_workspace(split_tokens, H, rep, D), pieces = pieces_of(rep, run_tokens);
+  const int64_t rep = Hq / H, need = joins ? kvq_paged_decode_workspace(split_tokens, H, rep, D) : 0, pieces = pieces_of(rep, run_tokens);
   KVQ_REQUIRE(need >= 0, "kvq_paged_decode: too many split tokens (%lld)", static_cast<long long>(split_tokens));
   KVQ_REQUIRE(workspace_floats >= need, "kvq_paged_decode: workspace of %lld floats, %lld needed", static_cast<long long>(workspace_floats),
               static_cast<long long>(need));

@@ -161,7 +161,7 @@ class PagedCache:
                 raise ValueError("counts must not be negative, and below 2^31")
             st = Step()
             st.host = np.empty(words, dtype=np.int32)
-            st.desc = torch.empty(words, dtype=torch.int32, device=self.device)
+            st.desc = self.table.new_empty(words)
             st.ptr = st.desc.data_ptr()
             st.splits = max(n, -(-SPLIT_BLOCKS[self.d] // self.Hkv))
             st.run_tokens = st.split_tokens = 1 << 31
@@ -227,7 +227,7 @@ class PagedCache:
             raise IndexError(f"no layer {layer} (of {self.layers})")
         s = _ints(slots, "slots")
         total = sum(self._lens.take(s, mode="clip").tolist())
-        out = torch.empty((2, total, self.Hkv, self.d), dtype=self.dtype, device=self.device)
+        out = self.k_open.new_empty((2, total, self.Hkv, self.d))
         k, v = out.unbind(0)
         _lib.call_on(self.device, "kvq_pages_rows", self._host[0], self._host[3], self.slots, _address(s), s.size,
                      *self._fixed, self._type, *self._at[layer], k.data_ptr(), v.data_ptr(), k.numel(), _lib.stream_of(out))
@@ -289,6 +289,10 @@ class PagedCache:
 
 
 def paged_workspace_floats(step: Step, Hq: int, Hkv: int, d: int) -> int:
+    """Float32 scratch of a decode of this step, and of those that are written into it: none where every sequence is one
+    split item."""
+    if not step.joins:
+        return 0
     n = _lib.load().kvq_paged_decode_workspace(step.split_tokens, Hkv, Hq // Hkv, d)
     if n < 0:
         raise _lib.KVQError("kvq_paged_decode_workspace rejected the shape")
@@ -316,11 +320,14 @@ def paged_decode(q: torch.Tensor, scaling: float, cache: PagedCache, layer: int,
         cache.check_step(step, "paged_decode")
     q, qt, qh = rows16(q)
     Hq, device = shape[1], cache.device
-    out = torch.empty(shape, dtype=cache.dtype, device=device) if out is None else _lib.out_or_new(out, shape, cache.dtype, device, "paged_decode")
+    if out is None:
+        out = torch.empty_like(q, memory_format=torch.contiguous_format)
+    else:
+        _lib.out_or_new(out, shape, cache.dtype, device, "paged_decode")
     if step.rows == 0:
         return out
     if workspace is None:
-        workspace = torch.empty((paged_workspace_floats(step, Hq, Hkv, d),), dtype=torch.float32, device=device)
+        workspace = cache.sc.new_empty(paged_workspace_floats(step, Hq, Hkv, d))
     elif workspace.dtype != torch.float32 or not workspace.is_contiguous() or workspace.device != device:
         raise ValueError("workspace must be contiguous float32 on the cache's device")
     table, max_blocks, _, _, page, code = cache._fixed

@@ -79,7 +79,7 @@ def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, scaling:
         _lib.require_gpu(q, k, v)
         raise ValueError(f"prompt_attention: the plan is for {device}")
     if out is None:
-        out = torch.empty(qs, dtype=dtype, device=device)
+        out = torch.empty_like(q, memory_format=torch.contiguous_format)
     else:
         _lib.out_or_new(out, qs, dtype, device, "prompt_attention")
     if plan.keys == 0:

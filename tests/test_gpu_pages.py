@@ -297,6 +297,7 @@ def test_joins_within_the_launch(rep, T):
     m = Mirror(slots=3, pages=200, max_tokens=7000, Hkv=2, d=128, page=64, seed=22)
     m.push([0, 1, 2], [6000, 900, 1])
     step = m.push([0, 1, 2], [T] * 3)
+    assert step.joins
     q, out = m.decode(step, 2 * rep, what="joined")
     for _ in range(3):
         assert torch.equal(out, kvq.paged_decode(q.cuda(), 128 ** -0.5, m.cache, 0, step))
@@ -324,8 +325,12 @@ def test_a_captured_step_without_joins():
     with torch.cuda.graph(gr):
         m.cache.append(0, kd, vd, step)
         kvq.paged_decode(q, 0.125, m.cache, 0, step, out=out, workspace=ws)
+    assert ws.numel() == 0
     for i in range(3):
         m.push([3, 40], [300, 33])
+        if i == 2:                             # neighbours that share pages
+            m.free([4])
+            m.fork([3], [4])
         step, [(k, v)] = m.extend(list(range(n)), counts, into=step)
         kd.copy_(k)
         vd.copy_(v)
@@ -559,8 +564,11 @@ def test_gpu_refusals():
         kvq.paged_decode(q[:, :3], 0.1, c, 0, step)
     with pytest.raises(TypeError):
         kvq.paged_decode(q.half(), 0.1, c, 0, step)
+    long = kvq.PagedCache(1, 1, 11, 700, 2, 64)
+    long.extend([0], [690])
+    many = long.extend([0], [4])               # several items: their results need room
     with pytest.raises(kvq.KVQError, match="workspace"):
-        kvq.paged_decode(q, 0.1, c, 0, step, workspace=torch.empty(10, device="cuda"))
+        kvq.paged_decode(q, 0.1, long, 0, many, workspace=torch.empty(10, device="cuda"))
     with pytest.raises(kvq.KVQError, match="no slot"):
         c.rows(0, [0, 3])
     with pytest.raises(ValueError, match="same counts"):
