@@ -16,7 +16,7 @@
 //
 // What bounds it: long caches, the codes' way from memory: 16 sequences of 32768 tokens, 8 KV heads of 128, 186-201 us
 // for 1.07 GB (5.4-5.8 TB/s, 88-94% of the 6.1 TB/s of a read-only stream; the matrix cores are busy 10% of the time, the
-// vector unit, which widens the codes, 33%), and 4.7 us of joins.  One sequence of 4096 tokens, 128 workgroups: 9.2 us,
+// vector unit, which widens the codes, 33%), and 4.7 us of joins.  One sequence of 4096 tokens, 128 workgroups: 8.8 us,
 // the round trips of one unit: description, page number, codes, join.  Registers for two workgroups a CU instead
 // of three were no faster.
 #include <type_traits>

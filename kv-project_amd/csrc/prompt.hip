@@ -17,8 +17,8 @@
 // KV heads of 128, bf16: 1913-2040 us by card (1.08-1.15 PFLOP/s; a library product of the largest size reaches 1.36),
 // matrix cores busy 63%, vector unit 55% of the cycles, at 1.7 GHz of 2.4; no LDS conflicts; keys and values come
 // from memory 4.5 times, otherwise from the caches.  With head_dim 64 a score costs half the products and the same
-// exponential, so the vector unit leads (68%; matrix cores 42%): four sequences of 512 to 1531 tokens behind up to 9000,
-// 235-269 us (0.76-0.87 PFLOP/s).  24 sequences of 1 to 2901 tokens, fp16, head_dim 128: 182 us (0.76 PFLOP/s): 71
+// exponential, so the vector unit leads (70%; matrix cores 43%): four sequences of 512 to 1531 tokens behind up to 9000,
+// 235-269 us (0.76-0.87 PFLOP/s).  24 sequences of 1 to 2901 tokens, fp16, head_dim 128: 180 us (0.77 PFLOP/s): 71
 // iterations for each of 512 places, 133 us at the long prompt's rate, and the starts and ends of five tiles.  20
 // tokens: 7 us, a launch and the round trips of one tile.
 // Measured and not kept: 64 rows a wavefront (half the LDS reads, but accumulators move between the register files:
