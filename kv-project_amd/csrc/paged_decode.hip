@@ -111,8 +111,9 @@ __device__ __forceinline__ float get(const float* p) {
   else return *p;
 }
 
-// N rows joined by one wavefront: the maxima, the sums, its channels of the weighted sums
-template <int D, bool SHARED, int N>
+// N rows joined by one wavefront: the maxima, the sums, its channels of the weighted sums.  LONG: of many items, 32 on
+// their way at once
+template <int D, bool SHARED, int N, bool LONG = false>
 struct Join {
   float top[N], l[N], o[N][D / 64];
   __device__ __forceinline__ Join() {
@@ -126,22 +127,32 @@ struct Join {
   }
   // DEEP items of every row on their way at once; behind the last: it again, unused
   template <int DEEP>
-  __device__ __forceinline__ void some(const float* const (&p)[N], int64_t stride, int k0, int most, const float (&f)[N]) {
+  struct Items {
     float x[N][DEEP][D / 64];
+    __device__ __forceinline__ void load(const float* const (&p)[N], int64_t stride, int k0, int most) {
 #pragma unroll
-    for (int n = 0; n < N; ++n)
+      for (int n = 0; n < N; ++n)
 #pragma unroll
-      for (int k = 0; k < DEEP; ++k)
+        for (int k = 0; k < DEEP; ++k)
 #pragma unroll
-        for (int e = 0; e < D / 64; ++e) x[n][k][e] = get<SHARED>(p[n] + (k0 + k < most ? k0 + k : most - 1) * stride * D + e);
+          for (int e = 0; e < D / 64; ++e) x[n][k][e] = get<SHARED>(p[n] + (k0 + k < most ? k0 + k : most - 1) * stride * D + e);
+    }
+    __device__ __forceinline__ void add_to(Join& j, int k0, int most, const float (&f)[N]) const {
 #pragma unroll
-    for (int n = 0; n < N; ++n)
+      for (int n = 0; n < N; ++n)
 #pragma unroll
-      for (int k = 0; k < DEEP; ++k) {
-        const float fk = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(f[n]), k0 + k < most ? k0 + k : 0));
+        for (int k = 0; k < DEEP; ++k) {
+          const float fk = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(f[n]), k0 + k < most ? k0 + k : 0));
 #pragma unroll
-        for (int e = 0; e < D / 64; ++e) o[n][e] += k0 + k < most ? fk * x[n][k][e] : 0.0f;
-      }
+          for (int e = 0; e < D / 64; ++e) j.o[n][e] += k0 + k < most ? fk * x[n][k][e] : 0.0f;
+        }
+    }
+  };
+  template <int DEEP>
+  __device__ __forceinline__ void some(const float* const (&p)[N], int64_t stride, int k0, int most, const float (&f)[N]) {
+    Items<DEEP> x;
+    x.load(p, stride, k0, most);
+    x.add_to(*this, k0, most, f);
   }
   // rows R of a run's split items from .. to - 1, 64 maxima at a time
   __device__ __forceinline__ void add(const DecodeArgs& a, const StepRun& run, const int (&R)[N], int h, int from, int to) {
@@ -159,6 +170,8 @@ struct Join {
         st[n] = make_float2(-INFINITY, 0.0f);
         if (i < to) st[n] = make_float2(get<SHARED>(stat + 2 * (first + i * stride)), get<SHARED>(stat + 2 * (first + i * stride) + 1));
       }
+      Items<8> early;                         // on their way with the maxima
+      early.load(p, stride, 0, most);
       float f[N];
 #pragma unroll
       for (int n = 0; n < N; ++n) {
@@ -170,8 +183,9 @@ struct Join {
         for (int e = 0; e < D / 64; ++e) o[n][e] *= old;
         top[n] = m;
       }
-      int k0 = 0;
-      if constexpr (!SHARED)
+      early.add_to(*this, 0, most, f);
+      int k0 = 8;
+      if constexpr (LONG)
         for (; k0 + 32 <= most; k0 += 32) some<32>(p, stride, k0, most, f);
       for (; k0 < most; k0 += 8) some<8>(p, stride, k0, most, f);
     }
@@ -250,11 +264,17 @@ __global__ __launch_bounds__(kThreads, 3) void paged_split_kernel(DecodeArgs a) 
   const int group = blockIdx.x / (8 * a.pieces), within = blockIdx.x % (8 * a.pieces);
   const int64_t ih = static_cast<int64_t>(group) * 8 + within % 8;
   const int piece = within / 8, item = static_cast<int>(ih / a.H), h = static_cast<int>(ih % a.H);
-  if (item >= step[2]) return;
   const int* runs = step_runs(step, a.n);
-  // no look where a run is one item, or one sequence the only run
-  const int ri = step[11] ? item : a.n == 1 ? 0 : __builtin_amdgcn_readfirstlane(last_not_above(runs + 5, kStepRun, step[8], item));
-  const StepRun run = step_run(runs, ri);
+  // no look where a run is one item, or one sequence the only run: that run is read with the header (there is room for
+  // 2 n + 1 of them)
+  const int near = a.n == 1 ? 0 : item < a.n ? item : a.n;
+  StepRun run = step_run(runs, near);
+  if (item >= step[2]) return;
+  int ri = near;
+  if (a.n > 1 && !(step[11] && item == near)) {
+    ri = __builtin_amdgcn_readfirstlane(last_not_above(runs + 5, kStepRun, step[8], item));
+    run = step_run(runs, ri);
+  }
   const int rows = a.rep * run.tokens;
   if (piece * kRows >= rows) return;
   const bool own = run.seq >= 0;              // or a shared front: whole pages that every row sees
@@ -534,18 +554,20 @@ __global__ __launch_bounds__(kThreads) void paged_merge_kernel(DecodeArgs a, int
   if (at >= total) return;
   const int Hq = a.H * a.rep;
   const int n = static_cast<int>(at / Hq), head = static_cast<int>(at % Hq), h = head / a.rep;
-  const StepSeq s = step_seq(a.step, a.n == 1 ? 0 : step_find(a.step, a.n, 3, n));
-  if (n >= s.row0 + s.count) return;
+  // as many sequences as rows, none with two: one of each; without fronts a sequence is the run of its number
+  const int longest = a.step[5], count = a.step[8];
+  const int i = a.n == 1 ? 0 : longest == 1 && total == static_cast<int64_t>(a.n) * Hq ? n : step_find(a.step, a.n, 3, n);
   const int* runs = step_runs(a.step, a.n);
-  const StepRun own = step_run(runs, s.run);
-  if (own.items < 2 && !s.front) return;      // its workgroup has written the result
-  Join<D, false, 1> j;
-  if (s.front) {
-    const StepRun front = step_run(runs, s.front - 1);
+  const StepRun own = step_run(runs, count == a.n ? i : step_seq(a.step, i).run);
+  if (n >= own.row0 + own.tokens) return;
+  if (own.items < 2 && !own.front) return;    // its workgroup has written the result
+  Join<D, false, 1, (WAVES > 1)> j;
+  if (own.front) {
+    const StepRun front = step_run(runs, own.front - 1);
     const int R[1] = {(n - front.row0) * a.rep + head % a.rep};
     j.add(a, front, R, h, front.items * part / WAVES, front.items * (part + 1) / WAVES);
   }
-  const int R[1] = {(n - s.row0) * a.rep + head % a.rep};
+  const int R[1] = {(n - own.row0) * a.rep + head % a.rep};
   j.add(a, own, R, h, own.items * part / WAVES, own.items * (part + 1) / WAVES);
   if constexpr (WAVES > 1) {
     __shared__ float sums[kWaves][D], stats[kWaves][2];
@@ -561,7 +583,7 @@ __global__ __launch_bounds__(kThreads) void paged_merge_kernel(DecodeArgs a, int
 #pragma unroll
     for (int i = 1; i < WAVES; ++i) top = fmaxf(top, stats[i][0]);
     const float safe = top == -INFINITY ? 0.0f : top;
-    j = Join<D, false, 1>();
+    j = Join<D, false, 1, (WAVES > 1)>();
 #pragma unroll
     for (int i = 0; i < WAVES; ++i) {
       const float f = __builtin_amdgcn_exp2f(stats[i][0] - safe);
