@@ -52,7 +52,7 @@ def _address(a: np.ndarray) -> int:
 class Step:
     """New tokens of some slots: ``rows`` packed rows, slot by slot.  Made by ``PagedCache.extend``."""
 
-    __slots__ = ("slots", "counts", "ends", "rows", "items", "splits", "run_tokens", "split_tokens", "joins", "fronts", "shares",
+    __slots__ = ("cache", "slots", "counts", "made", "rows", "items", "splits", "run_tokens", "split_tokens", "joins", "fronts", "shares",
                  "desc", "ptr", "host", "generation", "stamp")
 
 
@@ -91,6 +91,7 @@ class PagedCache:
         self._account = np.array([self.pages, 0], dtype=np.int64)   # free pages, none of them below
         self._generation = 0                   # of the pools
         self._stamp = 0                        # of the slots' lengths
+        self._touched = np.zeros(self.slots, dtype=np.int64)        # the stamp when a slot took tokens or was emptied
         self.table = torch.zeros((self.slots, self.max_blocks), dtype=torch.int32, device=self.device)
         self.kc, self.vc, self.sc = self._pool(self.pages)
         rows = (self.layers, self.slots, 2, self.Hkv, self.page * self.d)
@@ -160,6 +161,7 @@ class PagedCache:
             if words < 0:
                 raise ValueError("counts must not be negative, and below 2^31")
             st = Step()
+            st.cache = self
             st.host = np.empty(words, dtype=np.int32)
             st.desc = self.table.new_empty(words)
             st.ptr = st.desc.data_ptr()
@@ -168,6 +170,8 @@ class PagedCache:
             few = (-(-FEW_BLOCKS // self.Hkv), FEW_UNITS // self.Hkv)
         else:
             st = into
+            if st.cache is not self:
+                raise ValueError("a step is rewritten by its own cache only")
             if not np.array_equal(st.counts, c):
                 raise ValueError("a step is rewritten for the same counts only")
             few = (0, 0)
@@ -186,13 +190,16 @@ class PagedCache:
         if into is None:
             st.shares = st.fronts
         self._stamp += 1
-        st.slots, st.counts, st.ends, st.generation, st.stamp = s, c, self._lens[s], self._generation, self._stamp
+        self._touched[s[c > 0] if 0 in counts else s] = self._stamp
+        st.slots, st.counts, st.generation, st.made, st.stamp = s, c, self._generation, self._stamp, self._stamp
         return st
 
     def check_step(self, step: Step, what: str) -> None:
         """A step describes its slots only until they take more tokens or are freed."""
+        if step.cache is not self:
+            raise ValueError(f"{what}: the step is of another cache")
         if step.stamp != self._stamp:
-            if not (self._lens[step.slots] == step.ends).all():
+            if (self._touched[step.slots] > step.made).any():
                 raise ValueError(f"{what}: the step's slots have changed since it was made")
             step.stamp = self._stamp           # what changed were other slots
 
@@ -209,7 +216,7 @@ class PagedCache:
         if k.get_device() != self._index or v.get_device() != self._index:
             _lib.require_gpu(k, v)
             raise ValueError(f"append: the cache is on {self.device}")
-        if step.stamp != self._stamp:
+        if step.cache is not self or step.stamp != self._stamp:
             self.check_step(step, "append")
         if step.generation != self._generation:
             raise ValueError("append: the pages have moved since the step was made")
@@ -245,12 +252,14 @@ class PagedCache:
                      _address(t), s.size, self.layers, self.Hkv, self.d, self.table.data_ptr(), self.k_open.data_ptr(), self.v_open.data_ptr(),
                      _lib.stream_of(self.table))
         self._stamp += 1
+        self._touched[t] = self._stamp
 
     def free(self, slots: Sequence[int]) -> None:
         """Empty the slots; pages that no other sequence shares become free."""
         s = _ints(slots, "slots")
         _lib.call("kvq_pages_free", *self._host, self.slots, self.max_blocks, self.page, _address(s), s.size)
         self._stamp += 1
+        self._touched[s] = self._stamp
 
     def compact(self) -> int:
         """Move the pages at the end of the pool to the free places below, in order, so that the pages in use are the
@@ -316,7 +325,7 @@ def paged_decode(q: torch.Tensor, scaling: float, cache: PagedCache, layer: int,
     if q.get_device() != cache._index:
         _lib.require_gpu(q)
         raise ValueError(f"paged_decode: the cache is on {cache.device}")
-    if step.stamp != cache._stamp:
+    if step.cache is not cache or step.stamp != cache._stamp:
         cache.check_step(step, "paged_decode")
     q, qt, qh = rows16(q)
     Hq, device = shape[1], cache.device

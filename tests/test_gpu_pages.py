@@ -564,6 +564,25 @@ def test_gpu_refusals():
         kvq.paged_decode(q[:, :3], 0.1, c, 0, step)
     with pytest.raises(TypeError):
         kvq.paged_decode(q.half(), 0.1, c, 0, step)
+    # a step of another cache; of a slot that has been freed and holds as many tokens again
+    other = kvq.PagedCache(2, 3, 4, 300, 2, 64, page=64)
+    same = other.extend([0, 1], [3, 1])
+    with pytest.raises(ValueError, match="another cache"):
+        c.append(0, k, k, same)
+    with pytest.raises(ValueError, match="another cache"):
+        kvq.paged_decode(q, 0.1, c, 0, same)
+    with pytest.raises(ValueError, match="own cache"):
+        c.extend([0, 1], [3, 1], into=same)
+    other.extend([2], [0])
+    other.append(0, k, k, same)                # what changed were other slots, or nothing
+    other.extend([0], [0])
+    other.append(1, k, k, same)
+    other.free([0])
+    other.extend([0], [3])
+    with pytest.raises(ValueError, match="changed"):
+        other.append(1, k, k, same)
+    with pytest.raises(ValueError, match="changed"):
+        kvq.paged_decode(q, 0.1, other, 1, same)
     long = kvq.PagedCache(1, 1, 11, 700, 2, 64)
     long.extend([0], [690])
     many = long.extend([0], [4])               # several items: their results need room
