@@ -24,6 +24,7 @@
 // Measured and not kept: 64 rows a wavefront (half the LDS reads, but accumulators move between the register files:
 // 2040-2680 us); sums by a product with ones at head_dim 64 (235 -> 258 us); other wave priorities (3-5% slower).
 #include <algorithm>
+#include <cfloat>
 #include <cmath>
 #include <type_traits>
 
@@ -487,9 +488,11 @@ extern "C" int kvq_prompt_attention(const void* q, int64_t q_st, int64_t q_sh, c
   KVQ_REQUIRE(parts == 0 || (workspace && workspace_floats >= kvq_prompt_workspace(parts, H, D)),
               "kvq_prompt_attention: workspace of %lld floats, %lld needed", static_cast<long long>(workspace_floats),
               static_cast<long long>(kvq_prompt_workspace(parts, H, D)));
+  // a scaling of nothing would make a NaN of a hidden score's -inf: the smallest one, which makes zeros of the others
+  const float scale = std::fabs(scaling) * 1.44269504088896341f;
   const PromptArgs a{static_cast<const uint16_t*>(q), static_cast<const uint16_t*>(k), static_cast<const uint16_t*>(v),
                      q_st, q_sh, k_st, k_sh, v_st, v_sh, words, static_cast<int>(H), static_cast<int>(Hq / H),
-                     std::fabs(scaling) * 1.44269504088896341f, std::signbit(scaling) ? 0x80008000u : 0u,
+                     scale < FLT_MIN ? FLT_MIN : scale, std::signbit(scaling) ? 0x80008000u : 0u,
                      static_cast<uint16_t*>(out), workspace};
   const dim3 grid(static_cast<uint32_t>(items * H)), joins(static_cast<uint32_t>(merges * H), kTileRows * 64 / kThreads);
   hipStream_t s = static_cast<hipStream_t>(stream);

@@ -61,7 +61,8 @@ class PromptPlan:
 def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, scaling: float, plan: PromptPlan, *,
                      out: Optional[torch.Tensor] = None, workspace: Optional[torch.Tensor] = None) -> torch.Tensor:
     """Attention of the packed rows q (rows, Hq, d) over k, v (keys, Hkv, d), bf16 or fp16 of one type, head_dim 64
-    or 128, any row and head strides of whole 16 bytes (others are copied); returns (rows, Hq, d)."""
+    or 128, any row and head strides of whole 16 bytes (others are copied); returns (rows, Hq, d).  Forward only, as the
+    decodes: no gradient is recorded."""
     qs, ks = q.shape, k.shape
     if len(qs) != 3 or len(ks) != 3 or v.shape != ks:
         raise ValueError(f"prompt_attention takes q (rows, Hq, d) and k, v (keys, Hkv, d), got {tuple(qs)}, "

@@ -356,6 +356,18 @@ def test_uneven_sequences():
     m.decode(m.push([64, 65], [1, 3]), 16, what="long and short")
 
 
+def test_a_scaling_of_nothing():
+    import kvq
+    m = Mirror(slots=2, pages=60, max_tokens=1000, Hkv=1, d=64, page=32, seed=25)
+    m.push([0, 1], [900, 20])
+    step = m.push([0, 1], [3, 2])
+    q = m.rand(5, 2)
+    out = kvq.paged_decode(q.cuda(), 0.0, m.cache, 0, step)
+    for s, a, b in ((0, 0, 3), (1, 3, 5)):
+        kk, vv = cached(m.k[0][s], 32, "int8"), cached(m.v[0][s], 32, "int8")
+        check(out[a:b], attend(q[a:b], kk, vv, 0.0), float(vv.abs().max()), kk.shape[0], 64, torch.bfloat16, PAIR, f"slot {s}")
+
+
 def test_random_life():
     """A few hundred random steps, forks, frees and moves."""
     rng = random.Random(11)

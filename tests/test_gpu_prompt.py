@@ -132,6 +132,20 @@ def test_expanded_rows_and_a_negative_scaling():
                        kvq.prompt_attention(-q.cuda(), k.cuda(), v.cuda(), 0.1, plan))
 
 
+@pytest.mark.parametrize("scaling", [0.0, -0.0, 1e-45])
+def test_a_scaling_of_nothing(scaling):
+    """Every visible value weighs the same; hidden ones nothing."""
+    import kvq
+    lens, lens_k = [70, 3], [70, 900]
+    q, k, v = _inputs(lens, lens_k, 4, 2, 64, torch.bfloat16, 52)
+    out = kvq.prompt_attention(q.cuda(), k.cuda(), v.cuda(), scaling, kvq.PromptPlan(lens, 4, 2, lens_k=lens_k))
+    a = x = 0
+    for t, n in zip(lens, lens_k):
+        ref = attend(q[a:a + t], k[x:x + n], v[x:x + n], 0.0)
+        check(out[a:a + t], ref, float(v[x:x + n].abs().max()), n, 64, torch.bfloat16, HALF[torch.bfloat16], f"{t} of {n}")
+        a, x = a + t, x + n
+
+
 def test_offsets_past_32_bits():
     """Rows whose offsets pass 2^32 bytes and 2^31 elements."""
     import kvq
