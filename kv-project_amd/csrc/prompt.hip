@@ -22,7 +22,9 @@
 // iterations for each of 512 places, 133 us at the long prompt's rate, and the starts and ends of five tiles.  20
 // tokens: 7 us, a launch and the round trips of one tile.
 // Measured and not kept: 64 rows a wavefront (half the LDS reads, but accumulators move between the register files:
-// 2040-2680 us); sums by a product with ones at head_dim 64 (235 -> 258 us); other wave priorities (3-5% slower).
+// 2040-2680 us); sums by a product with ones at head_dim 64 (235 -> 258 us); other wave priorities (3-5% slower);
+// workgroups that stay for several tiles and fetch the next one's first keys during the last steps (24 sequences of 256
+// tokens 61 -> 54 us, but 3% slower over 273 shapes and 9% at head_dim 64, for its registers).
 #include <algorithm>
 #include <cfloat>
 #include <cmath>
