@@ -160,9 +160,13 @@ def call(name: str, *args) -> int:
     return rc
 
 
+# without torch.cuda's look at whether the GPU has been initialised: there are tensors on it
+_current_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
+
+
 def call_on(device: torch.device, name: str, *args) -> int:
     """``call`` with ``device`` as the current one: a launch on a default stream goes to the current device."""
-    if device.index == torch.cuda.current_device():
+    if device.index == _current_device():
         return call(name, *args)
     with torch.cuda.device(device):
         return call(name, *args)

@@ -222,9 +222,8 @@ class PagedCache:
             raise ValueError("append: the pages have moved since the step was made")
         if step.rows == 0:
             return
-        k, kt, kh = rows16(k)
-        v, vt, vh = rows16(v)
-        _lib.call_on(self.device, "kvq_pages_append", k.data_ptr(), kt, kh, v.data_ptr(), vt, vh, self._type, step.ptr, step.items,
+        (k, kp, kt, kh), (v, vp, vt, vh) = rows16(k), rows16(v)
+        _lib.call_on(self.device, "kvq_pages_append", kp, kt, kh, vp, vt, vh, self._type, step.ptr, step.items,
                      *self._fixed, *self._at[layer], _lib.stream_of(k))
 
     def rows(self, layer: int, slots: Sequence[int]) -> Tuple[torch.Tensor, torch.Tensor]:
@@ -327,7 +326,7 @@ def paged_decode(q: torch.Tensor, scaling: float, cache: PagedCache, layer: int,
         raise ValueError(f"paged_decode: the cache is on {cache.device}")
     if step.cache is not cache or step.stamp != cache._stamp:
         cache.check_step(step, "paged_decode")
-    q, qt, qh = rows16(q)
+    q, qp, qt, qh = rows16(q)
     Hq, device = shape[1], cache.device
     if out is None:
         out = torch.empty_like(q, memory_format=torch.contiguous_format)
@@ -340,7 +339,7 @@ def paged_decode(q: torch.Tensor, scaling: float, cache: PagedCache, layer: int,
     elif workspace.dtype != torch.float32 or not workspace.is_contiguous() or workspace.device != device:
         raise ValueError("workspace must be contiguous float32 on the cache's device")
     table, max_blocks, _, _, page, code = cache._fixed
-    _lib.call_on(device, "kvq_paged_decode", q.data_ptr(), qt, qh, cache._type, step.rows, Hq, Hkv, d, float(scaling), step.ptr,
+    _lib.call_on(device, "kvq_paged_decode", qp, qt, qh, cache._type, step.rows, Hq, Hkv, d, float(scaling), step.ptr,
                  step.slots.size, step.splits, step.run_tokens, step.split_tokens, step.joins, table, max_blocks, page,
                  code, *cache._at[layer], out.data_ptr(), workspace.data_ptr(), workspace.numel(),
                  None if step.shares else cache._tickets[layer], _lib.stream_of(q))

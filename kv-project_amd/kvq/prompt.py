@@ -85,7 +85,7 @@ def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, scaling:
         _lib.out_or_new(out, qs, dtype, device, "prompt_attention")
     if plan.keys == 0:
         return out.zero_()
-    (q, qt, qh), (k, kt, kh), (v, vt, vh) = rows16(q), rows16(k), rows16(v)
+    (q, qp, qt, qh), (k, kp, kt, kh), (v, vp, vt, vh) = rows16(q), rows16(k), rows16(v)
     ws, floats = None, 0
     if workspace is not None:
         if workspace.dtype != torch.float32 or not workspace.is_contiguous() or workspace.device != device:
@@ -94,16 +94,18 @@ def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, scaling:
         workspace = torch.empty((plan.workspace_floats(d),), dtype=torch.float32, device=device)
     if workspace is not None:
         ws, floats = workspace.data_ptr(), workspace.numel()
-    _lib.call_on(device, "kvq_prompt_attention", q.data_ptr(), qt, qh, k.data_ptr(), kt, kh, v.data_ptr(), vt, vh,
+    _lib.call_on(device, "kvq_prompt_attention", qp, qt, qh, kp, kt, kh, vp, vt, vh,
                  _lib.DTYPE_CODE[dtype], plan.Hq, plan.Hkv, d, float(scaling), plan.words.data_ptr(), plan.items, plan.merges, plan.parts,
                  out.data_ptr(), ws, floats, _lib.stream_of(q))
     return out
 
 
 def rows16(x: torch.Tensor):
-    """x (rows, heads, d) with its row and head strides, or a copy where the kernels cannot read it in 16-byte pieces."""
+    """x (rows, heads, d) with its address, row and head strides, or a copy where the kernels cannot read it in 16-byte
+    pieces."""
+    at = x.data_ptr()
     st, sh, sd = x.stride()
-    if sd != 1 or (st | sh) % 8 or x.data_ptr() % 16 or not 0 <= st < 1 << 24:
+    if sd != 1 or (st | sh) % 8 or at % 16 or not 0 <= st < 1 << 24:
         x = x.detach().clone(memory_format=torch.contiguous_format)
-        st, sh, _ = x.stride()
-    return x, st, sh
+        at, (st, sh, _) = x.data_ptr(), x.stride()
+    return x, at, st, sh
