@@ -107,7 +107,8 @@ class PagedCache:
         return new(self.page, self.d), new(self.d, self.page), new(2, dt=torch.float32)
 
     def _set_addresses(self) -> None:
-        """Of each layer's codes, scales and open blocks; what every call passes."""
+        """Of each layer's codes, scales and open blocks; what every call passes.  Called where the pools are allocated."""
+        self._pool_stream = _lib.stream_of(self.table)
         self._host = tuple(x.ctypes.data for x in (self._lens, self._table, self._refs, self._open, self._account))
         self._index, self._type = self.device.index, _lib.DTYPE_CODE[self.dtype]
         self._fixed = (self.table.data_ptr(), self.max_blocks, self.Hkv, self.d, self.page, CODES[self.code])
@@ -288,9 +289,10 @@ class PagedCache:
                      *[x.data_ptr() for x in src], *[x.data_ptr() for x in (src if pool is None else pool)], self._fixed[0],
                      _lib.stream_of(self.table))
         if pool is not None:
-            stream = torch.cuda.current_stream(self.device)
-            for x in src:                      # may be another stream than the pools': they are read until it gets there
-                x.record_stream(stream)
+            if _lib.stream_of(self.table) != self._pool_stream:
+                stream = torch.cuda.current_stream(self.device)
+                for x in src:                  # on another stream than the pools': they are read until it gets there
+                    x.record_stream(stream)
             (self.kc, self.vc, self.sc), self.pages, self._refs = pool, pages, refs
             self._set_addresses()
         self._generation += 1
