@@ -53,7 +53,7 @@ class Step:
     """New tokens of some slots: ``rows`` packed rows, slot by slot.  Made by ``PagedCache.extend``."""
 
     __slots__ = ("cache", "slots", "counts", "made", "rows", "items", "splits", "run_tokens", "split_tokens", "joins", "fronts", "shares",
-                 "desc", "ptr", "host", "generation", "stamp")
+                 "desc", "ptr", "host", "generation", "pools", "stamp")
 
 
 class PagedCache:
@@ -64,7 +64,8 @@ class PagedCache:
     Calls on one cache run in the order in which they are made: on one stream, or on streams that wait for each other
     (the accounts of slots and pages are on the host and change at once; not thread-safe).  append and paged_decode may be
     captured in a graph, for steps that ``extend(..., into=step)`` writes in front of each replay; the calls that change
-    slots or pages may not."""
+    slots or pages may not.  A captured graph reads and writes the cache's memory and its step's: both have to live as long
+    as it is replayed, and resize() ends its use."""
 
     def __init__(self, layers: int, slots: int, pages: int, max_tokens: int, Hkv: int, d: int, *, page: int = 64,
                  code: str = "int8", dtype: torch.dtype = torch.bfloat16, device="cuda"):
@@ -89,7 +90,8 @@ class PagedCache:
         self._open = np.zeros(self.slots, dtype=np.uint8)
         self._refs = np.zeros(self.pages, dtype=np.int32)
         self._account = np.array([self.pages, 0], dtype=np.int64)   # free pages, none of them below
-        self._generation = 0                   # of the pools
+        self._generation = 0                   # of the pages' places
+        self._pools = 0                        # of the pools
         self._stamp = 0                        # of the slots' lengths
         self._touched = np.zeros(self.slots, dtype=np.int64)        # the stamp when a slot took tokens or was emptied
         self.table = torch.zeros((self.slots, self.max_blocks), dtype=torch.int32, device=self.device)
@@ -151,7 +153,8 @@ class PagedCache:
         """Claim room for counts[i] more tokens (or none) of slots[i] (each slot once): the lowest free page for each
         block that gets full.  Raises KVQError ("decode buffer exhausted") and changes nothing when a slot or the pool is
         full.  ``into``: a step of the same counts whose description is rewritten in place, so that a
-        captured graph of its append and decode runs the new step when it is replayed."""
+        captured graph of its append and decode runs the new step when it is replayed; refused for a step from before a
+        resize(), whose graphs hold pools that are gone."""
         s, c = _ints(slots, "slots"), _ints(counts, "counts")
         if s.shape != c.shape:
             raise ValueError("slots and counts must have the same length")
@@ -162,7 +165,7 @@ class PagedCache:
             if words < 0:
                 raise ValueError("counts must not be negative, and below 2^31")
             st = Step()
-            st.cache = self
+            st.cache, st.pools = self, self._pools
             st.host = np.empty(words, dtype=np.int32)
             st.desc = self.table.new_empty(words)
             st.ptr = st.desc.data_ptr()
@@ -175,6 +178,8 @@ class PagedCache:
                 raise ValueError("a step is rewritten by its own cache only")
             if not np.array_equal(st.counts, c):
                 raise ValueError("a step is rewritten for the same counts only")
+            if st.pools != self._pools:
+                raise ValueError("a step from before resize() is not rewritten: graphs captured with it hold the old pools")
             few = (0, 0)
         # a captured decode joins shared fronts only if it was captured with some
         run_tokens = st.run_tokens if into is None or st.shares else 0
@@ -270,7 +275,8 @@ class PagedCache:
 
     def resize(self, pages: int) -> None:
         """Give the pool ``pages`` pages: those beyond the new end move to the lowest free places, in order, the others
-        keep theirs.  New pools are allocated beside the old ones; graphs that were captured hold the old ones."""
+        keep theirs.  New pools are allocated beside the old ones, whose memory is then given back: graphs captured before may
+        not be replayed any more, and their steps not be rewritten."""
         pages = int(pages)
         if pages < max(1, self.pages - self.free_pages):
             raise ValueError(f"{self.pages - self.free_pages} pages are in use")
@@ -294,6 +300,7 @@ class PagedCache:
                 for x in src:                  # on another stream than the pools': they are read until it gets there
                     x.record_stream(stream)
             (self.kc, self.vc, self.sc), self.pages, self._refs = pool, pages, refs
+            self._pools += 1
             self._set_addresses()
         self._generation += 1
 

@@ -617,3 +617,27 @@ def test_gpu_refusals():
     c.resize(9)
     with pytest.raises(ValueError, match="moved"):
         c.append(0, k, k, step)
+
+
+def test_a_step_is_not_rewritten_after_resize():
+    """The graphs that were captured with a step hold the pools of then, which resize gives back; compact keeps them."""
+    import kvq
+    m = Mirror(slots=2, pages=20, max_tokens=300, Hkv=1, d=64, page=32, seed=31)
+    m.push([0, 1], [70, 40])
+    step, [(k, v)] = m.extend([0, 1], [3, 1])
+    m.cache.append(0, k.cuda(), v.cuda(), step)
+    m.cache.compact()
+    m.model.move(3, 20)
+    step, [(k, v)] = m.extend([0, 1], [3, 1], into=step)
+    m.cache.append(0, k.cuda(), v.cuda(), step)
+    m.cache.resize(30)
+    m.model.move(30, 30)
+    with pytest.raises(ValueError, match="resize"):
+        m.cache.extend([0, 1], [3, 1], into=step)
+    m.check("refused")
+    m.decode(step, 2, what="the last step, over the new pools")
+    step = m.push([0, 1], [3, 1])              # a new one
+    step, [(k, v)] = m.extend([0, 1], [3, 1], into=step)
+    m.cache.append(0, k.cuda(), v.cuda(), step)
+    m.decode(step, 2, what="a new step")
+    m.check("a new step")
