@@ -53,7 +53,7 @@ class Step:
     """New tokens of some slots: ``rows`` packed rows, slot by slot.  Made by ``PagedCache.extend``."""
 
     __slots__ = ("cache", "slots", "counts", "made", "rows", "items", "splits", "run_tokens", "split_tokens", "joins", "fronts", "shares",
-                 "desc", "ptr", "host", "generation", "pools", "stamp")
+                 "desc", "ptr", "host", "generation", "pools", "stamp", "streams")
 
 
 class PagedCache:
@@ -64,8 +64,9 @@ class PagedCache:
     Calls on one cache run in the order in which they are made: on one stream, or on streams that wait for each other
     (the accounts of slots and pages are on the host and change at once; not thread-safe).  append and paged_decode may be
     captured in a graph, for steps that ``extend(..., into=step)`` writes in front of each replay; the calls that change
-    slots or pages may not.  A captured graph reads and writes the cache's memory and its step's: both have to live as long
-    as it is replayed, and resize() ends its use."""
+    slots or pages may not.  Memory that is dropped (a step's, the pools' by resize(), the cache's) is kept until the
+    streams that the calls were made on are done with it.  A captured graph reads and writes the cache's memory and its
+    step's: both have to live as long as it is replayed, and resize() ends its use."""
 
     def __init__(self, layers: int, slots: int, pages: int, max_tokens: int, Hkv: int, d: int, *, page: int = 64,
                  code: str = "int8", dtype: torch.dtype = torch.bfloat16, device="cuda"):
@@ -110,12 +111,26 @@ class PagedCache:
 
     def _set_addresses(self) -> None:
         """Of each layer's codes, scales and open blocks; what every call passes.  Called where the pools are allocated."""
-        self._pool_stream = _lib.stream_of(self.table)
+        self._streams = {_lib.stream_of(self.table)}     # that the pools and the other memory belong to, or are recorded for
         self._host = tuple(x.ctypes.data for x in (self._lens, self._table, self._refs, self._open, self._account))
         self._index, self._type = self.device.index, _lib.DTYPE_CODE[self.dtype]
         self._fixed = (self.table.data_ptr(), self.max_blocks, self.Hkv, self.d, self.page, CODES[self.code])
         parts = [(x.data_ptr(), x.stride(0) * x.element_size()) for x in (self.kc, self.vc, self.sc, self.k_open, self.v_open)]
         self._at = [tuple(p + l * step for p, step in parts) for l in range(self.layers)]
+
+    def _use(self, stream: int, step: Optional[Step] = None) -> None:
+        """The current stream, ``stream``, reads and writes the memory of the cache and of ``step``: what is dropped before it is
+        done is not given out again until then.  (What a graph is captured with has to outlive it in any case.)"""
+        if torch.cuda.is_current_stream_capturing():
+            return
+        current = torch.cuda.current_stream(self.device)
+        if stream not in self._streams:
+            for x in (self.table, self.kc, self.vc, self.sc, self.k_open, self.v_open, self._counters):
+                x.record_stream(current)
+            self._streams.add(stream)
+        if step is not None and stream not in step.streams:
+            step.desc.record_stream(current)
+            step.streams.add(stream)
 
     # ---- what is held ------------------------------------------------------------------------
 
@@ -159,7 +174,7 @@ class PagedCache:
         if s.shape != c.shape:
             raise ValueError("slots and counts must have the same length")
         n, pc = s.size, _address(c)
-        lib = _lib.load()
+        lib, stream = _lib.load(), _lib.stream_of(self.table)
         if into is None:
             words = lib.kvq_pages_step_words(self.page, pc, n)
             if words < 0:
@@ -168,7 +183,7 @@ class PagedCache:
             st.cache, st.pools = self, self._pools
             st.host = np.empty(words, dtype=np.int32)
             st.desc = self.table.new_empty(words)
-            st.ptr = st.desc.data_ptr()
+            st.ptr, st.streams = st.desc.data_ptr(), {stream}
             st.splits = max(n, -(-SPLIT_BLOCKS[self.d] // self.Hkv))
             st.run_tokens = st.split_tokens = 1 << 31
             few = (-(-FEW_BLOCKS // self.Hkv), FEW_UNITS // self.Hkv)
@@ -181,11 +196,13 @@ class PagedCache:
             if st.pools != self._pools:
                 raise ValueError("a step from before resize() is not rewritten: graphs captured with it hold the old pools")
             few = (0, 0)
+            if stream not in st.streams:
+                self._use(stream, st)
         # a captured decode joins shared fronts only if it was captured with some
         run_tokens = st.run_tokens if into is None or st.shares else 0
         _lib.call_on(self.device, "kvq_pages_extend", *self._host, self.slots, self.pages, self.max_blocks, self.page,
                      self.max_tokens, _address(s), pc, n, st.splits, *few, run_tokens, st.split_tokens,
-                     _address(st.host), st.host.size, st.ptr, _lib.stream_of(st.desc))
+                     _address(st.host), st.host.size, st.ptr, stream)
         head = st.host[:11].tolist()
         if into is None:
             # what later steps written into this one keep to: without shared fronts any of them does
@@ -229,8 +246,11 @@ class PagedCache:
         if step.rows == 0:
             return
         (k, kp, kt, kh), (v, vp, vt, vh) = rows16(k), rows16(v)
+        stream = _lib.stream_of(k)
+        if stream not in step.streams or stream not in self._streams:
+            self._use(stream, step)
         _lib.call_on(self.device, "kvq_pages_append", kp, kt, kh, vp, vt, vh, self._type, step.ptr, step.items,
-                     *self._fixed, *self._at[layer], _lib.stream_of(k))
+                     *self._fixed, *self._at[layer], stream)
 
     def rows(self, layer: int, slots: Sequence[int]) -> Tuple[torch.Tensor, torch.Tensor]:
         """All tokens of the slots, one behind the other, as dense rows k, v (tokens, Hkv, d): code times scale, rounded
@@ -241,8 +261,11 @@ class PagedCache:
         total = sum(self._lens.take(s, mode="clip").tolist())
         out = self.k_open.new_empty((2, total, self.Hkv, self.d))
         k, v = out.unbind(0)
+        stream = _lib.stream_of(out)
+        if stream not in self._streams:
+            self._use(stream)
         _lib.call_on(self.device, "kvq_pages_rows", self._host[0], self._host[3], self.slots, _address(s), s.size,
-                     *self._fixed, self._type, *self._at[layer], k.data_ptr(), v.data_ptr(), k.numel(), _lib.stream_of(out))
+                     *self._fixed, self._type, *self._at[layer], k.data_ptr(), v.data_ptr(), k.numel(), stream)
         return k, v
 
     # ---- sequences and pages -----------------------------------------------------------------
@@ -253,9 +276,12 @@ class PagedCache:
         s, t = _ints(src, "src"), _ints(dst, "dst")
         if s.shape != t.shape:
             raise ValueError("src and dst must have the same length")
+        stream = _lib.stream_of(self.table)
+        if stream not in self._streams:
+            self._use(stream)
         _lib.call_on(self.device, "kvq_pages_fork", *self._host[:4], self.slots, self.max_blocks, self.page, _address(s),
                      _address(t), s.size, self.layers, self.Hkv, self.d, self.table.data_ptr(), self.k_open.data_ptr(), self.v_open.data_ptr(),
-                     _lib.stream_of(self.table))
+                     stream)
         self._stamp += 1
         self._touched[t] = self._stamp
 
@@ -289,16 +315,13 @@ class PagedCache:
         pages = self.pages if pool is None else end
         refs = self._refs if pool is None else np.empty(pages, dtype=np.int32)
         place = np.empty(self.pages, dtype=np.int32)
-        src = (self.kc, self.vc, self.sc)
+        src, stream = (self.kc, self.vc, self.sc), _lib.stream_of(self.table)
+        if stream not in self._streams:
+            self._use(stream)
         _lib.call_on(self.device, "kvq_pages_move", *self._host[:3], _address(refs), self._host[4], self.slots, self.pages,
                      pages, end, self.max_blocks, self.page, _address(place), self.layers, self.Hkv, self.d,
-                     *[x.data_ptr() for x in src], *[x.data_ptr() for x in (src if pool is None else pool)], self._fixed[0],
-                     _lib.stream_of(self.table))
+                     *[x.data_ptr() for x in src], *[x.data_ptr() for x in (src if pool is None else pool)], self._fixed[0], stream)
         if pool is not None:
-            if _lib.stream_of(self.table) != self._pool_stream:
-                stream = torch.cuda.current_stream(self.device)
-                for x in src:                  # on another stream than the pools': they are read until it gets there
-                    x.record_stream(stream)
             (self.kc, self.vc, self.sc), self.pages, self._refs = pool, pages, refs
             self._pools += 1
             self._set_addresses()
@@ -336,7 +359,7 @@ def paged_decode(q: torch.Tensor, scaling: float, cache: PagedCache, layer: int,
     if step.cache is not cache or step.stamp != cache._stamp:
         cache.check_step(step, "paged_decode")
     q, qp, qt, qh = rows16(q)
-    Hq, device = shape[1], cache.device
+    Hq, device, stream = shape[1], cache.device, _lib.stream_of(q)
     if out is None:
         out = torch.empty_like(q, memory_format=torch.contiguous_format)
     else:
@@ -347,9 +370,11 @@ def paged_decode(q: torch.Tensor, scaling: float, cache: PagedCache, layer: int,
         workspace = cache.sc.new_empty(paged_workspace_floats(step, Hq, Hkv, d))
     elif workspace.dtype != torch.float32 or not workspace.is_contiguous() or workspace.device != device:
         raise ValueError("workspace must be contiguous float32 on the cache's device")
+    if stream not in step.streams or stream not in cache._streams:
+        cache._use(stream, step)
     table, max_blocks, _, _, page, code = cache._fixed
     _lib.call_on(device, "kvq_paged_decode", qp, qt, qh, cache._type, step.rows, Hq, Hkv, d, float(scaling), step.ptr,
                  step.slots.size, step.splits, step.run_tokens, step.split_tokens, step.joins, table, max_blocks, page,
                  code, *cache._at[layer], out.data_ptr(), workspace.data_ptr(), workspace.numel(),
-                 None if step.shares else cache._tickets[layer], _lib.stream_of(q))
+                 None if step.shares else cache._tickets[layer], stream)
     return out

@@ -641,3 +641,32 @@ def test_a_step_is_not_rewritten_after_resize():
     m.cache.append(0, k.cuda(), v.cuda(), step)
     m.decode(step, 2, what="a new step")
     m.check("a new step")
+
+
+def test_a_step_dropped_before_another_stream_is_done():
+    """Append and decode on a stream that is busy, step and cache gone: what their own stream allocates next is other memory."""
+    import kvq
+    m = Mirror(slots=2, pages=40, max_tokens=1000, Hkv=2, d=64, page=32, seed=32)
+    m.push([0, 1], [600, 40])
+    step, [(k, v)] = m.extend([0, 1], [40, 1])
+    k, v, q = k.cuda(), v.cuda(), m.rand(41, 4).cuda()
+    m.cache.append(0, k, v, step)
+    want, size = kvq.paged_decode(q, 0.125, m.cache, 0, step), step.desc.numel()
+    out, ws = torch.empty_like(want), torch.empty(kvq.paged_workspace_floats(step, 4, 2, 64), device="cuda")
+    x = torch.ones(4096, 4096, device="cuda")
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        for _ in range(20):
+            x = x @ x * 1e-4
+        m.cache.append(0, k, v, step)
+        kvq.paged_decode(q, 0.125, m.cache, 0, step, out=out, workspace=ws)
+    del step
+    held = [torch.zeros(size, dtype=torch.int32, device="cuda") for _ in range(64)]
+    parts = (m.cache.table, m.cache.kc, m.cache.vc, m.cache.sc, m.cache.k_open, m.cache.v_open, m.cache._counters)
+    like = [torch.empty_like(p, device="meta") for p in parts]
+    del parts
+    m.cache = None
+    held += [torch.zeros_like(p, device="cuda") for p in like for _ in range(4)]
+    torch.cuda.synchronize()
+    assert torch.equal(out, want) and not any(bool(h.any()) for h in held)
