@@ -28,7 +28,8 @@ def device_of(device) -> torch.device:
 class PromptPlan:
     """The work of an attention over packed sequences of ``lens`` new tokens each, in front of the last of
     ``lens_k`` keys (as many as the new tokens when not given).  Causal: query t of a sequence sees keys
-    0 .. t + len_k - len; one that sees none gets zeros.  For ``Hq`` query heads over ``Hkv`` KV heads."""
+    0 .. t + len_k - len; one that sees none gets zeros.  For ``Hq`` query heads over ``Hkv`` KV heads.  A plan that is dropped is
+    kept until the streams of its calls are done with it; it has to live as long as a graph captured with it is replayed."""
 
     def __init__(self, lens: Sequence[int], Hq: int, Hkv: int, *, lens_k: Optional[Sequence[int]] = None,
                  causal: bool = True, device="cuda"):
@@ -52,6 +53,7 @@ class PromptPlan:
         _lib.call("kvq_prompt_plan", *args, words.ctypes.data, words.size, info.ctypes.data)
         self.items, self.merges, self.parts = info.tolist()
         self.words = torch.from_numpy(words).to(self.device)
+        self._streams = {_lib.stream_of(self.words)}     # that the words belong to, or are recorded for
 
     def workspace_floats(self, d: int) -> int:
         """Float32 scratch of a call at head_dim ``d``: none where the rows fill the chip without cutting along the keys."""
@@ -94,9 +96,13 @@ def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, scaling:
         workspace = torch.empty((plan.workspace_floats(d),), dtype=torch.float32, device=device)
     if workspace is not None:
         ws, floats = workspace.data_ptr(), workspace.numel()
+    stream = _lib.stream_of(q)
+    if stream not in plan._streams and not torch.cuda.is_current_stream_capturing():
+        plan.words.record_stream(torch.cuda.current_stream(device))
+        plan._streams.add(stream)
     _lib.call_on(device, "kvq_prompt_attention", qp, qt, qh, kp, kt, kh, vp, vt, vh,
                  _lib.DTYPE_CODE[dtype], plan.Hq, plan.Hkv, d, float(scaling), plan.words.data_ptr(), plan.items, plan.merges, plan.parts,
-                 out.data_ptr(), ws, floats, _lib.stream_of(q))
+                 out.data_ptr(), ws, floats, stream)
     return out
 
 

@@ -213,3 +213,24 @@ def test_refusals():
         kvq.prompt_attention(q, k, k, 0.1, plan, out=torch.empty((5, 64, 4), dtype=torch.bfloat16, device="cuda"))
     with pytest.raises(kvq.KVQError):
         kvq.prompt_attention(q.cpu(), k, k, 0.1, plan)
+
+
+def test_a_plan_dropped_before_another_stream_is_done():
+    """A call on a stream that is busy, its plan gone: what the plan's own stream allocates next is other memory."""
+    import kvq
+    lens, lens_k, Hq, Hkv, d = [30, 4], [3000, 70], 4, 2, 64
+    q, k, v = (x.cuda() for x in _inputs(lens, lens_k, Hq, Hkv, d, torch.bfloat16, 65))
+    plan = kvq.PromptPlan(lens, Hq, Hkv, lens_k=lens_k)
+    want, size = kvq.prompt_attention(q, k, v, 0.125, plan), plan.words.numel()
+    out, ws = torch.empty_like(want), torch.empty(plan.workspace_floats(d), device="cuda")
+    x = torch.ones(4096, 4096, device="cuda")
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        for _ in range(20):
+            x = x @ x * 1e-4
+        kvq.prompt_attention(q, k, v, 0.125, plan, out=out, workspace=ws)
+    del plan
+    held = [torch.zeros(size, dtype=torch.int32, device="cuda") for _ in range(64)]
+    torch.cuda.synchronize()
+    assert torch.equal(out, want) and not any(bool(h.any()) for h in held)
