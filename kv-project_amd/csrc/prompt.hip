@@ -132,7 +132,7 @@ __global__ __launch_bounds__(kThreads, 2) void prompt_kernel(PromptArgs a) {
   const int v_at = (xr * static_cast<int>(a.v_st) + (xc ^ v_swz(xr)) * 8) * 2;
   const int wave0 = __builtin_amdgcn_readfirstlane(wave) * 512;     // elements
   // Straight to LDS, 16 bytes a lane, written down here so that it can run beside the transposing reads (the compiler
-  // has those wait for every load to LDS).  No register is written but m0, which nothing else here uses; end() waits.
+  // has those wait for every load to LDS).  m0 is set by the compiler, which so knows of it; end() waits.
   auto fetch = [&](uint16_t* to, const uint16_t* base, int64_t st, int at, int j) KVQ_INLINE {
     // rows behind the last one read as zeros: the buffer ends with the last row
     const int64_t left = keys - static_cast<int64_t>(j) * kTileKeys;
@@ -143,9 +143,9 @@ __global__ __launch_bounds__(kThreads, 2) void prompt_kernel(PromptArgs a) {
     const uint32_t lds = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((lds_void*)(to + wave0)));
 #pragma unroll
     for (int i = 0; i < kPer; ++i)
-      asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
+      asm volatile("s_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
                    :
-                   : "s"(lds + i * kThreads * 16), "v"(at + i * kStep * static_cast<int>(st) * 2), "s"(rsrc)
+                   : "{m0}"(lds + i * kThreads * 16), "v"(at + i * kStep * static_cast<int>(st) * 2), "s"(rsrc)
                    : "memory");
   };
   const int tiles = ((keys + kTileKeys - 1) / kTileKeys) | 1;
