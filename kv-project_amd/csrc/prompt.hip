@@ -375,7 +375,7 @@ __global__ __launch_bounds__(kThreads) void prompt_merge_kernel(PromptArgs a, co
     }
     top = m;
   }
-  const float inv = top == -INFINITY && l == 0.0f ? 0.0f : 1.0f / l;
+  const float inv = 1.0f / l;                 // a tile that was cut has a visible key for every row
   uint16_t* out = a.out + ((w[2] + static_cast<int64_t>(tok)) * a.H * a.rep + h * a.rep + row % a.rep) * D + lane * (D / 64);
 #pragma unroll
   for (int e = 0; e < D / 64; ++e) out[e] = BF16 ? f32_to_bf16(o[e] * inv) : f32_to_f16(o[e] * inv);

@@ -234,3 +234,20 @@ def test_a_plan_dropped_before_another_stream_is_done():
     held = [torch.zeros(size, dtype=torch.int32, device="cuda") for _ in range(64)]
     torch.cuda.synchronize()
     assert torch.equal(out, want) and not any(bool(h.any()) for h in held)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("lens,lens_k", [([40], [40]), ([40], [3040])])
+def test_rows_whose_scores_are_all_minus_infinity(lens, lens_k, dtype):
+    """Visible keys with scores of -inf only leave a row without a sum, a NaN, whether its tile is cut along the keys or not;
+    one finite score takes all the weight."""
+    import kvq
+    q, k, v = _inputs(lens, lens_k, 4, 2, 64, dtype, 61)
+    q[..., 0], k[..., 0] = 1.0, float("-inf")
+    plan = kvq.PromptPlan(lens, 4, 2, lens_k=lens_k)
+    assert bool(plan.parts) == (lens_k[0] > 512)
+    out = kvq.prompt_attention(q.cuda(), k.cuda(), v.cuda(), 0.125, plan)
+    assert torch.isnan(out).all()
+    k[lens_k[0] - 30, :, 0] = 0.0
+    out = kvq.prompt_attention(q.cuda(), k.cuda(), v.cuda(), 0.125, plan).cpu()
+    assert torch.isnan(out[:10]).all() and torch.equal(out[10:], v[-30].repeat_interleave(2, 0).expand(30, -1, -1))
