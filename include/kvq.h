@@ -664,7 +664,8 @@ int kvq_selftest_mfma_layout(const uint16_t* a, const uint16_t* b, float* out, v
  * Packed rows of n sequences: q (sum lens_q, Hq, D), k, v (sum lens_k, Hq / rep, D) of one 16-bit dtype,
  * element strides per row and head, channels contiguous, pointers and strides multiples of 16 bytes; D 64
  * or 128, rep <= 128, row strides below 2^24.  Query t of a sequence sees keys 0 .. t + len_k - len_q (causal), or
- * all of them; one that sees none gets zeros.  out (sum lens_q, Hq, D), contiguous.
+ * all of them; one that sees none gets zeros.  A visible value that is infinite or NaN is its channel's result, whatever its
+ * weight; hidden ones change nothing.  out (sum lens_q, Hq, D), contiguous.
  * kvq_prompt_plan (host memory): fills `words` for a call over such sequences and H KV heads; info[3] = {items,
  * merges, parts}.  8 items + 4 merges words are needed: with less room only info is set.  The words go to the
  * device as they are; they bound what kvq_prompt_attention reads.  workspace: kvq_prompt_workspace floats

@@ -75,6 +75,11 @@ __device__ __forceinline__ void each(F&& f) {
   }
 }
 
+__device__ __forceinline__ bool finite(float x) { return fabsf(x) < INFINITY; }
+
+// A sum times its weight; an infinity or a NaN stays one where the weight has become zero
+__device__ __forceinline__ float weigh(float f, float x) { return finite(x) ? f * x : x; }
+
 struct PromptArgs {
   const uint16_t *q, *k, *v;
   int64_t q_st, q_sh, k_st, k_sh, v_st, v_sh;
@@ -247,7 +252,7 @@ __global__ __launch_bounds__(kThreads, 2) void prompt_kernel(PromptArgs a) {
     if (__builtin_amdgcn_ballot_w64(grow != 1.0f)) each<0, D / 32>([&](auto c) KVQ_INLINE { o[c.value] *= grow; });
   };
   // A value that is hidden from some row may be an infinity or a NaN: in LDS it becomes a zero, and the rows that
-  // do see it get it at the end.  A thread looks at the pieces that it fetched itself.
+  // do see it have it at the end.  A thread looks at the pieces that it fetched itself.
   auto watch = [&](uint16_t* to, int j) KVQ_INLINE {
 #pragma unroll
     for (int i = 0; i < kPer; ++i) {
@@ -310,6 +315,36 @@ __global__ __launch_bounds__(kThreads, 2) void prompt_kernel(PromptArgs a) {
       step(even, j + 1);
     }
     each<0, kV>([&](auto t) KVQ_INLINE { add_v(even, t, read_v(even, t.value)); });
+    // A visible value that is infinite or NaN is its channel's result, however small its weight has become (zero times it would
+    // be a NaN).  In tiles that every row sees it has made the sum infinite or NaN: they are looked through, each lane 8 channels
+    // of every (64 / kRow)-th token (bits e, 8 + e, 16 + e: an infinity, a negative one, a NaN in channel e).  In the others
+    // it was left out of the sum.
+    l = xsum32(l);
+    float all = 0.0f;
+    each<0, D / 32>([&](auto c) KVQ_INLINE { each<0, 16>([&](auto e) KVQ_INLINE { all += o[c.value][e.value]; }); });
+    if (__builtin_amdgcn_ballot_w64(live && l == l && !finite(all))) {
+      uint32_t found = 0;
+#pragma unroll 8
+      for (int r = lane / kRow; r < open * kTileKeys; r += 64 / kRow) {
+        const u32x4 w = *reinterpret_cast<const u32x4*>(vb + r * a.v_st + lane % kRow * 8);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const uint32_t x = w[e / 2] >> (16 * (e % 2)) & 0xffffu;
+          if ((x & kInf) == kInf) found |= 1u << (e + ((x & 0x7fffu) != kInf ? 16 : x >> 15 ? 8 : 0));
+        }
+      }
+#pragma unroll
+      for (int i = kRow; i < 64; i *= 2) found |= __shfl_xor(found, i);
+      each<0, D / 8>([&](auto i) KVQ_INLINE {
+        const uint32_t f = __shfl(found, i.value) >> (4 * g);
+        each<0, 4>([&](auto e) KVQ_INLINE {
+          const bool up = f >> e.value & 1, down = f >> (8 + e.value) & 1, nan = f >> (16 + e.value) & 1;
+          auto& x = o[i.value / 4];
+          constexpr int at = i.value % 4 * 4 + e.value;
+          x[at] = nan || (up && down) ? NAN : up ? INFINITY : down ? -INFINITY : x[at];
+        });
+      });
+    }
     for (int j = open; j < tiles; ++j)
       if (flag[j - open])
         for (int r = j * kTileKeys; r < j * kTileKeys + kTileKeys && r < keys; ++r)
@@ -322,7 +357,6 @@ __global__ __launch_bounds__(kThreads, 2) void prompt_kernel(PromptArgs a) {
   }
 
   if (!live) return;
-  l = xsum32(l);
   const int piece = it[6];
   if (piece >= 0) {
     float* part = a.part + (static_cast<int64_t>(piece) * a.H + h) * (kTileRows * (D + 2));
@@ -365,13 +399,13 @@ __global__ __launch_bounds__(kThreads) void prompt_merge_kernel(PromptArgs a, co
     const float old = __builtin_amdgcn_exp2f(top - safe), f = __builtin_amdgcn_exp2f(st.x - safe);
     l = l * old + wave_sum(f * st.y);
 #pragma unroll
-    for (int e = 0; e < D / 64; ++e) o[e] *= old;
+    for (int e = 0; e < D / 64; ++e) o[e] = weigh(old, o[e]);
     const int most = parts - i0 < 64 ? parts - i0 : 64;
     for (int k = 0; k < most; ++k) {
       const float fk = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(f), k));
       const float* x = part + (i0 + k) * stride + row * D + lane * (D / 64);
 #pragma unroll
-      for (int e = 0; e < D / 64; ++e) o[e] += fk * x[e];
+      for (int e = 0; e < D / 64; ++e) o[e] += weigh(fk, x[e]);
     }
     top = m;
   }

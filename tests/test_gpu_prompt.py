@@ -251,3 +251,38 @@ def test_rows_whose_scores_are_all_minus_infinity(lens, lens_k, dtype):
     k[lens_k[0] - 30, :, 0] = 0.0
     out = kvq.prompt_attention(q.cuda(), k.cuda(), v.cuda(), 0.125, plan).cpu()
     assert torch.isnan(out[:10]).all() and torch.equal(out[10:], v[-30].repeat_interleave(2, 0).expand(30, -1, -1))
+
+
+def _far_query_and_key(q, k, at):
+    """The key ``at`` takes all the weight: by e^400 and more over every other visible one."""
+    q[..., 0], k[..., 0] = 16.0, 0.0
+    k[at, :, 0] = 25.0 * q.shape[2] ** 0.5
+
+
+@pytest.mark.parametrize("far", [False, True])
+@pytest.mark.parametrize("bad", [float("inf"), float("-inf"), float("nan")])
+@pytest.mark.parametrize("dtype,d", [(torch.bfloat16, 64), (torch.bfloat16, 128), (torch.float16, 64), (torch.float16, 128)])
+@pytest.mark.parametrize("t,n,ats", [(300, 300, (10, 130, 299)), (90, 3090, (5, 1000, 2990, 3040))])
+def test_a_visible_infinity_is_its_channels_result(t, n, ats, dtype, d, bad, far):
+    """In tiles that every row sees and in those that some see in part, in whole sequences and in parts, and however small its
+    weight: the rows that see an infinite value have it in that channel, the others and other channels do not change."""
+    import kvq
+    lens, lens_k, Hq, Hkv = [t], [n], 4, 2
+    q, k, v = _inputs(lens, lens_k, Hq, Hkv, d, dtype, 62)
+    if far:
+        _far_query_and_key(q, k, 700 % n)
+    plan = kvq.PromptPlan(lens, Hq, Hkv, lens_k=lens_k)
+    assert bool(plan.parts) == (n > 512)
+    run = lambda x: kvq.prompt_attention(q.cuda(), k.cuda(), x.cuda(), d ** -0.5, plan).cpu()
+    clean = run(v)
+    assert torch.isfinite(clean).all()
+    for at in ats:
+        for channel in (1, d - 1):
+            vb, want = v.clone(), clean.clone()
+            vb[at, 1, channel] = bad
+            want[max(0, at - (n - t)):, 2:, channel] = bad
+            assert torch.equal(torch.nan_to_num(run(vb), 7.0, 8.0, 9.0), torch.nan_to_num(want, 7.0, 8.0, 9.0)), (at, channel)
+    vb = v.clone()
+    vb[0, 0, 3], vb[n - t // 2, 0, 3] = float("inf"), float("-inf")
+    out = run(vb)[:, :2, 3]
+    assert torch.isposinf(out[:t - t // 2]).all() and torch.isnan(out[t - t // 2:]).all()
