@@ -734,7 +734,8 @@ int kvq_pages_move(const int64_t* lens, int32_t* table, const int32_t* refs, int
 
 /* ------------------------------------------------------------------------------------------
  * Attention of a step's query rows over the paged cache: q (rows, Hq, D), the step's rows in order; query
- * i of a sequence with `count` new tokens sees all tokens up to its own.  sequences: of the step; split_items,
+ * i of a sequence with `count` new tokens sees all tokens up to its own; a visible value of the open block that is infinite
+ * or NaN is its channel's result, whatever its weight.  sequences: of the step; split_items,
  * run_tokens and split_tokens: at least the description's third, seventh and eighth word; they give the grid and the
  * workspace.  joins: its eleventh word, or 1: results of several split items are joined; without, no workspace is
  * needed.  out (rows, Hq, D) contiguous.  workspace: kvq_paged_decode_workspace floats, no clearing; calls that share

@@ -90,6 +90,10 @@ __device__ __forceinline__ float row_max16(float x) {
 __device__ __forceinline__ float wave_sum(float x) { return xsum32(xsum16(row_sum16(x))); }
 __device__ __forceinline__ float wave_max(float x) { return xmax32(xmax16(row_max16(x))); }
 
+__device__ __forceinline__ bool finite(float x) { return fabsf(x) < INFINITY; }
+// A sum times its weight; an infinity or a NaN stays one where the weight has become zero
+__device__ __forceinline__ float weigh(float f, float x) { return finite(x) ? f * x : x; }
+
 __device__ __forceinline__ uint32_t pack_h2(_Float16 a, _Float16 b) {
   return static_cast<uint32_t>(__builtin_bit_cast(uint16_t, a)) |
          (static_cast<uint32_t>(__builtin_bit_cast(uint16_t, b)) << 16);

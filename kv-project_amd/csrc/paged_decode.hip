@@ -144,7 +144,7 @@ struct Join {
         for (int k = 0; k < DEEP; ++k) {
           const float fk = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(f[n]), k0 + k < most ? k0 + k : 0));
 #pragma unroll
-          for (int e = 0; e < D / 64; ++e) j.o[n][e] += k0 + k < most ? fk * x[n][k][e] : 0.0f;
+          for (int e = 0; e < D / 64; ++e) j.o[n][e] += k0 + k < most ? weigh(fk, x[n][k][e]) : 0.0f;
         }
     }
   };
@@ -180,7 +180,7 @@ struct Join {
         f[n] = __builtin_amdgcn_exp2f(st[n].x - safe);
         l[n] = l[n] * old + wave_sum(f[n] * st[n].y);
 #pragma unroll
-        for (int e = 0; e < D / 64; ++e) o[n][e] *= old;
+        for (int e = 0; e < D / 64; ++e) o[n][e] = weigh(old, o[n][e]);
         top[n] = m;
       }
       early.add_to(*this, 0, most, f);
@@ -434,7 +434,8 @@ __global__ __launch_bounds__(kThreads, 3) void paged_split_kernel(DecodeArgs a) 
       else split_f16(t, 8 * e, hi[e], lo[e]);
     }
     // what lies behind the sequence or is hidden from a row may be an infinity or a NaN: it goes in as zero, and
-    // the rows that do see such a value get it afterwards
+    // the rows that do see such a value have it in that channel, however small its weight: a wavefront has one unit of the open
+    // block at most, its last, and the joins keep it
     constexpr uint32_t kInf = BF16 ? 0x7f80u : 0x7c00u;
     const uint32_t at = col * P + (off + 16 * g < P ? off + 16 * g : 0);
     uint32_t worst = 0;
@@ -490,7 +491,7 @@ __global__ __launch_bounds__(kThreads, 3) void paged_split_kernel(DecodeArgs a) 
     const float f = __builtin_amdgcn_exp2f(stat[i][r][0] - safe);
     l += f * stat[i][r][1];
 #pragma unroll
-    for (int e = 0; e < kPer; ++e) o[e] += f * join[i][r][c0 + e];
+    for (int e = 0; e < kPer; ++e) o[e] += weigh(f, join[i][r][c0 + e]);
   }
   const int R = piece * kRows + r;
   const int64_t Hq = static_cast<int64_t>(a.H) * a.rep;
@@ -589,7 +590,7 @@ __global__ __launch_bounds__(kThreads) void paged_merge_kernel(DecodeArgs a, int
       const float f = __builtin_amdgcn_exp2f(stats[i][0] - safe);
       j.l[0] += f * stats[i][1];
 #pragma unroll
-      for (int e = 0; e < D / 64; ++e) j.o[0][e] += f * sums[i][lane * (D / 64) + e];
+      for (int e = 0; e < D / 64; ++e) j.o[0][e] += weigh(f, sums[i][lane * (D / 64) + e]);
     }
   }
   j.template put<BF16>(0, a.out + at * D);

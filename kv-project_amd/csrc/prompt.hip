@@ -75,11 +75,6 @@ __device__ __forceinline__ void each(F&& f) {
   }
 }
 
-__device__ __forceinline__ bool finite(float x) { return fabsf(x) < INFINITY; }
-
-// A sum times its weight; an infinity or a NaN stays one where the weight has become zero
-__device__ __forceinline__ float weigh(float f, float x) { return finite(x) ? f * x : x; }
-
 struct PromptArgs {
   const uint16_t *q, *k, *v;
   int64_t q_st, q_sh, k_st, k_sh, v_st, v_sh;

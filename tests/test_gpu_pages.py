@@ -670,3 +670,41 @@ def test_a_step_dropped_before_another_stream_is_done():
     held += [torch.zeros_like(p, device="cuda") for p in like for _ in range(4)]
     torch.cuda.synchronize()
     assert torch.equal(out, want) and not any(bool(h.any()) for h in held)
+
+
+@pytest.mark.parametrize("bad", [float("inf"), float("-inf")])
+@pytest.mark.parametrize("page,d,dtype", [(32, 64, torch.bfloat16), (64, 128, torch.float16), (128, 64, torch.bfloat16), (128, 128, torch.float16)])
+def test_a_visible_infinity_of_the_open_block_stays(page, d, dtype, bad):
+    """However small its weight beside what other tokens, wavefronts and items hold: the rows that see it have it in that
+    channel.  Joined in the launch, by a launch, and behind a shared front."""
+    import kvq
+    m = Mirror(slots=4, pages=160, max_tokens=30 * page + 10, Hkv=1, d=d, page=page, dtype=dtype, seed=33)
+    n = 23 * page + page - 4                   # page - 4 tokens in the open block, then three more
+    for big in (3, 12 * page, 23 * page + 1, 23 * page + page - 5, n + 2):
+        step, [(k, v)] = m.extend([0], [n])
+        k[..., 0] = 0
+        if big < n:
+            k[big, :, 0] = 25.0 * d ** 0.5
+        at = 23 * page + (0 if big % 2 else page - 6)
+        vb = v.clone()
+        vb[at, :, 5] = bad
+        m.cache.append(0, k.cuda(), vb.cuda(), step)
+        m.fork([0], [1])
+        for slots, counts in (([0], [1]), ([1], [2]), ([0, 1], [2, 1])):
+            step, [(k, v)] = m.extend(slots, counts)
+            k[..., 0] = 0
+            if big >= n:
+                k[:, :, 0] = 25.0 * d ** 0.5
+            m.cache.append(0, k.cuda(), v.cuda(), step)
+            q = m.rand(sum(counts), 4)
+            q[..., 0] = 16.0
+            tickets = m.cache._tickets
+            for way in (tickets, [None]):
+                m.cache._tickets = way
+                out = kvq.paged_decode(q.cuda(), d ** -0.5, m.cache, 0, step).float()
+                what = (big, at, slots, way[0] is None)
+                assert (out[..., 5] == bad).all(), what
+                assert torch.isfinite(out[..., :5]).all() and torch.isfinite(out[..., 6:]).all(), what
+            m.cache._tickets = tickets
+        assert step.fronts
+        m.free([0, 1])
