@@ -8,7 +8,8 @@
 // O^T += V^T P^T.  The accumulator layout of S^T is the operand layout of P^T once V^T takes its tokens in
 // the same order, so probabilities never leave their lanes: V^T comes from LDS by transposing reads.
 // Probabilities are rounded to the inputs' type (half a step of the output's type); the sums, the
-// references and the accumulators are float32.
+// references and the accumulators are float32.  fp16 has no room below 2^-24: there the reference weighs 2^7, so that
+// weights lose at most 2^-32 of it (200000 keys of 2^-26 each, 0.3% of the sum, were zeros without).
 //
 // Where the rows are too few to fill the chip, a tile of rows is cut along its keys into parts, each
 // with its own sums, and prompt_merge_kernel joins them in order.
@@ -167,6 +168,7 @@ __global__ __launch_bounds__(kThreads, 2) void prompt_kernel(PromptArgs a) {
   };
   // the softmax of tile j in 18 shares: 0 and 1 find the reference, 2 + i the weights 2 i, 2 i + 1.
   // register 16 x + 4 b + e of lane half g: token 32 x + 8 b + 4 g + e
+  constexpr float kLift = BF16 ? 0.0f : 7.0f; // log2 of the reference's weight
   float top, safe, sum;
   auto share = [&](auto par, bool masked, int j, auto which) KVQ_INLINE {
     constexpr int i = decltype(which)::value;
@@ -180,12 +182,13 @@ __global__ __launch_bounds__(kThreads, 2) void prompt_kernel(PromptArgs a) {
       each<1, 16>([&](auto e) KVQ_INLINE { x = fmaxf(x, t[i][e.value]); });
       top = x;
       if constexpr (i == 1) {
-        // the reference moves only when a score passes it by 2^8: weights up to 256 cost no accuracy, and the
+        // the reference moves only when a score passes it by 2^8: weights up to 256 (fp16: 2^15) cost no accuracy, and the
         // accumulators are hardly ever scaled
         x = xmax32(x) * a.scale;
         x = x > m + 8.0f ? x : m;
         safe = x == -INFINITY ? 0.0f : x;
         grow = __builtin_amdgcn_exp2f(m - safe);
+        safe -= kLift;
         m = x;
         sum = 0.0f;
       }

@@ -1,5 +1,7 @@
 """Attention over packed prompts against the float64 oracle: lengths from none to many, chunks behind a past,
 rows without a key, grouped heads, strides, values that a row must not see, replays and other streams."""
+import math
+
 import pytest
 import torch
 
@@ -286,3 +288,23 @@ def test_a_visible_infinity_is_its_channels_result(t, n, ats, dtype, d, bad, far
     vb[0, 0, 3], vb[n - t // 2, 0, 3] = float("inf"), float("-inf")
     out = run(vb)[:, :2, 3]
     assert torch.isposinf(out[:t - t // 2]).all() and torch.isnan(out[t - t // 2:]).all()
+
+
+def test_many_small_fp16_weights():
+    """A key without a value takes nearly all the weight, 200000 keys of value one 2^-26 of it each: 0.003 together, in tiles
+    that are not cut."""
+    import kvq
+    t, n, d = 600, 200000, 64
+    q, k, v = torch.zeros(t, 128, d), torch.zeros(n, 1, d), torch.ones(n, 1, d)
+    q[..., 0], k[0, :, 0], v[0] = 1.0, 26.0, 0.0
+    q, k, v = (x.half().cuda() for x in (q, k, v))
+    plan = kvq.PromptPlan([t], 128, 1, lens_k=[n])
+    assert plan.items == t and not plan.parts
+    out = kvq.prompt_attention(q, k, v, math.log(2.0), plan).double().cpu()
+    w = torch.arange(n - t, n, dtype=torch.float64)[:, None, None] * 2.0 ** -26
+    # a weight of 2^-26 is rounded by 2^-6 of itself at most (2^-25 as a number of the type, 2^-19 with the reference at 2^7), the
+    # sums by n roundings each, the result by half a step
+    tol = 2.0 ** -6 + 2 * n * 2.0 ** -24 + 2.0 ** -11
+    worst = float((out / (w / (1 + w)) - 1).abs().max())
+    print(f"relative error {worst:.2e}, bound {tol:.2e}")
+    assert worst <= tol
