@@ -801,8 +801,8 @@ extern "C" int kvq_pages_move(const int64_t* lens, int32_t* table, const int32_t
                   end >= 0 && end <= pages_to,
               "kvq_pages_move: bad sizes");
   KVQ_REQUIRE(!table_device || (kc && vc && sc && kc_to && vc_to && sc_to), "kvq_pages_move: null pointer");
-  const bool same = kc == kc_to;
-  KVQ_REQUIRE(!same || (pages == pages_to && refs == refs_to), "kvq_pages_move: one pool has one size");
+  const bool same = refs == refs_to;          // the pools may be null where only the accounts move
+  KVQ_REQUIRE((!same || pages == pages_to) && (!table_device || same == (kc == kc_to)), "kvq_pages_move: one pool has one size");
   int64_t used = 0;
   for (int64_t p = 0; p < pages; ++p) used += refs[p] != 0;
   KVQ_REQUIRE(used <= end, "kvq_pages_move: %lld pages are in use", static_cast<long long>(used));

@@ -282,3 +282,26 @@ def test_kernel_entries_refuse_before_any_launch():
     rc = lib.kvq_paged_decode(one, 256, 64, 2, 1, 4, 2, 64, 0.1, one, 1, 4, 1, 4, 1, one, 4, 64, 0, one, one, one, one, one, one, one, need - 1, None, None)
     assert rc == 1 and b"workspace" in lib.kvq_last_error()
     assert lib.kvq_paged_decode_workspace(4, 2, 2, 96) == -1
+
+
+def test_accounts_move_without_a_device():
+    """Without a table on the device the pools are not looked at: null ones do, for one pool and for another."""
+    host, model = Host(3, 20, 640, 64), Accounts(3, 20, 64)
+    for f in (host, model):
+        f.extend([0, 1, 2], [200, 300, 130])
+        f.free([0])
+    for end, pages, same in ((6, 20, True), (9, 9, False), (30, 30, False)):
+        place, refs = np.zeros(len(host.refs), np.int32), host.refs if same else np.zeros(pages, np.int32)
+        assert host.lib.kvq_pages_move(*host.p[:3], refs.ctypes.data, host.p[4], 3, host.pages, pages, end, host.blocks, 64,
+                                       place.ctypes.data, 1, 1, 64, *[None] * 8) == 0, host.error()
+        host.refs, host.pages = refs, pages
+        host.p[2] = refs.ctypes.data
+        model.move(end, pages)
+        host.same(model)
+    # one pool of two sizes, or in two places
+    place, refs = np.zeros(30, np.int32), np.zeros(30, np.int32)
+    for to, pages, kc, kc_to in ((host.refs, 31, 16, 16), (host.refs, 30, 16, 32), (refs, 30, 16, 16)):
+        assert host.lib.kvq_pages_move(*host.p[:3], to.ctypes.data, host.p[4], 3, 30, pages, 30, host.blocks, 64, place.ctypes.data, 1, 1,
+                                       64, kc, kc, kc, kc_to, kc_to, kc_to, 16, None) == 1
+        assert b"one size" in host.error()
+    host.same(model)
