@@ -36,7 +36,8 @@ class PagedCtl:
 
     def begin(self, counts: Union[int, Sequence[int]]) -> None:
         """Claim the next step: ``counts`` new tokens of every sequence, or of each one (in a batch padded on the left:
-        the last counts[b] tokens of row b are its own).  Once per forward pass, before it."""
+        the last counts[b] tokens of row b are its own).  Once per forward pass, before it: a layer that comes a second time
+        in a step is refused, its tokens would take the places of the first ones."""
         n = [int(counts)] * len(self.slots) if isinstance(counts, int) else [int(c) for c in counts]
         if len(n) != len(self.slots):
             raise ValueError("counts must be one number or one per sequence")
@@ -45,6 +46,7 @@ class PagedCtl:
         self.step = self.cache.extend(self.slots, n)
         self.counts, self.lens, self.fresh = n, [a + b for a, b in zip(before, n)], not any(before)
         self.plan = self.index = None
+        self.seen = set()                      # layers that have appended the step
 
     def _plan(self, Hq: int, lens_k) -> PromptPlan:
         if self.plan is None or self.plan.Hq != Hq:           # one for all layers of the step
@@ -71,8 +73,11 @@ class PagedCtl:
         scaling = kwargs.get("scaling")
         scaling = module.scaling if scaling is None else scaling
         layer, cache = module.layer_idx, self.cache
+        if layer in self.seen:
+            raise RuntimeError(f"PagedCtl: layer {layer} has had this step; begin() claims one for each forward pass")
         qp, kp, vp = (self._packed(x, T) for x in (q, k, v))
         cache.append(layer, kp, vp, self.step)
+        self.seen.add(layer)
         if self.fresh:
             out = prompt_attention(qp, kp, vp, scaling, self._plan(Hq, None))
         elif Hq // cache.Hkv * max(self.counts) < MANY_ROWS:

@@ -121,3 +121,25 @@ def test_a_model_through_the_router():
     assert torch.equal(one, two)
     assert torch.isfinite(got).all() and got.shape == want.shape
     print("logits: largest difference", float((got - want).abs().max()), "of", float(want.abs().max()))
+
+
+def test_a_forward_pass_without_begin():
+    """A layer that comes a second time in a step is refused, and the step's rows stay; begin claims the next one."""
+    import kvq
+    cache = kvq.PagedCache(2, 2, 10, 300, 2, 64)
+    ctl = kvq.PagedCtl(cache, [0, 1])
+    g = torch.Generator().manual_seed(1)
+    q, k, v = (torch.randn(2, h, 3, 64, generator=g).bfloat16().cuda() for h in (4, 2, 2))
+    layers = [SimpleNamespace(layer_idx=l, scaling=0.125) for l in (0, 1)]
+    for _ in range(2):
+        ctl.begin(3)
+        with pytest.raises(ValueError):
+            ctl.attend(layers[0], q[:, :, :2], k[:, :, :2], v[:, :, :2], None, {})
+        for m in layers:                       # the one that was refused has not come yet
+            ctl.attend(m, q, k, v, None, {})
+        held = [x.clone() for l in (0, 1) for x in cache.rows(l, [0, 1])]
+        for m in layers:
+            with pytest.raises(RuntimeError, match="begin"):
+                ctl.attend(m, q, -k, -v, None, {})
+        assert all(torch.equal(a, b) for a, b in zip(held, [x for l in (0, 1) for x in cache.rows(l, [0, 1])]))
+    assert cache.lengths == [6, 6]
