@@ -4,7 +4,7 @@
 registered under ``kvq.register()`` (STRATA_KV.py:495-523) on the slots of the cache: each layer's new keys
 and values are appended to its pages, and its queries attend
 
-* over the prompt itself (prompt_attention, exact keys and values) where all of the sequences begin,
+* over the prompt itself (prompt_attention, exact keys and values) where a sequence begins, whoever else is in the batch,
 * over the cache by ``paged_decode`` in steps of a few tokens,
 * over the cache's rows by ``rows`` and prompt_attention in steps of many tokens (a further question, a chunk of
   a prompt): the same attention as paged_decode's, with the codes read once rather than once per 16 query rows.
@@ -13,6 +13,7 @@ Layer ``module.layer_idx`` of the model is layer ``layer_idx`` of the cache.
 """
 from __future__ import annotations
 
+import itertools
 from typing import Sequence, Union
 
 import torch
@@ -44,14 +45,25 @@ class PagedCtl:
         before = [self.cache.length(s) for s in self.slots]
         self.step = None                       # none is left if this one does not fit
         self.step = self.cache.extend(self.slots, n)
-        self.counts, self.lens, self.fresh = n, [a + b for a, b in zip(before, n)], not any(before)
-        self.plan = self.index = None
+        self.counts, self.lens = n, [a + b for a, b in zip(before, n)]
+        self.begins, self.runs = ([b for b, c in enumerate(n) if c and bool(before[b]) == held] for held in (False, True))
+        self.plans, self.index, self.own = {}, None, None
         self.seen = set()                      # layers that have appended the step
 
-    def _plan(self, Hq: int, lens_k) -> PromptPlan:
-        if self.plan is None or self.plan.Hq != Hq:           # one for all layers of the step
-            self.plan = PromptPlan(self.counts, Hq, self.cache.Hkv, lens_k=lens_k, device=self.cache.device)
-        return self.plan
+    def _plan(self, Hq: int, which, lens_k) -> PromptPlan:
+        key = (Hq, lens_k is None)                            # one for all layers of the step
+        if key not in self.plans:
+            self.plans[key] = PromptPlan([self.counts[b] for b in which], Hq, self.cache.Hkv, device=self.cache.device,
+                                         lens_k=None if lens_k is None else [lens_k[b] for b in which])
+        return self.plans[key]
+
+    def _rows_of(self, which, device):
+        """The packed rows of some of the sequences: a slice where they lie behind one another."""
+        first = [0, *itertools.accumulate(self.counts)]
+        parts = [(first[b], first[b + 1]) for b in which]
+        if all(x[1] == y[0] for x, y in zip(parts, parts[1:])):
+            return slice(parts[0][0], parts[-1][1])
+        return torch.cat([torch.arange(*x) for x in parts]).to(device)
 
     def _packed(self, x: torch.Tensor, T: int) -> torch.Tensor:
         """(B, H, T, d) -> the sequences' own rows (rows, H, d)."""
@@ -78,14 +90,28 @@ class PagedCtl:
         qp, kp, vp = (self._packed(x, T) for x in (q, k, v))
         cache.append(layer, kp, vp, self.step)
         self.seen.add(layer)
-        if self.fresh:
-            out = prompt_attention(qp, kp, vp, scaling, self._plan(Hq, None))
-        elif Hq // cache.Hkv * max(self.counts) < MANY_ROWS:
-            out = paged_decode(qp, scaling, cache, layer, self.step)
-        else:
-            out = prompt_attention(qp, *cache.rows(layer, self.slots), scaling, self._plan(Hq, self.lens))
+        few = Hq // cache.Hkv * max(self.counts) < MANY_ROWS
+        if not self.runs:
+            out = prompt_attention(qp, kp, vp, scaling, self._plan(Hq, self.begins, None))
+        elif not self.begins:
+            out = paged_decode(qp, scaling, cache, layer, self.step) if few else self._over_rows(qp, scaling, layer)
+        else:                                  # each kind of sequence its own way
+            if self.own is None:
+                self.own = [self._rows_of(which, q.device) for which in (self.begins, self.runs)]
+            begins, runs = self.own
+            if few:
+                out = paged_decode(qp, scaling, cache, layer, self.step)
+            else:
+                out = torch.empty_like(qp)
+                out[runs] = self._over_rows(qp[runs], scaling, layer)
+            out[begins] = prompt_attention(qp[begins], kp[begins], vp[begins], scaling, self._plan(Hq, self.begins, None))
         if self.index is None:
             return out.view(B, T, Hq, d), None
         whole = torch.zeros((B * T, Hq, d), dtype=out.dtype, device=out.device)
         whole.index_copy_(0, self.index, out)
         return whole.view(B, T, Hq, d), None
+
+    def _over_rows(self, q: torch.Tensor, scaling: float, layer: int) -> torch.Tensor:
+        """The running sequences' rows q over the cache's rows, read back."""
+        k, v = self.cache.rows(layer, [self.slots[b] for b in self.runs])
+        return prompt_attention(q, k, v, scaling, self._plan(q.shape[1], self.runs, self.lens))

@@ -143,3 +143,38 @@ def test_a_forward_pass_without_begin():
                 ctl.attend(m, q, -k, -v, None, {})
         assert all(torch.equal(a, b) for a, b in zip(held, [x for l in (0, 1) for x in cache.rows(l, [0, 1])]))
     assert cache.lengths == [6, 6]
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("counts", [[1, 70, 0, 131], [1, 5, 0, 6], [60, 33, 2, 8], [0, 70, 0, 3]])
+def test_prompts_that_begin_beside_running_sequences(counts, dtype):
+    """A prompt attends its own exact keys, whoever else is in the batch; the running sequences attend what the cache holds."""
+    import kvq
+    from kvq.paged_ctl import MANY_ROWS
+    Hq, Hkv, d = 8, 2, 64
+    cache = kvq.PagedCache(1, 4, 40, 500, Hkv, d, page=32, dtype=dtype)
+    ctl = kvq.PagedCtl(cache, [3, 0, 1, 2])    # slots 3 and 1 hold tokens when the others begin
+    g = torch.Generator().manual_seed(5)
+    rand = lambda T: tuple(torch.randn(4, h, T, d, generator=g).to(dtype) for h in (Hq, Hkv, Hkv))
+    m = SimpleNamespace(layer_idx=0, scaling=0.125)
+    first = [90, 0, 40, 0]
+    held = []
+    for c in (first, counts):
+        T = max(c)
+        q, k, v = rand(T)
+        ctl.begin(c)
+        out, _ = ctl.attend(m, q.cuda(), k.cuda(), v.cuda(), None, {})
+        held.append((k, v))
+    many = Hq // Hkv * max(counts) >= MANY_ROWS
+    for b, n in enumerate(counts):
+        if n == 0:
+            continue
+        kk, vv = (x[b].transpose(0, 1)[T - n:] for x in (k, v))
+        if first[b]:
+            kk, vv = (cached(torch.cat([x[b].transpose(0, 1)[90 - first[b]:], y]), 32, "int8") for x, y in zip(held[0], (kk, vv)))
+            if many:
+                kk, vv = kk.to(dtype), vv.to(dtype)
+        weight = PAIR if first[b] and not many else HALF[dtype]
+        check(out[b, T - n:], attend(q[b].transpose(0, 1)[T - n:], kk, vv, 0.125), float(vv.abs().max()), kk.shape[0], d, dtype,
+              weight, f"sequence {b}: {n} behind {first[b]}")
+        assert not out[b, :T - n].any()
