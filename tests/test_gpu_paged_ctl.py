@@ -178,3 +178,79 @@ def test_prompts_that_begin_beside_running_sequences(counts, dtype):
         check(out[b, T - n:], attend(q[b].transpose(0, 1)[T - n:], kk, vv, 0.125), float(vv.abs().max()), kk.shape[0], d, dtype,
               weight, f"sequence {b}: {n} behind {first[b]}")
         assert not out[b, :T - n].any()
+
+
+class Kept:
+    """The router's controller as it should be, on the CPU: every step attends over what a paged cache holds by then, the first one
+    over its own keys.  ``mistake``: one that the comparison has to see."""
+
+    def __init__(self, page, mistake=None, dtype=torch.bfloat16):
+        self.page, self.mistake, self.dtype, self.held = page, mistake, dtype, {}
+
+    def attend(self, module, q, k, v, mask, kwargs):
+        kv = [x.to(self.dtype).transpose(1, 2) for x in (k, v)]        # (B, T, H, d)
+        layer = module.layer_idx
+        if self.mistake == "layer" and layer in self.held:
+            layer = 1 - layer
+        first = layer not in self.held
+        past = [] if first else self.held[layer]
+        self.held[layer] = kv = kv if first else [torch.cat(x, 1) for x in zip(past, kv)]
+        out = []
+        for b in range(q.shape[0]):
+            kk, vv = (x[b].double() if first else cached(x[b], self.page, "int8") for x in kv)
+            if self.mistake == "heads":
+                kk, vv = kk.flip(1), vv.flip(1)
+            if self.mistake == "offset" and not first:
+                kk, vv = kk[:-1], vv[:-1]
+            scaling = module.scaling * (0.5 if self.mistake == "scaling" else 1.0)
+            out.append(attend(q[b].transpose(0, 1), kk, vv, scaling)[0])
+        return torch.stack(out).to(q.dtype), None
+
+
+def test_a_models_logits_through_the_router():
+    """The logits of a small bf16 model through the paged cache, prompt and later steps, lie as near those of the same weights in
+    float32 with attention in 64 bits as the logits of bf16 arithmetic with SDPA do: both carry the same roundings, so within
+    twice their largest distance.  Mistakes move the logits by four times that and more."""
+    import kvq
+    name = kvq.register()
+    exact_sdpa, exact = (x.float() for x in _small_models(name))
+    ids = torch.randint(0, 97, (2, 150), generator=torch.Generator().manual_seed(7))
+    cuts = ((0, 140), (140, 141), (141, 145), (145, 150))
+
+    def steps(model, ctl, device):
+        logits = []
+        with torch.no_grad(), kvq.routed(ctl):
+            for a, b in cuts:
+                if hasattr(ctl, "begin"):
+                    ctl.begin(b - a)
+                pos = torch.arange(a, b, device=device).expand(2, -1)
+                logits.append(model(input_ids=ids[:, a:b].to(device), position_ids=pos, use_cache=False).logits.double().cpu())
+        return torch.cat(logits, 1)
+
+    with torch.no_grad():
+        plain = exact_sdpa(input_ids=ids, use_cache=False).logits.double()
+    # the oracle's prompt is SDPA's, where it keeps float32 keys and values
+    assert float((steps(exact, Kept(32, dtype=torch.float32), "cpu") - plain)[:, :140].abs().max()) < 1e-4
+    want = steps(exact, Kept(32), "cpu")
+    whole, parts = (x.cuda() for x in _small_models(name))
+    with torch.no_grad():
+        near = whole(input_ids=ids.cuda(), use_cache=False).logits.double().cpu()
+    got = steps(parts, kvq.PagedCtl(kvq.PagedCache(2, 2, 12, 300, 2, 64, page=32), [0, 1]), "cuda")
+    noise = float((near - plain).abs().max())
+    first, later = (float((got - want)[:, s].abs().max()) for s in (slice(0, 140), slice(140, 150)))
+    print(f"bf16 arithmetic {noise:.4f}, prompt {first:.4f}, later steps {later:.4f}")
+    assert max(first, later) <= 2 * noise
+    for mistake in ("layer", "heads", "offset", "scaling"):            # what these bounds can tell
+        wrong = float((steps(exact, Kept(32, mistake), "cpu") - want)[:, 140:].abs().max())
+        print(f"{mistake}: {wrong:.4f}")
+        assert wrong > 4 * noise, mistake
+
+
+def _small_models(name):
+    from transformers import LlamaConfig, LlamaForCausalLM
+    torch.manual_seed(0)
+    cfg = LlamaConfig(vocab_size=97, hidden_size=256, intermediate_size=320, num_hidden_layers=2, num_attention_heads=4,
+                      num_key_value_heads=2, head_dim=64, max_position_embeddings=512, initializer_range=0.05)
+    models = [LlamaForCausalLM._from_config(cfg, attn_implementation=a, dtype=torch.bfloat16).eval() for a in ("sdpa", name)]
+    models[1].load_state_dict(models[0].state_dict())
+    return models
