@@ -308,3 +308,36 @@ def test_many_small_fp16_weights():
     worst = float((out / (w / (1 + w)) - 1).abs().max())
     print(f"relative error {worst:.2e}, bound {tol:.2e}")
     assert worst <= tol
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("t,n,Hq,Hkv,d", [(600, 20000, 128, 1, 64), (530, 4333, 128, 1, 128), (1050, 1050, 64, 1, 64)])
+def test_long_loops_of_many_tiles(t, n, Hq, Hkv, d, dtype):
+    """More tiles of rows than places, so that each goes over all of its keys: up to 313 key tiles a workgroup, the largest
+    score early, late and in between."""
+    import kvq
+    q, k, v = _inputs([t], [n], Hq, Hkv, d, dtype, 63)
+    plan = kvq.PromptPlan([t], Hq, Hkv, lens_k=[n])
+    assert plan.items * Hkv > 512 and not plan.parts
+    rows = [0, 1, t // 2, t - 2, t - 1]
+    for i, at in zip(rows, (n - t, 100, n - t, n - t + t // 2, 0)):
+        k[at] = 6 * q[i, 0] / q[i, 0].norm()
+        q[i] = q[i] * 4
+    out = kvq.prompt_attention(q.cuda(), k.cuda(), v.cuda(), d ** -0.5, plan)
+    for i in rows:
+        m = n - t + i + 1
+        check(out[i:i + 1], attend(q[i:i + 1], k[:m], v[:m], d ** -0.5), float(v[:m].abs().max()), m, d, dtype, HALF[dtype], f"row {i}")
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("late", [0, 12000, 39990])
+def test_more_parts_than_a_wavefront_has_lanes(late, dtype):
+    """A tile in more than 64 parts, joined in two rounds of maxima, the largest score in an early and in a late one."""
+    import kvq
+    n, d = 40000, 128
+    q, k, v = _inputs([1], [n], 4, 1, d, dtype, 64)
+    k[late] = 30 * q[0, 0] / q[0, 0].norm()
+    plan = kvq.PromptPlan([1], 4, 1, lens_k=[n])
+    assert plan.merges == 1 and plan.parts > 64
+    out = kvq.prompt_attention(q.cuda(), k.cuda(), v.cuda(), d ** -0.5, plan)
+    _check(out, q, k, v, [1], [n], True, dtype, f"late {late}")
