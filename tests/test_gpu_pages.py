@@ -708,3 +708,52 @@ def test_a_visible_infinity_of_the_open_block_stays(page, d, dtype, bad):
             m.cache._tickets = tickets
         assert step.fronts
         m.free([0, 1])
+
+
+@pytest.mark.parametrize("late", [50, 70000, 100010])
+@pytest.mark.parametrize("tickets", [True, False])
+def test_joins_of_more_items_than_a_wavefront_has_lanes(tickets, late):
+    """A sequence of more than 64 items beside 39 short ones: two rounds of maxima, the largest score in an early and in a
+    late one."""
+    m = Mirror(slots=40, pages=1750, max_tokens=100100, Hkv=1, d=128, page=64, seed=34)
+    if not tickets:
+        m.cache._tickets = [None]
+    q = _one_strong_key(m, 0, 100020, late, 4)
+    m.push(list(range(1, 40)), [40 + i for i in range(39)])
+    step = m.push(list(range(40)), [1] * 40)
+    first = step.host[12 + 8 * 41:].reshape(-1)[:12]
+    assert first[7] == 0 and first[11] > 64
+    _check_rows(m, step, q, 40, 4)
+
+
+@pytest.mark.parametrize("late", [50, 70000, 131060])
+@pytest.mark.parametrize("rows", [1, 3])
+def test_joins_with_a_workgroup_for_each_row(rows, late):
+    """One long sequence of many items, whose rows are joined by four wavefronts each, 32 partial results on their way."""
+    m = Mirror(slots=1, pages=2100, max_tokens=131100, Hkv=1, d=128, page=64, seed=35)
+    q = _one_strong_key(m, 0, 131070, late, 8)
+    step = m.push([0], [rows])
+    assert step.splits >= 160 and step.joins
+    _check_rows(m, step, q, rows, 8)
+
+
+def _one_strong_key(m, slot, n, at, Hq):
+    """n tokens for the slot, the one at ``at`` along the query that is returned."""
+    step, [(k, v)] = m.extend([slot], [n])
+    q = m.rand(1, Hq)
+    k[at] = (30 * q[0, :1] / q[0, :1].float().norm()).to(k.dtype)
+    m.k[0][slot] = k
+    m.cache.append(0, k.cuda(), v.cuda(), step)
+    return q
+
+
+def _check_rows(m, step, q, rows, Hq):
+    import kvq
+    c = m.cache
+    qs = torch.cat([q, m.rand(rows - 1, Hq)])
+    out = kvq.paged_decode(qs.cuda(), c.d ** -0.5, c, 0, step)
+    a = 0
+    for s, n in zip(step.slots.tolist(), step.counts.tolist()):
+        kk, vv = cached(m.k[0][s], c.page, c.code), cached(m.v[0][s], c.page, c.code)
+        check(out[a:a + n], attend(qs[a:a + n], kk, vv, c.d ** -0.5), float(vv.abs().max()), kk.shape[0], c.d, c.dtype, PAIR, f"slot {s}")
+        a += n
