@@ -44,7 +44,7 @@ __device__ __forceinline__ uint32_t pack_bf16(float a, float b) {
   return __builtin_bit_cast(uint32_t, __builtin_convertvector(v, bf16x2));
 }
 
-// Two codes as two numbers of the 16-bit type: exact.  `hi` selects the upper pair of the word.
+// Four codes as two pairs of numbers of the 16-bit type: exact.
 template <int CODE, bool BF16>
 __device__ __forceinline__ void widen4(uint32_t w, uint32_t& a, uint32_t& b) {
   if constexpr (CODE == kCodeE4M3) {

@@ -110,8 +110,9 @@ __global__ __launch_bounds__(kThreads) void append_kernel(Rows16 k, Rows16 v, co
                                                           uint16_t* __restrict__ ko, uint16_t* __restrict__ vo) {
   constexpr int kChunks = P * D / 8, kPer = kChunks / kThreads;      // pieces of 8 elements, per thread
   constexpr int kRow = D / 8;                                       // pieces of a token
-  // values turn to channel-major order in LDS: channel c's tokens 8 u .. at piece u ^ (c / 8) of its row, so that
-  // the channels of a wavefront's writes (8 apart) do not meet in the same banks
+  // values turn to channel-major order in LDS: channel c's tokens 8 u .. at piece u ^ (c / 8) of its row, which spreads the
+  // channels of a wavefront's writes (8 apart) over P / 8 places; with 128 channels two of them still share the banks
+  // at 64 tokens, four at 32 (31 conflict cycles a wavefront, 1.8 million of a large fill of 144 us)
   __shared__ __align__(16) uint16_t turn[D * P];
   auto place = [](int c, int t) { return c * P + (((t >> 3) ^ (c >> 3)) & (P / 8 - 1)) * 8 + (t & 7); };
   __shared__ uint32_t top[8];
@@ -425,11 +426,13 @@ constexpr int64_t kFront = 4;
 constexpr int64_t kUneven = 16;
 
 // Fills the description from lens (before), counts and open buffers; pages are written by the caller.  split_cap bounds
-// the split items (those of a front weighted by the workgroups that its rows take at four query heads per KV head).
+// the split items (those of a front weighted by the workgroups that its rows take at four query heads per KV head: the real
+// number is not known here, with one or eight of them the weight is four times too large or half).
 // With few_cap, the workgroups that have a CU each: of no more than few_units units there are few_cap items, unless that
 // makes the longest one more than twice an even share, or there are more sequences and long ones among them; and up to twice split_cap where the longest item is kUneven units
 // and 1.5 times an even share at least, and all sequences start at once (8 KV heads of 128: 64 sequences of 100 to 4000
-// tokens 61 -> 54 us, but 64 of 3000 to 4000 94 -> 98, and 256 of 16 to 3000 with 16 rows each 187 -> 209).
+// tokens 61 -> 54 us, but 64 of 3000 to 4000 94 -> 98, and 256 of 16 to 3000 with 16 rows each 187 -> 209).  More sequences
+// than places are one item each, however long: 64 of 1000 tokens beside one of 32768 wait for its 513 units, 16 with 63.
 // most_run, most_tokens: where the step has to fit a launch that was captured; fronts that do not are left out.
 void describe(const int64_t* lens, const uint8_t* open, const int32_t* table, int64_t max_blocks, int64_t page, const int64_t* seq,
               const int64_t* counts, int64_t n, int64_t split_cap, int64_t few_cap, int64_t few_units, int64_t most_run, int64_t most_tokens,

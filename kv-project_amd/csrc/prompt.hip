@@ -15,13 +15,13 @@
 // with its own sums, and prompt_merge_kernel joins them in order.
 //
 // What bounds it: the matrix cores and the power they draw.  One causal prompt of 16384 tokens, 32 query heads over 8
-// KV heads of 128, bf16: 1913-2040 us by card (1.08-1.15 PFLOP/s; a library product of the largest size reaches 1.36),
-// matrix cores busy 63%, vector unit 55% of the cycles, at 1.7 GHz of 2.4; no LDS conflicts; keys and values come
+// KV heads of 128, bf16: 1913-2078 us by card (1.06-1.15 PFLOP/s; a library product of the largest size reaches 1.36),
+// matrix cores busy 62%, vector unit 55% of the cycles, at 1.7 GHz of 2.4; no LDS conflicts; keys and values come
 // from memory 4.5 times, otherwise from the caches.  With head_dim 64 a score costs half the products and the same
-// exponential, so the vector unit leads (70%; matrix cores 43%): four sequences of 512 to 1531 tokens behind up to 9000,
-// 235-269 us (0.76-0.87 PFLOP/s).  24 sequences of 1 to 2901 tokens, fp16, head_dim 128: 180 us (0.77 PFLOP/s): 71
-// iterations for each of 512 places, 133 us at the long prompt's rate, and the starts and ends of five tiles.  20
-// tokens: 7 us, a launch and the round trips of one tile.
+// exponential, so the vector unit leads (68%; matrix cores 42%): four sequences of 512 to 1531 tokens behind up to 9000,
+// 235-245 us (0.84-0.87 PFLOP/s; 250-283 traced over 30 passes).  24 sequences of 1 to 2901 tokens, fp16, head_dim 128:
+// 172-182 us (0.76-0.80 PFLOP/s; 179-214 traced): 71 iterations for each of 512 places, 133 us at the long prompt's rate,
+// and the starts and ends of five tiles.  20 tokens: 7 us, a launch and the round trips of one tile.
 // Measured and not kept: 64 rows a wavefront (half the LDS reads, but accumulators move between the register files:
 // 2040-2680 us); sums by a product with ones at head_dim 64 (235 -> 258 us); other wave priorities (3-5% slower);
 // workgroups that stay for several tiles and fetch the next one's first keys during the last steps (24 sequences of 256
@@ -444,7 +444,9 @@ extern "C" int kvq_prompt_plan(const int64_t* lens_q, const int64_t* lens_k, int
   // Where the tiles of rows do not fill kSlots places (two on each of 256 CUs), they are cut into the shortest parts that
   // fit: 8 key tiles at least, which pay for the part's sums (64 KB).  Parts beyond the places start a second round, which
   // costs more than uneven ones: 8 sequences of 1024 tokens, 8 heads of 128, 512 tiles whole 36 us, 768 parts of an even
-  // share at most 53; 24 of 16 tokens behind 32768, 384 parts 605, 576 of them 723.
+  // share at most 53; 24 of 16 tokens behind 32768, 384 parts 605, 576 of them 723.  Batches whose tiles fill the places
+  // stay whole, however uneven: 64 tokens behind 60000 beside twelve prompts of 256 (32 query heads over 8) wait for
+  // tiles of 939 steps, 33 of them an even share.
   int64_t most = kMinPart, high = longest > kMinPart ? longest : kMinPart;
   if (tiles * H > kSlots) most = high;
   while (most < high) {
