@@ -38,7 +38,8 @@ class PagedCtl:
     def begin(self, counts: Union[int, Sequence[int]]) -> None:
         """Claim the next step: ``counts`` new tokens of every sequence, or of each one (in a batch padded on the left:
         the last counts[b] tokens of row b are its own).  Once per forward pass, before it: a layer that comes a second time
-        in a step is refused, its tokens would take the places of the first ones."""
+        in a step is refused, its tokens would take the places of the first ones.  To run a step again on purpose (a pass that
+        failed, one in front of a capture) clear ``seen``."""
         n = [int(counts)] * len(self.slots) if isinstance(counts, int) else [int(c) for c in counts]
         if len(n) != len(self.slots):
             raise ValueError("counts must be one number or one per sequence")

@@ -254,3 +254,39 @@ def _small_models(name):
     models = [LlamaForCausalLM._from_config(cfg, attn_implementation=a, dtype=torch.bfloat16).eval() for a in ("sdpa", name)]
     models[1].load_state_dict(models[0].state_dict())
     return models
+
+
+def test_a_step_run_again_and_captured():
+    """A step's pass repeated on purpose, then captured; its replays run the steps that are written into it."""
+    import kvq
+    cache = kvq.PagedCache(1, 2, 20, 300, 2, 64, page=32)
+    ctl = kvq.PagedCtl(cache, [0, 1])
+    m = SimpleNamespace(layer_idx=0, scaling=0.125)
+    g = torch.Generator(device="cuda").manual_seed(3)
+    rand = lambda T: [torch.randn(2, h, T, 64, generator=g, device="cuda").bfloat16() for h in (4, 2, 2)]
+    ctl.begin([70, 33])
+    ctl.attend(m, *rand(70), None, {})
+    ctl.begin(1)
+    q, k, v = rand(1)
+    first, _ = ctl.attend(m, q, k, v, None, {})
+    ctl.seen.clear()
+    again, _ = ctl.attend(m, q, k, v, None, {})
+    assert torch.equal(first, again)
+    ctl.seen.clear()
+    torch.cuda.synchronize()
+    gr = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(gr):
+        out, _ = ctl.attend(m, q, k, v, None, {})
+    for i in range(4):
+        if i:
+            cache.extend([0, 1], [1, 1], into=ctl.step)
+            for x, y in zip((q, k, v), rand(1)):
+                x.copy_(y)
+        _ = (q.float() * 2).sum()
+        gr.replay()
+        torch.cuda.synchronize()
+        want = kvq.paged_decode(q.transpose(1, 2).reshape(2, 4, 64), 0.125, cache, 0, ctl.step)
+        assert torch.equal(out.view(2, 4, 64), want), i
+        kk, vv = cache.rows(0, [0, 1])
+        assert torch.equal(kk[70 + i], k[0, :, 0]) and torch.equal(vv[-1], v[1, :, 0])
+    assert cache.lengths == [74, 37]
