@@ -179,6 +179,8 @@ class PagedCache:
             words = lib.kvq_pages_step_words(self.page, pc, n)
             if words < 0:
                 raise ValueError("counts must not be negative, and below 2^31")
+            if words > 32 * n + 32 + n * (self.max_blocks + 1):         # before memory is taken for its description
+                raise _lib.KVQError(f"decode buffer exhausted: a slot holds {self.max_tokens} tokens, {int(c.max())} more asked for")
             st = Step()
             st.cache, st.pools = self, self._pools
             st.host = np.empty(words, dtype=np.int32)

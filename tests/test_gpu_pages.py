@@ -757,3 +757,17 @@ def _check_rows(m, step, q, rows, Hq):
         kk, vv = cached(m.k[0][s], c.page, c.code), cached(m.v[0][s], c.page, c.code)
         check(out[a:a + n], attend(qs[a:a + n], kk, vv, c.d ** -0.5), float(vv.abs().max()), kk.shape[0], c.d, c.dtype, PAIR, f"slot {s}")
         a += n
+
+
+def test_a_step_beyond_every_slot_takes_no_memory():
+    """Counts that no slot can hold are refused before their description is allocated (268 MB for 2^31 - 1 tokens)."""
+    import kvq
+    c = kvq.PagedCache(1, 2, 4, 300, 2, 64, page=32)
+    before = torch.cuda.memory_allocated()
+    torch.cuda.reset_peak_memory_stats()
+    for counts in ([(1 << 31) - 1], [301], [1, 1 << 30], [(1 << 31) - 1] * 2):
+        with pytest.raises(kvq.KVQError, match="exhausted"):
+            c.extend(list(range(len(counts))), counts)
+    assert torch.cuda.max_memory_allocated() - before < 1 << 20
+    assert c.lengths == [0, 0] and c.free_pages == 4
+    assert c.extend([0, 1], [64, 64]).rows == 128
