@@ -15,12 +15,12 @@
 // with its own sums, and prompt_merge_kernel joins them in order.
 //
 // What bounds it: the matrix cores and the power they draw.  One causal prompt of 16384 tokens, 32 query heads over 8
-// KV heads of 128, bf16: 1913-2078 us by card (1.06-1.15 PFLOP/s; a library product of the largest size reaches 1.36),
+// KV heads of 128, bf16: 1913-2085 us by card (1.06-1.15 PFLOP/s; a library product of the largest size reaches 1.36),
 // matrix cores busy 62%, vector unit 55% of the cycles, at 1.7 GHz of 2.4; no LDS conflicts; keys and values come
 // from memory 4.5 times, otherwise from the caches.  With head_dim 64 a score costs half the products and the same
 // exponential, so the vector unit leads (68%; matrix cores 42%): four sequences of 512 to 1531 tokens behind up to 9000,
-// 235-245 us (0.84-0.87 PFLOP/s; 250-283 traced over 30 passes).  24 sequences of 1 to 2901 tokens, fp16, head_dim 128:
-// 172-182 us (0.76-0.80 PFLOP/s; 179-214 traced): 71 iterations for each of 512 places, 133 us at the long prompt's rate,
+// 235-253 us (0.81-0.87 PFLOP/s; 250-283 traced over 30 passes).  24 sequences of 1 to 2901 tokens, fp16, head_dim 128:
+// 172-188 us (0.73-0.80 PFLOP/s; 179-214 traced): 71 iterations for each of 512 places, 133 us at the long prompt's rate,
 // and the starts and ends of five tiles.  20 tokens: 7 us, a launch and the round trips of one tile.
 // Measured and not kept: 64 rows a wavefront (half the LDS reads, but accumulators move between the register files:
 // 2040-2680 us); sums by a product with ones at head_dim 64 (235 -> 258 us); other wave priorities (3-5% slower);
