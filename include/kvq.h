@@ -752,6 +752,27 @@ int kvq_paged_decode(const void* q, int64_t q_st, int64_t q_sh, int dtype, int64
                      const uint8_t* kc, const uint8_t* vc, const float* sc, const void* ko, const void* vo, void* out,
                      float* workspace, int64_t workspace_floats, int32_t* tickets, void* stream);
 
+/* ------------------------------------------------------------------------------------------
+ * Attention of many rows straight over the paged cache.  Packed rows q (rows, Hq, D), counts[i] of them for slot
+ * seq[i] (a slot may be named more than once).  Causal: they are the slot's last tokens, and row t sees tokens 0 .. t +
+ * len - count; otherwise every row sees all tokens of the slot, and rows of an empty one get zeros.  A visible value of the
+ * open block that is infinite or NaN is its channel's result, whatever its weight; what is hidden changes nothing.
+ * kvq_paged_plan (host memory: the accounts of the cache as they are, slots named, counts): fills `words` for a call of such rows,
+ * rep <= 128 query heads to each of H KV heads; info[3] = {items, merges, parts}.  12 items + 8 merges words are needed: with
+ * less room only info is set.  Pages that neighbours share in front are read once for all of them where that saves work.
+ * The words go to the device as they are; they bound what kvq_paged_attention reads, together with the table on the
+ * device.  workspace: kvq_paged_attention_workspace floats (none without parts), no clearing; calls that share one must not
+ * overlap in time.
+ * ---------------------------------------------------------------------------------------- */
+int kvq_paged_plan(const int64_t* lens, const int32_t* table, const uint8_t* open, int64_t slots, int64_t max_blocks,
+                   int64_t page, const int64_t* seq, const int64_t* counts, int64_t n, int64_t rep, int64_t H, int causal,
+                   int32_t* words, int64_t words_cap, int64_t* info);
+int64_t kvq_paged_attention_workspace(int64_t parts, int64_t H, int64_t D);
+int kvq_paged_attention(const void* q, int64_t q_st, int64_t q_sh, int dtype, int64_t Hq, int64_t H, int64_t D, float scaling,
+                        const int32_t* words, int64_t items, int64_t merges, int64_t parts, const int32_t* table,
+                        int64_t max_blocks, int64_t page, int code, const uint8_t* kc, const uint8_t* vc, const float* sc,
+                        const void* ko, const void* vo, void* out, float* workspace, int64_t workspace_floats, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

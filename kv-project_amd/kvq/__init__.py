@@ -24,6 +24,7 @@ from .coverage import coverage_groups, coverage_plan, coverage_stats
 from .strata_compress import StrataCompressor, rotation_matrix
 from .prompt import PromptPlan, prompt_attention
 from .pages import PagedCache, paged_decode, paged_workspace_floats
+from .paged import PagedPlan, paged_attention
 from .paged_ctl import PagedCtl
 
 __all__ = [
@@ -41,4 +42,5 @@ __all__ = [
     "EvictedState", "MTLPState", "mtlp_budget", "mtlp_select", "snapkv_keep", "streaming_keep", "PackedState",
     "exact_rows_cache", "quasar_scores", "quasar_values", "retained_decode",
     "retained_workspace_floats", "PromptPlan", "prompt_attention", "PagedCache", "paged_decode", "paged_workspace_floats", "PagedCtl",
+    "PagedPlan", "paged_attention",
 ]

@@ -117,6 +117,10 @@ SIGNATURES = {
     "kvq_paged_decode_workspace": (i64, [i64, i64, i64, i64]),
     "kvq_paged_decode": (i32, [vp, i64, i64, i32, i64, i64, i64, i64, f32, vp, i64, i64, i64, i64, i32, vp, i64, i64, i32, vp, vp, vp,
                                vp, vp, vp, vp, i64, vp, vp]),
+    "kvq_paged_plan": (i32, [vp, vp, vp, i64, i64, i64, vp, vp, i64, i64, i64, i32, vp, i64, vp]),
+    "kvq_paged_attention_workspace": (i64, [i64, i64, i64]),
+    "kvq_paged_attention": (i32, [vp, i64, i64, i32, i64, i64, i64, f32, vp, i64, i64, i64, vp, i64, i64, i32, vp, vp, vp, vp, vp, vp, vp,
+                                  i64, vp]),
 }
 
 

@@ -1,0 +1,222 @@
+"""Attention of many rows over the paged cache against the float64 oracle: chunks of prompts, questions behind a shared text,
+cross attention; cut and joined rows, values that a row must not see, replays and other streams, and what is refused."""
+import pytest
+import torch
+
+from attention_bounds import HALF, check
+from oracle.paged import attend, cached
+from test_gpu_pages import Mirror
+
+pytestmark = pytest.mark.gpu
+
+# a weight times a scale: rounded once for bf16, kept as two bf16 for fp16
+WEIGHT = {torch.bfloat16: HALF[torch.bfloat16], torch.float16: 2.0 ** -17}
+
+
+def run(m, slots, counts, Hq, causal=True, layer=0, what="", scaling=None, q=None):
+    """One call, every row checked; returns (plan, q, out)."""
+    import kvq
+    c = m.cache
+    scaling = c.d ** -0.5 if scaling is None else scaling
+    plan = kvq.PagedPlan(c, slots, counts, Hq, causal=causal)
+    q = m.rand(sum(counts), Hq) if q is None else q
+    out = kvq.paged_attention(q.cuda(), scaling, c, layer, plan)
+    a = 0
+    for s, n in zip(slots, counts):
+        if n:
+            k, v = cached(m.k[layer][s], c.page, c.code), cached(m.v[layer][s], c.page, c.code)
+            ref = attend(q[a:a + n], k, v, scaling, causal)
+            check(out[a:a + n], ref, float(v.abs().max()) if len(v) else 0.0, k.shape[0], c.d, c.dtype, WEIGHT[c.dtype],
+                  f"{what} slot {s}, {n} of {k.shape[0]}")
+        a += n
+    return plan, q, out
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("code", ["int8", "e4m3"])
+@pytest.mark.parametrize("page,d,Hkv,rep", [(32, 64, 2, 4), (64, 128, 1, 3), (128, 64, 1, 7), (32, 128, 1, 1), (128, 128, 2, 2), (64, 64, 1, 8)])
+def test_chunks(page, d, Hkv, rep, code, dtype):
+    """Chunks from one token to all of the slot's, lengths around the blocks' borders, nothing for one of them."""
+    m = Mirror(page=page, d=d, Hkv=Hkv, code=code, dtype=dtype, seed=page + d + rep)
+    m.push([0, 1, 2, 3, 4], [1, page, 2 * page + 40, 3 * page - 1, 64])
+    run(m, [0, 1, 2, 3, 4], [1, page, 41, 60, 0], rep * Hkv, what="chunks")
+    run(m, [4, 2], [64, 1], rep * Hkv, what="whole")
+    m.push([0, 1], [70, 33])
+    run(m, [1, 0], [33, 70], rep * Hkv, what="later")
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("page,d,Hkv,rep", [(32, 64, 2, 4), (64, 128, 1, 3), (128, 64, 1, 8)])
+def test_shared_text(page, d, Hkv, rep, dtype):
+    """Questions of forks side by side, others between, uneven; and the same rows again, and each alone."""
+    import kvq
+    m = Mirror(slots=10, pages=200, max_tokens=1500, Hkv=Hkv, d=d, page=page, dtype=dtype, seed=page)
+    m.push([0, 1], [900, 333])
+    m.fork([0] * 5 + [1] * 2, [2, 3, 4, 5, 6, 7, 8])
+    counts = [1, 5, 17, 3, 90, 2, 40, 8]
+    m.push([0, 2, 3, 4, 5, 7, 8, 9], [1, 5, 17, 3, 90, 2, 40, 8])
+    plan, q, out = run(m, [0, 2, 3, 4, 5, 7, 8, 9], counts, rep * Hkv, what="forks")
+    # the seven that share a text are joined, a tile of their rows at a time
+    assert plan.merges >= 7 and torch.equal(out, kvq.paged_attention(q.cuda(), d ** -0.5, m.cache, 0, plan))
+    run(m, [2, 9, 3, 6, 4], [5, 0, 17, 9, 3], rep * Hkv, what="between")
+    run(m, [6, 6], [900, 30], Hkv, what="the text itself, twice")
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("code", ["int8", "e4m3"])
+@pytest.mark.parametrize("page,d,Hkv,rep", [(32, 64, 2, 1), (64, 128, 1, 4), (128, 128, 1, 2)])
+def test_cross(page, d, Hkv, rep, code, dtype):
+    """Every row sees every token: beams of one encoder, one without states, single tokens and prompts, shared pages."""
+    m = Mirror(slots=8, pages=100, max_tokens=900, Hkv=Hkv, d=d, page=page, code=code, dtype=dtype, seed=page + rep)
+    m.push([0, 1, 2, 3], [750, 1, page, 200])
+    m.fork([0, 0], [5, 6])
+    m.push([5], [70])
+    run(m, [0, 0, 0, 4, 1, 2, 3], [1, 1, 1, 2, 3, 1, 100], rep * Hkv, causal=False, what="beams")
+    run(m, [0, 5, 6, 3], [7, 1, 2, 0], rep * Hkv, causal=False, what="shared pages")
+    run(m, [4, 4], [1, 0], rep * Hkv, causal=False, what="none")
+
+
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("n,rep,d", [(4099, 4, 64), (2600, 1, 128), (5000, 2, 64)])
+def test_cut_along_the_tokens(n, rep, d, causal):
+    """Few rows over many tokens: parts and their joins, with and without a shared text."""
+    m = Mirror(slots=4, pages=300, max_tokens=5200, Hkv=1, d=d, page=64, seed=n)
+    m.push([0, 1], [n, 700])
+    plan, _, _ = run(m, [0, 1], [3, 2], rep, causal, what="cut")
+    assert plan.parts > 2 and plan.merges == 2
+    m.fork([0, 0], [2, 3])
+    m.push([2, 3], [5, 40])
+    run(m, [2, 3], [5, 7], rep, causal, what="cut text")
+
+
+def test_one_query_head_to_many():
+    """128 query heads over one KV head: a tile for each token."""
+    m = Mirror(Hkv=1, d=64, page=32, seed=5)
+    m.push([0], [150])
+    run(m, [0], [3], 128, what="128 heads")
+    run(m, [0], [2], 20, what="20 heads")
+
+
+def test_layers_after_moves():
+    m = Mirror(layers=3, slots=4, pages=30, max_tokens=600, Hkv=2, d=64, page=32, seed=4)
+    m.push([0, 1, 2], [100, 164, 31])
+    m.free([0])
+    m.cache.compact()
+    for l in range(3):
+        run(m, [1, 2], [50, 31], 4, layer=l, what=f"layer {l}")
+    m.cache.resize(20)
+    run(m, [2, 1], [3, 164], 4, layer=2, what="resized")
+
+
+@pytest.mark.parametrize("scaling", [0.0, -0.3, 2.5])
+def test_scaling(scaling):
+    m = Mirror(Hkv=1, d=64, page=32, seed=6)
+    m.push([0], [150])
+    run(m, [0], [40], 4, what=f"scaling {scaling}", scaling=scaling)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("page", [32, 64, 128])
+@pytest.mark.parametrize("value", [float("inf"), float("-inf"), float("nan")])
+@pytest.mark.parametrize("side", ["k", "v"])
+def test_hidden_values_change_nothing(side, value, page, dtype):
+    """An infinity or a NaN behind what a row sees, in a block that was coded (its scale is NaN) and in the open one: the rows in
+    front of the block are as without it; in the open block a visible value is its channel's result."""
+    import kvq
+    d, n = 64, 3 * page + 20
+    m = Mirror(slots=2, Hkv=1, d=d, page=page, dtype=dtype, max_tokens=600, seed=7)
+    k, v = m.rand(n, 1), m.rand(n, 1)
+    q = m.rand(n, 2)
+    for slot, bad in ((0, [2 * page + 5]), (1, [3 * page + 11])):
+        kk, vv = k.clone(), v.clone()
+        for j in bad:
+            (kk if side == "k" else vv)[j, 0, 3] = value
+        step = m.cache.extend([slot], [n])
+        m.cache.append(0, kk.cuda(), vv.cuda(), step)
+        plan = kvq.PagedPlan(m.cache, [slot], [n], 2)
+        out = kvq.paged_attention(q.cuda(), d ** -0.5, m.cache, 0, plan).cpu()
+        first = bad[0] // page * page if slot == 0 else bad[0]       # rows in front of the block, or of the token
+        if slot == 0:
+            first = 2 * page                                        # row i sees the block's first token from i = first on
+        ref = attend(q, cached(k, page, "int8"), cached(v, page, "int8"), d ** -0.5)
+        vmax = float(v.abs().max())
+        check(out[:first], tuple(x[:first] for x in ref), vmax, n, d, dtype, WEIGHT[dtype], f"slot {slot}")
+        late = out[first:].float()
+        if slot == 0 or side == "k" and value != value:
+            assert late.isnan().all()
+        elif side == "v":
+            hit = late[..., 3]
+            assert bool(hit.isnan().all()) if value != value else bool((hit == value).all())
+            rest = [i for i in range(d) if i != 3]
+            check(out[first:][..., rest], tuple(x[first:][..., rest] if x.shape[-1] == d else x[first:] for x in ref), vmax, n, d, dtype,
+                  WEIGHT[dtype], "other channels")
+
+
+def test_replays_streams_and_strides():
+    """A captured call replayed with other rows, another stream, expanded rows, the caller's output and workspace."""
+    import kvq
+    m = Mirror(slots=4, pages=120, max_tokens=3100, Hkv=2, d=64, page=32, seed=8)
+    m.push([0], [3001])
+    m.fork([0, 0], [1, 2])
+    m.push([1, 2], [4, 9])
+    plan = kvq.PagedPlan(m.cache, [1, 2], [4, 9], 8)
+    assert plan.parts
+    q = m.rand(13, 8).cuda()
+    out = torch.empty_like(q)
+    ws = torch.full((plan.workspace_floats(),), float("nan"), device="cuda")
+    kvq.paged_attention(q, 0.125, m.cache, 0, plan, out=out, workspace=ws)
+    torch.cuda.synchronize()
+    gr = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(gr):
+        kvq.paged_attention(q, 0.125, m.cache, 0, plan, out=out, workspace=ws)
+    for i in range(3):
+        q.copy_(m.rand(13, 8))
+        _ = (q.float() * 2).sum()
+        gr.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, kvq.paged_attention(q, 0.125, m.cache, 0, plan)), i
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        one = m.rand(1, 8).cuda()
+        got = kvq.paged_attention(one.expand(13, -1, -1), 0.125, m.cache, 0, plan)
+    torch.cuda.current_stream().wait_stream(side)
+    assert torch.equal(got, kvq.paged_attention(one.expand(13, -1, -1).contiguous(), 0.125, m.cache, 0, plan))
+    wide = torch.empty((13, 8, 96), dtype=q.dtype, device="cuda")
+    wide[..., 32:] = q
+    assert torch.equal(kvq.paged_attention(wide[..., 32:], 0.125, m.cache, 0, plan), out)
+    odd = torch.empty((13, 8, 67), dtype=q.dtype, device="cuda")
+    odd[..., 3:] = q
+    assert torch.equal(kvq.paged_attention(odd[..., 3:], 0.125, m.cache, 0, plan), out)
+
+
+def test_refusals():
+    import kvq
+    m = Mirror(slots=3, Hkv=2, d=64, page=32)
+    m.push([0, 1], [40, 10])
+    c = m.cache
+    for slots, counts, what in (([], [], "length"), ([0], [1, 2], "length"), ([3], [1], "slot"), ([-1], [1], "slot"), ([0], [-1], "negative"),
+                                ([0], [41], "last"), ([2], [1], "last")):
+        with pytest.raises((ValueError, kvq.KVQError), match=what):
+            kvq.PagedPlan(c, slots, counts, 4)
+    for Hq in (0, 3, 2 * 129):
+        with pytest.raises(ValueError, match="query heads"):
+            kvq.PagedPlan(c, [0], [1], Hq)
+    plan = kvq.PagedPlan(c, [0, 1], [5, 2], 4)
+    q = m.rand(7, 4).cuda()
+    ws = torch.empty(0, device="cuda")
+    call = lambda q=q, layer=0, cache=c, p=plan, **kw: kvq.paged_attention(q, 0.1, cache, layer, p, **kw)
+    call()
+    for bad, error in ((dict(layer=1), IndexError), (dict(layer=-1), IndexError), (dict(q=q[:6]), ValueError), (dict(q=q[..., :32]), ValueError),
+                       (dict(q=q.half()), TypeError), (dict(q=q.cpu()), kvq.KVQError), (dict(out=torch.empty_like(q)[:6]), ValueError),
+                       (dict(out=torch.empty(7, 4, 64, device="cuda")), ValueError), (dict(workspace=ws.double()), ValueError)):
+        with pytest.raises(error):
+            call(**bad)
+    other = Mirror(slots=3, Hkv=2, d=64, page=32).cache
+    with pytest.raises(ValueError, match="another cache"):
+        call(cache=other)
+    m.push([2], [3])
+    call()                                     # another slot's tokens
+    m.push([1], [1])
+    with pytest.raises(ValueError, match="changed"):
+        call()
