@@ -773,6 +773,26 @@ int kvq_paged_attention(const void* q, int64_t q_st, int64_t q_sh, int dtype, in
                         int64_t max_blocks, int64_t page, int code, const uint8_t* kc, const uint8_t* vc, const float* sc,
                         const void* ko, const void* vo, void* out, float* workspace, int64_t workspace_floats, void* stream);
 
+/* ------------------------------------------------------------------------------------------
+ * The paged cache's accounts in device memory, for counts that only the device knows: lens (slots), refs (pages), open
+ * (slots) int32, account[3] int32 = {free pages, no free page below this one, steps refused}, and the table.  slots (n,
+ * different ones), counts (n) int32 are device memory too.
+ * kvq_tables_extend: what kvq_pages_extend does for n sequences of 0 .. most tokens each, whose rows lie at i * most: the lowest free page
+ * for each block that gets full, in order, in the table, and the step's description (kvq_tables_step_words words; n sequences without shared
+ * fronts, `splits` >= n split items at most) for kvq_pages_append and kvq_paged_decode, whose grids go by the items (words - 32 n - 32),
+ * `splits`, run_tokens = most and split_tokens = splits * most.  positions (n most): a row's place in its sequence, or -1; places (n
+ * most): page * P + offset of a row whose block is full after the step, else -1.  A step that does not fit (a count out of range, more than
+ * max_tokens or the free pages) changes no slot, describes no tokens and is counted in account[2].  scratch: n + items words.
+ * kvq_tables_free empties the slots, or those with which[i] != 0.  Both may be captured.
+ * ---------------------------------------------------------------------------------------- */
+int64_t kvq_tables_step_words(int64_t page, int64_t n, int64_t most);
+int kvq_tables_extend(const int32_t* slots, const int32_t* counts, int64_t n, int64_t most, int64_t page, int64_t max_tokens,
+                      int64_t pages, int64_t max_blocks, int64_t splits, int32_t* lens, int32_t* refs, int32_t* open,
+                      int32_t* account, int32_t* table, int32_t* desc, int64_t desc_words, int32_t* scratch,
+                      int64_t scratch_words, int32_t* positions, int64_t* places, void* stream);
+int kvq_tables_free(const int32_t* slots, const uint8_t* which, int64_t n, int64_t page, int64_t max_blocks, int32_t* lens,
+                    int32_t* refs, int32_t* open, int32_t* account, const int32_t* table, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

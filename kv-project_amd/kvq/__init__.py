@@ -25,6 +25,7 @@ from .strata_compress import StrataCompressor, rotation_matrix
 from .prompt import PromptPlan, prompt_attention
 from .pages import PagedCache, paged_decode, paged_workspace_floats
 from .paged import PagedPlan, paged_attention
+from .tables import DeviceAccounts
 from .paged_ctl import PagedCtl
 
 __all__ = [
@@ -42,5 +43,5 @@ __all__ = [
     "EvictedState", "MTLPState", "mtlp_budget", "mtlp_select", "snapkv_keep", "streaming_keep", "PackedState",
     "exact_rows_cache", "quasar_scores", "quasar_values", "retained_decode",
     "retained_workspace_floats", "PromptPlan", "prompt_attention", "PagedCache", "paged_decode", "paged_workspace_floats", "PagedCtl",
-    "PagedPlan", "paged_attention",
+    "PagedPlan", "paged_attention", "DeviceAccounts",
 ]

@@ -28,6 +28,7 @@ class PagedPlan:
     live as long as a graph captured with it is replayed."""
 
     def __init__(self, cache: PagedCache, slots: Sequence[int], counts: Sequence[int], Hq: int, *, causal: bool = True):
+        cache.at_home()
         s, c = (np.array(x, dtype=np.int64).reshape(-1) for x in (slots, counts))
         if s.size == 0 or s.shape != c.shape:
             raise ValueError("slots and counts must have the same length, one at least")

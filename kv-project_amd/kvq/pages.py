@@ -95,6 +95,7 @@ class PagedCache:
         self._pools = 0                        # of the pools
         self._stamp = 0                        # of the slots' lengths
         self._touched = np.zeros(self.slots, dtype=np.int64)        # the stamp when a slot took tokens or was emptied
+        self._away = None                      # the DeviceAccounts that have the accounts meanwhile
         self.table = torch.zeros((self.slots, self.max_blocks), dtype=torch.int32, device=self.device)
         self.kc, self.vc, self.sc = self._pool(self.pages)
         rows = (self.layers, self.slots, 2, self.Hkv, self.page * self.d)
@@ -134,19 +135,27 @@ class PagedCache:
 
     # ---- what is held ------------------------------------------------------------------------
 
+    def at_home(self) -> None:
+        """Refused while the accounts are on the device."""
+        if self._away is not None:
+            raise _lib.KVQError("the cache's accounts are on the device: DeviceAccounts.close() hands them back")
+
     @property
     def lengths(self) -> List[int]:
         """Tokens of each slot."""
+        self.at_home()
         return self._lens.tolist()
 
     def length(self, slot: int) -> int:
         """Tokens of one slot."""
+        self.at_home()
         if not 0 <= slot < self.slots:
             raise IndexError(f"no slot {slot} (of {self.slots})")
         return int(self._lens[slot])
 
     @property
     def free_pages(self) -> int:
+        self.at_home()
         return int(self._account[0])
 
     def codes(self) -> Tuple[torch.Tensor, torch.Tensor]:
@@ -170,6 +179,8 @@ class PagedCache:
         full.  ``into``: a step of the same counts whose description is rewritten in place, so that a
         captured graph of its append and decode runs the new step when it is replayed; refused for a step from before a
         resize(), whose graphs hold pools that are gone."""
+        if self._away is not None:
+            self.at_home()
         s, c = _ints(slots, "slots"), _ints(counts, "counts")
         if s.shape != c.shape:
             raise ValueError("slots and counts must have the same length")
@@ -193,7 +204,7 @@ class PagedCache:
             st = into
             if st.cache is not self:
                 raise ValueError("a step is rewritten by its own cache only")
-            if not np.array_equal(st.counts, c):
+            if st.host is None or not np.array_equal(st.counts, c):
                 raise ValueError("a step is rewritten for the same counts only")
             if st.pools != self._pools:
                 raise ValueError("a step from before resize() is not rewritten: graphs captured with it hold the old pools")
@@ -259,6 +270,7 @@ class PagedCache:
         once, and the open blocks as they are.  With prompt_attention this is the attention of many new tokens."""
         if not 0 <= layer < self.layers:
             raise IndexError(f"no layer {layer} (of {self.layers})")
+        self.at_home()
         s = _ints(slots, "slots")
         total = sum(self._lens.take(s, mode="clip").tolist())
         out = self.k_open.new_empty((2, total, self.Hkv, self.d))
@@ -275,6 +287,7 @@ class PagedCache:
     def fork(self, src: Sequence[int], dst: Sequence[int]) -> None:
         """Empty slots dst[i] become continuations of src[i]: they share its pages and get copies of its open block, in all
         layers.  Call it when every layer has appended its steps."""
+        self.at_home()
         s, t = _ints(src, "src"), _ints(dst, "dst")
         if s.shape != t.shape:
             raise ValueError("src and dst must have the same length")
@@ -289,6 +302,7 @@ class PagedCache:
 
     def free(self, slots: Sequence[int]) -> None:
         """Empty the slots; pages that no other sequence shares become free."""
+        self.at_home()
         s = _ints(slots, "slots")
         _lib.call("kvq_pages_free", *self._host, self.slots, self.max_blocks, self.page, _address(s), s.size)
         self._stamp += 1
@@ -363,7 +377,9 @@ def paged_decode(q: torch.Tensor, scaling: float, cache: PagedCache, layer: int,
     q, qp, qt, qh = rows16(q)
     Hq, device, stream = shape[1], cache.device, _lib.stream_of(q)
     if out is None:
-        out = torch.empty_like(q, memory_format=torch.contiguous_format)
+        # a step of counts that the host does not know may leave rows out
+        new = torch.empty_like if step.host is not None else torch.zeros_like
+        out = new(q, memory_format=torch.contiguous_format)
     else:
         _lib.out_or_new(out, shape, cache.dtype, device, "paged_decode")
     if step.rows == 0:
