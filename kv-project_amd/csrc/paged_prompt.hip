@@ -7,9 +7,10 @@
 // token major, values channel major, as their pages are.  S^T = K Q^T, the softmax in base 2 with one running reference
 // and sum per column, O^T += V^T P^T.  Row m = 8 a + 4 g + b of tile s of S^T is token 32 g + 16 s + 4 a + b, so that lane
 // half g holds the scores of tokens 32 g .. 32 g + 31 in order, which is how it reads a channel of V: 16 bytes, 8 tokens.
-// The key scale multiplies the scores, the value scale the weights; both are float32.
-// Weights times scale are bfloat16 (a scale has float32's range): rounded once for bfloat16 outputs, half a step of the
-// type; as a pair that keeps 16 bits for half ones.
+// The key scale multiplies the scores, the value scale the weights; both are float32.  Weights times scale are rounded once to
+// the inputs' type, half a step of the outputs'.  bfloat16 has a scale's range; for half types the accumulators are held in
+// units of a power of two near the scale, and the reference weighs 2^7: what a weight loses below 2^-14 is at most 2^-32 of its
+// block's largest value (pages of 32 tokens: of the two blocks of a unit).
 #include <algorithm>
 #include <cfloat>
 #include <cmath>
@@ -41,13 +42,6 @@ __device__ __forceinline__ uint32_t pack2(float a, float b) {
   const f32x2 v = {a, b};
   if constexpr (BF16) return __builtin_bit_cast(uint32_t, __builtin_convertvector(v, bf16x2));
   else return __builtin_bit_cast(uint32_t, __builtin_convertvector(v, half2v));
-}
-
-// What rounding a pair of weights leaves, in the same type
-template <bool BF16>
-__device__ __forceinline__ uint32_t rest2(float a, float b, uint32_t w) {
-  if constexpr (BF16) return pack2<true>(a - __uint_as_float(w << 16), b - __uint_as_float(w & 0xffff0000u));
-  else return pack2<false>(a - h2f(w, 0), b - h2f(w, 1));
 }
 
 // Four codes as two pairs of numbers of the 16-bit type: exact.
@@ -111,116 +105,296 @@ struct WideArgs {
   float* part;                                // (parts, H): 128 x D sums, then 128 x {reference, sum}
 };
 
+// Iteration j takes unit j of the codes through the softmax, beside matrix products that do not depend on it: O += V(j-1)
+// P(j-1); then S(j+1) = K(j+1) Q, beside the widening of K(j+2) and V(j) from registers to LDS (two buffers each, one barrier an
+// iteration), whose codes were fetched an iteration earlier.  The number of units is rounded up to an odd one, so that buffers
+// and registers of even and odd ones have fixed places.  Units of the open block follow, one at a time.
 template <int D, int P, int CODE, bool BF16>
 __global__ __launch_bounds__(kThreads, 2) void paged_wide_kernel(WideArgs a) {
   constexpr int kPieces = D / 8;              // 16-byte pieces of a token's keys in LDS
-  constexpr int kChunks = 4 * D, kPer = kChunks / kThreads;         // 16-byte pieces of a unit's codes, of a thread
+  constexpr int kPer = 4 * D / kThreads;      // 16-byte pieces of a unit's key codes of a thread, and of its value codes
+  constexpr int kBuf = kUnit * D;
   constexpr uint32_t kInf = BF16 ? 0x7f80u : 0x7c00u;
-  __shared__ __align__(16) uint16_t ks[kUnit * D], vs[D * kUnit];
+  constexpr bool kOne = P >= kUnit;           // a unit lies in one page
+  __shared__ __align__(16) uint16_t ks[2][kBuf], vs[2][kBuf];
   __shared__ int flag[2];
   const int* it = a.items + kItemWords * (blockIdx.x / a.H);
   const int h = blockIdx.x % a.H;
   const int row0 = it[0], toks = it[1], slot = it[2], u0 = it[3], u1 = it[4], vis0 = it[5], vis_step = it[6], len = it[7], buf = it[8], piece = it[9];
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, col = lane & 31, g = lane >> 5;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), col = lane & 31, g = lane >> 5;
   const int full = len / P * P, u_full = (full + kUnit - 1) / kUnit, last = full / P - 1;
   const int u_end = u1 < u_full ? u1 : u_full;
 
   const int row = wave * 32 + col, tok = row / a.rep, hq = row % a.rep;
   const bool live = tok < toks;
   const int sees = vis0 + vis_step * tok, visible = !live ? 0 : sees < len ? sees : len;
+  // every lane reads a row, dead ones the first
   u32x4 q[D / 16];
   const uint32_t mask = live ? ~0u : 0u;
   const uint16_t* qp = a.q + (row0 + static_cast<int64_t>(live ? tok : 0)) * a.q_st + (static_cast<int64_t>(h) * a.rep + hq) * a.q_sh + 8 * g;
-  each<0, D / 16>([&](auto i) { q[i.value] = (*reinterpret_cast<const u32x4*>(qp + 16 * i.value) ^ a.sign) & mask; });
-  f32x16 o[D / 32], s[2];
-  float m = -INFINITY, l = 0.0f;
+  each<0, D / 16>([&](auto i) { q[i.value] = *reinterpret_cast<const u32x4*>(qp + 16 * i.value); });
+  f32x16 o[D / 32], s[2][2];                  // s, p: of even and odd units
+  u32x4 p[2][4];
+  float m = -INFINITY, l = 0.0f, grow = 1.0f; // the exponents' reference, this lane's part of the sum, what o is to be scaled by
   each<0, D / 32>([&](auto c) { each<0, 16>([&](auto e) { o[c.value][e.value] = 0.0f; }); });
 
   // Piece c of row r of keys lies at place c ^ k_swz(r) of its row, of values at c ^ v_swz(r): 16 lanes of a read meet 256
   // different bytes of the banks, and so do 16 of a write
   auto k_swz = [](int r) { return D == 128 ? (r & 7) | (r >> 5 & 1) << 3 : (r >> 1 & 3) | (r >> 5 & 1) << 2; };
   auto v_swz = [](int r) { return r >> 1 & 7; };
-  auto k_put = [&](int r, int c, u32x4 w) KVQ_INLINE { *reinterpret_cast<u32x4*>(ks + r * D + (c ^ k_swz(r)) * 8) = w; };
-  auto v_put = [&](int r, int c, u32x4 w) KVQ_INLINE { *reinterpret_cast<u32x4*>(vs + r * kUnit + (c ^ v_swz(r)) * 8) = w; };
-  const int k_tok = 32 * (col >> 2 & 1) + 4 * (col >> 3) + (col & 3);
-  auto read_k = [&](int i, int t) KVQ_INLINE {                      // channels 16 i + 8 g .., tile t
-    const int r = k_tok + 16 * t;
-    return *reinterpret_cast<const u32x4*>(ks + r * D + ((2 * i + g) ^ k_swz(r)) * 8);
+  auto k_put = [&](int par, int r, int c, u32x4 w) KVQ_INLINE { *reinterpret_cast<u32x4*>(ks[par] + r * D + (c ^ k_swz(r)) * 8) = w; };
+  auto v_put = [&](int par, int r, int c, u32x4 w) KVQ_INLINE { *reinterpret_cast<u32x4*>(vs[par] + r * kUnit + (c ^ v_swz(r)) * 8) = w; };
+  const int k_tok = 32 * (col >> 2 & 1) + 4 * (col >> 3) + (col & 3), k_x = g ^ k_swz(k_tok), v_x = (4 * g) ^ v_swz(col);
+  auto read_k = [&](auto par, int t) KVQ_INLINE {        // operand t of K: channels 16 (t / 2) + 8 g .., tile t % 2 (rows 16 apart have the
+    return *reinterpret_cast<const u32x4*>(ks[decltype(par)::value] + (k_tok + 16 * (t % 2)) * D + ((2 * (t / 2)) ^ k_x) * 8);   // same swizzle)
   };
-  auto read_v = [&](int c, int y) KVQ_INLINE {                      // channel 32 c + col, tokens 32 g + 8 y ..
-    const int r = 32 * c + col;
-    return *reinterpret_cast<const u32x4*>(vs + r * kUnit + ((4 * g + y) ^ v_swz(r)) * 8);
-  };
-  auto scores = [&]() KVQ_INLINE {
-    each<0, 16>([&](auto e) { s[0][e.value] = s[1][e.value] = 0.0f; });
-    each<0, D / 16>([&](auto i) { each<0, 2>([&](auto t) { s[t.value] = mfma32<BF16>(read_k(i.value, t.value), q[i.value], s[t.value]); }); });
-  };
-  // scores (register 16 t + e: token 32 g + 16 t + e of the unit) -> weights in s; o and l brought to the reference
-  auto soft = [&](float scale, bool masked, int lim) KVQ_INLINE {
-    if (masked)
-      each<0, 32>([&](auto i) { s[i.value / 16][i.value % 16] = i.value < lim ? s[i.value / 16][i.value % 16] : -INFINITY; });
-    float x = s[0][0];
-    each<1, 32>([&](auto i) { x = fmaxf(x, s[i.value / 16][i.value % 16]); });
-    // the reference moves only when a score passes it by 2^8: the accumulators are hardly ever scaled
-    x = xmax32(x * scale);
-    x = x > m + 8.0f ? x : m;
-    const float safe = x == -INFINITY ? 0.0f : x, grow = __builtin_amdgcn_exp2f(m - safe);
-    m = x;
-    float sum = 0.0f;
-    each<0, 32>([&](auto i) {
-      const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i.value / 16][i.value % 16], scale, -safe));
-      s[i.value / 16][i.value % 16] = p;
-      sum += p;
-    });
-    l = l * grow + sum;
-    if (__builtin_amdgcn_ballot_w64(grow != 1.0f)) each<0, D / 32>([&](auto c) { o[c.value] *= grow; });
+  auto read_v = [&](auto par, int t) KVQ_INLINE {        // operand t of V^T: channels 32 c + col, tokens 32 g + 8 y ..
+    const int y = t / (D / 32), c = t % (D / 32);
+    return *reinterpret_cast<const u32x4*>(vs[decltype(par)::value] + (32 * c + col) * kUnit + (y ^ v_x) * 8);
   };
 
   const int* pages = a.table + slot * a.max_blocks;
-  for (int u = u0; u < u_end; ++u) {
-    const int t0 = u * kUnit;
-    // the page of each half of the unit; half of the last one may lie behind the last page: masked
-    const int b0 = t0 / P, b1 = (t0 + 32) / P < last ? (t0 + 32) / P : last;
-    const int64_t p0 = static_cast<int64_t>(pages[b0]) * a.H + h, p1 = P == 32 ? static_cast<int64_t>(pages[b1]) * a.H + h : p0;
-    u32x4 kw[kPer], vw[kPer];
-    each<0, kPer>([&](auto i) {
-      const int x = tid + i.value * kThreads, r = x / (D / 16), c = x % (D / 16), ch = x / 4, t = x % 4 * 16;
-      kw[i.value] = *reinterpret_cast<const u32x4*>(a.kc + ((r < 32 ? p0 : p1) * P + ((t0 + r) & (P - 1))) * D + 16 * c);
-      vw[i.value] = *reinterpret_cast<const u32x4*>(a.vc + ((t < 32 ? p0 : p1) * D + ch) * P + ((t0 + t) & (P - 1)));
+  const int units = u_end - u0, tiles = units > 0 ? units | 1 : 0;
+  int whole = (vis0 < full ? vis0 : full) / kUnit - u0;             // units that every row sees whole
+  whole = whole < 0 ? 0 : whole < units ? whole : units;
+  // Codes of unit j, its pages a unit ahead of them.  (Behind the last unit: it again, masked; half of the last one may lie behind
+  // the last page.)
+  struct Ids {
+    int a, b;                                 // of the unit's halves
+  };
+  auto unit_of = [&](int j) KVQ_INLINE { return u0 + (j < units ? j : units - 1); };
+  auto ids_of = [&](int j) KVQ_INLINE {
+    const int b0 = unit_of(j) * kUnit / P, b1 = b0 < last ? b0 + 1 : last;
+    Ids r;
+    r.a = pages[b0];
+    r.b = kOne ? r.a : pages[b1];
+    return r;
+  };
+  auto at_of = [&](int id) KVQ_INLINE { return static_cast<int64_t>(__builtin_amdgcn_readfirstlane(id)) * a.H + h; };
+  u32x4 kw[kPer], vw[kPer];
+  auto fetch_k = [&](Ids ids, int j, auto i) KVQ_INLINE {
+    if constexpr (kOne) {
+      const uint8_t* base = a.kc + at_of(ids.a) * (P * D) + (unit_of(j) * kUnit & (P - 1)) * D;
+      kw[i.value] = *reinterpret_cast<const u32x4*>(base + (tid + i.value * kThreads) * 16);
+    } else if constexpr (D == 128) {          // a thread's pieces are of one half each
+      kw[i.value] = *reinterpret_cast<const u32x4*>(a.kc + at_of(i.value ? ids.b : ids.a) * (P * D) + tid * 16);
+    } else {
+      kw[i.value] = *reinterpret_cast<const u32x4*>(a.kc + at_of(wave >= 2 ? ids.b : ids.a) * (P * D) + (tid & 127) * 16);
+    }
+  };
+  auto fetch_v = [&](Ids ids, int j, auto i) KVQ_INLINE {
+    const int x = tid + i.value * kThreads, ch = x / 4, t = x % 4 * 16;
+    if constexpr (kOne) {
+      const uint8_t* base = a.vc + at_of(ids.a) * (P * D) + (unit_of(j) * kUnit & (P - 1));
+      vw[i.value] = *reinterpret_cast<const u32x4*>(base + ch * P + t);
+    } else {
+      const int64_t at = t < 32 ? at_of(ids.a) : at_of(ids.b);
+      vw[i.value] = *reinterpret_cast<const u32x4*>(a.vc + at * (P * D) + ch * P + (t & 31));
+    }
+  };
+  auto scales_of = [&](Ids ids) KVQ_INLINE { return reinterpret_cast<const float2*>(a.sc)[kOne || !g ? at_of(ids.a) : at_of(ids.b)]; };
+  // 8 codes of piece i / 2 each
+  auto widen_k = [&](int par, auto i) KVQ_INLINE {
+    const int x = tid + i.value / 2 * kThreads;
+    const u32x4 w = kw[i.value / 2];
+    k_put(par, x / (D / 16), 2 * (x % (D / 16)) + i.value % 2, widen8<CODE, BF16>(w[2 * (i.value % 2)], w[2 * (i.value % 2) + 1]));
+  };
+  auto widen_v = [&](int par, auto i) KVQ_INLINE {
+    const int x = tid + i.value / 2 * kThreads;
+    const u32x4 w = vw[i.value / 2];
+    v_put(par, x / 4, 2 * (x % 4) + i.value % 2, widen8<CODE, BF16>(w[2 * (i.value % 2)], w[2 * (i.value % 2) + 1]));
+  };
+
+  // The softmax of a unit in 18 shares: 0 and 1 find the reference, 2 + i the weights 2 i, 2 i + 1 (register 16 t + e: token 32
+  // g + 16 t + e).  lim: how many of this lane's 32 tokens the row sees; kz: what makes exponents of scores; r: what the weights
+  // are multiplied by.
+  constexpr float kLift = BF16 ? 0.0f : 7.0f; // log2 of the reference's weight
+  float top, safe, sum, kz, r, unit = 1.0f;   // of half types: o is held in units of a power of two near the value scale
+  bool unit_set = false;
+  auto share = [&](auto par, bool masked, int lim, auto which) KVQ_INLINE {
+    constexpr int i = decltype(which)::value;
+    auto& t = s[decltype(par)::value];
+    if constexpr (i < 2) {
+      if (masked) each<0, 16>([&](auto e) KVQ_INLINE { t[i][e.value] = 16 * i + e.value < lim ? t[i][e.value] : -INFINITY; });
+      float x = i == 0 ? t[0][0] : fmaxf(top, t[1][0]);
+      each<1, 16>([&](auto e) KVQ_INLINE { x = fmaxf(x, t[i][e.value]); });
+      top = x;
+      if constexpr (i == 1) {
+        // the reference moves only when a score passes it by 2^8: weights up to 256 (fp16: 2^15) cost no accuracy, and the
+        // accumulators are hardly ever scaled
+        x = xmax32(x * kz);
+        x = x > m + 8.0f ? x : m;
+        safe = x == -INFINITY ? 0.0f : x;
+        grow = __builtin_amdgcn_exp2f(m - safe);
+        safe -= kLift;
+        m = x;
+        l *= grow;
+        sum = 0.0f;
+      }
+    } else {
+      constexpr int k = 2 * (i - 2);
+      const float x = __builtin_amdgcn_exp2f(__builtin_fmaf(t[k / 16][k % 16], kz, -safe));
+      const float z = __builtin_amdgcn_exp2f(__builtin_fmaf(t[k / 16][k % 16 + 1], kz, -safe));
+      sum += x;
+      sum += z;
+      uint32_t w = pack2<BF16>(x * r, z * r);
+      asm volatile("" : "+v"(w));             // here, not behind the branch of the rescaling
+      p[decltype(par)::value][k / 8][k % 8 / 2] = w;
+      if constexpr (i == 17) {
+        l += sum;
+        asm volatile("" : "+v"(l));
+      }
+    }
+  };
+  constexpr int kV = 4 * (D / 32), kK = 2 * (D / 16);               // steps of the two products
+  constexpr std::integral_constant<int, 0> even{};
+  constexpr std::integral_constant<int, 1> odd{};
+  constexpr std::false_type no{};
+  constexpr std::true_type yes{};
+  auto add_v = [&](auto par, auto t, const u32x4& w) KVQ_INLINE {   // o += V P, operand t
+    constexpr int c = decltype(t)::value % (D / 32), y = decltype(t)::value / (D / 32);
+    o[c] = mfma32<BF16>(w, p[decltype(par)::value][y], o[c]);
+  };
+  // o += V P of the other parity (if `with`) beside the softmax of this one
+  auto values = [&](auto par, bool masked, auto with, int lim) KVQ_INLINE {
+    constexpr bool kWith = decltype(with)::value;
+    constexpr std::integral_constant<int, 1 - decltype(par)::value> other{};
+    u32x4 w[3];
+    if constexpr (kWith) {
+      w[0] = read_v(other, 0);
+      w[1] = read_v(other, 1);
+    }
+    each<0, kV>([&](auto t) KVQ_INLINE {
+      if constexpr (kWith) {
+        if constexpr (t.value + 2 < kV) w[(t.value + 2) % 3] = read_v(other, t.value + 2);
+        add_v(other, t, w[t.value % 3]);
+      }
+      each<t.value * 18 / kV, (t.value + 1) * 18 / kV>([&](auto i) KVQ_INLINE { share(par, masked, lim, i); });
+      __builtin_amdgcn_sched_barrier(0);
     });
-    const float2 z = reinterpret_cast<const float2*>(a.sc)[g ? p1 : p0];
-    __syncthreads();
-    each<0, kPer>([&](auto i) {
-      const int x = tid + i.value * kThreads, r = x / (D / 16), c = x % (D / 16), ch = x / 4, t = x % 4;
-      k_put(r, 2 * c, widen8<CODE, BF16>(kw[i.value][0], kw[i.value][1]));
-      k_put(r, 2 * c + 1, widen8<CODE, BF16>(kw[i.value][2], kw[i.value][3]));
-      v_put(ch, 2 * t, widen8<CODE, true>(vw[i.value][0], vw[i.value][1]));
-      v_put(ch, 2 * t + 1, widen8<CODE, true>(vw[i.value][2], vw[i.value][3]));
+  };
+  // S = K Q of the units of the other parity, beside `job` of each of its steps
+  auto products = [&](auto par, auto&& job) KVQ_INLINE {
+    constexpr int next = 1 - decltype(par)::value;
+    constexpr std::integral_constant<int, next> other{};
+    u32x4 w[4];
+    each<0, 16>([&](auto e) KVQ_INLINE { s[next][0][e.value] = s[next][1][e.value] = 0.0f; });
+    each<0, 3>([&](auto t) KVQ_INLINE { w[t.value] = read_k(other, t.value); });
+    each<0, kK>([&](auto t) KVQ_INLINE {
+      if constexpr (t.value + 3 < kK) w[(t.value + 3) % 4] = read_k(other, t.value + 3);
+      s[next][t.value % 2] = mfma32<BF16>(w[t.value % 4], q[t.value / 2], s[next][t.value % 2]);
+      job(t);
+      __builtin_amdgcn_sched_barrier(0);
     });
-    __syncthreads();
-    scores();
-    // a block that a row sees nothing of may hold a NaN scale
-    const int lim = (visible < full ? visible : full) - t0 - 32 * g;
-    float kz = z.x * a.scale, vz = z.y;
+  };
+  auto nothing = [](auto) {};
+  auto rescale = [&]() KVQ_INLINE {
+    if (__builtin_amdgcn_ballot_w64(grow != 1.0f)) each<0, D / 32>([&](auto c) KVQ_INLINE { o[c.value] *= grow; });
+  };
+  // kz and r of unit j from its scales; what o is to be scaled by for a new unit.  A block that a row sees nothing of may have the
+  // scale NaN.
+  float turn = 1.0f;
+  auto scale_for = [&](float2 z, bool masked, int lim) KVQ_INLINE {
+    kz = z.x * a.scale;
     kz = kz < FLT_MIN ? FLT_MIN : kz;
-    kz = lim > 0 ? kz : 1.0f;
-    vz = lim > 0 ? vz : 0.0f;
-    soft(kz, true, lim);
-    each<0, 4>([&](auto y) {
-      u32x4 hi, lo;
-      each<0, 4>([&](auto e) {
-        constexpr int at = y.value * 8 + 2 * e.value;
-        const float p = s[at / 16][at % 16] * vz, r = s[at / 16][at % 16 + 1] * vz;
-        hi[e.value] = pack2<true>(p, r);
-        if constexpr (!BF16) lo[e.value] = rest2<true>(p, r, hi[e.value]);
-      });
-      each<0, D / 32>([&](auto c) {
-        const u32x4 w = read_v(c.value, y.value);
-        o[c.value] = mfma32<true>(w, hi, o[c.value]);
-        if constexpr (!BF16) o[c.value] = mfma32<true>(w, lo, o[c.value]);
+    r = z.y;
+    turn = 1.0f;
+    if constexpr (!BF16) {
+      // half weights need the value scale near one: o is held in units of 2^k, changed where a scale is not within 2^-4 .. 1 of
+      // it (blocks of zeros, below 2^-100, and NaN change nothing)
+      const float v0 = __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(z.y)));
+      const float v1 = kOne ? v0 : __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(z.y), 32));
+      const float v = kOne ? v0 : fmaxf(v0, v1);
+      if (v > 0x1p-100f && !(v <= unit && v >= unit * 0x1p-4f && unit_set)) {
+        const float now = __uint_as_float((__float_as_uint(v) & 0x7f800000u) + 0x00800000u);      // 2^k above v
+        if (unit_set) turn = unit / now;
+        unit = now;
+        unit_set = true;
+      }
+      r = z.y < 0x1p-100f ? 0.0f : z.y * __builtin_amdgcn_rcpf(unit);              // of a power of two: exact
+    }
+    if (masked) {
+      kz = lim > 0 ? kz : 1.0f;
+      r = lim > 0 ? r : 0.0f;
+    }
+  };
+  auto lim_of = [&](int j) KVQ_INLINE { return j < units ? (visible < full ? visible : full) - (u0 + j) * kUnit - 32 * g : 0; };
+  // Pages of units on their way: id[i] of unit j + 1 + i when iteration j begins
+  Ids id[3], next_id;
+  float2 z_now, z_next;
+  auto step = [&](auto par, int j) KVQ_INLINE {
+    constexpr int kPar = decltype(par)::value;
+    const bool masked = j >= whole;
+    const int lim = lim_of(j);
+    scale_for(z_now, masked, lim);
+    z_now = scales_of(id[0]);
+    next_id = ids_of(j + 4);
+    __builtin_amdgcn_s_setprio(1);            // the softmax goes before the other wavefront's products
+    values(par, masked, yes, lim);
+    __builtin_amdgcn_s_setprio(0);
+    grow *= turn;
+    // unit j + 2 of K and j of V into the buffers of this parity, then the codes of the ones after them
+    products(par, [&](auto t) KVQ_INLINE {
+      constexpr int kJobs = 4 * kPer, kFirst = t.value * kJobs / kK, kEnd = (t.value + 1) * kJobs / kK;
+      each<kFirst, kEnd>([&](auto i) KVQ_INLINE {
+        if constexpr (i.value < 2 * kPer) {
+          widen_k(kPar, i);
+          if constexpr (i.value % 2) fetch_k(id[2], j + 3, std::integral_constant<int, i.value / 2>{});
+        } else {
+          constexpr std::integral_constant<int, i.value - 2 * kPer> v{};
+          widen_v(kPar, v);
+          if constexpr (v.value % 2) fetch_v(id[0], j + 1, std::integral_constant<int, v.value / 2>{});
+        }
       });
     });
+    rescale();
+    id[0] = id[1];
+    id[1] = id[2];
+    id[2] = next_id;
+    block_lds_barrier();
+  };
+  each<0, D / 16>([&](auto i) { q[i.value] = (q[i.value] ^ a.sign) & mask; });
+  if (tiles) {
+    const Ids first = ids_of(0);
+    id[0] = ids_of(1);
+    id[1] = ids_of(2);
+    id[2] = ids_of(3);
+    each<0, kPer>([&](auto i) { fetch_k(first, 0, i); });
+    each<0, kPer>([&](auto i) { fetch_v(first, 0, i); });
+    z_now = scales_of(first);
+    each<0, 2 * kPer>([&](auto i) { widen_k(0, i); });
+    each<0, kPer>([&](auto i) { fetch_k(id[0], 1, i); });
+    each<0, 2 * kPer>([&](auto i) { widen_v(0, i); });
+    each<0, kPer>([&](auto i) { fetch_v(id[0], 1, i); });
+    each<0, 2 * kPer>([&](auto i) { widen_k(1, i); });
+    each<0, kPer>([&](auto i) { fetch_k(id[1], 2, i); });
+    block_lds_barrier();
+    products(odd, nothing);                   // unit 0
+    const bool masked = whole == 0;
+    const int lim = lim_of(0);
+    scale_for(z_now, masked, lim);
+    z_now = scales_of(id[0]);
+    if (tiles > 1) {
+      block_lds_barrier();                    // K(2) takes the place of K(0)
+      each<0, 2 * kPer>([&](auto i) { widen_k(0, i); });
+      each<0, kPer>([&](auto i) { fetch_k(id[2], 3, i); });
+    }
+    values(even, masked, no, lim);
+    if (tiles > 1) {
+      products(even, nothing);                // unit 1
+      // ids of units 2, 3, 4
+      id[0] = id[1];
+      id[1] = id[2];
+      id[2] = ids_of(4);
+      block_lds_barrier();
+    }
+    for (int j = 1; j < tiles; j += 2) {
+      step(odd, j);
+      step(even, j + 1);
+    }
+    each<0, kV>([&](auto t) KVQ_INLINE { add_v(even, t, read_v(even, t.value)); });
   }
+  if constexpr (!BF16) each<0, D / 32>([&](auto c) KVQ_INLINE { o[c.value] *= unit; });
 
   // Units of the open block
   const int64_t open = ((static_cast<int64_t>(slot) * 2 + buf) * a.H + h) * P * D;
@@ -231,20 +405,20 @@ __global__ __launch_bounds__(kThreads, 2) void paged_wide_kernel(WideArgs a) {
     __syncthreads();
     if (tid == 0) flag[u - u_full] = 0;
     for (int x = tid; x < kUnit * kPieces; x += kThreads) {
-      const int r = x / kPieces, c = x % kPieces;
+      const int t = x / kPieces, c = x % kPieces;
       u32x4 w = {0, 0, 0, 0};
-      if (r < rest) w = *reinterpret_cast<const u32x4*>(ko + (off + r) * D + 8 * c);
-      k_put(r, c, w);
+      if (t < rest) w = *reinterpret_cast<const u32x4*>(ko + (off + t) * D + 8 * c);
+      k_put(0, t, c, w);
     }
     __syncthreads();
     // what is hidden from a row may be an infinity or a NaN, and what lies behind the last token anything: such values go in as
     // zeros, and the rows that do see one have it afterwards
     for (int x = tid; x < D * 8; x += kThreads) {
-      const int r = x / 8, c = x % 8;
+      const int ch = x / 8, c = x % 8;
       u32x4 w = {0, 0, 0, 0};
       bool bad = false;
       if (8 * c < rest) {
-        w = *reinterpret_cast<const u32x4*>(vo + r * P + off + 8 * c);
+        w = *reinterpret_cast<const u32x4*>(vo + ch * P + off + 8 * c);
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           const bool i0 = (w[e] & kInf) == kInf, i1 = (w[e] >> 16 & kInf) == kInf;
@@ -252,36 +426,26 @@ __global__ __launch_bounds__(kThreads, 2) void paged_wide_kernel(WideArgs a) {
           w[e] = (i0 ? 0u : w[e] & 0xffffu) | (i1 ? 0u : w[e] & 0xffff0000u);
         }
       }
-      v_put(r, c, w);
+      v_put(0, ch, c, w);
       if (bad) flag[u - u_full] = 1;
     }
     __syncthreads();
-    scores();
-    soft(a.scale, true, visible - t0 - 32 * g);
-    each<0, 4>([&](auto y) {
-      u32x4 hi, lo;
-      each<0, 4>([&](auto e) {
-        constexpr int at = y.value * 8 + 2 * e.value;
-        const float p = s[at / 16][at % 16], r = s[at / 16][at % 16 + 1];
-        hi[e.value] = pack2<BF16>(p, r);
-        if constexpr (!BF16) lo[e.value] = rest2<false>(p, r, hi[e.value]);
-      });
-      each<0, D / 32>([&](auto c) {
-        const u32x4 w = read_v(c.value, y.value);
-        o[c.value] = mfma32<BF16>(w, hi, o[c.value]);
-        if constexpr (!BF16) o[c.value] = mfma32<false>(w, lo, o[c.value]);
-      });
-    });
+    products(odd, nothing);
+    kz = a.scale;
+    r = 1.0f;
+    values(even, true, no, visible - t0 - 32 * g);
+    rescale();
+    each<0, kV>([&](auto t) KVQ_INLINE { add_v(even, t, read_v(even, t.value)); });
   }
   // A visible value that is infinite or NaN is its channel's result, however small its weight
   for (int u = first_open; u < u1; ++u) {
     const int off = (u - u_full) * kUnit, t0 = full + off, rest = len - t0 < kUnit ? len - t0 : kUnit;
     if (!flag[u - u_full]) continue;
-    for (int r = 0; r < rest; ++r)
+    for (int t = 0; t < rest; ++t)
       each<0, D / 32>([&](auto c) {
         each<0, 16>([&](auto e) {
-          const uint16_t x = vo[(32 * c.value + 8 * (e.value / 4) + 4 * g + e.value % 4) * P + off + r];
-          if (t0 + r < visible && (x & kInf) == kInf) o[c.value][e.value] += BF16 ? bf16_to_f32(x) : f16_to_f32(x);
+          const uint16_t x = vo[(32 * c.value + 8 * (e.value / 4) + 4 * g + e.value % 4) * P + off + t];
+          if (t0 + t < visible && (x & kInf) == kInf) o[c.value][e.value] += BF16 ? bf16_to_f32(x) : f16_to_f32(x);
         });
       });
   }

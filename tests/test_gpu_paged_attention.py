@@ -9,8 +9,9 @@ from test_gpu_pages import Mirror
 
 pytestmark = pytest.mark.gpu
 
-# a weight times a scale: rounded once for bf16, kept as two bf16 for fp16
-WEIGHT = {torch.bfloat16: HALF[torch.bfloat16], torch.float16: 2.0 ** -17}
+# A weight times its block's value scale is one number of the type, rounded to nearest once: off by at most half a step, 2^-8 (bf16) or
+# 2^-11 (fp16) of itself, 2^-32 of the block's largest value where it is below fp16's normal range (the bound has 2^-25 of it)
+WEIGHT = HALF
 
 
 def run(m, slots, counts, Hq, causal=True, layer=0, what="", scaling=None, q=None):
