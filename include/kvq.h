@@ -758,20 +758,31 @@ int kvq_paged_decode(const void* q, int64_t q_st, int64_t q_sh, int dtype, int64
  * len - count; otherwise every row sees all tokens of the slot, and rows of an empty one get zeros.  A visible value of the
  * open block that is infinite or NaN is its channel's result, whatever its weight; what is hidden changes nothing.
  * kvq_paged_plan (host memory: the accounts of the cache as they are, slots named, counts): fills `words` for a call of such rows,
- * rep <= 128 query heads to each of H KV heads; info[3] = {items, merges, parts}.  12 items + 8 merges words are needed: with
- * less room only info is set.  Pages that neighbours share in front are read once for all of them where that saves work.
- * The words go to the device as they are; they bound what kvq_paged_attention reads, together with the table on the
- * device.  workspace: kvq_paged_attention_workspace floats (none without parts), no clearing; calls that share one must not
- * overlap in time.
+ * rep <= 128 query heads to each of H KV heads.  Pages that neighbours share in front are read once for all of them where that
+ * saves work.  info[12] = {items, merges, parts, waves of a workgroup; words of the rest, its sequences, split items, run
+ * tokens, split tokens, joins, whether there are shared fronts, 0}: 12 items + 8 merges words go to kvq_paged_attention; behind
+ * them lies what kvq_paged_decode_held takes, which has the rows of sequences of at most few_rows rows a KV head (neighbours over
+ * shared pages: four times as many), where they are all, or of few_work units (64 tokens of a KV head) at least, cut as kvq_pages_extend cuts them by split_cap, few_cap and few_units.  With less room for words only
+ * info is set.  The words go to the device as they are; they bound what the calls read, together with the table on the device.
+ * Each writes its own rows of out (rows, Hq, D).
+ * kvq_paged_attention's workspace: kvq_paged_attention_workspace floats (none without parts), no clearing; calls that share one
+ * must not overlap in time.  kvq_paged_decode_held is kvq_paged_decode for rows whose tokens are in the cache (all = 0), or which
+ * see all tokens of the slot (all = 1); tickets only where no slot is named twice.
  * ---------------------------------------------------------------------------------------- */
 int kvq_paged_plan(const int64_t* lens, const int32_t* table, const uint8_t* open, int64_t slots, int64_t max_blocks,
-                   int64_t page, const int64_t* seq, const int64_t* counts, int64_t n, int64_t rep, int64_t H, int causal,
-                   int32_t* words, int64_t words_cap, int64_t* info);
-int64_t kvq_paged_attention_workspace(int64_t parts, int64_t H, int64_t D);
+                   int64_t page, const int64_t* seq, const int64_t* counts, int64_t n, int64_t rep, int64_t H, int64_t D, int causal,
+                   int64_t few_rows, int64_t few_work, int64_t split_cap, int64_t few_cap, int64_t few_units, int32_t* words, int64_t words_cap,
+                   int64_t* info);
+int64_t kvq_paged_attention_workspace(int64_t parts, int64_t waves, int64_t H, int64_t D);
 int kvq_paged_attention(const void* q, int64_t q_st, int64_t q_sh, int dtype, int64_t Hq, int64_t H, int64_t D, float scaling,
-                        const int32_t* words, int64_t items, int64_t merges, int64_t parts, const int32_t* table,
+                        const int32_t* words, int64_t items, int64_t merges, int64_t parts, int64_t waves, const int32_t* table,
                         int64_t max_blocks, int64_t page, int code, const uint8_t* kc, const uint8_t* vc, const float* sc,
                         const void* ko, const void* vo, void* out, float* workspace, int64_t workspace_floats, void* stream);
+int kvq_paged_decode_held(const void* q, int64_t q_st, int64_t q_sh, int dtype, int64_t rows, int64_t Hq, int64_t H, int64_t D,
+                          float scaling, const int32_t* words, int64_t sequences, int64_t split_items, int64_t run_tokens,
+                          int64_t split_tokens, int joins, const int32_t* table, int64_t max_blocks, int64_t page, int code,
+                          const uint8_t* kc, const uint8_t* vc, const float* sc, const void* ko, const void* vo, void* out,
+                          float* workspace, int64_t workspace_floats, int32_t* tickets, int all, void* stream);
 
 /* ------------------------------------------------------------------------------------------
  * The paged cache's accounts in device memory, for counts that only the device knows: lens (slots), refs (pages), open

@@ -92,6 +92,7 @@ struct DecodeArgs {
   uint16_t* out;                              // (rows, Hq, D)
   float* part;                                // (part_rows, H): D sums; behind them {max, sum} each
   int64_t part_rows;                          // rows of all split items
+  bool all;                                   // rows are no tokens of their slots: they see all tokens before
   int* tickets;                               // (slots, H, kApart) zeros, or none: joins by a launch of its own
 };
 constexpr int kApart = 32;                    // a cache line for each ticket: 208 workgroups 10.7 us, 12.2 with them side by side
@@ -279,14 +280,14 @@ __global__ __launch_bounds__(kThreads, 3) void paged_split_kernel(DecodeArgs a) 
   if (piece * kRows >= rows) return;
   const bool own = run.seq >= 0;              // or a shared front: whole pages that every row sees
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), col = lane & 15, g = lane >> 4;
-  const int pos0 = own ? run.pos0 : run.u1 * kUnit, len = own ? run.pos0 + run.tokens : run.u1 * kUnit, full = len / P * P;
+  const int pos0 = own ? run.pos0 : run.u1 * kUnit, len = own && !a.all ? run.pos0 + run.tokens : pos0, full = len / P * P;
   const int u_full = (full + kUnit - 1) / kUnit;
   const int u0 = run.u0 + (item - run.split0) * per, u1 = u0 + per < run.u1 ? u0 + per : run.u1;
 
   // the query rows: column col of B, channels 64 j + 16 g + 8 e ..
   const int row = piece * kRows + col, tok = row / a.rep, hq = row % a.rep;
   const bool live = row < rows;
-  const int visible = live ? pos0 + tok + 1 : 0;
+  const int visible = !live ? 0 : a.all ? len : pos0 + tok + 1;
   u32x4 q[2 * kJ];
   {
     const uint16_t* qp = a.q + (run.row0 + (live ? tok : 0)) * a.q_st + (static_cast<int64_t>(h) * a.rep + (live ? hq : 0)) * a.q_sh;
@@ -497,7 +498,7 @@ __global__ __launch_bounds__(kThreads, 3) void paged_split_kernel(DecodeArgs a) 
   const int64_t Hq = static_cast<int64_t>(a.H) * a.rep;
   if (single) {
     if (R >= rows) return;
-    const float inv = 1.0f / l;
+    const float inv = len ? 1.0f / l : 0.0f;  // rows of a slot without tokens: zeros
     uint16_t* out = a.out + ((static_cast<int64_t>(run.row0) + R / a.rep) * Hq + h * a.rep + R % a.rep) * D + c0;
     uint32_t p[kPer / 2];
 #pragma unroll
@@ -608,11 +609,11 @@ extern "C" int64_t kvq_paged_decode_workspace(int64_t split_tokens, int64_t H, i
   return split_tokens * rep * H * (D + 2);
 }
 
-extern "C" int kvq_paged_decode(const void* q, int64_t q_st, int64_t q_sh, int dtype, int64_t rows, int64_t Hq, int64_t H, int64_t D,
+static int paged_decode(const void* q, int64_t q_st, int64_t q_sh, int dtype, int64_t rows, int64_t Hq, int64_t H, int64_t D,
                                 float scaling, const int32_t* step, int64_t sequences, int64_t split_items, int64_t run_tokens,
                                 int64_t split_tokens, int joins, const int32_t* table, int64_t max_blocks, int64_t P, int code, const uint8_t* kc, const uint8_t* vc, const float* sc,
                                 const void* ko, const void* vo, void* out, float* workspace, int64_t workspace_floats, int32_t* tickets,
-                                void* stream) {
+                                bool all, void* stream) {
   KVQ_REQUIRE(D == 64 || D == 128, "kvq_paged_decode: head_dim must be 64 or 128 (got %lld)", static_cast<long long>(D));
   KVQ_REQUIRE(P == 32 || P == 64 || P == 128, "kvq_paged_decode: pages hold 32, 64 or 128 tokens");
   KVQ_REQUIRE(dtype == KVQ_F16 || dtype == KVQ_BF16, "kvq_paged_decode: queries must be fp16 or bf16");
@@ -629,7 +630,7 @@ extern "C" int kvq_paged_decode(const void* q, int64_t q_st, int64_t q_sh, int d
   DecodeArgs a{static_cast<const uint16_t*>(q), q_st, q_sh, step, static_cast<int>(sequences), table, max_blocks,
                static_cast<int>(H), static_cast<int>(rep), static_cast<int>(pieces), scaling * 1.44269504088896341f, kc, vc, sc,
                static_cast<const uint16_t*>(ko), static_cast<const uint16_t*>(vo), static_cast<uint16_t*>(out), workspace,
-               split_tokens * rep, rep * run_tokens * D <= kWaves * 128 && split_items * H <= 256 && split_items <= 64 * sequences ? tickets : nullptr};
+               split_tokens * rep, all, rep * run_tokens * D <= kWaves * 128 && split_items * H <= 256 && split_items <= 64 * sequences ? tickets : nullptr};
   // Joining in the launch, against a launch for it, in us.  One sequence, 8 KV heads: of 128 and 4096 tokens, 136 workgroups,
   // with one row 9.5 / 11.1, four 10.4 / 11.2, eight 12.6 / 11.2 (a wavefront's rows share its loads past the caches); of 64, four
   // rows 8.0 / 10.2, eight 8.7 / 10.2.  768 workgroups 26.1 / 23.9 (their stores and the wait for the last one); 2 KV heads, 30000
@@ -673,4 +674,20 @@ extern "C" int kvq_paged_decode(const void* q, int64_t q_st, int64_t q_sh, int d
   else by_page(std::integral_constant<int, 128>{});
   KVQ_LAUNCH_CHECK("kvq_paged_decode");
   return KVQ_OK;
+}
+
+extern "C" int kvq_paged_decode(const void* q, int64_t q_st, int64_t q_sh, int dtype, int64_t rows, int64_t Hq, int64_t H, int64_t D,
+                                float scaling, const int32_t* step, int64_t sequences, int64_t split_items, int64_t run_tokens,
+                                int64_t split_tokens, int joins, const int32_t* table, int64_t max_blocks, int64_t P, int code, const uint8_t* kc, const uint8_t* vc, const float* sc,
+                                const void* ko, const void* vo, void* out, float* workspace, int64_t workspace_floats, int32_t* tickets,
+                                void* stream) {
+  return paged_decode(q, q_st, q_sh, dtype, rows, Hq, H, D, scaling, step, sequences, split_items, run_tokens, split_tokens, joins, table, max_blocks, P, code, kc, vc, sc, ko, vo, out, workspace, workspace_floats, tickets, false, stream);
+}
+
+extern "C" int kvq_paged_decode_held(const void* q, int64_t q_st, int64_t q_sh, int dtype, int64_t rows, int64_t Hq, int64_t H, int64_t D,
+                                float scaling, const int32_t* step, int64_t sequences, int64_t split_items, int64_t run_tokens,
+                                int64_t split_tokens, int joins, const int32_t* table, int64_t max_blocks, int64_t P, int code, const uint8_t* kc, const uint8_t* vc, const float* sc,
+                                const void* ko, const void* vo, void* out, float* workspace, int64_t workspace_floats, int32_t* tickets,
+                                int all, void* stream) {
+  return paged_decode(q, q_st, q_sh, dtype, rows, Hq, H, D, scaling, step, sequences, split_items, run_tokens, split_tokens, joins, table, max_blocks, P, code, kc, vc, sc, ko, vo, out, workspace, workspace_floats, tickets, all != 0, stream);
 }

@@ -13,8 +13,17 @@ import numpy as np
 import torch
 
 from . import _lib
-from .pages import PagedCache, _address
+from .pages import FEW_BLOCKS, FEW_UNITS, SPLIT_BLOCKS, PagedCache, _address
 from .prompt import MAX_REP, rows16
+
+# Rows (query heads of a KV head times tokens) of a sequence up to which paged_decode's kernels take them, 16 at a time, and in
+# fours of these for neighbours over a shared text.  Theirs / those of tiles of 128 rows, 8 KV heads of 128: 16 sequences of
+# 16384 tokens with 32 rows 128 / 153 us, with 48 169 / 154; 64 of 1000 37 / 41 and 48 / 42; 8 behind a text of 8192, 16 rows each 23 / 25,
+# 32 each 35 / 28.
+FEW_ROWS = 32
+# Beside sequences of many rows those of few have launches of their own from this many units (64 tokens of a KV head) on: 10 us of
+# the chip's tiles.
+FEW_WORK = 2048
 
 
 class PagedPlan:
@@ -37,19 +46,28 @@ class PagedPlan:
         self.cache, self.Hq, self.causal = cache, int(Hq), bool(causal)
         self.slots, self.counts = s, c
         lens, table, _, open_, _ = cache._host
-        info = np.zeros(3, dtype=np.int64)
+        info = np.zeros(12, dtype=np.int64)
         args = (lens, table, open_, cache.slots, cache.max_blocks, cache.page, _address(s), _address(c), s.size,
-                self.Hq // cache.Hkv, cache.Hkv, int(self.causal))
-        words = np.empty(1024, dtype=np.int32)
+                self.Hq // cache.Hkv, cache.Hkv, cache.d, int(self.causal), FEW_ROWS, FEW_WORK, -(-SPLIT_BLOCKS[cache.d] // cache.Hkv),
+                -(-FEW_BLOCKS // cache.Hkv), FEW_UNITS // cache.Hkv)
+        words = np.empty(2048, dtype=np.int32)
         _lib.call("kvq_paged_plan", *args, _address(words), words.size, _address(info))
-        need = 12 * int(info[0]) + 8 * int(info[1])
+        many = 12 * int(info[0]) + 8 * int(info[1])
+        need = many + int(info[4])
         if need > words.size:
             words = np.empty(need, dtype=np.int32)
             _lib.call("kvq_paged_plan", *args, _address(words), words.size, _address(info))
         self.rows = int(c.sum())
-        self.items, self.merges, self.parts = info.tolist()
+        self.items, self.merges, self.parts, self.waves, _, self.sequences, *self._few, self._joins, fronts, _ = info.tolist()
         self.words = torch.from_numpy(words[:max(need, 1)]).to(cache.device)
-        self._empty = bool((cache._lens[s][c > 0] == 0).any())
+        self._at = (self.words.data_ptr(), self.words.data_ptr() + 4 * many)
+        lib = _lib.load()
+        self._floats = lib.kvq_paged_attention_workspace(self.parts, self.waves, cache.Hkv, cache.d) if self.parts else 0
+        self._few_floats = 0
+        if self._joins:
+            self._few_floats = lib.kvq_paged_decode_workspace(self._few[2], cache.Hkv, self.Hq // cache.Hkv, cache.d)
+        # a slot's tickets are one call's
+        self._tickets = not fronts and np.unique(s).size == s.size
         self._stamp = cache._stamp
         self._streams = {_lib.stream_of(self.words)}     # that the words belong to, or are recorded for
 
@@ -61,8 +79,8 @@ class PagedPlan:
                 raise ValueError("paged_attention: the plan's slots have changed since it was made")
 
     def workspace_floats(self) -> int:
-        """Float32 scratch of a call: none where the rows fill the chip without cutting along the tokens."""
-        return _lib.load().kvq_paged_attention_workspace(self.parts, self.cache.Hkv, self.cache.d)
+        """Float32 scratch of a call: none where nothing is cut along the tokens."""
+        return self._floats + self._few_floats
 
 
 def paged_attention(q: torch.Tensor, scaling: float, cache: PagedCache, layer: int, plan: PagedPlan, *,
@@ -93,18 +111,27 @@ def paged_attention(q: torch.Tensor, scaling: float, cache: PagedCache, layer: i
     if plan.rows == 0:
         return out
     q, qp, qt, qh = rows16(q)
-    stream = _lib.stream_of(q)
+    stream, floats = _lib.stream_of(q), plan._floats + plan._few_floats
     if workspace is None:
-        workspace = cache.sc.new_empty(plan.workspace_floats())
+        workspace = cache.sc.new_empty(floats)
     elif workspace.dtype != torch.float32 or not workspace.is_contiguous() or workspace.device != device:
         raise ValueError("workspace must be contiguous float32 on the cache's device")
+    elif workspace.numel() < floats:
+        raise ValueError(f"a workspace of {workspace.numel()} floats, {floats} needed")
     if (stream not in cache._streams or stream not in plan._streams) and not torch.cuda.is_current_stream_capturing():
         cache._use(stream)
         if stream not in plan._streams:
             plan.words.record_stream(torch.cuda.current_stream(device))
             plan._streams.add(stream)
     table, max_blocks, Hkv, d, page, code = cache._fixed
-    _lib.call_on(device, "kvq_paged_attention", qp, qt, qh, cache._type, plan.Hq, Hkv, d, float(scaling), plan.words.data_ptr(),
-                 plan.items, plan.merges, plan.parts, table, max_blocks, page, code, *cache._at[layer], out.data_ptr(),
-                 workspace.data_ptr(), workspace.numel(), stream)
+    at, few = plan._at
+    ws = workspace.data_ptr()
+    if plan.items:
+        _lib.call_on(device, "kvq_paged_attention", qp, qt, qh, cache._type, plan.Hq, Hkv, d, float(scaling), at,
+                     plan.items, plan.merges, plan.parts, plan.waves, table, max_blocks, page, code, *cache._at[layer], out.data_ptr(),
+                     ws, plan._floats, stream)
+    if plan.sequences:
+        _lib.call_on(device, "kvq_paged_decode_held", qp, qt, qh, cache._type, plan.rows, plan.Hq, Hkv, d, float(scaling), few,
+                     plan.sequences, *plan._few, plan._joins, table, max_blocks, page, code, *cache._at[layer], out.data_ptr(),
+                     ws + 4 * plan._floats, plan._few_floats, cache._tickets[layer] if plan._tickets else None, int(not plan.causal), stream)
     return out

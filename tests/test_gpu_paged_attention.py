@@ -14,6 +14,17 @@ pytestmark = pytest.mark.gpu
 WEIGHT = HALF
 
 
+@pytest.fixture(params=[0, None, 1 << 30], ids=["tiles", "by rows", "16 rows"], autouse=True)
+def few_rows(request, monkeypatch):
+    """Every call by the kernels of many rows, by those that it gets, and by the decode's."""
+    import kvq.paged
+    if request.param is not None:
+        monkeypatch.setattr(kvq.paged, "FEW_ROWS", request.param)
+    else:
+        monkeypatch.setattr(kvq.paged, "FEW_WORK", 1)                # however short they are
+    return request.param
+
+
 def run(m, slots, counts, Hq, causal=True, layer=0, what="", scaling=None, q=None):
     """One call, every row checked; returns (plan, q, out)."""
     import kvq
@@ -48,7 +59,7 @@ def test_chunks(page, d, Hkv, rep, code, dtype):
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
 @pytest.mark.parametrize("page,d,Hkv,rep", [(32, 64, 2, 4), (64, 128, 1, 3), (128, 64, 1, 8)])
-def test_shared_text(page, d, Hkv, rep, dtype):
+def test_shared_text(page, d, Hkv, rep, dtype, few_rows):
     """Questions of forks side by side, others between, uneven; and the same rows again, and each alone."""
     import kvq
     m = Mirror(slots=10, pages=200, max_tokens=1500, Hkv=Hkv, d=d, page=page, dtype=dtype, seed=page)
@@ -58,7 +69,7 @@ def test_shared_text(page, d, Hkv, rep, dtype):
     m.push([0, 2, 3, 4, 5, 7, 8, 9], [1, 5, 17, 3, 90, 2, 40, 8])
     plan, q, out = run(m, [0, 2, 3, 4, 5, 7, 8, 9], counts, rep * Hkv, what="forks")
     # the seven that share a text are joined, a tile of their rows at a time
-    assert plan.merges >= 7 and torch.equal(out, kvq.paged_attention(q.cuda(), d ** -0.5, m.cache, 0, plan))
+    assert (few_rows != 0 or plan.merges >= 7) and torch.equal(out, kvq.paged_attention(q.cuda(), d ** -0.5, m.cache, 0, plan))
     run(m, [2, 9, 3, 6, 4], [5, 0, 17, 9, 3], rep * Hkv, what="between")
     run(m, [6, 6], [900, 30], Hkv, what="the text itself, twice")
 
@@ -79,12 +90,15 @@ def test_cross(page, d, Hkv, rep, code, dtype):
 
 @pytest.mark.parametrize("causal", [True, False])
 @pytest.mark.parametrize("n,rep,d", [(4099, 4, 64), (2600, 1, 128), (5000, 2, 64)])
-def test_cut_along_the_tokens(n, rep, d, causal):
+def test_cut_along_the_tokens(n, rep, d, causal, few_rows):
     """Few rows over many tokens: parts and their joins, with and without a shared text."""
     m = Mirror(slots=4, pages=300, max_tokens=5200, Hkv=1, d=d, page=64, seed=n)
     m.push([0, 1], [n, 700])
     plan, _, _ = run(m, [0, 1], [3, 2], rep, causal, what="cut")
-    assert plan.parts > 2 and plan.merges == 2
+    if few_rows == 0:
+        assert plan.parts > 2 and plan.merges == 2 and not plan.sequences
+    else:
+        assert not plan.items and plan.sequences == 2
     m.fork([0, 0], [2, 3])
     m.push([2, 3], [5, 40])
     run(m, [2, 3], [5, 7], rep, causal, what="cut text")
@@ -153,6 +167,21 @@ def test_hidden_values_change_nothing(side, value, page, dtype):
                   WEIGHT[dtype], "other channels")
 
 
+def test_few_and_many_rows_in_one_call(few_rows):
+    """Single tokens, drafts and long chunks side by side, nothing for one, a shared text among the chunks, a slot named twice."""
+    m = Mirror(slots=9, pages=200, max_tokens=1500, Hkv=2, d=64, page=32, seed=12)
+    m.push([0, 1, 2, 3, 4], [900, 31, 640, 70, 1])
+    m.fork([2, 2], [5, 6])
+    m.push([5, 6], [100, 60])
+    slots, counts = [4, 0, 2, 5, 6, 3, 7, 1], [1, 2, 50, 100, 60, 70, 0, 1]
+    plan, _, _ = run(m, slots, counts, 8, what="mixed")
+    assert few_rows is not None or plan.items and plan.sequences == 7
+    run(m, [1, 4, 0], [1, 1, 100], 8, what="few in front")
+    run(m, [0, 4, 1], [100, 1, 1], 8, what="many in front")
+    run(m, [0, 0, 1, 0, 7, 3], [2, 1, 3, 40, 2, 1], 8, causal=False, what="cross")
+    run(m, [0, 1, 0], [1, 1, 1], 8, causal=False, what="named twice")
+
+
 def test_replays_streams_and_strides():
     """A captured call replayed with other rows, another stream, expanded rows, the caller's output and workspace."""
     import kvq
@@ -161,7 +190,7 @@ def test_replays_streams_and_strides():
     m.fork([0, 0], [1, 2])
     m.push([1, 2], [4, 9])
     plan = kvq.PagedPlan(m.cache, [1, 2], [4, 9], 8)
-    assert plan.parts
+    assert plan.workspace_floats()
     q = m.rand(13, 8).cuda()
     out = torch.empty_like(q)
     ws = torch.full((plan.workspace_floats(),), float("nan"), device="cuda")
@@ -216,6 +245,12 @@ def test_refusals():
     other = Mirror(slots=3, Hkv=2, d=64, page=32).cache
     with pytest.raises(ValueError, match="another cache"):
         call(cache=other)
+    long = Mirror(slots=1, pages=200, max_tokens=6000, Hkv=1, d=64, page=32)
+    long.push([0], [5000])
+    cut = kvq.PagedPlan(long.cache, [0], [2], 4)
+    assert cut.workspace_floats() > 0
+    with pytest.raises(ValueError, match="workspace"):
+        kvq.paged_attention(long.rand(2, 4).cuda(), 0.1, long.cache, 0, cut, workspace=ws)
     m.push([2], [3])
     call()                                     # another slot's tokens
     m.push([1], [1])
