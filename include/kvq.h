@@ -760,7 +760,8 @@ int kvq_paged_decode(const void* q, int64_t q_st, int64_t q_sh, int dtype, int64
  * kvq_paged_plan (host memory: the accounts of the cache as they are, slots named, counts): fills `words` for a call of such rows,
  * rep <= 128 query heads to each of H KV heads.  Pages that neighbours share in front are read once for all of them where that
  * saves work.  info[12] = {items, merges, parts, waves of a workgroup; words of the rest, its sequences, split items, run
- * tokens, split tokens, joins, whether there are shared fronts, 0}: 12 items + 8 merges words go to kvq_paged_attention; behind
+ * tokens, split tokens, joins, whether there are shared fronts; the
+ * most parts of a join}: 12 items + 8 merges words go to kvq_paged_attention; behind
  * them lies what kvq_paged_decode_held takes, which has the rows of sequences of at most few_rows rows a KV head (neighbours over
  * shared pages: four times as many), where they are all, or of few_work units (64 tokens of a KV head) at least, cut as kvq_pages_extend cuts them by split_cap, few_cap and few_units.  With less room for words only
  * info is set.  The words go to the device as they are; they bound what the calls read, together with the table on the device.
@@ -775,7 +776,7 @@ int kvq_paged_plan(const int64_t* lens, const int32_t* table, const uint8_t* ope
                    int64_t* info);
 int64_t kvq_paged_attention_workspace(int64_t parts, int64_t waves, int64_t H, int64_t D);
 int kvq_paged_attention(const void* q, int64_t q_st, int64_t q_sh, int dtype, int64_t Hq, int64_t H, int64_t D, float scaling,
-                        const int32_t* words, int64_t items, int64_t merges, int64_t parts, int64_t waves, const int32_t* table,
+                        const int32_t* words, int64_t items, int64_t merges, int64_t parts, int64_t most_parts, int64_t waves, const int32_t* table,
                         int64_t max_blocks, int64_t page, int code, const uint8_t* kc, const uint8_t* vc, const float* sc,
                         const void* ko, const void* vo, void* out, float* workspace, int64_t workspace_floats, void* stream);
 int kvq_paged_decode_held(const void* q, int64_t q_st, int64_t q_sh, int dtype, int64_t rows, int64_t Hq, int64_t H, int64_t D,

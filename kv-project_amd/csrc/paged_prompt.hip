@@ -23,7 +23,7 @@ struct PlanMerge {
 struct PlanWords {
   std::vector<PlanItem> items;
   std::vector<PlanMerge> merges;
-  int64_t parts = 0;
+  int64_t parts = 0, most_parts = 0;          // of a row that is joined
   int waves = 4;                              // of a workgroup: 32 rows of a tile each
 };
 
@@ -127,14 +127,14 @@ Cut best_cut(const std::vector<Tile>& tiles, int64_t places, int64_t H) {
   Cut best{longest, INT64_MAX};
   std::vector<int64_t> costs, ends(places);
   for (int64_t k : {1, 2, 3, 4, 5, 6, 8, 10, 12, 16, 20, 24, 32, 48, 64, 96, 128}) {
-    const int64_t most = std::max<int64_t>((longest + k - 1) / k, 2);
+    const int64_t most = (longest + k - 1) / k | 1;          // the kernel rounds units up to an odd number
     costs.clear();
     int64_t parts = 0;
     for (const Tile& t : tiles) {
       const int64_t cut = cut_of(t, most), units = t.u1 - t.u0;
       const bool joins = t.joins || cut > 1;
       parts += joins ? cut : 0;
-      for (int64_t c = 0; c < cut; ++c) costs.push_back(units * (c + 1) / cut - units * c / cut + kStartUnits + joins);
+      for (int64_t c = 0; c < cut; ++c) costs.push_back(((units * (c + 1) / cut - units * c / cut) | 1) + kStartUnits + joins);
     }
     if (static_cast<int64_t>(costs.size()) > many) break;
     std::sort(costs.begin(), costs.end(), std::greater<int64_t>());
@@ -146,7 +146,7 @@ Cut best_cut(const std::vector<Tile>& tiles, int64_t places, int64_t H) {
     }
     const int64_t end = *std::max_element(ends.begin(), ends.end()) + (parts ? kMergeUnits + parts * H / kPartsPerUnit : 0);
     if (end < best.end) best = {most, end};
-    if (most == 2) break;
+    if (most <= 3) break;
   }
   return best;
 }
@@ -197,6 +197,7 @@ void plan_wide(const std::vector<Seq>& some, const std::vector<Group>& groups, c
         w[7] = in;
       }
       w[1] = toks;
+      out.most_parts = std::max(out.most_parts, std::max(w[3], w[6]));
       PlanMerge m;
       for (int k = 0; k < kMergeWords; ++k) m.w[k] = static_cast<int32_t>(w[k]);
       out.merges.push_back(m);
@@ -271,7 +272,7 @@ extern "C" int kvq_paged_plan(const int64_t* lens, const int32_t* table, const u
       }, open, table, max_blocks, page, m, std::max(split_cap, m), few_cap, few_units, INT64_C(1) << 31, INT64_C(1) << 31, desc.data());
     const int64_t found[12] = {static_cast<int64_t>(p.items.size()), static_cast<int64_t>(p.merges.size()), p.parts, p.waves,
                                static_cast<int64_t>(desc.size()), few ? m : 0, few ? desc[2] : 0, few ? desc[6] : 0, few ? desc[7] : 0,
-                               few ? desc[10] : 0, few ? desc[8] > m : 0, 0};
+                               few ? desc[10] : 0, few ? desc[8] > m : 0, p.most_parts};
     memcpy(info, found, sizeof(found));
     KVQ_REQUIRE(!few || found[8] >= 0, "kvq_paged_plan: too many rows");
     if (!words || words_cap < kItemWords * info[0] + kMergeWords * info[1] + info[4]) return KVQ_OK;
@@ -289,7 +290,7 @@ extern "C" int64_t kvq_paged_attention_workspace(int64_t parts, int64_t waves, i
 }
 
 extern "C" int kvq_paged_attention(const void* q, int64_t q_st, int64_t q_sh, int dtype, int64_t Hq, int64_t H, int64_t D, float scaling,
-                                   const int32_t* words, int64_t items, int64_t merges, int64_t parts, int64_t waves, const int32_t* table,
+                                   const int32_t* words, int64_t items, int64_t merges, int64_t parts, int64_t most_parts, int64_t waves, const int32_t* table,
                                    int64_t max_blocks, int64_t P, int code, const uint8_t* kc, const uint8_t* vc, const float* sc,
                                    const void* ko, const void* vo, void* out, float* workspace, int64_t workspace_floats, void* stream) {
   KVQ_REQUIRE(D == 64 || D == 128, "kvq_paged_attention: head_dim must be 64 or 128 (got %lld)", static_cast<long long>(D));
@@ -312,7 +313,7 @@ extern "C" int kvq_paged_attention(const void* q, int64_t q_st, int64_t q_sh, in
   const WideArgs a{static_cast<const uint16_t*>(q), q_st, q_sh, words, table, max_blocks, static_cast<int>(H), static_cast<int>(Hq / H),
                    scale < FLT_MIN ? FLT_MIN : scale, std::signbit(scaling) ? 0x80008000u : 0u, kc, vc, sc,
                    static_cast<const uint16_t*>(ko), static_cast<const uint16_t*>(vo), static_cast<uint16_t*>(out), workspace};
-  (D == 64 ? launch_wide_64 : launch_wide_128)(a, static_cast<int>(P), code, dtype == KVQ_BF16, static_cast<int>(waves), items, merges, static_cast<hipStream_t>(stream));
+  (D == 64 ? launch_wide_64 : launch_wide_128)(a, static_cast<int>(P), code, dtype == KVQ_BF16, static_cast<int>(waves), items, merges, most_parts, static_cast<hipStream_t>(stream));
   KVQ_LAUNCH_CHECK("kvq_paged_attention");
   return KVQ_OK;
 }

@@ -40,10 +40,11 @@ struct WideArgs {
 };
 
 constexpr int kItemWords = 12, kMergeWords = 8;
+constexpr int64_t kSpread = 12;               // parts of a row from which on a workgroup joins it
 
 // The launches of one head_dim: the rows, then the joins
-void launch_wide_64(const WideArgs& a, int page, int code, bool bf16, int waves, int64_t items, int64_t merges, hipStream_t stream);
-void launch_wide_128(const WideArgs& a, int page, int code, bool bf16, int waves, int64_t items, int64_t merges, hipStream_t stream);
+void launch_wide_64(const WideArgs& a, int page, int code, bool bf16, int waves, int64_t items, int64_t merges, int64_t most_parts, hipStream_t stream);
+void launch_wide_128(const WideArgs& a, int page, int code, bool bf16, int waves, int64_t items, int64_t merges, int64_t most_parts, hipStream_t stream);
 
 namespace {
 
@@ -167,6 +168,7 @@ __global__ __launch_bounds__(64 * W, 2) void paged_wide_kernel(WideArgs a) {
     return *reinterpret_cast<const u32x4*>(vs[decltype(par)::value] + (32 * c + col) * kUnit + (y ^ v_x) * 8);
   };
 
+  if (tid < 2) flag[tid] = 0;                 // a barrier later
   const int* pages = a.table + slot * a.max_blocks;
   const int units = u_end - u0, tiles = units > 0 ? units | 1 : 0;
   int whole = (vis0 < full ? vis0 : full) / kUnit - u0;             // units that every row sees whole
@@ -306,7 +308,6 @@ __global__ __launch_bounds__(64 * W, 2) void paged_wide_kernel(WideArgs a) {
       if constexpr (t.value + 3 < kK) w[(t.value + 3) % 4] = read_k(other, t.value + 3);
       s[next][t.value % 2] = mfma32<BF16>(w[t.value % 4], q[t.value / 2], s[next][t.value % 2]);
       job(t);
-      __builtin_amdgcn_sched_barrier(0);
     });
   };
   auto nothing = [](auto) {};
@@ -384,15 +385,19 @@ __global__ __launch_bounds__(64 * W, 2) void paged_wide_kernel(WideArgs a) {
     id[0] = ids_of(1);
     id[1] = ids_of(2);
     id[2] = ids_of(3);
+    // keys of two units and values of one on their way at once
+    each<0, kPer>([&](auto i) { fetch_k(id[0], 1, i); });
+    u32x4 later[kPer];
+    each<0, kPer>([&](auto i) { later[i.value] = kw[i.value]; });
     each<0, kPer>([&](auto i) { fetch_k(first, 0, i); });
     each<0, kPer>([&](auto i) { fetch_v(first, 0, i); });
     z_now = scales_of(first);
     each<0, 2 * kPer>([&](auto i) { widen_k(0, i); });
-    each<0, kPer>([&](auto i) { fetch_k(id[0], 1, i); });
-    each<0, 2 * kPer>([&](auto i) { widen_v(0, i); });
-    each<0, kPer>([&](auto i) { fetch_v(id[0], 1, i); });
+    each<0, kPer>([&](auto i) { kw[i.value] = later[i.value]; });
     each<0, 2 * kPer>([&](auto i) { widen_k(1, i); });
     each<0, kPer>([&](auto i) { fetch_k(id[1], 2, i); });
+    each<0, 2 * kPer>([&](auto i) { widen_v(0, i); });
+    each<0, kPer>([&](auto i) { fetch_v(id[0], 1, i); });
     block_lds_barrier();
     products(odd, nothing);                   // unit 0
     const bool masked = whole == 0;
@@ -427,31 +432,31 @@ __global__ __launch_bounds__(64 * W, 2) void paged_wide_kernel(WideArgs a) {
   const int first_open = u0 > u_full ? u0 : u_full;
   for (int u = first_open; u < u1; ++u) {
     const int off = (u - u_full) * kUnit, t0 = full + off, rest = len - t0 < kUnit ? len - t0 : kUnit;
-    __syncthreads();
-    if (tid == 0) flag[u - u_full] = 0;
-    for (int x = tid; x < kUnit * kPieces; x += kThreads) {
-      const int t = x / kPieces, c = x % kPieces;
-      u32x4 w = {0, 0, 0, 0};
-      if (t < rest) w = *reinterpret_cast<const u32x4*>(ko + (off + t) * D + 8 * c);
-      k_put(0, t, c, w);
+    constexpr int kMine = kUnit * kPieces / kThreads;
+    u32x4 kx[kMine], vx[kMine];               // behind the last token: zeros
+#pragma unroll
+    for (int i = 0; i < kMine; ++i) {
+      const int x = tid + i * kThreads, t = x / kPieces, ch = x / 8;
+      kx[i] = vx[i] = u32x4{0, 0, 0, 0};
+      if (t < rest) kx[i] = *reinterpret_cast<const u32x4*>(ko + (off + t) * D + 8 * (x % kPieces));
+      if (8 * (x % 8) < rest) vx[i] = *reinterpret_cast<const u32x4*>(vo + ch * P + off + 8 * (x % 8));
     }
     __syncthreads();
     // what is hidden from a row may be an infinity or a NaN, and what lies behind the last token anything: such values go in as
     // zeros, and the rows that do see one have it afterwards
-    for (int x = tid; x < D * 8; x += kThreads) {
-      const int ch = x / 8, c = x % 8;
-      u32x4 w = {0, 0, 0, 0};
-      bool bad = false;
-      if (8 * c < rest) {
-        w = *reinterpret_cast<const u32x4*>(vo + ch * P + off + 8 * c);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const bool i0 = (w[e] & kInf) == kInf, i1 = (w[e] >> 16 & kInf) == kInf;
-          bad |= i0 || i1;
-          w[e] = (i0 ? 0u : w[e] & 0xffffu) | (i1 ? 0u : w[e] & 0xffff0000u);
-        }
+    for (int i = 0; i < kMine; ++i) {
+      const int x = tid + i * kThreads;
+      k_put(0, x / kPieces, x % kPieces, kx[i]);
+      u32x4 w = vx[i];
+      bool bad = false;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const bool i0 = (w[e] & kInf) == kInf, i1 = (w[e] >> 16 & kInf) == kInf;
+        bad |= i0 || i1;
+        w[e] = (i0 ? 0u : w[e] & 0xffffu) | (i1 ? 0u : w[e] & 0xffff0000u);
       }
-      v_put(0, ch, c, w);
+      v_put(0, x / 8, x % 8, w);
       if (bad) flag[u - u_full] = 1;
     }
     __syncthreads();
@@ -501,61 +506,90 @@ __global__ __launch_bounds__(64 * W, 2) void paged_wide_kernel(WideArgs a) {
   });
 }
 
-// One wavefront per row that is joined of several parts: those of its own tile and those of a tile of its shared front
-template <int D, bool BF16, int W>
+// D / 4 lanes per row that is joined of several parts, its sums 16 bytes a lane: those of its own tile and those of a tile of its
+// shared front, four on their way at once.  SPREAD: a workgroup per row, for many parts of few rows.  What bounds it: the parts'
+// way from memory (16 questions of 17 to 391 tokens behind 8131, 123 MB of them: 20 us).
+template <int D, bool BF16, int W, bool SPREAD>
 __global__ __launch_bounds__(kThreads) void paged_wide_merge_kernel(WideArgs a, const int* __restrict__ merges) {
-  constexpr int kTileRows = 32 * W;
+  constexpr int kTileRows = 32 * W, kLanes = D / 4, kGroups = kThreads / kLanes;
   const int* w = merges + kMergeWords * (blockIdx.x / a.H);
-  const int h = blockIdx.x % a.H, lane = threadIdx.x & 63, row = blockIdx.y * (kThreads / 64) + (threadIdx.x >> 6);
+  const int group = threadIdx.x / kLanes, h = blockIdx.x % a.H, lane = threadIdx.x % kLanes, row = SPREAD ? blockIdx.y : blockIdx.y * kGroups + group;
   const int tok = row / a.rep, hq = row % a.rep;
   if (tok >= w[1]) return;
   constexpr int64_t kPart = kTileRows * (D + 2);
   const int64_t stride = a.H * kPart;
-  float top = -INFINITY, l = 0.0f, o[D / 64] = {};
+  float top = -INFINITY, l = 0.0f;
+  f32x4 o = {0, 0, 0, 0};
 #pragma unroll
   for (int side = 0; side < 2; ++side) {
     const int first = w[2 + 3 * side], parts = w[3 + 3 * side], r = (w[4 + 3 * side] + tok) * a.rep + hq;
+    const int from = SPREAD ? parts * group / kGroups : 0, to = SPREAD ? parts * (group + 1) / kGroups : parts;
     const float* part = a.part + (static_cast<int64_t>(first) * a.H + h) * kPart;
-    for (int i0 = 0; i0 < parts; i0 += 64) {
-      const int i = i0 + lane;
-      const float2 st = i < parts ? *reinterpret_cast<const float2*>(part + i * stride + kTileRows * D + 2 * r) : make_float2(-INFINITY, 0.0f);
-      const float m = fmaxf(top, wave_max(st.x)), safe = m == -INFINITY ? 0.0f : m;
-      const float old = __builtin_amdgcn_exp2f(top - safe), f = __builtin_amdgcn_exp2f(st.x - safe);
-      l = l * old + wave_sum(f * st.y);
+    for (int i0 = from; i0 < to; i0 += 4) {   // behind the last: it again, unused
+      f32x4 x[4];
+      float2 st[4];
 #pragma unroll
-      for (int e = 0; e < D / 64; ++e) o[e] = weigh(old, o[e]);
-      const int most = parts - i0 < 64 ? parts - i0 : 64;
-      for (int k0 = 0; k0 < most; k0 += 8) {  // 8 on their way at once; behind the last: it again, unused
-        float x[8][D / 64];
-#pragma unroll
-        for (int k = 0; k < 8; ++k)
-#pragma unroll
-          for (int e = 0; e < D / 64; ++e) x[k][e] = part[(i0 + (k0 + k < most ? k0 + k : most - 1)) * stride + r * D + lane * (D / 64) + e];
-#pragma unroll
-        for (int k = 0; k < 8; ++k) {
-          const float fk = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(f), k0 + k < most ? k0 + k : 0));
-#pragma unroll
-          for (int e = 0; e < D / 64; ++e) o[e] += k0 + k < most ? weigh(fk, x[k][e]) : 0.0f;
-        }
+      for (int k = 0; k < 4; ++k) {
+        const float* at = part + (i0 + k < to ? i0 + k : to - 1) * stride;
+        x[k] = *reinterpret_cast<const f32x4*>(at + r * D + 4 * lane);
+        st[k] = *reinterpret_cast<const float2*>(at + kTileRows * D + 2 * r);
       }
+      float m = top;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) m = fmaxf(m, st[k].x);
+      const float safe = m == -INFINITY ? 0.0f : m, old = __builtin_amdgcn_exp2f(top - safe);
       top = m;
+      l *= old;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) o[e] = weigh(old, o[e]);
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        if (i0 + k >= to) break;
+        const float f = __builtin_amdgcn_exp2f(st[k].x - safe);
+        l += f * st[k].y;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[e] += weigh(f, x[k][e]);
+      }
+    }
+  }
+  if constexpr (SPREAD) {
+    __shared__ f32x4 sums[kGroups][kLanes];
+    __shared__ float2 stats[kGroups];
+    sums[group][lane] = o;
+    if (lane == 0) stats[group] = make_float2(top, l);
+    __syncthreads();                          // a workgroup is one row: all or none get here
+    if (group) return;
+    top = stats[0].x;
+#pragma unroll
+    for (int k = 1; k < kGroups; ++k) top = fmaxf(top, stats[k].x);
+    const float safe = top == -INFINITY ? 0.0f : top;
+    l = 0.0f;
+    o = f32x4{0, 0, 0, 0};
+#pragma unroll
+    for (int k = 0; k < kGroups; ++k) {
+      const float f = __builtin_amdgcn_exp2f(stats[k].x - safe);
+      l += f * stats[k].y;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) o[e] += weigh(f, sums[k][lane][e]);
     }
   }
   const float inv = 1.0f / l;                 // a row that is joined sees a token at least
-  uint16_t* out = a.out + ((w[0] + static_cast<int64_t>(tok)) * a.H * a.rep + h * a.rep + hq) * D + lane * (D / 64);
-#pragma unroll
-  for (int e = 0; e < D / 64; ++e) out[e] = BF16 ? f32_to_bf16(o[e] * inv) : f32_to_f16(o[e] * inv);
+  uint16_t* out = a.out + ((w[0] + static_cast<int64_t>(tok)) * a.H * a.rep + h * a.rep + hq) * D + 4 * lane;
+  *reinterpret_cast<uint2*>(out) = make_uint2(pack2<BF16>(o[0] * inv, o[1] * inv), pack2<BF16>(o[2] * inv, o[3] * inv));
 }
 
 template <int D>
-void launch_wide(const WideArgs& a, int page, int code, bool bf16, int waves, int64_t items, int64_t merges, hipStream_t stream) {
+void launch_wide(const WideArgs& a, int page, int code, bool bf16, int waves, int64_t items, int64_t merges, int64_t most_parts, hipStream_t stream) {
   auto run = [&](auto p, auto c, auto t, auto w) {
     constexpr int P_ = decltype(p)::value, C_ = decltype(c)::value, W_ = decltype(w)::value;
     constexpr bool T_ = decltype(t)::value;
     hipLaunchKernelGGL((paged_wide_kernel<D, P_, C_, T_, W_>), dim3(static_cast<uint32_t>(items * a.H)), dim3(64 * W_), 0, stream, a);
-    if (merges)
-      hipLaunchKernelGGL((paged_wide_merge_kernel<D, T_, W_>), dim3(static_cast<uint32_t>(merges * a.H), 32 * W_ * 64 / kThreads), dim3(kThreads),
-                         0, stream, a, a.items + kItemWords * items);
+    const uint32_t x = static_cast<uint32_t>(merges * a.H);
+    const int* words = a.items + kItemWords * items;
+    if (merges && most_parts >= kSpread)
+      hipLaunchKernelGGL((paged_wide_merge_kernel<D, T_, W_, true>), dim3(x, 32 * W_), dim3(kThreads), 0, stream, a, words);
+    else if (merges)
+      hipLaunchKernelGGL((paged_wide_merge_kernel<D, T_, W_, false>), dim3(x, 32 * W_ * (D / 4) / kThreads), dim3(kThreads), 0, stream, a, words);
   };
   auto by_waves = [&](auto p, auto c, auto t) {
     if constexpr (D == 128) {

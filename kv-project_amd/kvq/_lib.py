@@ -121,7 +121,7 @@ SIGNATURES = {
                                vp, vp, vp, vp, i64, vp, i32, vp]),
     "kvq_paged_plan": (i32, [vp, vp, vp, i64, i64, i64, vp, vp, i64, i64, i64, i64, i32, i64, i64, i64, i64, i64, vp, i64, vp]),
     "kvq_paged_attention_workspace": (i64, [i64, i64, i64, i64]),
-    "kvq_paged_attention": (i32, [vp, i64, i64, i32, i64, i64, i64, f32, vp, i64, i64, i64, i64, vp, i64, i64, i32, vp, vp, vp, vp, vp, vp, vp,
+    "kvq_paged_attention": (i32, [vp, i64, i64, i32, i64, i64, i64, f32, vp, i64, i64, i64, i64, i64, vp, i64, i64, i32, vp, vp, vp, vp, vp, vp, vp,
                                   i64, vp]),
     "kvq_tables_step_words": (i64, [i64, i64, i64]),
     "kvq_tables_extend": (i32, [vp, vp, i64, i64, i64, i64, i64, i64, i64, vp, vp, vp, vp, vp, vp, i64, vp, i64, vp, vp, vp]),

@@ -58,7 +58,7 @@ class PagedPlan:
             words = np.empty(need, dtype=np.int32)
             _lib.call("kvq_paged_plan", *args, _address(words), words.size, _address(info))
         self.rows = int(c.sum())
-        self.items, self.merges, self.parts, self.waves, _, self.sequences, *self._few, self._joins, fronts, _ = info.tolist()
+        self.items, self.merges, self.parts, self.waves, _, self.sequences, *self._few, self._joins, fronts, self._most_parts = info.tolist()
         self.words = torch.from_numpy(words[:max(need, 1)]).to(cache.device)
         self._at = (self.words.data_ptr(), self.words.data_ptr() + 4 * many)
         lib = _lib.load()
@@ -112,8 +112,10 @@ def paged_attention(q: torch.Tensor, scaling: float, cache: PagedCache, layer: i
         return out
     q, qp, qt, qh = rows16(q)
     stream, floats = _lib.stream_of(q), plan._floats + plan._few_floats
+    ws = None
     if workspace is None:
-        workspace = cache.sc.new_empty(floats)
+        if floats:
+            workspace = cache.sc.new_empty(floats)
     elif workspace.dtype != torch.float32 or not workspace.is_contiguous() or workspace.device != device:
         raise ValueError("workspace must be contiguous float32 on the cache's device")
     elif workspace.numel() < floats:
@@ -125,13 +127,14 @@ def paged_attention(q: torch.Tensor, scaling: float, cache: PagedCache, layer: i
             plan._streams.add(stream)
     table, max_blocks, Hkv, d, page, code = cache._fixed
     at, few = plan._at
-    ws = workspace.data_ptr()
+    if floats:
+        ws = workspace.data_ptr()
     if plan.items:
         _lib.call_on(device, "kvq_paged_attention", qp, qt, qh, cache._type, plan.Hq, Hkv, d, float(scaling), at,
-                     plan.items, plan.merges, plan.parts, plan.waves, table, max_blocks, page, code, *cache._at[layer], out.data_ptr(),
+                     plan.items, plan.merges, plan.parts, plan._most_parts, plan.waves, table, max_blocks, page, code, *cache._at[layer], out.data_ptr(),
                      ws, plan._floats, stream)
     if plan.sequences:
         _lib.call_on(device, "kvq_paged_decode_held", qp, qt, qh, cache._type, plan.rows, plan.Hq, Hkv, d, float(scaling), few,
                      plan.sequences, *plan._few, plan._joins, table, max_blocks, page, code, *cache._at[layer], out.data_ptr(),
-                     ws + 4 * plan._floats, plan._few_floats, cache._tickets[layer] if plan._tickets else None, int(not plan.causal), stream)
+                     ws + 4 * plan._floats if plan._few_floats else None, plan._few_floats, cache._tickets[layer] if plan._tickets else None, int(not plan.causal), stream)
     return out
