@@ -7,7 +7,9 @@ and values are appended to its pages, and its queries attend
 * over the prompt itself (prompt_attention, exact keys and values) where a sequence begins, whoever else is in the batch,
 * over the cache by ``paged_decode`` in steps of a few tokens,
 * over the cache's rows by ``rows`` and prompt_attention in steps of many tokens (a further question, a chunk of
-  a prompt): the same attention as paged_decode's, with the codes read once rather than once per 16 query rows.
+  a prompt): the same attention as paged_decode's, with the codes read once rather than once per 16 query rows; or, with
+  ``over_pages``, straight over the pages by ``paged_attention``: without the rows' rounding and their memory, and a text that
+  neighbouring slots share (forks side by side) once for all of them.
 
 Layer ``module.layer_idx`` of the model is layer ``layer_idx`` of the cache.
 """
@@ -18,6 +20,8 @@ from typing import Sequence, Union
 
 import torch
 
+from . import paged
+from .paged import PagedPlan, paged_attention
 from .pages import PagedCache, paged_decode
 from .prompt import PromptPlan, prompt_attention
 
@@ -29,10 +33,11 @@ MANY_ROWS = 192
 
 
 class PagedCtl:
-    """Sequences in ``slots`` of ``cache``, the rows of the model's batch in that order."""
+    """Sequences in ``slots`` of ``cache``, the rows of the model's batch in that order.  ``over_pages``: steps of many tokens
+    attend straight over the pages (the codes as they are, where reading back rounds them to the model's type)."""
 
-    def __init__(self, cache: PagedCache, slots: Sequence[int]):
-        self.cache, self.slots = cache, [int(s) for s in slots]
+    def __init__(self, cache: PagedCache, slots: Sequence[int], *, over_pages: bool = False):
+        self.cache, self.slots, self.over_pages = cache, [int(s) for s in slots], bool(over_pages)
         self.step = None
 
     def begin(self, counts: Union[int, Sequence[int]]) -> None:
@@ -91,7 +96,7 @@ class PagedCtl:
         qp, kp, vp = (self._packed(x, T) for x in (q, k, v))
         cache.append(layer, kp, vp, self.step)
         self.seen.add(layer)
-        few = Hq // cache.Hkv * max(self.counts) < MANY_ROWS
+        few = Hq // cache.Hkv * max(self.counts) < (paged.FEW_ROWS + 1 if self.over_pages else MANY_ROWS)
         if not self.runs:
             out = prompt_attention(qp, kp, vp, scaling, self._plan(Hq, self.begins, None))
         elif not self.begins:
@@ -113,6 +118,12 @@ class PagedCtl:
         return whole.view(B, T, Hq, d), None
 
     def _over_rows(self, q: torch.Tensor, scaling: float, layer: int) -> torch.Tensor:
-        """The running sequences' rows q over the cache's rows, read back."""
-        k, v = self.cache.rows(layer, [self.slots[b] for b in self.runs])
+        """The running sequences' rows q over the cache: straight over its pages, or its rows, read back."""
+        slots = [self.slots[b] for b in self.runs]
+        if self.over_pages:
+            key = (q.shape[1], "pages")
+            if key not in self.plans:
+                self.plans[key] = PagedPlan(self.cache, slots, [self.counts[b] for b in self.runs], q.shape[1])
+            return paged_attention(q, scaling, self.cache, layer, self.plans[key])
+        k, v = self.cache.rows(layer, slots)
         return prompt_attention(q, k, v, scaling, self._plan(q.shape[1], self.runs, self.lens))

@@ -220,6 +220,67 @@ def test_replays_streams_and_strides():
     assert torch.equal(kvq.paged_attention(odd[..., 3:], 0.125, m.cache, 0, plan), out)
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_through_the_router(dtype):
+    """Prompts, tokens, questions and branches of a batch through router_attention, questions straight over the pages."""
+    from types import SimpleNamespace
+    import kvq
+    m = Mirror(layers=2, slots=6, pages=90, max_tokens=900, Hkv=2, d=64, page=32, dtype=dtype, seed=13)
+    c = m.cache
+
+    def step(ctl, counts, T):
+        begins = [c.length(s) == 0 for s in ctl.slots]
+        with kvq.routed(ctl):
+            ctl.begin(counts)
+            for l in range(2):
+                q, k, v = (torch.randn(len(counts), h, T, 64, generator=m.g).to(dtype) for h in (8, 2, 2))
+                out, _ = kvq.router_attention(SimpleNamespace(layer_idx=l, scaling=0.125), q.cuda(), k.cuda(), v.cuda(), None)
+                for b, (s, n) in enumerate(zip(ctl.slots, counts)):
+                    assert not out[b, :T - n].any()
+                    kk, vv = (x[b].transpose(0, 1)[T - n:] for x in (k, v))
+                    m.k[l][s], m.v[l][s] = torch.cat([m.k[l][s], kk]), torch.cat([m.v[l][s], vv])
+                    if n == 0:
+                        continue
+                    kk, vv = m.k[l][s], m.v[l][s]
+                    if not begins[b]:
+                        kk, vv = cached(kk, 32, "int8"), cached(vv, 32, "int8")
+                    check(out[b, T - n:], attend(q[b].transpose(0, 1)[T - n:], kk, vv, 0.125), float(vv.abs().max()), kk.shape[0], 64, dtype,
+                          WEIGHT[dtype], f"layer {l} slot {s}")
+
+    ctl = kvq.PagedCtl(c, [0, 1, 2], over_pages=True)
+    step(ctl, [300, 131, 64], 300)
+    step(ctl, [1, 1, 1], 1)
+    step(ctl, [60, 0, 49], 60)
+    c.fork([0, 0], [3, 4])
+    for l in range(2):
+        for x in (m.k[l], m.v[l]):
+            x[3] = x[4] = x[0]
+    step(kvq.PagedCtl(c, [0, 3, 4, 5, 1], over_pages=True), [20, 33, 1, 70, 50], 70)
+    step(ctl, [2, 1, 3], 3)
+
+
+def test_blocks_of_very_different_scales():
+    """Value scales that grow and fall from block to block by factors of up to 2^60 (bf16) and 2^14 (fp16), blocks of zeros between: each
+    row against the blocks that it sees."""
+    import kvq
+    for dtype, big in ((torch.bfloat16, 60), (torch.float16, 14)):
+        for page in (32, 64):
+            n, d = 9 * page + 7, 64
+            m = Mirror(slots=1, Hkv=1, d=d, page=page, dtype=dtype, max_tokens=1000, seed=page)
+            k, v = m.rand(n, 1), torch.randn(n, 1, d, generator=m.g)
+            for j, e in enumerate([0, -big, 0, None, big // 2, -big // 2, 3, None, -big, 0]):
+                v[j * page:(j + 1) * page] *= 0.0 if e is None else 2.0 ** (e - (big if dtype == torch.bfloat16 else 0))
+            v, q = v.to(dtype), m.rand(n, 2)
+            step = m.cache.extend([0], [n])
+            m.cache.append(0, k.cuda(), v.cuda(), step)
+            out = kvq.paged_attention(q.cuda(), d ** -0.5, m.cache, 0, kvq.PagedPlan(m.cache, [0], [n], 2))
+            vv = cached(v, page, "int8")
+            ref = attend(q, cached(k, page, "int8"), vv, d ** -0.5)
+            for a in range(0, n, page):        # a row's bound has the largest value that it sees
+                b = min(n, a + page)
+                check(out[a:b], tuple(x[a:b] for x in ref), float(vv[:b].abs().max()), b, d, dtype, WEIGHT[dtype], f"{dtype} page {page} rows {a}")
+
+
 def test_refusals():
     import kvq
     m = Mirror(slots=3, Hkv=2, d=64, page=32)
