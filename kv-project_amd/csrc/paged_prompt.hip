@@ -4,6 +4,7 @@
 #include <cmath>
 #include <cstring>
 #include <functional>
+#include <utility>
 #include <vector>
 
 #include "paged_wide.hpp"
@@ -38,7 +39,7 @@ struct Tile {
 
 // What a call costs, in units of 64 tokens of a tile of 128 rows (2.2 us with two workgroups to a CU): the start of a tile; the
 // joins' launch; a tile's sums out and in, which the places share (128 KB at 5 TB/s: 26 ns of all of them)
-constexpr int64_t kStartUnits = 2, kMergeUnits = 2, kPartsPerUnit = 80, kPartUnits = 7;
+constexpr int64_t kStartUnits = 2, kMergeUnits = 2, kPartsPerUnit = 80, kPartUnits = 9, kLeastUnits = 3;
 // Rows a KV head of neighbours over shared pages that the decode's kernels take, in multiples of those of one sequence
 constexpr int64_t kFewShared = 4;
 
@@ -109,45 +110,75 @@ std::vector<Tile> tiles_for(const std::vector<Seq>& some, const std::vector<Grou
   return tiles;
 }
 
-int64_t cut_of(const Tile& t, int64_t most) { return std::max<int64_t>((t.u1 - t.u0 + most - 1) / most, 1); }
-
-// The units of the longest part with which a call is done the earliest, and when that is: the places take the longest workgroup
-// first, each the next when it is done.  Tiles that are many to a place stay whole.
+// How the tiles are cut along the tokens: into even parts of `most` units at most, or, with the tiles' work in a row, where a place's
+// share of it ends
 struct Cut {
-  int64_t most, end;
+  int64_t most, share, end;                   // end: when the call is done
 };
+// f(first unit, end) of each part of a tile, `before` units of work behind the first; returns their number
+template <class F>
+int64_t parts_of(const Tile& t, const Cut& c, int64_t before, F&& f) {
+  const int64_t units = t.u1 - t.u0;
+  int64_t count = 0;
+  if (c.share == 0) {
+    count = std::max<int64_t>((units + c.most - 1) / c.most, 1);
+    for (int64_t i = 0; i < count; ++i) f(units * i / count, units * (i + 1) / count);
+    return count;
+  }
+  before += kStartUnits;
+  int64_t from = 0;
+  for (int64_t at = (before / c.share + 1) * c.share - before; at < units; at += c.share) {
+    if (at - from < kLeastUnits || units - at < kLeastUnits) continue;
+    f(from, at);
+    from = at;
+    ++count;
+  }
+  f(from, units);
+  return count + 1;
+}
+
+// The way with which a call is done the earliest: the places take the longest workgroup first, each the next when it is done.  Tiles
+// that are many to a place stay whole.
 Cut best_cut(const std::vector<Tile>& tiles, int64_t places, int64_t H) {
-  int64_t longest = 1, all = 0;
+  int64_t longest = 1, all = 0, work = 0;
   for (const Tile& t : tiles) {
     longest = std::max(longest, t.u1 - t.u0);
+    work += t.u1 - t.u0 + kStartUnits;
     all += t.u1 - t.u0 + kStartUnits + (t.joins ? kPartUnits : 0);
   }
   const int64_t many = 4 * places;
-  if (static_cast<int64_t>(tiles.size()) > many) return {longest, all / places};
-  Cut best{longest, INT64_MAX};
+  if (static_cast<int64_t>(tiles.size()) > many) return {longest, 0, all / places};
+  Cut best{longest, 0, INT64_MAX};
   std::vector<int64_t> costs, ends(places);
-  for (int64_t k : {1, 2, 3, 4, 5, 6, 8, 10, 12, 16, 20, 24, 32, 48, 64, 96, 128}) {
-    const int64_t most = (longest + k - 1) / k | 1;          // the kernel rounds units up to an odd number
+  auto look = [&](Cut c) {
     costs.clear();
-    int64_t parts = 0;
+    int64_t parts = 0, before = 0;
     for (const Tile& t : tiles) {
-      const int64_t cut = cut_of(t, most), units = t.u1 - t.u0;
-      const bool joins = t.joins || cut > 1;
-      parts += joins ? cut : 0;
-      for (int64_t c = 0; c < cut; ++c) costs.push_back(((units * (c + 1) / cut - units * c / cut) | 1) + kStartUnits + joins);
+      const size_t at = costs.size();
+      // the kernel rounds units up to an odd number
+      const int64_t count = parts_of(t, c, before, [&](int64_t a, int64_t b) { costs.push_back(((b - a) | 1) + kStartUnits); });
+      before += t.u1 - t.u0 + kStartUnits;
+      if (!t.joins && count == 1) continue;
+      parts += count;
+      for (size_t i = at; i < costs.size(); ++i) ++costs[i];
     }
-    if (static_cast<int64_t>(costs.size()) > many) break;
+    if (static_cast<int64_t>(costs.size()) > many) return false;
     std::sort(costs.begin(), costs.end(), std::greater<int64_t>());
     std::fill(ends.begin(), ends.end(), 0);
-    for (int64_t c : costs) {
+    for (int64_t x : costs) {
       std::pop_heap(ends.begin(), ends.end(), std::greater<int64_t>());
-      ends.back() += c;
+      ends.back() += x;
       std::push_heap(ends.begin(), ends.end(), std::greater<int64_t>());
     }
-    const int64_t end = *std::max_element(ends.begin(), ends.end()) + (parts ? kMergeUnits + parts * H / kPartsPerUnit : 0);
-    if (end < best.end) best = {most, end};
-    if (most <= 3) break;
+    c.end = *std::max_element(ends.begin(), ends.end()) + (parts ? kMergeUnits + parts * H / kPartsPerUnit : 0);
+    if (c.end < best.end) best = c;
+    return true;
+  };
+  for (int64_t k : {1, 2, 3, 4, 5, 6, 8, 10, 12, 16, 20, 24, 32, 48, 64, 96, 128}) {
+    const int64_t most = (longest + k - 1) / k | 1;
+    if (!look({most, 0, 0}) || most <= kLeastUnits) break;
   }
+  for (int64_t k : {1, 2}) look({longest, std::max((work + k * places - 1) / (k * places), kLeastUnits), 0});
   return best;
 }
 
@@ -170,15 +201,18 @@ void plan_wide(const std::vector<Seq>& some, const std::vector<Group>& groups, c
       out.waves = 8;
     }
   }
+  int64_t before = 0;
   for (Tile& t : tiles) {
-    t.cut = t.u1 > t.u0 ? cut_of(t, cut.most) : 0;
+    std::vector<std::pair<int64_t, int64_t>> parts;
+    t.cut = parts_of(t, cut, before, [&](int64_t a, int64_t b) { parts.push_back({a, b}); });
+    before += t.u1 - t.u0 + kStartUnits;
     t.joins = t.joins || t.cut > 1;
+    if (t.joins && t.u1 == t.u0) t.cut = 0;   // all of it is in the front
     t.part = out.parts;
     if (t.joins) out.parts += t.cut;
-    const int64_t count = t.joins ? t.cut : 1;
-    for (int64_t c = 0; c < count; ++c) {
-      const int64_t units = t.u1 - t.u0, a = t.u0 + units * c / count, b = t.u0 + units * (c + 1) / count;
-      const int64_t w[kItemWords] = {t.row0, t.toks, t.slot, a, b, t.vis0, t.step, t.len, t.buf, t.joins ? t.part + c : -1, 0, 0};
+    for (int64_t c = 0; c < (t.joins ? t.cut : 1); ++c) {
+      const int64_t w[kItemWords] = {t.row0, t.toks, t.slot, t.u0 + parts[c].first, t.u0 + parts[c].second, t.vis0, t.step, t.len, t.buf,
+                                     t.joins ? t.part + c : -1, 0, 0};
       PlanItem it;
       for (int k = 0; k < kItemWords; ++k) it.w[k] = static_cast<int32_t>(w[k]);
       out.items.push_back(it);
