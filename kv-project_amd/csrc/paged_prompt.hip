@@ -337,11 +337,14 @@ extern "C" int kvq_paged_attention(const void* q, int64_t q_st, int64_t q_sh, in
   KVQ_REQUIRE((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(out) | reinterpret_cast<uintptr_t>(workspace)) % 16 == 0 &&
                   (q_st | q_sh) % 8 == 0,
               "kvq_paged_attention: rows and strides must be multiples of 16 bytes");
-  KVQ_REQUIRE(items * H <= kMaxGrid && merges * H <= kMaxGrid, "kvq_paged_attention: too many rows");
   const int64_t need = kvq_paged_attention_workspace(parts, waves, H, D);
   KVQ_REQUIRE(need >= 0, "kvq_paged_attention: workgroups of 4 wavefronts, or of 8 with head_dim 128 (got %lld)", static_cast<long long>(waves));
   KVQ_REQUIRE(workspace_floats >= need, "kvq_paged_attention: workspace of %lld floats, %lld needed",
               static_cast<long long>(workspace_floats), static_cast<long long>(need));
+  // a launch counts its threads in 32 bits
+  const int64_t rows = 32 * waves, join_threads = most_parts >= kSpread ? rows * 256 : rows * (D / 4);
+  KVQ_REQUIRE(items <= (INT64_C(1) << 32) / (2 * rows) / H && merges <= ((INT64_C(1) << 32) - 1) / join_threads / H && items * H < INT64_C(1) << 24,
+              "kvq_paged_attention: too many rows");
   // a scaling of nothing would make a NaN of a hidden score's -inf: the smallest one, which makes zeros of the others
   const float scale = std::fabs(scaling) * 1.44269504088896341f;
   const WideArgs a{static_cast<const uint16_t*>(q), q_st, q_sh, words, table, max_blocks, static_cast<int>(H), static_cast<int>(Hq / H),

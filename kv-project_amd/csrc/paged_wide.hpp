@@ -335,7 +335,10 @@ __global__ __launch_bounds__(64 * W, 2) void paged_wide_kernel(WideArgs a) {
       unit = now;
       unit_set = true;
     }
-    const float r = z.y < 0x1p-100f ? 1.0f : z.y * __builtin_amdgcn_rcpf(unit);         // of a power of two: exact
+    // (the quotient of a power of two is exact; of two blocks of one unit the smaller one's scale is taken for 2^-100 of the larger
+    // one's at least)
+    float r = z.y < 0x1p-100f ? 1.0f : z.y * __builtin_amdgcn_rcpf(unit);
+    r = r < 0x1p-100f ? 0x1p-100f : r;
     lr = __builtin_amdgcn_logf(r);
     inv_r = __builtin_amdgcn_rcpf(r);
     if (masked) {

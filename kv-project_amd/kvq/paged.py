@@ -66,8 +66,11 @@ class PagedPlan:
         self._few_floats = 0
         if self._joins:
             self._few_floats = lib.kvq_paged_decode_workspace(self._few[2], cache.Hkv, self.Hq // cache.Hkv, cache.d)
-        # a slot's tickets are one call's
-        self._tickets = not fronts and np.unique(s).size == s.size
+        # a slot's tickets are one run's
+        named = s[c > 0]
+        if not causal:
+            named = named[np.append(True, named[1:] != named[:-1])] if named.size else named
+        self._tickets = not fronts and np.unique(named).size == named.size
         self._stamp = cache._stamp
         self._streams = {_lib.stream_of(self.words)}     # that the words belong to, or are recorded for
 

@@ -86,6 +86,11 @@ def test_cross(page, d, Hkv, rep, code, dtype):
     run(m, [0, 0, 0, 4, 1, 2, 3], [1, 1, 1, 2, 3, 1, 100], rep * Hkv, causal=False, what="beams")
     run(m, [0, 5, 6, 3], [7, 1, 2, 0], rep * Hkv, causal=False, what="shared pages")
     run(m, [4, 4], [1, 0], rep * Hkv, causal=False, what="none")
+    # forks of a whole number of units: nothing of their own
+    m.free([0, 5, 6])
+    m.push([0], [512])
+    m.fork([0, 0], [5, 6])
+    run(m, [0, 5, 6, 4], [3, 1, 40, 1], rep * Hkv, causal=False, what="all shared")
 
 
 @pytest.mark.parametrize("causal", [True, False])
@@ -116,10 +121,14 @@ def test_layers_after_moves():
     m = Mirror(layers=3, slots=4, pages=30, max_tokens=600, Hkv=2, d=64, page=32, seed=4)
     m.push([0, 1, 2], [100, 164, 31])
     m.free([0])
+    import kvq
+    plan = kvq.PagedPlan(m.cache, [1, 2], [50, 31], 4)               # made before the pages move
     m.cache.compact()
     for l in range(3):
-        run(m, [1, 2], [50, 31], 4, layer=l, what=f"layer {l}")
+        _, q, out = run(m, [1, 2], [50, 31], 4, layer=l, what=f"layer {l}")
+        assert torch.equal(out, kvq.paged_attention(q.cuda(), 0.125, m.cache, l, plan))
     m.cache.resize(20)
+    assert torch.equal(out, kvq.paged_attention(q.cuda(), 0.125, m.cache, 2, plan))
     run(m, [2, 1], [3, 164], 4, layer=2, what="resized")
 
 
