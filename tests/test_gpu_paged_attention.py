@@ -109,6 +109,29 @@ def test_cut_along_the_tokens(n, rep, d, causal, few_rows):
     run(m, [2, 3], [5, 7], rep, causal, what="cut text")
 
 
+@pytest.mark.parametrize("page,code,dtype,causal", [(32, "int8", torch.bfloat16, True), (64, "e4m3", torch.float16, True),
+                                                     (128, "int8", torch.float16, False), (64, "int8", torch.bfloat16, False)])
+def test_a_full_chip(page, code, dtype, causal):
+    """As many tiles as the chip has places: workgroups of 256 rows, alone and with a text that is shared; some heads of all rows."""
+    import kvq
+    H, d, heads = 64, 128, [0, 31, 63]
+    m = Mirror(slots=9, pages=9 * (1100 // page + 1), max_tokens=1100, Hkv=H, d=d, page=page, code=code, dtype=dtype, seed=page)
+    lens = [300, 256, 290, 300]
+    m.push([0, 1, 2, 3, 4], [*lens, 640])
+    m.fork([4] * 4, [5, 6, 7, 8])
+    m.push([5, 6, 7, 8], lens)
+    for slots in ([0, 1, 2, 3], [5, 6, 7, 8]):
+        plan = kvq.PagedPlan(m.cache, slots, [256] * 4, H, causal=causal)
+        assert plan.sequences or plan.waves == 8
+        q = m.rand(1024, H)
+        out = kvq.paged_attention(q.cuda(), d ** -0.5, m.cache, 0, plan)
+        for i, s in enumerate(slots):
+            k, v = (cached(x[0][s][:, heads], page, code) for x in (m.k, m.v))
+            rows = slice(256 * i, 256 * (i + 1))
+            check(out[rows][:, heads], attend(q[rows][:, heads], k, v, d ** -0.5, causal), float(v.abs().max()), k.shape[0], d, dtype,
+                  WEIGHT[dtype], f"slot {s}")
+
+
 def test_one_query_head_to_many():
     """128 query heads over one KV head: a tile for each token."""
     m = Mirror(Hkv=1, d=64, page=32, seed=5)
