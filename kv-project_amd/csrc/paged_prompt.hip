@@ -343,7 +343,7 @@ extern "C" int kvq_paged_attention(const void* q, int64_t q_st, int64_t q_sh, in
               static_cast<long long>(workspace_floats), static_cast<long long>(need));
   // a launch counts its threads in 32 bits
   const int64_t rows = 32 * waves, join_threads = most_parts >= kSpread ? rows * 256 : rows * (D / 4);
-  KVQ_REQUIRE(items <= (INT64_C(1) << 32) / (2 * rows) / H && merges <= ((INT64_C(1) << 32) - 1) / join_threads / H && items * H < INT64_C(1) << 24,
+  KVQ_REQUIRE(items <= ((INT64_C(1) << 32) - 1) / (2 * rows) / H && merges <= ((INT64_C(1) << 32) - 1) / join_threads / H && items * H < INT64_C(1) << 24,
               "kvq_paged_attention: too many rows");
   // a scaling of nothing would make a NaN of a hidden score's -inf: the smallest one, which makes zeros of the others
   const float scale = std::fabs(scaling) * 1.44269504088896341f;

@@ -29,7 +29,7 @@ class DeviceAccounts:
     """Takes the cache's accounts to the device; until ``close`` hands them back, the cache's own calls that need them (extend, rows,
     fork, free, compact, resize, its lengths, plans) are refused, and so are steps and plans that were made before.  Calls run in the
     order in which they are made, as the cache's do; what a captured graph reads and writes (these accounts, the cache, its steps)
-    has to live as long as it is replayed.
+    has to live as long as it is replayed, and graphs of extend and free are not replayed after ``close``.
 
     ``lengths`` (slots,) int32 is each slot's tokens, ``free_pages`` and ``refused`` () int32 the free pages and the steps that did not
     fit, all on the device."""
@@ -48,7 +48,9 @@ class DeviceAccounts:
         self.lengths, self._open, self._refs, account = self._state.split([n, n, p, 4])
         self.free_pages, self.refused = account[0], account[2]
         self._at = tuple(x.data_ptr() for x in (self.lengths, self._refs, self._open, account))
-        self._streams = {_lib.stream_of(self._state)}
+        stream = _lib.stream_of(self._state)
+        self._streams = {stream}
+        cache._use(stream)
         cache._away = self
         self._changed(slice(None))
 

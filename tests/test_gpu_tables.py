@@ -232,6 +232,23 @@ def test_a_captured_loop(n, Hkv):
     m.check("handed back")
 
 
+@pytest.mark.parametrize("slots,most", [([1], 1), ([1], 40), ([2, 0, 1], 1), ([2, 0, 1], 40)])
+def test_a_step_before_its_first_extend(slots, most):
+    """Describes no tokens: nothing is appended, and its rows of a decode are zeros."""
+    import kvq
+    m = Mirror(slots=3, pages=20, max_tokens=300, Hkv=2, d=64, page=32, seed=12)
+    m.push([0, 1], [70, 33])
+    acc = kvq.DeviceAccounts(m.cache)
+    step = acc.step(slots, most)
+    assert not (step.positions + 1).any() and not (step.places + 1).any()
+    new = m.rand(step.rows, 2).cuda()
+    m.cache.append(0, new, new, step)
+    decode(m, step, [0] * len(slots), 4)
+    same(m, acc)
+    acc.close()
+    m.check("before")
+
+
 def test_another_stream():
     import kvq
     m = Mirror(slots=3, pages=20, max_tokens=300, Hkv=1, d=64, page=32, seed=9)
