@@ -204,11 +204,14 @@ __global__ __launch_bounds__(64 * W, 2) void paged_wide_kernel(WideArgs a) {
       const uint8_t* base = a.vc + at_of(ids.a) * (P * D) + (unit_of(j) * kUnit & (P - 1));
       vw[i.value] = load16(base + ch * P + t);
     } else {
-      const int64_t at = t < 32 ? at_of(ids.a) : at_of(ids.b);
+      const int64_t first = at_of(ids.a), second = at_of(ids.b), at = t < 32 ? first : second;
       vw[i.value] = load16(a.vc + at * (P * D) + ch * P + (t & 31));
     }
   };
-  auto scales_of = [&](Ids ids) KVQ_INLINE { return reinterpret_cast<const float2*>(a.sc)[kOne || !g ? at_of(ids.a) : at_of(ids.b)]; };
+  auto scales_of = [&](Ids ids) KVQ_INLINE {
+    const int64_t first = at_of(ids.a), second = at_of(ids.b);        // not behind a branch, which would part the products' steps
+    return reinterpret_cast<const float2*>(a.sc)[kOne || !g ? first : second];
+  };
   // 8 codes of piece i / 2 each
   auto widen_k = [&](int par, auto i) KVQ_INLINE {
     const int x = tx + i.value / 2 * kThreads;
