@@ -224,54 +224,62 @@ __global__ __launch_bounds__(64 * W, 2) void paged_wide_kernel(WideArgs a) {
     v_put(par, x / 4, 2 * (x % 4) + i.value % 2, widen8<CODE, BF16>(w[2 * (i.value % 2)], w[2 * (i.value % 2) + 1]));
   };
 
-  // The softmax of a unit in 18 shares: 0 and 1 find the reference, 2 + i the weights 2 i, 2 i + 1 (register 16 t + e: token 32
-  // g + 16 t + e).  lim: how many of this lane's 32 tokens the row sees; kz: what makes exponents of scores.  The weights come
-  // multiplied by the value scale, as its logarithm lr in the exponent, and their sum is divided by it once.
+  // The softmax of a unit: share i is the weights 2 i, 2 i + 1 (register 16 t + e: token 32 g + 16 t + e).  The weights come
+  // multiplied by the value scale, as its logarithm lr in the exponent, and their sum is divided by it once.  kz: what makes
+  // exponents of scores.
   constexpr float kLift = BF16 ? 0.0f : 7.0f; // log2 of the reference's weight
-  float top, safe, sum, kz, lr, inv_r, unit = 1.0f, wx, wz;
+  constexpr float kMost = BF16 ? 0x1p13f : 0x1p15f;
+  float base = 0.0f, safe, sum, kz, lr, inv_r, unit = 1.0f, wx, wz;
   bool unit_set = false;                      // o is held in units of a power of two near the value scale
-  auto share = [&](auto par, bool masked, int lim, auto which) KVQ_INLINE {
-    constexpr int i = decltype(which)::value;
+  // The reference from the unit's scores, where one passes it by more than 2^slack.  lim: how many of this lane's 32 tokens the row
+  // sees.  Only units that some row does not see whole look for it: in the others the weights are taken by the one there is, and
+  // where a lane's come to more than kMost, taken again.  Weights of up to that cost no accuracy, and a maximum of every unit costs 30 of
+  // its 230 vector instructions with head_dim 64, in a row before the first weight (four fp16 chunks 398 -> 376 us; 32 questions
+  // behind 16384, head_dim 128, 3925 -> 3777).
+  auto find = [&](auto par, bool masked, int lim, float slack) KVQ_INLINE {
     auto& t = s[decltype(par)::value];
-    if constexpr (i < 2) {
-      if (masked) each<0, 16>([&](auto e) KVQ_INLINE { t[i][e.value] = 16 * i + e.value < lim ? t[i][e.value] : -INFINITY; });
-      float x = i == 0 ? t[0][0] : fmaxf(top, t[1][0]);
-      each<1, 16>([&](auto e) KVQ_INLINE { x = fmaxf(x, t[i][e.value]); });
-      top = x;
-      if constexpr (i == 1) {
-        // the reference moves only when a score passes it by 2^8: weights up to 256 (fp16: 2^15) cost no accuracy, and the
-        // accumulators are hardly ever scaled
-        x = xmax32(x * kz);
-        x = x > m + 8.0f ? x : m;
-        safe = x == -INFINITY ? 0.0f : x;
-        grow = __builtin_amdgcn_exp2f(m - safe);
-        safe -= kLift + lr;
-        m = x;
-        l *= grow;
-        sum = 0.0f;
-      }
-    } else {
-      // a pair's exponentials, then the pair before it: no wait for a result
-      constexpr int k = 2 * (i - 2);
-      auto finish = [&](auto at) KVQ_INLINE {
-        constexpr int n = decltype(at)::value;
-        uint32_t w = pack2<BF16>(wx, wz);
-        asm volatile("" : "+v"(w));           // here, not behind the branch of the rescaling
-        p[decltype(par)::value][n / 8][n % 8 / 2] = w;
-        sum += wx;
-        sum += wz;
-      };
-      const float x = __builtin_amdgcn_exp2f(__builtin_fmaf(t[k / 16][k % 16], kz, -safe));
-      const float z = __builtin_amdgcn_exp2f(__builtin_fmaf(t[k / 16][k % 16 + 1], kz, -safe));
-      if constexpr (i > 2) finish(std::integral_constant<int, k - 2>{});
-      wx = x;
-      wz = z;
-      if constexpr (i == 17) {
-        finish(std::integral_constant<int, k>{});
-        l = __builtin_fmaf(sum, inv_r, l);
-        asm volatile("" : "+v"(l));
-      }
+    if (masked)
+      each<0, 32>([&](auto e) KVQ_INLINE {
+        constexpr int n = decltype(e)::value;
+        t[n / 16][n % 16] = n < lim ? t[n / 16][n % 16] : -INFINITY;
+      });
+    float x = t[0][0];
+    each<1, 32>([&](auto e) KVQ_INLINE { x = fmaxf(x, t[e.value / 16][e.value % 16]); });
+    x = xmax32(x * kz);
+    x = x > m + slack ? x : m;
+    base = x == -INFINITY ? 0.0f : x;
+    const float f = __builtin_amdgcn_exp2f(m - base);
+    m = x;
+    grow *= f;
+    l *= f;
+  };
+  auto begin = [&]() KVQ_INLINE {
+    safe = base - (kLift + lr);
+    sum = 0.0f;
+  };
+  auto share = [&](auto par, auto which, auto again) KVQ_INLINE {
+    // a pair's exponentials, then the pair before it: no wait for a result
+    constexpr int i = decltype(which)::value, k = 2 * i;
+    auto& t = s[decltype(par)::value];
+    auto finish = [&](auto at) KVQ_INLINE {
+      constexpr int n = decltype(at)::value;
+      uint32_t w = pack2<BF16>(wx, wz);
+      asm volatile("" : "+v"(w));             // here, not behind a branch
+      p[decltype(par)::value][n / 8][n % 8 / 2] = w;
+      sum += wx;
+      sum += wz;
+    };
+    float x = __builtin_fmaf(t[k / 16][k % 16], kz, -safe), z = __builtin_fmaf(t[k / 16][k % 16 + 1], kz, -safe);
+    if constexpr (decltype(again)::value) {   // not above the reference's: it is off by much where scores pass 2^24 (a NaN stays one)
+      x = x > kLift + lr ? kLift + lr : x;
+      z = z > kLift + lr ? kLift + lr : z;
     }
+    x = __builtin_amdgcn_exp2f(x);
+    z = __builtin_amdgcn_exp2f(z);
+    if constexpr (i > 0) finish(std::integral_constant<int, k - 2>{});
+    wx = x;
+    wz = z;
+    if constexpr (i == 15) finish(std::integral_constant<int, k>{});
   };
   constexpr int kV = 4 * (D / 32), kK = 2 * (D / 16);               // steps of the two products
   constexpr std::integral_constant<int, 0> even{};
@@ -287,6 +295,9 @@ __global__ __launch_bounds__(64 * W, 2) void paged_wide_kernel(WideArgs a) {
     constexpr bool kWith = decltype(with)::value;
     constexpr std::integral_constant<int, 1 - decltype(par)::value> other{};
     u32x4 w[3];
+    grow = 1.0f;
+    if (masked) find(par, true, lim, 8.0f);
+    begin();
     if constexpr (kWith) {
       w[0] = read_v(other, 0);
       w[1] = read_v(other, 1);
@@ -296,9 +307,18 @@ __global__ __launch_bounds__(64 * W, 2) void paged_wide_kernel(WideArgs a) {
         if constexpr (t.value + 2 < kV) w[(t.value + 2) % 3] = read_v(other, t.value + 2);
         add_v(other, t, w[t.value % 3]);
       }
-      each<t.value * 18 / kV, (t.value + 1) * 18 / kV>([&](auto i) KVQ_INLINE { share(par, masked, lim, i); });
+      each<t.value * 16 / kV, (t.value + 1) * 16 / kV>([&](auto i) KVQ_INLINE { share(par, i, no); });
       __builtin_amdgcn_sched_barrier(0);
     });
+    float add = sum * inv_r;
+    if (__builtin_amdgcn_ballot_w64(add > kMost)) {
+      find(par, false, lim, 0.0f);
+      begin();
+      each<0, 16>([&](auto i) KVQ_INLINE { share(par, i, yes); });
+      add = sum * inv_r;
+    }
+    l += add;
+    asm volatile("" : "+v"(l));
   };
   // S = K Q of the units of the other parity, beside `job` of each of its steps
   auto products = [&](auto par, auto&& job) KVQ_INLINE {
@@ -406,16 +426,16 @@ __global__ __launch_bounds__(64 * W, 2) void paged_wide_kernel(WideArgs a) {
     each<0, kPer>([&](auto i) { fetch_v(id[0], 1, i); });
     block_lds_barrier();
     products(odd, nothing);                   // unit 0
-    const bool masked = whole == 0;
     const int lim = lim_of(0);
-    scale_for(z_now, masked, lim);
+    scale_for(z_now, whole == 0, lim);
     z_now = scales_of(id[0]);
     if (tiles > 1) {
       block_lds_barrier();                    // K(2) takes the place of K(0)
       each<0, 2 * kPer>([&](auto i) { widen_k(0, i); });
       each<0, kPer>([&](auto i) { fetch_k(id[2], 3, i); });
     }
-    values(even, masked, no, lim);
+    values(even, true, no, lim);
+    if (__builtin_amdgcn_ballot_w64(live && m == -INFINITY)) whole = 0;      // a row without a reference yet
     if (tiles > 1) {
       products(even, nothing);                // unit 1
       // ids of units 2, 3, 4

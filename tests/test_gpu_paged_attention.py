@@ -313,6 +313,46 @@ def test_blocks_of_very_different_scales():
                 check(out[a:b], tuple(x[a:b] for x in ref), float(vv[:b].abs().max()), b, d, dtype, WEIGHT[dtype], f"{dtype} page {page} rows {a}")
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("page,d", [(32, 128), (64, 64), (128, 128)])
+@pytest.mark.parametrize("way", ["climb", "jumps", "from far below", "down"])
+def test_scores_that_climb(way, page, d, dtype):
+    """Scores that climb along the text, for some rows slowly, for others fast, for others not: by less than a weight has room for,
+    by far more from one block to the next, and from far below the others."""
+    import kvq
+    n = 640 + 9
+    at = torch.arange(n, dtype=torch.float64)
+    c = {"climb": at * 0.06, "jumps": 45.0 * (at // 130), "from far below": torch.where(at < 200, -150.0, 20.0), "down": 120.0 - at * 0.2}[way]
+    m = Mirror(slots=1, Hkv=2, d=d, page=page, dtype=dtype, max_tokens=1000, seed=page + d)
+    u = torch.randint(0, 2, (2, d), generator=m.g).double() * 2 - 1
+    k = (c[:, None, None] * u + 0.3 * torch.randn(n, 2, d, generator=m.g)).to(dtype)
+    v = m.rand(n, 2)
+    q = torch.tensor([1.0, -1.0, 0.25, 0.0, 0.5] * 8, dtype=torch.float64)[:, None, None] * u.repeat_interleave(2, 0)
+    m.cache.append(0, k.cuda(), v.cuda(), m.cache.extend([0], [n]))
+    m.k[0][0], m.v[0][0] = k, v
+    run(m, [0], [40], 4, what=way, scaling=1.0 / d, q=q.to(dtype))
+    run(m, [0], [40], 4, causal=False, what=way, scaling=1.0 / d, q=q.to(dtype))
+
+
+def test_scores_of_minus_infinity():
+    """A text whose first block gives a row scores of -inf alone (keys and queries near the type's largest): the row is what the
+    rest of it gives."""
+    import kvq
+    d, n = 64, 64 * 5 + 3
+    m = Mirror(slots=1, Hkv=1, d=d, page=64, max_tokens=600, seed=3)
+    k, v, q = m.rand(n, 1), m.rand(n, 1), m.rand(40, 2)
+    k[:64] = -3e37
+    k[:, 0, 1:] = 0
+    q[:, :, 0] = torch.where(torch.arange(40)[:, None] % 2 == 0, 3e37, 1.0)
+    k[64:, 0, 0] = 0
+    m.cache.append(0, k.cuda(), v.cuda(), m.cache.extend([0], [n]))
+    out = kvq.paged_attention(q.cuda(), 1.0, m.cache, 0, kvq.PagedPlan(m.cache, [0], [40], 2))
+    kk, vv = cached(k, 64, "int8"), cached(v, 64, "int8")
+    # the others of the first block weigh exp(-3e37), nothing
+    ref = attend(q, kk[64:], vv[64:], 1.0)
+    check(out, ref, float(vv.abs().max()), n, d, torch.bfloat16, WEIGHT[torch.bfloat16], "-inf in front")
+
+
 def test_refusals():
     import kvq
     m = Mirror(slots=3, Hkv=2, d=64, page=32)
