@@ -291,12 +291,12 @@ __global__ __launch_bounds__(64 * W, 2) void paged_wide_kernel(WideArgs a) {
     o[c] = mfma32<BF16>(w, p[decltype(par)::value][y], o[c]);
   };
   // o += V P of the other parity (if `with`) beside the softmax of this one
-  auto values = [&](auto par, bool masked, auto with, int lim) KVQ_INLINE {
+  auto values = [&](auto par, bool look, bool masked, auto with, int lim) KVQ_INLINE {
     constexpr bool kWith = decltype(with)::value;
     constexpr std::integral_constant<int, 1 - decltype(par)::value> other{};
     u32x4 w[3];
     grow = 1.0f;
-    if (masked) find(par, true, lim, 8.0f);
+    if (look) find(par, masked, lim, 8.0f);
     begin();
     if constexpr (kWith) {
       w[0] = read_v(other, 0);
@@ -311,7 +311,7 @@ __global__ __launch_bounds__(64 * W, 2) void paged_wide_kernel(WideArgs a) {
       __builtin_amdgcn_sched_barrier(0);
     });
     float add = sum * inv_r;
-    if (__builtin_amdgcn_ballot_w64(add > kMost)) {
+    if (__builtin_expect(__builtin_amdgcn_ballot_w64(add > kMost) != 0, 0)) {
       find(par, false, lim, 0.0f);
       begin();
       each<0, 16>([&](auto i) KVQ_INLINE { share(par, i, yes); });
@@ -382,7 +382,7 @@ __global__ __launch_bounds__(64 * W, 2) void paged_wide_kernel(WideArgs a) {
     z_now = scales_of(id[0]);
     next_id = ids_of(j + 4);
     __builtin_amdgcn_s_setprio(1);            // the softmax goes before the other wavefront's products
-    values(par, masked, yes, lim);
+    values(par, masked, true, yes, lim);
     __builtin_amdgcn_s_setprio(0);
     grow *= turn;
     // unit j + 2 of K and j of V into the buffers of this parity, then the codes of the ones after them
@@ -434,7 +434,7 @@ __global__ __launch_bounds__(64 * W, 2) void paged_wide_kernel(WideArgs a) {
       each<0, 2 * kPer>([&](auto i) { widen_k(0, i); });
       each<0, kPer>([&](auto i) { fetch_k(id[2], 3, i); });
     }
-    values(even, true, no, lim);
+    values(even, true, whole == 0, no, lim);
     if (__builtin_amdgcn_ballot_w64(live && m == -INFINITY)) whole = 0;      // a row without a reference yet
     if (tiles > 1) {
       products(even, nothing);                // unit 1
@@ -490,7 +490,7 @@ __global__ __launch_bounds__(64 * W, 2) void paged_wide_kernel(WideArgs a) {
     kz = a.scale;
     lr = 0.0f;
     inv_r = 1.0f;
-    values(even, true, no, visible - t0 - 32 * g);
+    values(even, true, true, no, visible - t0 - 32 * g);
     rescale();
     each<0, kV>([&](auto t) KVQ_INLINE { add_v(even, t, read_v(even, t.value)); });
   }
