@@ -39,7 +39,7 @@ struct Tile {
 
 // What a call costs, in units of 64 tokens of a tile of 128 rows (2.2 us with two workgroups to a CU): the start of a tile; the
 // joins' launch; a tile's sums out and in, which the places share (128 KB at 5 TB/s: 26 ns of all of them)
-constexpr int64_t kStartUnits = 2, kMergeUnits = 2, kPartsPerUnit = 80, kPartUnits = 9, kLeastUnits = 3;
+constexpr int64_t kStartUnits = 2, kMergeUnits = 2, kPartsPerUnit = 80, kPartUnits = 9, kLeastUnits = 3, kAloneUnits = 2;
 // Rows a KV head of neighbours over shared pages that the decode's kernels take, in multiples of those of one sequence
 constexpr int64_t kFewShared = 4;
 
@@ -182,9 +182,11 @@ Cut best_cut(const std::vector<Tile>& tiles, int64_t places, int64_t H) {
   return best;
 }
 
-// Eight wavefronts to a workgroup, one of them to a CU, widen a code for twice the rows: a unit of their 256 rows takes 0.965 of the
-// time of two of 128 (32 questions of 301 to 700 tokens behind 16384, 8 KV heads of 128: 4418 -> 4272 us).  But a workgroup
-// that has a CU to itself is no faster, and tiles that are not full cost twice as much: only where the chip is full of tiles.
+// Eight wavefronts to a workgroup, one of them to a CU, widen a code for twice the rows: a unit of their 256 rows takes 0.92 of the
+// time of two of 128 (32 questions of 301 to 700 tokens behind 16384, 8 KV heads of 128: 4082 -> 3748 us; four of 1613 to 2146 behind
+// 10323, 4 KV heads: 691 -> 640).  But a workgroup that has a CU to itself is no faster, tiles that are not full cost twice as much, and
+// nothing runs beside a tile's start: only where the chip is full of tiles, with kAloneUnits more for each start (six texts of three
+// readers of 52 to 280 tokens: 30 us with 256 rows, 26 with 128).
 void plan_wide(const std::vector<Seq>& some, const std::vector<Group>& groups, const uint8_t* open, int64_t page, int64_t rep, int64_t H,
                int64_t D, bool causal, PlanWords& out) {
   out.waves = 4;
@@ -193,8 +195,10 @@ void plan_wide(const std::vector<Seq>& some, const std::vector<Group>& groups, c
   Cut cut = best_cut(tiles, std::max<int64_t>(kSlots / H, 1), H);
   if (D == 128 && static_cast<int64_t>(tiles.size()) * H >= kSlots) {
     std::vector<Tile> wider = tiles_for(some, groups, open, page, 256 / rep, causal);
-    const Cut other = best_cut(wider, std::max<int64_t>(kSlots / 2 / H, 1), 2 * H);
-    if (other.end * 965 < cut.end * 1000) {
+    const int64_t places = std::max<int64_t>(kSlots / 2 / H, 1);
+    const Cut other = best_cut(wider, places, 2 * H);
+    const int64_t starts = (static_cast<int64_t>(wider.size()) + places - 1) / places;       // of a place
+    if ((other.end + kAloneUnits * starts) * 92 < cut.end * 100) {
       tiles.swap(wider);
       cut = other;
       per_tile = 256 / rep;
