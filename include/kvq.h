@@ -767,7 +767,7 @@ int kvq_paged_decode(const void* q, int64_t q_st, int64_t q_sh, int dtype, int64
  * info is set.  The words go to the device as they are; they bound what the calls read, together with the table on the device.
  * Each writes its own rows of out (rows, Hq, D).
  * kvq_paged_attention's workspace: kvq_paged_attention_workspace floats (none without parts), no clearing; calls that share one
- * must not overlap in time.  kvq_paged_decode_held is kvq_paged_decode for rows whose tokens are in the cache (all = 0), or which
+ * must not overlap in time.  items, merges, parts, waves and most_parts are the plan's.  kvq_paged_decode_held is kvq_paged_decode for rows whose tokens are in the cache (all = 0), or which
  * see all tokens of the slot (all = 1); tickets only where no slot is named twice.
  * ---------------------------------------------------------------------------------------- */
 int kvq_paged_plan(const int64_t* lens, const int32_t* table, const uint8_t* open, int64_t slots, int64_t max_blocks,

@@ -39,7 +39,7 @@ struct Tile {
 
 // What a call costs, in units of 64 tokens of a tile of 128 rows (2.2 us with two workgroups to a CU): the start of a tile; the
 // joins' launch; a tile's sums out and in, which the places share (128 KB at 5 TB/s: 26 ns of all of them)
-constexpr int64_t kStartUnits = 2, kMergeUnits = 2, kPartsPerUnit = 80, kPartUnits = 9, kLeastUnits = 3, kAloneUnits = 2;
+constexpr int64_t kStartUnits = 2, kMergeUnits = 2, kPartsPerUnit = 80, kPartUnits = 9, kLeastUnits = 3, kAloneUnits = 3;
 // Rows a KV head of neighbours over shared pages that the decode's kernels take, in multiples of those of one sequence
 constexpr int64_t kFewShared = 4;
 
@@ -185,8 +185,8 @@ Cut best_cut(const std::vector<Tile>& tiles, int64_t places, int64_t H) {
 // Eight wavefronts to a workgroup, one of them to a CU, widen a code for twice the rows: a unit of their 256 rows takes 0.92 of the
 // time of two of 128 (32 questions of 301 to 700 tokens behind 16384, 8 KV heads of 128: 4082 -> 3748 us; four of 1613 to 2146 behind
 // 10323, 4 KV heads: 691 -> 640).  But a workgroup that has a CU to itself is no faster, tiles that are not full cost twice as much, and
-// nothing runs beside a tile's start: only where the chip is full of tiles, with kAloneUnits more for each start (six texts of three
-// readers of 52 to 280 tokens: 30 us with 256 rows, 26 with 128).
+// nothing runs beside the start of its next one: only where the chip is full of tiles, with kAloneUnits for each start behind the first
+// (six texts of three readers of 52 to 280 tokens: 31 us with 256 rows, 27 with 128).
 void plan_wide(const std::vector<Seq>& some, const std::vector<Group>& groups, const uint8_t* open, int64_t page, int64_t rep, int64_t H,
                int64_t D, bool causal, PlanWords& out) {
   out.waves = 4;
@@ -198,7 +198,7 @@ void plan_wide(const std::vector<Seq>& some, const std::vector<Group>& groups, c
     const int64_t places = std::max<int64_t>(kSlots / 2 / H, 1);
     const Cut other = best_cut(wider, places, 2 * H);
     const int64_t starts = (static_cast<int64_t>(wider.size()) + places - 1) / places;       // of a place
-    if ((other.end + kAloneUnits * starts) * 92 < cut.end * 100) {
+    if ((other.end + kAloneUnits * (starts - 1)) * 92 < cut.end * 100) {
       tiles.swap(wider);
       cut = other;
       per_tile = 256 / rep;
