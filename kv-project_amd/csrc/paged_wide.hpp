@@ -272,8 +272,16 @@ __global__ __launch_bounds__(64 * W, 2) void paged_wide_kernel(WideArgs a) {
       uint32_t w = pack2<BF16>(wx, wz);
       asm volatile("" : "+v"(w));             // here, not behind a branch
       p[decltype(par)::value][n / 8][n % 8 / 2] = w;
-      sum += wx;
-      sum += wz;
+      if constexpr (BF16) {
+        sum += wx;
+        sum += wz;
+      } else {                                // the rounded ones: what a large weight loses leaves the sum as well (error 1.38-1.46 of a
+                                              // float32 softmax's -> 1.21-1.33, at 1.00-1.01 of the time); subnormal ones count
+        float y = sum;
+        asm("v_fma_mix_f32 %0, %1, 1.0, %0 op_sel_hi:[1,0,0]" : "+v"(y) : "v"(w));
+        asm("v_fma_mix_f32 %0, %1, 1.0, %0 op_sel:[1,0,0] op_sel_hi:[1,0,0]" : "+v"(y) : "v"(w));
+        sum = y;
+      }
     };
     float x = __builtin_fmaf(t[k / 16][k % 16], kz, -safe), z = __builtin_fmaf(t[k / 16][k % 16 + 1], kz, -safe);
     if constexpr (decltype(again)::value) {   // not above the reference's: it is off by much where scores pass 2^24 (a NaN stays one)
