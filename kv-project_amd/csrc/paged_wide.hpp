@@ -15,7 +15,7 @@
 // What bounds it: matrix cores and vector unit together.  A unit of 128 rows is 32 products of 32x32x16 a wavefront with head_dim 128
 // (1024 cycles) beside 230 vector instructions, an exponential for 256 multiplications; two wavefronts to a SIMD fill each other's gaps,
 // and reading the codes once for 128 or 256 rows leaves memory idle.  32 questions of 301 to 700 tokens behind 16384, 32 / 8 heads
-// of 128, int8, bf16: 3750-3910 us by card, 1.06-1.10 PFLOP/s, matrix cores busy 55%, vector unit 58%, at 2.1 GHz of 2.4; four fp16 chunks
+// of 128, int8, bf16: 3750-4020 us by card, 1.03-1.10 PFLOP/s, matrix cores busy 55%, vector unit 58%, at 2.1 GHz of 2.4; four fp16 chunks
 // of 512 to 1531 tokens behind 9000, head_dim 64, e4m3: 346-376 us, 35% and 65%.
 #pragma once
 #include <cfloat>
@@ -272,11 +272,11 @@ __global__ __launch_bounds__(64 * W, 2) void paged_wide_kernel(WideArgs a) {
       uint32_t w = pack2<BF16>(wx, wz);
       asm volatile("" : "+v"(w));             // here, not behind a branch
       p[decltype(par)::value][n / 8][n % 8 / 2] = w;
+      // Sums of the rounded weights: what a large one loses leaves the sum as well (error against 64 bits, of a float32 softmax's: bf16
+      // 1.50 -> 1.31, fp16 1.38-1.46 -> 1.21-1.33; time 1.00-1.02, the largest case 1.01).  Subnormal fp16 ones count.
       if constexpr (BF16) {
-        sum += wx;
-        sum += wz;
-      } else {                                // the rounded ones: what a large weight loses leaves the sum as well (error 1.38-1.46 of a
-                                              // float32 softmax's -> 1.21-1.33, at 1.00-1.01 of the time); subnormal ones count
+        sum = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2, w), __builtin_bit_cast(bf16x2, 0x3f803f80u), sum, false);
+      } else {
         float y = sum;
         asm("v_fma_mix_f32 %0, %1, 1.0, %0 op_sel_hi:[1,0,0]" : "+v"(y) : "v"(w));
         asm("v_fma_mix_f32 %0, %1, 1.0, %0 op_sel:[1,0,0] op_sel_hi:[1,0,0]" : "+v"(y) : "v"(w));

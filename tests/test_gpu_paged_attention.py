@@ -11,9 +11,9 @@ pytestmark = pytest.mark.gpu
 
 # A weight times its block's value scale is one number of the type, rounded to nearest once: off by at most half a step, 2^-8 (bf16) or
 # 2^-11 (fp16) of itself, 2^-32 of the block's largest value where it is below fp16's normal range (the bound has 2^-25 of it)
-# fp16 sums the rounded weights p (1 + e), |e| <= h: its output is off by sum p e (v - o) / (1 + sum p e), at most h (sum p |v| + |o|) / (1 - h), and |o| is
+# The rounded weights p (1 + e), |e| <= h, are summed: the output is off by sum p e (v - o) / (1 + sum p e), at most h (sum p |v| + |o|) / (1 - h), and |o| is
 # no more than sum p |v|
-WEIGHT = {t: 2 * h / (1 - h) if t == torch.float16 else h for t, h in HALF.items()}
+WEIGHT = {t: 2 * h / (1 - h) for t, h in HALF.items()}
 
 
 @pytest.fixture(params=[0, None, 1 << 30], ids=["tiles", "by rows", "16 rows"], autouse=True)
