@@ -127,6 +127,7 @@ __global__ __launch_bounds__(T) void tables_extend_kernel(Tables a) {
     longest = tops[w][0] > longest ? tops[w][0] : longest;
     most_units = tops[w][1] > most_units ? tops[w][1] : most_units;
   }
+  __syncthreads();                            // the room is free for the scans
   const bool fit = !total[3] && total[0] <= free_pages;
   need = fit ? total[0] : 0;
   all = fit ? total[1] : 0;
