@@ -9,8 +9,8 @@
 // half g holds the scores of tokens 32 g .. 32 g + 31 in order, which is how it reads a channel of V: 16 bytes, 8 tokens.
 // The key scale multiplies the scores, the value scale the weights; both are float32.  Weights times scale are rounded once to
 // the inputs' type, half a step of the outputs'.  bfloat16 has a scale's range; for half types the accumulators are held in
-// units of a power of two near the scale, and the reference weighs 2^7: what a weight loses below 2^-14 is at most 2^-32 of its
-// block's largest value (pages of 32 tokens: of the two blocks of a unit).
+// units of a power of two near the scale (a row's own: only blocks that it sees count), and the reference weighs 2^7: what a weight loses
+// below 2^-14 is at most 2^-28 of its block's largest value, or with pages of 32 tokens 2^-32 of the larger one's of the two in a unit.
 //
 // What bounds it: matrix cores and vector unit together.  A unit of 128 rows is 32 products of 32x32x16 a wavefront with head_dim 128
 // (1024 cycles) beside 230 vector instructions, an exponential for 256 multiplications; two wavefronts to a SIMD fill each other's gaps,
@@ -235,8 +235,8 @@ __global__ __launch_bounds__(64 * W, 2) void paged_wide_kernel(WideArgs a) {
   // exponents of scores.
   constexpr float kLift = BF16 ? 0.0f : 7.0f; // log2 of the reference's weight
   constexpr float kMost = BF16 ? 0x1p13f : 0x1p15f;
-  float base = 0.0f, safe, sum, kz, lr, inv_r, unit = 1.0f, wx, wz;
-  bool unit_set = false;                      // o is held in units of a power of two near the value scale
+  float base = 0.0f, safe, sum, kz, lr, inv_r, wx, wz;
+  float unit = 0.0f;                          // a power of two near the value scales that the row has met: o is held in units of it; 0: none yet
   // The reference from the unit's scores, where one passes it by more than 2^slack.  lim: how many of this lane's 32 tokens the row
   // sees.  Only units that some row does not see whole look for it: in the others the weights are taken by the one there is, and
   // where a lane's come to more than kMost, taken again.  Weights of up to that cost no accuracy, and a maximum of every unit costs 30 of
@@ -351,26 +351,26 @@ __global__ __launch_bounds__(64 * W, 2) void paged_wide_kernel(WideArgs a) {
   auto rescale = [&]() KVQ_INLINE {
     if (__builtin_amdgcn_ballot_w64(grow != 1.0f)) each<0, D / 32>([&](auto c) KVQ_INLINE { o[c.value] *= grow; });
   };
-  // kz, lr and inv_r of a unit from its scales; what o is to be scaled by for a new unit of its own.  A block that a row sees
-  // nothing of may have the scale NaN; one of zeros (its scale is below 2^-100) weighs nothing in o, whatever its scale.
+  // kz, lr and inv_r of a unit from its scales; what o is to be scaled by for a new unit of its own, which is each row's: only the
+  // blocks that a row sees count (a hidden one may have any scale, NaN too; far larger ones behind a row cost it its fp16 weights).  A
+  // block of zeros (its scale is below 2^-100) weighs nothing in o, whatever its scale.
   float turn = 1.0f;
   auto scale_for = [&](float2 z, bool masked, int lim) KVQ_INLINE {
     kz = z.x * a.scale;
     kz = kz < FLT_MIN ? FLT_MIN : kz;
     turn = 1.0f;
+    float v = z.y;
+    if (masked) v = (kOne ? lim + 32 * g : lim) > 0 ? v : 0.0f;
+    if constexpr (!kOne) v = xmax32(v);
     // changed where a scale is not within the window below it (fp16: its weights have to stay normal numbers; bf16: their sum)
-    const float v0 = __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(z.y)));
-    const float v1 = kOne ? v0 : __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(z.y), 32));
-    const float v = kOne ? v0 : fmaxf(v0, v1);
     constexpr float kWindow = BF16 ? 0x1p-60f : 0x1p-4f;
-    if (v > 0x1p-100f && !(v <= unit && v >= unit * kWindow && unit_set)) {
-      float now = __uint_as_float((__float_as_uint(v) & 0x7f800000u) + 0x00800000u);    // 2^k above v
-      if (unit_set) {
-        if (now < unit * 0x1p-100f) now = unit * 0x1p-100f;
-        turn = unit / now;
-      }
-      unit = now;
-      unit_set = true;
+    const bool out = v != __builtin_amdgcn_fmed3f(v, unit * kWindow, unit);
+    if (__builtin_amdgcn_ballot_w64(out)) {
+      const bool change = out && v > 0x1p-100f;   // not for a NaN, or where the row sees nothing
+      float now = __uint_as_float((__float_as_uint(v) & 0x7f800000u) + 0x00800000u);        // 2^k above v
+      now = now < unit * 0x1p-100f ? unit * 0x1p-100f : now;
+      turn = change && unit > 0.0f ? unit / now : 1.0f;
+      unit = change ? now : unit;
     }
     // (the quotient of a power of two is exact; of two blocks of one unit the smaller one's scale is taken for 2^-100 of the larger
     // one's at least)
