@@ -355,6 +355,7 @@ __global__ __launch_bounds__(64 * W, 2) void paged_wide_kernel(WideArgs a) {
   // blocks that a row sees count (a hidden one may have any scale, NaN too; far larger ones behind a row cost it its fp16 weights).  A
   // block of zeros (its scale is below 2^-100) weighs nothing in o, whatever its scale.
   float turn = 1.0f;
+  auto above = [](float x) KVQ_INLINE { return __uint_as_float((__float_as_uint(x) & 0x7f800000u) + 0x00800000u); };  // the next 2^k
   auto scale_for = [&](float2 z, bool masked, int lim) KVQ_INLINE {
     kz = z.x * a.scale;
     kz = kz < FLT_MIN ? FLT_MIN : kz;
@@ -367,13 +368,18 @@ __global__ __launch_bounds__(64 * W, 2) void paged_wide_kernel(WideArgs a) {
     const bool out = v != __builtin_amdgcn_fmed3f(v, unit * kWindow, unit);
     if (__builtin_amdgcn_ballot_w64(out)) {
       const bool change = out && v > 0x1p-100f;   // not for a NaN, or where the row sees nothing
-      float now = __uint_as_float((__float_as_uint(v) & 0x7f800000u) + 0x00800000u);        // 2^k above v
-      now = now < unit * 0x1p-100f ? unit * 0x1p-100f : now;
+      float now = above(v);
+      if (__builtin_amdgcn_ballot_w64(change && now < unit)) {
+        // a fall multiplies o: not beyond 2^122, the products that are on their way to it (below 2^32) with it
+        float most = 0x1p32f;
+        each<0, D / 32>([&](auto c) KVQ_INLINE { each<0, 16>([&](auto e) KVQ_INLINE { most = fmaxf(most, fabsf(o[c.value][e.value])); }); });
+        const float least = unit * (above(fminf(xmax32(most), 0x1p120f)) * 0x1p-121f);
+        now = now < least ? least : now;
+      }
       turn = change && unit > 0.0f ? unit / now : 1.0f;
       unit = change ? now : unit;
     }
-    // (the quotient of a power of two is exact; of two blocks of one unit the smaller one's scale is taken for 2^-100 of the larger
-    // one's at least)
+    // (the quotient of a power of two is exact; a scale is taken for 2^-100 of its unit at least)
     float r = z.y < 0x1p-100f ? 1.0f : z.y * __builtin_amdgcn_rcpf(unit);
     r = r < 0x1p-100f ? 0x1p-100f : r;
     lr = __builtin_amdgcn_logf(r);

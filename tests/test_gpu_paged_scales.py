@@ -78,3 +78,13 @@ def test_large_values_that_a_row_does_not_see(dtype, small, big, page, code, hea
         e = [big if i == at else small for i in range(6)]
         t = Text(e, [0] * 6, page, page, code, dtype, heads, seed=page + at)
         t.check(t.n, what=f"large block {at}")
+
+
+@pytest.mark.parametrize("code", CODES)
+@pytest.mark.parametrize("page", PAGES)
+@pytest.mark.parametrize("e", [[83, 0, -63], [95, 30, -40, -85], [60, -80, 60, -80]], ids=str)
+def test_values_that_fall_again_and_again(e, page, code, heads):
+    """bf16 values that fall by more than 2^100 in several steps: sums of the large ones stay finite in units of the small."""
+    bf16 = torch.bfloat16
+    Text(e, [0] * len(e), 128, page, code, bf16, heads, seed=page).check(130, what="even")
+    Text([e[0]] * 2 + e, [0] * 2 + [8.0] * len(e), 128, page, code, bf16, heads, seed=page + 1).check(130, what="heavier later")
