@@ -352,8 +352,8 @@ __global__ __launch_bounds__(64 * W, 2) void paged_wide_kernel(WideArgs a) {
     if (__builtin_amdgcn_ballot_w64(grow != 1.0f)) each<0, D / 32>([&](auto c) KVQ_INLINE { o[c.value] *= grow; });
   };
   // kz, lr and inv_r of a unit from its scales; what o is to be scaled by for a new unit of its own, which is each row's: only the
-  // blocks that a row sees count (a hidden one may have any scale, NaN too; far larger ones behind a row cost it its fp16 weights).  A
-  // block of zeros (its scale is below 2^-100) weighs nothing in o, whatever its scale.
+  // blocks that a row sees count (a hidden one may have any scale, NaN too; far larger ones behind a row cost it its fp16 weights).  bf16
+  // blocks have scales down to 2^-109, with codes down to 2^-108; in fp16 what is below 2^-100 is a block of zeros, which weighs nothing in o.
   float turn = 1.0f;
   auto above = [](float x) KVQ_INLINE { return __uint_as_float((__float_as_uint(x) & 0x7f800000u) + 0x00800000u); };  // the next 2^k
   auto scale_for = [&](float2 z, bool masked, int lim) KVQ_INLINE {
@@ -364,10 +364,10 @@ __global__ __launch_bounds__(64 * W, 2) void paged_wide_kernel(WideArgs a) {
     if (masked) v = (kOne ? lim + 32 * g : lim) > 0 ? v : 0.0f;
     if constexpr (!kOne) v = xmax32(v);
     // changed where a scale is not within the window below it (fp16: its weights have to stay normal numbers; bf16: their sum)
-    constexpr float kWindow = BF16 ? 0x1p-60f : 0x1p-4f;
+    constexpr float kWindow = BF16 ? 0x1p-60f : 0x1p-4f, kEmpty = BF16 ? 0.0f : 0x1p-100f;
     const bool out = v != __builtin_amdgcn_fmed3f(v, unit * kWindow, unit);
     if (__builtin_amdgcn_ballot_w64(out)) {
-      const bool change = out && v > 0x1p-100f;   // not for a NaN, or where the row sees nothing
+      const bool change = out && v > kEmpty;   // not for a NaN, or where the row sees nothing
       float now = above(v);
       if (__builtin_amdgcn_ballot_w64(change && now < unit)) {
         // a fall multiplies o: not beyond 2^122, the products that are on their way to it (below 2^32) with it
@@ -380,7 +380,7 @@ __global__ __launch_bounds__(64 * W, 2) void paged_wide_kernel(WideArgs a) {
       unit = change ? now : unit;
     }
     // (the quotient of a power of two is exact; a scale is taken for 2^-100 of its unit at least)
-    float r = z.y < 0x1p-100f ? 1.0f : z.y * __builtin_amdgcn_rcpf(unit);
+    float r = z.y < kEmpty ? 1.0f : z.y * __builtin_amdgcn_rcpf(unit);
     r = r < 0x1p-100f ? 0x1p-100f : r;
     lr = __builtin_amdgcn_logf(r);
     inv_r = __builtin_amdgcn_rcpf(r);

@@ -88,3 +88,26 @@ def test_values_that_fall_again_and_again(e, page, code, heads):
     bf16 = torch.bfloat16
     Text(e, [0] * len(e), 128, page, code, bf16, heads, seed=page).check(130, what="even")
     Text([e[0]] * 2 + e, [0] * 2 + [8.0] * len(e), 128, page, code, bf16, heads, seed=page + 1).check(130, what="heavier later")
+
+
+@pytest.mark.parametrize("code", CODES)
+@pytest.mark.parametrize("page", PAGES)
+@pytest.mark.parametrize("e", [-94, -97, -103, -106])
+def test_small_values(e, page, code, heads):
+    """bf16 values down to where a block's codes are all zero, alone, between ordinary ones, and between ordinary ones that weigh nothing."""
+    bf16 = torch.bfloat16
+    Text([e] * 6, [0] * 6, 128, page, code, bf16, heads, seed=page).check(200, what="alone")
+    Text([0, e, e, 0, e, 0, e], [0] * 7, 128, page, code, bf16, heads, seed=page + 1).check(200, what="between")
+    t = Text([0, e, e, 0, e], [-60, 0, 0, -60, 0], 128, page, code, bf16, heads, rest=0, seed=page + 2)
+    t.check(128, what="heavy between light")
+    t.check(128, False, what="heavy between light")
+
+
+@pytest.mark.parametrize("code", CODES)
+@pytest.mark.parametrize("page", PAGES)
+@pytest.mark.parametrize("e", [[100, 30, -40, -80, -105], [-100, 100, -100], [0, -130, 90, -130, -60]], ids=str)
+def test_small_values_behind_large_ones(e, page, code, heads):
+    """bf16 values up to 2^205 of the smallest, blocks whose codes are all zero."""
+    bf16 = torch.bfloat16
+    Text(e, [0] * len(e), 128, page, code, bf16, heads, seed=page).check(130, what="even")
+    Text([e[0]] * 2 + e, [0] * 2 + [8.0] * len(e), 128, page, code, bf16, heads, seed=page + 1).check(130, what="heavier later")
