@@ -10,7 +10,8 @@
 // The key scale multiplies the scores, the value scale the weights; both are float32.  Weights times scale are rounded once to
 // the inputs' type, half a step of the outputs'.  bfloat16 has a scale's range; for half types the accumulators are held in
 // units of a power of two near the scale (a row's own: only blocks that it sees count), and the reference weighs 2^7: what a weight loses
-// below 2^-14 is at most 2^-28 of its block's largest value, or with pages of 32 tokens 2^-32 of the larger one's of the two in a unit.
+// below 2^-14 is at most 2^-28 of its block's largest value, or with pages of 32 tokens 2^-32 of the larger one's of the two in a unit;
+// the sum loses nothing of it.
 //
 // What bounds it: matrix cores and vector unit together.  A unit of 128 rows is 32 products of 32x32x16 a wavefront with head_dim 128
 // (1024 cycles) beside 230 vector instructions, an exponential for 256 multiplications; two wavefronts to a SIMD fill each other's gaps,
@@ -235,6 +236,7 @@ __global__ __launch_bounds__(64 * W, 2) void paged_wide_kernel(WideArgs a) {
   // exponents of scores.
   constexpr float kLift = BF16 ? 0.0f : 7.0f; // log2 of the reference's weight
   constexpr float kMost = BF16 ? 0x1p13f : 0x1p15f;
+  constexpr float kWindow = BF16 ? 0x1p-60f : 0x1p-4f;              // a scale in its unit, unless it shares that with a larger one
   float base = 0.0f, safe, sum, kz, lr, inv_r, wx, wz;
   float unit = 0.0f;                          // a power of two near the value scales that the row has met: o is held in units of it; 0: none yet
   // The reference from the unit's scores, where one passes it by more than 2^slack.  lim: how many of this lane's 32 tokens the row
@@ -295,6 +297,17 @@ __global__ __launch_bounds__(64 * W, 2) void paged_wide_kernel(WideArgs a) {
     wz = z;
     if constexpr (i == 15) finish(std::integral_constant<int, k>{});
   };
+  // The sum without the value scale, where that is so far below the unit that the type does not hold a weight times it: such weights may
+  // be lost in the products, where they are nothing beside the larger block's, but not in the sum
+  auto plain_sum = [&](auto par, auto again) KVQ_INLINE {
+    float y = 0.0f;
+    each<0, 32>([&](auto e) KVQ_INLINE {
+      float x = __builtin_fmaf(s[decltype(par)::value][e.value / 16][e.value % 16], kz, kLift - base);
+      if constexpr (decltype(again)::value) x = x > kLift ? kLift : x;
+      y += __builtin_amdgcn_exp2f(x);
+    });
+    return y;
+  };
   constexpr int kV = 4 * (D / 32), kK = 2 * (D / 16);               // steps of the two products
   constexpr std::integral_constant<int, 0> even{};
   constexpr std::integral_constant<int, 1> odd{};
@@ -325,11 +338,17 @@ __global__ __launch_bounds__(64 * W, 2) void paged_wide_kernel(WideArgs a) {
       __builtin_amdgcn_sched_barrier(0);
     });
     float add = sum * inv_r;
-    if (__builtin_expect(__builtin_amdgcn_ballot_w64(add > kMost) != 0, 0)) {
-      find(par, false, lim, 0.0f);
-      begin();
-      each<0, 16>([&](auto i) KVQ_INLINE { share(par, i, yes); });
-      add = sum * inv_r;
+    constexpr bool kFar = BF16 || !kOne;
+    const bool far = kFar && inv_r > 2.0f / kWindow;
+    if (__builtin_expect(__builtin_amdgcn_ballot_w64(add > kMost || far) != 0, 0)) {
+      if constexpr (kFar) add = far ? plain_sum(par, no) : add;
+      if (__builtin_amdgcn_ballot_w64(add > kMost)) {
+        find(par, false, lim, 0.0f);
+        begin();
+        each<0, 16>([&](auto i) KVQ_INLINE { share(par, i, yes); });
+        add = sum * inv_r;
+        if constexpr (kFar) add = far ? plain_sum(par, yes) : add;
+      }
     }
     l += add;
     asm volatile("" : "+v"(l));
@@ -364,7 +383,7 @@ __global__ __launch_bounds__(64 * W, 2) void paged_wide_kernel(WideArgs a) {
     if (masked) v = (kOne ? lim + 32 * g : lim) > 0 ? v : 0.0f;
     if constexpr (!kOne) v = xmax32(v);
     // changed where a scale is not within the window below it (fp16: its weights have to stay normal numbers; bf16: their sum)
-    constexpr float kWindow = BF16 ? 0x1p-60f : 0x1p-4f, kEmpty = BF16 ? 0.0f : 0x1p-100f;
+    constexpr float kEmpty = BF16 ? 0.0f : 0x1p-100f;
     const bool out = v != __builtin_amdgcn_fmed3f(v, unit * kWindow, unit);
     if (__builtin_amdgcn_ballot_w64(out)) {
       const bool change = out && v > kEmpty;   // not for a NaN, or where the row sees nothing

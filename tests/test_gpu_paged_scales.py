@@ -111,3 +111,31 @@ def test_small_values_behind_large_ones(e, page, code, heads):
     bf16 = torch.bfloat16
     Text(e, [0] * len(e), 128, page, code, bf16, heads, seed=page).check(130, what="even")
     Text([e[0]] * 2 + e, [0] * 2 + [8.0] * len(e), 128, page, code, bf16, heads, seed=page + 1).check(130, what="heavier later")
+
+
+@pytest.mark.parametrize("code", CODES)
+@pytest.mark.parametrize("dtype,apart", [(torch.float16, 12), (torch.float16, 20), (torch.float16, 24), (torch.float16, 27), (torch.float16, 30),
+                                         (torch.bfloat16, 60), (torch.bfloat16, 90), (torch.bfloat16, 99)])
+def test_neighbours_that_share_a_unit(dtype, apart, code, heads):
+    """Pages of 32 tokens whose values are 2^apart of each other's in one unit of 64, the small ones with nearly all of the weight: it counts
+    in the softmax's sum whatever is left of it in the products."""
+    big = 9 if dtype == torch.float16 else apart // 2
+    for first in (0, 1):
+        e = [big, big - apart] if first else [big - apart, big]
+        for light in (-2.0, -5.0, -9.0):
+            c = [light, 0] if first else [0, light]
+            t = Text(e * 2, c * 2, 32, 32, code, dtype, heads, seed=apart + first)
+            for causal in (True, False):
+                t.check(128, causal, what=f"light {light}")
+
+
+@pytest.mark.parametrize("code", CODES)
+@pytest.mark.parametrize("small,big", [(-60, 30), (-20, 70), (-94, 0)])
+def test_neighbours_of_which_the_small_one_is_all(small, big, code, heads):
+    """bf16, pages of 32 tokens in one unit, the far larger one of next to no weight, in front or behind."""
+    for first in (0, 1):
+        for light in (-25.0, -60.0, -90.0):
+            e, c = ([big, small], [light, 0]) if first else ([small, big], [0, light])
+            t = Text(e * 3, c * 3, 32, 32, code, torch.bfloat16, heads, rest=0 if first else 7, seed=first)
+            t.check(64, causal=False, what=f"light {light}")
+            t.check(32, what=f"light {light}")
