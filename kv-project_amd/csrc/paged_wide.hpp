@@ -10,8 +10,8 @@
 // The key scale multiplies the scores, the value scale the weights; both are float32.  Weights times scale are rounded once to
 // the inputs' type, half a step of the outputs'.  bfloat16 has a scale's range; for half types the accumulators are held in
 // units of a power of two near the scale (a row's own: only blocks that it sees count), and the reference weighs 2^7: what a weight loses
-// below 2^-14 is at most 2^-28 of its block's largest value, or with pages of 32 tokens 2^-32 of the larger one's of the two in a unit;
-// the sum loses nothing of it.
+// below 2^-14 is at most 2^-28 of its block's largest value, or with pages of 32 tokens of the larger one's of the two in a unit; the sum
+// loses nothing of it.
 //
 // What bounds it: matrix cores and vector unit together.  A unit of 128 rows is 32 products of 32x32x16 a wavefront with head_dim 128
 // (1024 cycles) beside 230 vector instructions, an exponential for 256 multiplications; two wavefronts to a SIMD fill each other's gaps,
@@ -412,7 +412,7 @@ __global__ __launch_bounds__(64 * W, 2) void paged_wide_kernel(WideArgs a) {
   auto lim_of = [&](int j) KVQ_INLINE { return j < units ? (visible < full ? visible : full) - (u0 + j) * kUnit - 32 * g : 0; };
   // Pages of units on their way: id[i] of unit j + 1 + i when iteration j begins
   Ids id[3], next_id;
-  float2 z_now, z_next;
+  float2 z_now;
   auto step = [&](auto par, int j) KVQ_INLINE {
     constexpr int kPar = decltype(par)::value;
     const bool masked = j >= whole;

@@ -89,8 +89,13 @@ class PagedPlan:
 def paged_attention(q: torch.Tensor, scaling: float, cache: PagedCache, layer: int, plan: PagedPlan, *,
                     out: Optional[torch.Tensor] = None, workspace: Optional[torch.Tensor] = None) -> torch.Tensor:
     """Attention of the plan's packed rows q (rows, Hq, d) over one layer of the cache; returns (rows, Hq, d).  The codes go into
-    the products as they are and their scales in float32; what a row does not see changes nothing, whatever it holds.  Forward only, as
-    the decodes: no gradient is recorded."""
+    the products as they are and their scales in float32; what a row does not see changes nothing, whatever it holds.  Rows beyond a few
+    (FEW_ROWS of a sequence) weigh with one number of the model's type, rounded once (half a step: bf16 2^-8, fp16 2^-11 of a weight, which is
+    summed as it was rounded), where paged_decode's few rows have two of them (2^-17): the same row differs by that between a call of
+    32 rows a KV head and one of 33.  Forward only, as the decodes: no gradient is recorded.
+
+    Value blocks of one sequence may lie far apart in size.  Of two pages of 32 tokens side by side (blocks 2 i and 2 i + 1) a token of the
+    smaller one's is off by up to 2^-28 of the larger one's largest value in fp16, and by 2^-100 of the largest that the row sees in bf16."""
     if not 0 <= layer < cache.layers:
         raise IndexError(f"no layer {layer} (of {cache.layers})")
     if plan.cache is not cache:

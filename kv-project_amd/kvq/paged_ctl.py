@@ -34,7 +34,9 @@ MANY_ROWS = 192
 
 class PagedCtl:
     """Sequences in ``slots`` of ``cache``, the rows of the model's batch in that order.  ``over_pages``: steps of many tokens
-    attend straight over the pages (the codes as they are, where reading back rounds them to the model's type)."""
+    attend straight over the pages (the codes as they are, where reading back rounds them to the model's type).  They are many from 33 rows a
+    KV head on, where reading back is from 192 on: steps between these leave paged_decode, whose weights have 17 bits, for
+    paged_attention's, one number of the model's type as in prompt_attention."""
 
     def __init__(self, cache: PagedCache, slots: Sequence[int], *, over_pages: bool = False):
         self.cache, self.slots, self.over_pages = cache, [int(s) for s in slots], bool(over_pages)
