@@ -409,7 +409,8 @@ __global__ __launch_bounds__(64 * W, 2) void paged_wide_kernel(WideArgs a) {
       inv_r = lim > 0 ? inv_r : 0.0f;
     }
   };
-  auto lim_of = [&](int j) KVQ_INLINE { return j < units ? (visible < full ? visible : full) - (u0 + j) * kUnit - 32 * g : 0; };
+  // (nothing of what lies behind the last unit, for either half)
+  auto lim_of = [&](int j) KVQ_INLINE { return j < units ? (visible < full ? visible : full) - (u0 + j) * kUnit - 32 * g : -kUnit; };
   // Pages of units on their way: id[i] of unit j + 1 + i when iteration j begins
   Ids id[3], next_id;
   float2 z_now;

@@ -56,8 +56,8 @@ class Text:
         out, q = out[:, some], q[:, some]
         k, v = cached(self.k, page, self.code), cached(self.v, page, self.code)
         ref = attend(q, k, v, 1.0 / self.d, causal)
-        for a in range(0, rows, page):
-            b = min(rows, a + page)
+        for a in [0, *range(-(n - rows) % page or page, rows, page)]:
+            b = min(rows, a + page - (n - rows + a) % page)
             mass = float(ref[1][a:b].max())
             unit = 2.0 ** -round(torch.log2(torch.tensor(mass)).item()) if self.dtype == torch.bfloat16 else 1.0
             got, (o, m, s) = out[a:b].double() * unit, (x[a:b] for x in ref)
@@ -139,3 +139,15 @@ def test_neighbours_of_which_the_small_one_is_all(small, big, code, heads):
             t = Text(e * 3, c * 3, 32, 32, code, torch.bfloat16, heads, rest=0 if first else 7, seed=first)
             t.check(64, causal=False, what=f"light {light}")
             t.check(32, what=f"light {light}")
+
+
+@pytest.mark.parametrize("code", CODES)
+@pytest.mark.parametrize("page", PAGES)
+@pytest.mark.parametrize("small,big", [(-70, 70), (-80, 90)])
+def test_tiles_over_the_border_of_a_large_block(small, big, page, code, heads):
+    """bf16 rows of one tile on both sides of where a far larger block begins, the tile's units in even and odd numbers."""
+    run = max(page, 64)
+    for at in (1, 2, 3):
+        t = Text([small] * at + [big], [0] * (at + 1), run, page, code, torch.bfloat16, heads, rest=0, seed=page + at)
+        for offset in (8, 20):
+            t.check(t.n - offset, what=f"large block {at}, rows from {offset}")
