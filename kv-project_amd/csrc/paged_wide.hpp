@@ -14,10 +14,11 @@
 // loses nothing of it.
 //
 // What bounds it: matrix cores and vector unit together.  A unit of 128 rows is 32 products of 32x32x16 a wavefront with head_dim 128
-// (1024 cycles) beside 230 vector instructions, an exponential for 256 multiplications; two wavefronts to a SIMD fill each other's gaps,
+// (1024 cycles) beside 220 vector instructions, an exponential for 256 multiplications; two wavefronts to a SIMD fill each other's gaps,
 // and reading the codes once for 128 or 256 rows leaves memory idle.  32 questions of 301 to 700 tokens behind 16384, 32 / 8 heads
-// of 128, int8, bf16: 3750-4020 us by card, 1.03-1.10 PFLOP/s, matrix cores busy 55%, vector unit 58%, at 2.1 GHz of 2.4; four fp16 chunks
-// of 512 to 1531 tokens behind 9000, head_dim 64, e4m3: 346-376 us, 35% and 65%.
+// of 128, int8, bf16: 3700-4020 us by card, 1.03-1.12 PFLOP/s, matrix cores busy 54-56%, vector unit 54-59%, at 2.1 GHz of 2.4; four fp16
+// chunks of 512 to 1531 tokens behind 9000, head_dim 64, e4m3: 346-382 us, 35% and 65%.  Four wavefronts at head_dim 128 spill 2 to 9 of
+// their 256 registers.
 #pragma once
 #include <cfloat>
 #include <type_traits>
@@ -242,7 +243,7 @@ __global__ __launch_bounds__(64 * W, 2) void paged_wide_kernel(WideArgs a) {
   // The reference from the unit's scores, where one passes it by more than 2^slack.  lim: how many of this lane's 32 tokens the row
   // sees.  Only units that some row does not see whole look for it: in the others the weights are taken by the one there is, and
   // where a lane's come to more than kMost, taken again.  Weights of up to that cost no accuracy, and a maximum of every unit costs 30 of
-  // its 230 vector instructions with head_dim 64, in a row before the first weight (four fp16 chunks 398 -> 376 us; 32 questions
+  // its 207 vector instructions with head_dim 64, in a row before the first weight (four fp16 chunks 398 -> 376 us; 32 questions
   // behind 16384, head_dim 128, 3925 -> 3777).
   auto find = [&](auto par, bool masked, int lim, float slack) KVQ_INLINE {
     auto& t = s[decltype(par)::value];
